@@ -347,6 +347,36 @@ int cavs_softmax_xent_part(float *loss, float *dlogits, const float *logits, con
 int cavs_softmax_xent_sum_rows(int n, int C);
 int cavs_softmax_xent_sums(float *loss, float *dlogits, const float *logits, const float *labels, float *sums, int n, int C,
                            void *stream);
+/* Softmax cross entropy of X W^T + b over a large vocabulary, and its gradients, without logits in memory: FullyConnected
+ * (cavs/backend/op_impl_fullyconnected_cublas.cc:71-79, gradients :150-163) and SoftmaxEntropyLoss
+ * (op_impl_softmax_entropy_logits_loss.cu:94-140, :212-250) where [n, C] logits and d logits would be the largest tensors of a step.
+ *   z = X W^T + b;  lse[r] = log sum_c exp(z[r,c]);  loss[r] = lse[r] - z[r, label[r]]
+ *   d[r,c] = scale * dloss[r] * (exp(z[r,c] - lse[r]) - (c == label[r]));  dX = d W;  dW = d^T X;  db[c] = sum_r d[r,c]
+ * X [n,H], W [C,H] and dX, dW are of `type` (row strides in elements, any of at least H), everything else is fp32; b and dloss (all ones)
+ * may be NULL.  What is NULL of loss, lse, dX, dW and db is not computed.  Outputs may not overlap inputs or each other.
+ * labels are class ids as floats; a row whose label is below 0, not below C or NaN takes no part: its loss is 0, it adds nothing
+ * to dW and db and its row of dX is 0, whatever X holds there.  A class with b = -infinity is masked: probability 0, gradient 0, whatever its row
+ * of W holds.  A row without any class that is not masked has lse = -infinity, loss = infinity and no gradient.  Otherwise infinities and NaN in
+ * X or W make their row's or column's results NaN.  n = 0 is allowed (dW and db become 0).
+ * CAVS_F32: products as sums of bf16 parts in full fp32 precision (the arithmetic of cavs_sgemm); CAVS_BF16: products of bf16 values
+ * in fp32 accumulators, d rounded to bf16 between its products, gradients rounded once.  Results are the same on every call.
+ *   _fwd  loss and lse
+ *   _bwd  the gradients, from the lse that _fwd (or cavs_vocab_xent) left for the same X, W and b
+ *   cavs_vocab_xent  both in one call
+ * The vocabulary goes by in pieces; the logits are computed once for lse and once more for the gradients.  The workspace (16-byte aligned, of
+ * at least cavs_vocab_xent_workspace(type, n, H, C, grads) bytes on this device, grads = 0 for _fwd) holds one piece's d, not
+ * [n, C] of anything; it may be reused by the next call on the same stream, not by one that overlaps in time.  At most 2^22 rows,
+ * 2^23 classes, H <= 2^16.  The workspace query returns 0 for a shape or type that is refused. */
+enum { CAVS_F32 = 0, CAVS_BF16 = 1 };
+size_t cavs_vocab_xent_workspace(int type, int n, int H, int C, int grads);
+int cavs_vocab_xent_fwd(int type, const void *X, int ldx, const void *W, int ldw, const float *b, const float *labels, float *loss,
+                        float *lse, int n, int H, int C, void *workspace, size_t workspace_bytes, void *stream);
+int cavs_vocab_xent_bwd(int type, const void *X, int ldx, const void *W, int ldw, const float *b, const float *labels,
+                        const float *lse, const float *dloss, float scale, void *dX, int lddx, void *dW, int lddw, float *db, int n,
+                        int H, int C, void *workspace, size_t workspace_bytes, void *stream);
+int cavs_vocab_xent(int type, const void *X, int ldx, const void *W, int ldw, const float *b, const float *labels, const float *dloss,
+                    float scale, float *loss, float *lse, void *dX, int lddx, void *dW, int lddw, float *db, int n, int H, int C,
+                    void *workspace, size_t workspace_bytes, void *stream);
 /* SGD (cavs/backend/op_impl_sgd.cu): w -= lr * g */
 int cavs_sgd(float *w, const float *g, float lr, size_t n, void *stream);
 

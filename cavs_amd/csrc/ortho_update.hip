@@ -1,0 +1,546 @@
+// Momentum, orthogonalised by Newton-Schulz products, for several matrices at once.
+//
+//   M <- mu M + G,  U = G + mu M or M,  X = U / (|U| + eps);  `steps` times  X <- (a I + b A + c A A) X, A = X X^T
+//
+// on the side that is smaller: m x n with m <= n.  Three products a step, each one launch over all matrices: A and a I + b A + c A A are
+// symmetric, so only tiles that reach the diagonal or below are made, and each is stored twice.  What a launch makes is
+// what the next ones read, as planes of bf16 parts (nt_product.h): X by rows (for A) and by columns (for the product
+// with it), A and the polynomial by rows, which are their columns.
+//
+// A singular value next to 0 grows a-fold a step, 485-fold in five, and so does a rounding error made beside it.  With three parts X, A and the
+// polynomial keep an fp32's bits and the result is as far off as in fp32.  Where the result is rounded to bf16, two parts will do: what
+// they leave off, 2^-17 of the largest, is 2^-8 then.  (One part, 2^-9, would come out as large as the result.)
+#include "nt_product.h"
+
+namespace cavs {
+namespace {
+
+constexpr int kMats = 16;       // matrices of a launch
+constexpr int kNormBlocks = 64; // workgroups that add up a matrix's squares
+
+struct Mat {
+  const void *G;
+  float *M, *W;
+  void *O;
+  long ldg, ldm, ldw, ldo;
+  int rows, cols;      // as the caller has them
+  int m, n, mp, np;    // of X, and padded to whole steps
+  u16 *X, *Xt[2], *A, *Q;  // planes: [m, np], [n, mp] (read, written), [m, mp], [m, mp]
+  float shrink;        // sqrt(max(1, rows / cols))
+};
+
+struct Common {
+  int count, nesterov;
+  float a, b, c, eps, momentum, lr, decay;
+  const int *guard;
+  double *squares;     // [kMats][kNormBlocks]
+  int *arrived;        // a counter for every tile of a launch, zero between launches
+  int counters;
+  float *part;         // tiles of stretches of K
+};
+
+__device__ inline bool held_back(const Common &c) { return c.guard && *c.guard != 0; }
+
+template <class Src>
+__device__ inline float update_of(const Mat &t, const Common &c, long r, int k) {
+  const float g = value_of(static_cast<const Src *>(t.G) + r * t.ldg + k);
+  if (!t.M) return g;
+  const float m = t.M[r * t.ldm + k];
+  return c.nesterov ? fmaf(c.momentum, m, g) : m;
+}
+
+// M <- mu M + G, and the squares of U, added up in 64 bits in a fixed order
+struct NormArgs {
+  Mat m[kMats];
+  Common c;
+};
+template <class Src>
+__global__ __launch_bounds__(256) void norm_kernel(NormArgs g) {
+  const Common &c = g.c;
+  const int who = blockIdx.y;
+  if (who == 0)
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < c.counters; i += gridDim.x * 256) c.arrived[i] = 0;
+  if (held_back(c)) return;
+  const Mat &t = g.m[who];
+  double sum = 0.;
+  for (long r = blockIdx.x; r < t.rows; r += gridDim.x)
+    for (int k = threadIdx.x; k < t.cols; k += 256) {
+      if (t.M) {
+        float *m = t.M + r * t.ldm + k;
+        *m = fmaf(c.momentum, *m, value_of(static_cast<const Src *>(t.G) + r * t.ldg + k));
+      }
+      const double u = update_of<Src>(t, c, r, k);
+      sum += u * u;
+    }
+  __shared__ double s[256];
+  s[threadIdx.x] = sum;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) s[threadIdx.x] += s[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) c.squares[who * kNormBlocks + blockIdx.x] = s[0];
+}
+
+// X by rows and by columns, 64 x 64 at a time
+struct StartArgs {
+  Mat m[kMats];
+  Common c;
+  int first[kMats + 1];
+};
+template <int P, class Src>
+__global__ __launch_bounds__(256) void start_kernel(StartArgs g) {
+  __shared__ float tile[64][65];
+  const Common &c = g.c;
+  if (held_back(c)) return;
+  int who = 0;
+  while (who + 1 < c.count && (int)blockIdx.x >= g.first[who + 1]) who++;
+  const Mat &t = g.m[who];
+  double sum = 0.;
+  for (int i = 0; i < kNormBlocks; i++) sum += c.squares[who * kNormBlocks + i];
+  const double by = 1. / (sqrt(sum) + (double)c.eps);
+  const bool flat = t.rows <= t.cols;
+  const int across = (flat ? t.np : t.mp) / 64, block = blockIdx.x - g.first[who];
+  const int r0 = block / across * 64, k0 = block % across * 64;
+  u16 *o = flat ? t.X : t.Xt[0], *tr = flat ? t.Xt[0] : t.X;
+  const int ldo = flat ? t.np : t.mp, ldt = flat ? t.mp : t.np;
+  const long po = (long)t.rows * ldo, pt = (long)t.cols * ldt;
+  {
+    const int k = threadIdx.x & 63;
+#pragma unroll 4
+    for (int i = threadIdx.x >> 6; i < 64; i += 4) {
+      const int r = r0 + i;
+      float x = 0.f;
+      if (r < t.rows && k0 + k < t.cols) x = (float)((double)update_of<Src>(t, c, r, k0 + k) * by);
+      if (r < t.rows) {
+        u16 part[P];
+        parts_of<P>(x, part);
+#pragma unroll
+        for (int p = 0; p < P; p++) o[p * po + (long)r * ldo + k0 + k] = part[p];
+      }
+      tile[i][k] = x;
+    }
+  }
+  __syncthreads();
+  const int i = threadIdx.x & 63;
+#pragma unroll 4
+  for (int k = threadIdx.x >> 6; k < 64; k += 4) {
+    if (k0 + k >= t.cols || r0 + i >= ldt) continue;
+    u16 part[P];
+    parts_of<P>(tile[i][k], part);
+#pragma unroll
+    for (int p = 0; p < P; p++) tr[p * pt + (long)(k0 + k) * ldt + r0 + i] = part[p];
+  }
+}
+
+enum { GRAM = 0, POLYNOMIAL = 1, APPLY = 2, LAST = 3 };
+
+struct ProductArgs {
+  Mat m[kMats];
+  Common c;
+  int first[kMats + 1];              // workgroups
+  int tilesN[kMats], splits[kMats], chunk[kMats], tiles0[kMats];  // tiles0: of the counters
+  long part0[kMats];
+};
+
+// Tile `t` of those of a symmetric m x m result that reach the diagonal or below
+template <class T>
+__device__ inline void lower_tile(int t, int m, int *tm, int *tn) {
+  const int tilesN = (m + T::BN - 1) / T::BN;
+  int row = 0;
+  for (;; row++) {
+    const int here = min(tilesN, (row * T::BM + T::BM + T::BN - 1) / T::BN);
+    if (t < here) break;
+    t -= here;
+  }
+  *tm = row, *tn = t;
+}
+template <class T>
+int lower_tiles(int m) {
+  const int tilesM = (m + T::BM - 1) / T::BM, tilesN = (m + T::BN - 1) / T::BN;
+  int all = 0;
+  for (int row = 0; row < tilesM; row++) {
+    const int here = (row * T::BM + T::BM + T::BN - 1) / T::BN;
+    all += here < tilesN ? here : tilesN;
+  }
+  return all;
+}
+
+// four neighbours of a row of planes
+template <int P>
+__device__ inline void put4(u16 *o, long plane, const u16 (&part)[4][P]) {
+#pragma unroll
+  for (int p = 0; p < P; p++)
+    *reinterpret_cast<uint2 *>(o + p * plane) = make_uint2(part[0][p] | (unsigned)part[1][p] << 16, part[2][p] | (unsigned)part[3][p] << 16);
+}
+
+template <class T, class Src, int STAGE>
+__global__ __launch_bounds__(T::THREADS, T::EU) void ortho_product_kernel(ProductArgs g) {
+  __shared__ __attribute__((aligned(16))) char S[T::LDS];
+  const Common &c = g.c;
+  if (held_back(c)) return;
+  int who = 0;
+  while (who + 1 < c.count && (int)blockIdx.x >= g.first[who + 1]) who++;
+  const Mat &t = g.m[who];
+  const int m = t.m, n = t.n, splits = g.splits[who];
+  int block = blockIdx.x - g.first[who];
+  const int tiles = (g.first[who + 1] - g.first[who]) / splits, split = block / tiles, id = block - split * tiles;
+  constexpr bool SYM = STAGE == GRAM || STAGE == POLYNOMIAL;
+  int tm, tn;
+  if constexpr (SYM) lower_tile<T>(xcd_remap(id, tiles), m, &tm, &tn);
+  else nt_tile_of(id, tiles / g.tilesN[who], g.tilesN[who], &tm, &tn);
+  const int m0 = tm * T::BM, n0 = tn * T::BN;
+  const long px = (long)m * t.np, pt = (long)n * t.mp, pa = (long)m * t.mp;
+  const PlanesRef A = STAGE == GRAM ? PlanesRef{t.X, px, t.np} : STAGE == POLYNOMIAL ? PlanesRef{t.A, pa, t.mp} : PlanesRef{t.Xt[0], pt, t.mp};
+  const PlanesRef B = STAGE == GRAM ? A : STAGE == POLYNOMIAL ? A : PlanesRef{t.Q, pa, t.mp};
+  const int K = STAGE == GRAM ? t.np : t.mp, kbeg = split * g.chunk[who], kend = min(K, kbeg + g.chunk[who]);
+  const int M = SYM ? m : n, N = m;
+  floatx16 acc[T::ACC][T::TM][T::TN];
+  nt_multiply<T>(A, M, m0, B, N, n0, kbeg, kend, S, acc);
+  if constexpr (T::ACC > 1)
+#pragma unroll
+    for (int i = 0; i < T::TM; i++)
+#pragma unroll
+      for (int j = 0; j < T::TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[0][i][j][r] += acc[T::ACC - 1][i][j][r];
+
+  if (splits > 1) {
+    // Each stretch of K leaves its tile; whoever is the last to arrive adds them up in their order and goes on.  (Past this XCD's L2, as the
+    // others may be anywhere.)
+    float *here = c.part + g.part0[who] + (long)id * splits * (T::BM * T::BN) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < T::TM; i++)
+#pragma unroll
+      for (int j = 0; j < T::TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          __hip_atomic_store(here + (long)split * (T::BM * T::BN) + ((i * T::TN + j) * 16 + r) * T::THREADS, acc[0][i][j][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    int *last = reinterpret_cast<int *>(S);
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int *counter = c.arrived + g.tiles0[who] + id;
+      const bool all = __hip_atomic_fetch_add(counter, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == splits - 1;
+      if (all) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      *last = all;
+    }
+    __syncthreads();
+    if (!*last) return;
+    __threadfence();
+#pragma unroll
+    for (int i = 0; i < T::TM; i++)
+#pragma unroll
+      for (int j = 0; j < T::TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[0][i][j][r] = 0.f;
+    for (int s = 0; s < splits; s++)
+#pragma unroll
+      for (int i = 0; i < T::TM; i++)
+#pragma unroll
+        for (int j = 0; j < T::TN; j++)
+#pragma unroll
+          for (int r = 0; r < 16; r++)
+            acc[0][i][j][r] += __hip_atomic_load(here + (long)s * (T::BM * T::BN) + ((i * T::TN + j) * 16 + r) * T::THREADS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int rbase = m0 + wave / T::WGN * T::WM + 4 * (lane >> 5), cbase = n0 + wave % T::WGN * T::WN + (lane & 31);
+#pragma unroll
+  for (int j = 0; j < T::TN; j++) {
+    const int col = cbase + 32 * j;
+#pragma unroll
+    for (int i = 0; i < T::TM; i++)
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const int row = rbase + 32 * i + 8 * q;
+        float x[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = acc[0][i][j][4 * q + k];
+        if constexpr (SYM) {
+          // element (row + k, col) on the diagonal or below, and its mirror image; zero between m and mp
+          if (col >= m || row >= t.mp || row + 3 < col) continue;
+          u16 part[4][T::P];
+          if constexpr (STAGE == POLYNOMIAL) {
+            u16 old[T::P][4];
+#pragma unroll
+            for (int p = 0; p < T::P; p++) {
+              const uint2 v = *reinterpret_cast<const uint2 *>(t.A + p * pa + (long)col * t.mp + row);
+              old[p][0] = v.x & 0xffff, old[p][1] = v.x >> 16, old[p][2] = v.y & 0xffff, old[p][3] = v.y >> 16;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              float A1 = bf16_float(old[T::P - 1][k]);
+#pragma unroll
+              for (int p = T::P - 2; p >= 0; p--) A1 += bf16_float(old[p][k]);
+              x[k] = fmaf(c.c, x[k], c.b * A1) + (row + k == col ? c.a : 0.f);
+            }
+          }
+          u16 *o = STAGE == GRAM ? t.A : t.Q;
+#pragma unroll
+          for (int k = 0; k < 4; k++) parts_of<T::P>(row + k < m ? x[k] : 0.f, part[k]);
+          if (row >= col) {
+            put4<T::P>(o + (long)col * t.mp + row, pa, part);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              if (row + k >= col)
+#pragma unroll
+                for (int p = 0; p < T::P; p++) o[p * pa + (long)col * t.mp + row + k] = part[k][p];
+          }
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            if (row + k > col && row + k < m)
+#pragma unroll
+              for (int p = 0; p < T::P; p++) o[p * pa + (long)(row + k) * t.mp + col] = part[k][p];
+        } else if constexpr (STAGE == APPLY) {
+          u16 part[4][T::P];
+#pragma unroll
+          for (int k = 0; k < 4; k++) parts_of<T::P>(row + k < n && col < m ? x[k] : 0.f, part[k]);
+          if (col < m && row < t.np) put4<T::P>(t.X + (long)col * t.np + row, px, part);
+          if (col < t.mp)
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              if (row + k < n)
+#pragma unroll
+                for (int p = 0; p < T::P; p++) t.Xt[1][p * pt + (long)(row + k) * t.mp + col] = part[k][p];
+        } else {
+          if (col >= m) continue;
+          const bool flat = t.rows <= t.cols;
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            if (row + k >= n) continue;
+            const long r = flat ? col : row + k, cc = flat ? row + k : col;
+            if (t.O) {
+              if constexpr (sizeof(Src) == 4) static_cast<float *>(t.O)[r * t.ldo + cc] = x[k];
+              else static_cast<u16 *>(t.O)[r * t.ldo + cc] = bf16_bits(x[k]);
+            }
+            if (t.W) {
+              float *w = t.W + r * t.ldw + cc;
+              *w = fmaf(1.f - c.lr * c.decay, *w, -c.lr * t.shrink * x[k]);
+            }
+          }
+        }
+      }
+  }
+}
+
+// ------------------------------------------------------------------ what a call consists of
+template <int P> struct Tiles;
+template <> struct Tiles<2> {
+  using L = NtTile<2, 256, 128, 32, 4, 2>;
+  using M = NtTile<2, 128, 128, 32, 2, 2>;
+  using S = NtTile<2, 64, 64, 32, 2, 2>;
+};
+template <> struct Tiles<3> {
+  using L = NtTile<3, 256, 128, 32, 4, 2>;
+  using M = NtTile<3, 128, 128, 16, 2, 2>;
+  using S = NtTile<3, 64, 64, 32, 2, 2>;
+};
+
+struct Plan {
+  size_t squares, arrived, part, bytes;
+  int counters;
+};
+
+struct Shape {
+  int m, n, mp, np;
+  explicit Shape(const cavs_ortho_desc &d) {
+    m = d.rows < d.cols ? d.rows : d.cols, n = d.rows < d.cols ? d.cols : d.rows;
+    mp = ceil_to(m, kPlaneAlign), np = ceil_to(n, kPlaneAlign);
+  }
+};
+
+// One launch's tiles: the largest that give most compute units one; where there are fewer, K in stretches, none of them short
+template <class T>
+struct LaunchPlan {
+  int first[kMats + 1], tilesN[kMats], splits[kMats], chunk[kMats], tiles0[kMats];
+  long part0[kMats], parts;
+  int tiles;
+  LaunchPlan(const cavs_ortho_desc *d, int count, int stage) {
+    long work = 0;  // tiles times k
+    tiles = 0;
+    int own[kMats], K[kMats];
+    for (int i = 0; i < count; i++) {
+      const Shape s(d[i]);
+      tilesN[i] = (s.m + T::BN - 1) / T::BN;
+      own[i] = stage == GRAM || stage == POLYNOMIAL ? lower_tiles<T>(s.m) : tilesN[i] * ((s.n + T::BM - 1) / T::BM);
+      K[i] = stage == GRAM ? s.np : s.mp;
+      tiles0[i] = tiles;
+      tiles += own[i];
+      work += (long)own[i] * K[i];
+    }
+    const long fits = 2l * num_cus();
+    int step = (int)((work + fits - 1) / fits);
+    step = step < 256 ? 256 : ceil_to(step, kPlaneAlign);
+    first[0] = 0, parts = 0;
+    for (int i = 0; i < count; i++) {
+      splits[i] = tiles >= num_cus() || K[i] <= step ? 1 : (K[i] + step - 1) / step;
+      chunk[i] = splits[i] == 1 ? K[i] : ceil_to((K[i] + splits[i] - 1) / splits[i], kPlaneAlign);
+      splits[i] = (K[i] + chunk[i] - 1) / chunk[i];
+      first[i + 1] = first[i] + own[i] * splits[i];
+      part0[i] = parts;
+      if (splits[i] > 1) parts += (long)own[i] * splits[i] * T::BM * T::BN;
+    }
+  }
+};
+
+template <int P, class F>
+auto with_tile(const cavs_ortho_desc *d, int count, int stage, F &&f) {
+  using TT = Tiles<P>;
+  if (LaunchPlan<typename TT::L>(d, count, stage).tiles >= num_cus() * 3 / 4) return f(typename TT::L{});
+  if (LaunchPlan<typename TT::M>(d, count, stage).tiles >= num_cus() * 3 / 4) return f(typename TT::M{});
+  return f(typename TT::S{});
+}
+
+// planes of a matrix: X, two Xt, A and the polynomial
+template <int P>
+size_t plane_bytes(const Shape &s) {
+  return ((size_t)s.m * s.np + 2 * (size_t)s.n * s.mp + 2 * (size_t)s.m * s.mp) * 2 * P;
+}
+
+template <int P>
+Plan plan_of(const cavs_ortho_desc *d, int count) {
+  Plan p{};
+  size_t most = 0;
+  long parts = 0;
+  for (int at = 0; at < count; at += kMats) {  // (batches come one after the other, in the same room)
+    const int k = count - at < kMats ? count - at : kMats;
+    size_t bytes = 0;
+    for (int i = 0; i < k; i++) bytes += (plane_bytes<P>(Shape(d[at + i])) + 255) & ~(size_t)255;
+    most = bytes > most ? bytes : most;
+    for (int stage = GRAM; stage <= APPLY; stage++)
+      with_tile<P>(d + at, k, stage, [&](auto t) {
+        const LaunchPlan<decltype(t)> l(d + at, k, stage);
+        parts = l.parts > parts ? l.parts : parts;
+        p.counters = l.tiles > p.counters ? l.tiles : p.counters;
+        return 0;
+      });
+  }
+  p.squares = most;
+  p.arrived = p.squares + sizeof(double) * kMats * kNormBlocks;
+  p.part = (p.arrived + sizeof(int) * p.counters + 255) & ~(size_t)255;
+  p.bytes = p.part + sizeof(float) * parts;
+  return p;
+}
+
+template <int P, class Src, int STAGE>
+void product(const cavs_ortho_desc *d, int count, const Mat *m, const Common &c, hipStream_t st) {
+  with_tile<P>(d, count, STAGE, [&](auto tile) {
+    using T = decltype(tile);
+    const LaunchPlan<T> l(d, count, STAGE);
+    ProductArgs a{};
+    a.c = c;
+    for (int i = 0; i < count; i++) {
+      a.m[i] = m[i];
+      a.tilesN[i] = l.tilesN[i], a.splits[i] = l.splits[i], a.chunk[i] = l.chunk[i], a.tiles0[i] = l.tiles0[i], a.part0[i] = l.part0[i];
+    }
+    for (int i = 0; i <= count; i++) a.first[i] = l.first[i];
+    launch(ortho_product_kernel<T, Src, STAGE>, l.first[count], T::THREADS, 0, st, a);
+    return 0;
+  });
+}
+
+template <int P, class Src>
+int run(const cavs_ortho_desc *d, int count, const cavs_ortho_options &o, const Plan &p, char *ws, hipStream_t st) {
+  Common c{};
+  c.nesterov = o.nesterov, c.a = o.a, c.b = o.b, c.c = o.c, c.eps = o.eps, c.momentum = o.momentum, c.lr = o.lr, c.decay = o.weight_decay, c.guard = o.guard;
+  c.squares = reinterpret_cast<double *>(ws + p.squares);
+  c.arrived = reinterpret_cast<int *>(ws + p.arrived);
+  c.counters = p.counters;
+  c.part = reinterpret_cast<float *>(ws + p.part);
+  for (int at = 0; at < count; at += kMats) {
+    const int k = count - at < kMats ? count - at : kMats;
+    const cavs_ortho_desc *b = d + at;
+    c.count = k;
+    StartArgs s{};
+    NormArgs nm{};
+    char *room = ws;
+    for (int i = 0; i < k; i++) {
+      const Shape h(b[i]);
+      u16 *at16 = reinterpret_cast<u16 *>(room);
+      auto take = [&](size_t n) {
+        u16 *here = at16;
+        at16 += n * P;
+        return here;
+      };
+      Mat t{b[i].G, b[i].M, b[i].W, b[i].O, b[i].ldg, b[i].ldm, b[i].ldw, b[i].ldo, b[i].rows, b[i].cols, h.m, h.n, h.mp, h.np};
+      t.X = take((size_t)h.m * h.np), t.Xt[0] = take((size_t)h.n * h.mp), t.Xt[1] = take((size_t)h.n * h.mp);
+      t.A = take((size_t)h.m * h.mp), t.Q = take((size_t)h.m * h.mp);
+      t.shrink = b[i].rows > b[i].cols ? (float)__builtin_sqrt((double)b[i].rows / b[i].cols) : 1.f;
+      room += (plane_bytes<P>(h) + 255) & ~(size_t)255;
+      s.m[i] = nm.m[i] = t;
+      s.first[i + 1] = s.first[i] + ceil_to(b[i].rows, 64) / 64 * (ceil_to(b[i].cols, 64) / 64);
+    }
+    s.c = nm.c = c;
+    launch(norm_kernel<Src>, dim3(kNormBlocks, k), 256, 0, st, nm);
+    launch(start_kernel<P, Src>, s.first[k], 256, 0, st, s);
+    for (int step = 0; step < o.steps; step++) {
+      product<P, Src, GRAM>(b, k, s.m, c, st);
+      product<P, Src, POLYNOMIAL>(b, k, s.m, c, st);
+      if (step + 1 < o.steps) product<P, Src, APPLY>(b, k, s.m, c, st);
+      else product<P, Src, LAST>(b, k, s.m, c, st);
+      for (int i = 0; i < k; i++) {
+        u16 *x = s.m[i].Xt[0];
+        s.m[i].Xt[0] = s.m[i].Xt[1], s.m[i].Xt[1] = x;
+      }
+    }
+  }
+  CAVS_LAUNCH_CHECK();
+  return CAVS_OK;
+}
+
+constexpr int kMostSide = 1 << 16;
+
+// two parts where nothing but a bf16 result is wanted
+bool two_parts(int type, int count, const cavs_ortho_desc *d) {
+  for (int i = 0; i < count; i++)
+    if (d[i].W) return false;
+  return type == CAVS_BF16;
+}
+
+bool sizes_ok(int type, int count, const cavs_ortho_desc *d) {
+  if ((type != CAVS_F32 && type != CAVS_BF16) || count < 0 || (count > 0 && !d)) return false;
+  for (int i = 0; i < count; i++)
+    if (d[i].rows <= 0 || d[i].cols <= 0 || d[i].rows > kMostSide || d[i].cols > kMostSide) return false;
+  return true;
+}
+
+}  // namespace
+}  // namespace cavs
+
+using namespace cavs;
+
+extern "C" {
+
+size_t cavs_ortho_update_workspace(int type, int count, const cavs_ortho_desc *d) {
+  if (count <= 0 || !sizes_ok(type, count, d)) return 0;
+  return (two_parts(type, count, d) ? plan_of<2>(d, count) : plan_of<3>(d, count)).bytes;
+}
+
+int cavs_ortho_update(int type, int count, const cavs_ortho_desc *d, const cavs_ortho_options *o, void *workspace, size_t workspace_bytes, void *stream) {
+  CAVS_REQUIRE(type == CAVS_F32 || type == CAVS_BF16, "cavs_ortho_update: type %d is neither CAVS_F32 nor CAVS_BF16", type);
+  CAVS_REQUIRE(count >= 0 && (count == 0 || d) && o, "cavs_ortho_update: bad count %d or null pointer", count);
+  CAVS_REQUIRE(o->steps >= 1 && o->steps <= 64, "cavs_ortho_update: %d steps (1 to 64)", o->steps);
+  CAVS_REQUIRE(o->eps >= 0.f, "cavs_ortho_update: eps is negative or not a number");
+  for (int i = 0; i < count; i++) {
+    const cavs_ortho_desc &e = d[i];
+    CAVS_REQUIRE(e.rows > 0 && e.cols > 0 && e.rows <= kMostSide && e.cols <= kMostSide, "cavs_ortho_update: matrix %d: unsupported shape %d x %d (1 to 2^16)", i,
+                 e.rows, e.cols);
+    CAVS_REQUIRE(e.G, "cavs_ortho_update: matrix %d: null pointer", i);
+    CAVS_REQUIRE(e.O || e.W, "cavs_ortho_update: matrix %d: neither O nor W is wanted", i);
+    CAVS_REQUIRE(e.ldg >= e.cols && (!e.M || e.ldm >= e.cols) && (!e.W || e.ldw >= e.cols) && (!e.O || e.ldo >= e.cols),
+                 "cavs_ortho_update: matrix %d: a row stride is below its %d columns", i, e.cols);
+  }
+  if (count == 0) return CAVS_OK;
+  const bool two = two_parts(type, count, d);
+  const Plan p = two ? plan_of<2>(d, count) : plan_of<3>(d, count);
+  CAVS_REQUIRE(workspace && workspace_bytes >= p.bytes, "cavs_ortho_update: workspace of %zu bytes needed, %zu given", p.bytes, workspace_bytes);
+  CAVS_REQUIRE(aligned16(workspace), "cavs_ortho_update: the workspace must be 16-byte aligned");
+  char *ws = static_cast<char *>(workspace);
+  hipStream_t st = as_stream(stream);
+  if (type == CAVS_F32) return run<3, float>(d, count, *o, p, ws, st);
+  return two ? run<2, u16>(d, count, *o, p, ws, st) : run<3, u16>(d, count, *o, p, ws, st);
+}
+
+}  // extern "C"

@@ -57,6 +57,17 @@ class BlockCopy(C.Structure):
 
 F32, BF16 = 0, 1  # the type of operands that may be either
 
+class OrthoDesc(C.Structure):
+    """cavs_ortho_desc: one matrix of cavs_ortho_update"""
+    _fields_ = [("rows", _I), ("cols", _I), ("G", _P), ("ldg", _I), ("M", _P), ("ldm", _I), ("W", _P), ("ldw", _I), ("O", _P), ("ldo", _I)]
+
+
+class OrthoOptions(C.Structure):
+    """cavs_ortho_options"""
+    _fields_ = [("steps", _I), ("nesterov", _I), ("a", _F), ("b", _F), ("c", _F), ("eps", _F), ("momentum", _F), ("lr", _F), ("weight_decay", _F),
+                ("guard", _P)]
+
+
 GEMM_C_UNUSED, GEMM_A_ZERO, GEMM_B_ZERO = 1, 2, 3
 
 
@@ -130,6 +141,7 @@ _SIGS = {
     "cavs_vocab_xent_bwd": [_I, _P, _I, _P, _I, _P, _P, _P, _P, _F, _P, _I, _P, _I, _P, _I, _I, _I, _P, _Z, _P],
     "cavs_vocab_xent": [_I, _P, _I, _P, _I, _P, _P, _P, _F, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _P, _Z, _P],
     "cavs_sgd": [_P, _P, _F, _Z, _P],
+    "cavs_ortho_update": [_I, _I, C.POINTER(OrthoDesc), C.POINTER(OrthoOptions), _P, _Z, _P],
     "cavs_ew_binary": [_I, _P, _P, _Z, _P, _Z, _Z, _I, _P],
     "cavs_ew_unary": [_I, _P, _P, _Z, _I, _P],
     "cavs_scale": [_P, _P, _F, _Z, _P],
@@ -204,7 +216,7 @@ _RESTYPE = {"cavs_last_error": C.c_char_p, "cavs_abi_version": _I, "cavs_sgemm_s
             "cavs_group_rounds_ok": _I, "cavs_group_max_groups": _I, "cavs_group_rows": _I, "cavs_tail_rounds_ok": _I, "cavs_tail_max_rounds": _I, "cavs_tail_max_groups": _I, "cavs_tail_sync_bytes": _Z,
             "cavs_sgemm_splitk_static_max_bytes": _Z,
             "cavs_embed_index_ints": _Z, "cavs_embed_index_workspace": _Z, "cavs_gather_sums_workspace": _Z,
-            "cavs_schedule_arena_scratch": _Z, "cavs_vocab_xent_workspace": _Z}
+            "cavs_schedule_arena_scratch": _Z, "cavs_vocab_xent_workspace": _Z, "cavs_ortho_update_workspace": _Z}
 _NOCHECK = {"cavs_last_error": [], "cavs_abi_version": [], "cavs_sgemm_splitk_workspace": [_I, _I, _I],
             "cavs_fc_softmax_xent_workspace": [_I, _I, _I], "cavs_colsum_blocks_workspace": [_I, _I, _I],
             "cavs_clip_grads_workspace": [_I], "cavs_sgemm_group_workspace": [_I, C.POINTER(GemmDesc)],
@@ -212,7 +224,8 @@ _NOCHECK = {"cavs_last_error": [], "cavs_abi_version": [], "cavs_sgemm_splitk_wo
             "cavs_lstm_round_packed_ok": [_I, _I], "cavs_sgemm_splitk_static_max_bytes": [],
             "cavs_group_rounds_ok": [_I], "cavs_group_max_groups": [_I], "cavs_group_rows": [], "cavs_tail_rounds_ok": [_I, _I], "cavs_tail_max_rounds": [], "cavs_tail_max_groups": [], "cavs_tail_sync_bytes": [],
             "cavs_embed_index_ints": [_I], "cavs_embed_index_workspace": [_I], "cavs_gather_sums_workspace": [_I, _I],
-            "cavs_schedule_arena_scratch": [_I, _I], "cavs_vocab_xent_workspace": [_I, _I, _I, _I, _I]}
+            "cavs_schedule_arena_scratch": [_I, _I], "cavs_vocab_xent_workspace": [_I, _I, _I, _I, _I],
+            "cavs_ortho_update_workspace": [_I, _I, C.POINTER(OrthoDesc)]}
 
 EW_BINARY = dict(add=0, sub=1, mul=2, div=3, sigmoid_grad=4, tanh_grad=5, relu_grad=6, equal=7)
 EW_UNARY = dict(assign=0, neg=1, abs=2, square=3, sigmoid=4, tanh=5, relu=6)

@@ -471,6 +471,40 @@ int cavs_fc_softmax_xent(const float *X, const float *W, const float *b, const f
 /* SGD (cavs/backend/op_impl_sgd.cu) over `count` tensors in one launch; the arrays are host arrays. */
 int cavs_sgd_multi(int count, float *const *w, const float *const *g, const size_t *n, float lr,
                    void *stream);
+/* Weight matrices updated by their momentum, orthogonalised (an optimizer step beside SGD, cavs/backend/op_impl_sgd.cu; the Muon rule:
+ * every direction of the update gets about the same size).  For each of `count` matrices:
+ *   M <- momentum M + G;  U = nesterov ? G + momentum M : M  (M NULL: U = G)
+ *   X = U / (|U| + eps), |U| the Frobenius norm;  `steps` times: A = X X^T, X <- a X + (b A + c A A) X  (rows > cols: of the transpose)
+ *   O = X (NULL: not wanted);  W <- (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) X (NULL: no weights)
+ * G and O are of `type`, M and W fp32; row strides in elements.  A matrix may be a block of a larger one (a gate's columns of a weight matrix);
+ * columns between `cols` and a row's stride are not touched.  O may be G; otherwise what is written may overlap nothing else.  U = 0 gives
+ * X = 0.  An infinity or a NaN in a matrix's G or M makes all of its X NaN.
+ * Products as sums of bf16 parts: three of them (full fp32 precision) where fp32 results are made, two (16 bits) where
+ * nothing but bf16 O are.  Sums of squares in 64 bits.  Results are the same on every call.
+ * steps 1 .. 64 (5 with a = 3.4445, b = -4.7750, c = 2.0315 bring singular values above 0.003 of the norm to 0.7 .. 1.2), rows and cols up to 2^16.
+ * guard (may be NULL): a device word; while it is not 0 the call leaves M, W and O as they are.
+ * The workspace: 16-byte aligned, at least cavs_ortho_update_workspace(type, count, d) bytes on this device (it depends on rows, cols and on
+ * which W are NULL; 0: refused, or count is 0); for the next call on the same stream to reuse, not for one that overlaps in time.
+ * The arrays are host arrays. */
+typedef struct {
+  int rows, cols;
+  const void *G;
+  int ldg;
+  float *M;
+  int ldm;
+  float *W;
+  int ldw;
+  void *O;
+  int ldo;
+} cavs_ortho_desc;
+typedef struct {
+  int steps, nesterov;
+  float a, b, c, eps, momentum, lr, weight_decay;
+  const int *guard;
+} cavs_ortho_options;
+size_t cavs_ortho_update_workspace(int type, int count, const cavs_ortho_desc *d);
+int cavs_ortho_update(int type, int count, const cavs_ortho_desc *d, const cavs_ortho_options *options, void *workspace,
+                      size_t workspace_bytes, void *stream);
 /* Clip (cavs/backend/op_impl_clip.cu:26-50): scales every gradient in place by
  * clip / max(sum_i ||g_i||_2, clip) -- the sum of the tensors' 2-norms, as the reference adds
  * them; at most 8 non-empty tensors per call; the arrays are host arrays.  After the call

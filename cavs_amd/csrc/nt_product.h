@@ -1,14 +1,23 @@
-// Products C = A B^T of operands laid out for the bf16 matrix pipe: `P` planes of bf16, k-contiguous.
+// Products C = A B^T of operands packed for the bf16 matrix pipe.
 //
-// An operand of type bf16 is one plane.  A float is the sum of bf16 parts, h = bf16(x), m = bf16(x - h), l = bf16(x - h - m); three of
+// An operand of type bf16 is one part.  A float is the sum of bf16 parts, h = bf16(x), m = bf16(x - h), l = bf16(x - h - m); three of
 // them hold all its bits, two hold 16.  A product of operands of P parts adds up the P (P + 1) / 2 products of weight 2^-8(P-1) and
 // above: six of nine, three of four.  The products of the first parts go into one set of accumulators and all the others, a 2^-8
 // smaller, into a second: the pipe loses an addend of less than about an eighth of its accumulator's last place, and beside their own
-// kind the small ones are not lost.  (gemm_split.h splits on the way into LDS; here whoever makes an operand writes its
-// planes, as the same operand goes into several products, and a tile's loads go to LDS without passing through registers.)
+// kind the small ones are not lost.  (gemm_split.h splits on the way into LDS; here whoever makes an operand writes its parts,
+// as the same operand goes into several products, and a tile's loads go to LDS without passing through registers.)
 //
-// Planes are zero from K up to `ld`, a multiple of 64: the loops below know no k that is not there.  Rows beyond the last read the last
-// one again; what comes of them is not stored.
+// A packed operand [rows, K] is blocks of 32 rows by 16 k, 1 KB a part: lane l of a wavefront finds its piece for the 32x32x16 instruction,
+// eight k of row l % 32, at byte 16 l.  Blocks follow each other part by part, then along k, then along the rows.  So a wavefront's load is 1 KB in
+// one piece, and LDS is read in the order it was written.  (Rows of bf16 as they lie in memory, 32 or 128 bytes of each to a tile: the loads of a
+// 128 x 128 x 16 tile alone took 2277 us of 7088 x 4096 x 3584, all of it takes 836 now.)  K is padded with zeros to whole steps: the loops
+// below know no k that is not there.  Blocks of rows beyond the last read the last one again; what comes of them is not stored.
+//
+// A workgroup is four wavefronts and its LDS two stages, so that a CU holds three of them that know nothing of each other: while one waits
+// for its loads the others multiply.  TFLOP/s of the bf16 pipe, random operands (power holds the clock at 1.9 GHz):
+//   one part     8192 x 8192 x 4096   256 x 128 x 32 1287    256 x 256 x 32, eight wavefronts, five stages 1162    128 x 128 x 32 1240
+//   three parts  7088 x 4096 x 3584   128 x 128 x 16 1493 (249 of the fp32 product)   256 x 128 x 32, eight wavefronts 1329
+//   two parts    4096 x 4096 x 4096   128 x 128 x 16, three stages 1355   256 x 128 x 32, eight wavefronts 1344
 #pragma once
 #include "gemm_common.h"
 
@@ -19,11 +28,16 @@ typedef unsigned short u16;
 
 constexpr int kPlaneAlign = 64;  // of K, in elements
 
-struct PlanesRef {
+struct PackedRef {
   const u16 *p;
-  long plane;  // elements from one plane to the next
-  int ld;      // of a row: a multiple of kPlaneAlign
+  int K;  // a multiple of kPlaneAlign
 };
+struct PackedOut {
+  u16 *p;
+  int K;
+};
+template <int P>
+constexpr size_t packed_bytes(long rows, int K) { return (size_t)((rows + 31) / 32 * 32) * K * 2 * P; }
 
 // bf16 of a float (to nearest), its bits
 __device__ inline u16 bf16_bits(float x) { return __builtin_bit_cast(u16, (__bf16)x); }
@@ -45,36 +59,43 @@ __device__ inline void parts_of(float x, u16 (&o)[P]) {
   }
 }
 
-template <int P_, int BM_, int BN_, int BK_, int WGM_, int WGN_>
+// NS: stages in LDS.  RA: the blocks a step begins with are read while the one before it multiplies.
+template <int P_, int BM_, int BN_, int BK_, int WGM_, int WGN_, int NS_ = 2, bool RA_ = false>
 struct NtTile {
-  static constexpr int P = P_, BM = BM_, BN = BN_, BK = BK_, WGM = WGM_, WGN = WGN_;
+  static constexpr int P = P_, BM = BM_, BN = BN_, BK = BK_, WGM = WGM_, WGN = WGN_, NS = NS_;
+  static constexpr bool RA = RA_;
   static constexpr int WAVES = WGM * WGN, THREADS = 64 * WAVES;
   static constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 32, TN = WN / 32;
-  static constexpr int ROWB = 2 * BK, PPR = BK / 8;           // bytes of a row of a tile, 16-byte pieces of it
-  static constexpr int RPC = 1024 / ROWB;                     // rows a wavefront loads with one instruction
-  static constexpr int CA = BM / RPC / WAVES, CB = BN / RPC / WAVES;  // such instructions per wavefront, plane and operand
-  static constexpr int PA = BM * ROWB, PB = BN * ROWB, STAGE = P * (PA + PB), LDS = 2 * STAGE;
+  static constexpr int STEPS = BK / 16, ROWB = 1024 * P * STEPS;    // bytes a row of blocks takes of a stage
+  static constexpr int CA = BM / 32 * P * STEPS / WAVES, CB = BN / 32 * P * STEPS / WAVES;  // blocks a wavefront loads per stage
+  static constexpr int PA = BM / 32 * ROWB, STAGE = (BM + BN) / 32 * ROWB, LDS = NS * STAGE;
+  static constexpr int LOADS = CA + CB;
   static constexpr int ACC = P > 1 ? 2 : 1;
-  static constexpr int EU = THREADS == 512 || WM == 64 ? 2 : P == 1 ? 4 : 3;  // wavefronts a SIMD is to hold: what LDS has room for
-  static_assert(BM % (RPC * WAVES) == 0 && BN % (RPC * WAVES) == 0, "a tile's loads are the same for every wavefront");
-  static_assert(kPlaneAlign % BK == 0, "planes end on a step");
+  static constexpr int GROUPS = 160 * 1024 / LDS;                   // workgroups a CU's LDS has room for
+  static constexpr int EU = GROUPS * WAVES / 4 < 4 ? GROUPS * WAVES / 4 : WM < 64 ? 4 : 3;  // wavefronts a SIMD is to hold
+  static_assert(BM / 32 * P * STEPS % WAVES == 0 && BN / 32 * P * STEPS % WAVES == 0, "a tile's loads are the same for every wavefront");
+  static_assert(kPlaneAlign % BK == 0, "operands end on a step");
+  static_assert(NS >= (RA ? 3 : 2) && LDS <= 160 * 1024, "stages");
 };
 
-// Byte of a tile's row x where its piece `oct` (8 k) lies: pieces change places so that sixteen rows read at one k touch all banks once.
-template <class T>
-__device__ inline int nt_at(int x, int oct) {
-  return x * T::ROWB + ((oct ^ ((x * T::ROWB >> 8) & (T::PPR - 1))) << 4);
+// Until at most N of this wavefront's loads are on their way and all it read from LDS is there; then until every wavefront is here.  (A barrier
+// by itself waits for neither, and __syncthreads would wait for all loads.)
+template <int N>
+__device__ __forceinline__ void nt_arrive() {
+  if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // acc[ACC][TM][TN] of the tile at rows m0 of A and n0 of B over k in [kbeg, kend), both multiples of BK.  S: T::LDS bytes.
-// Two stages: while one is multiplied the other is on its way from memory; a step's one barrier says that the stage to come has arrived
-// and that nobody reads the one before it any more.
+// NS stages in a ring: while one is multiplied the others are on their way from memory; a step's one barrier says that the stage to come
+// has arrived and that nobody reads the one before it any more, so that its place takes the load of the stage NS - 1 ahead.
 template <class T>
-__device__ __forceinline__ void nt_multiply(const PlanesRef &A, int M, int m0, const PlanesRef &B, int N, int n0, int kbeg, int kend, char *S,
+__device__ __forceinline__ void nt_multiply(const PackedRef &A, int M, int m0, const PackedRef &B, int N, int n0, int kbeg, int kend, char *S,
                                             floatx16 (&acc)[T::ACC][T::TM][T::TN]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WGN, wn = wave % T::WGN;
-  static_assert((32 * T::ROWB >> 8) % T::PPR == 0, "");
 #pragma unroll
   for (int s = 0; s < T::ACC; s++)
 #pragma unroll
@@ -84,72 +105,105 @@ __device__ __forceinline__ void nt_multiply(const PlanesRef &A, int M, int m0, c
 #pragma unroll
         for (int r = 0; r < 16; r++) acc[s][i][j][r] = 0.f;
 
-  // what this lane loads: piece lane % PPR of row lane / PPR of a wavefront's stretch of rows, as it lies in LDS
-  int va[T::CA], vb[T::CB];
-  auto offset = [&](int x, int x0, int X, int ld) {
-    const int piece = (lane % T::PPR) ^ ((x * T::ROWB >> 8) & (T::PPR - 1));
-    return (int)((unsigned)min(x, X - 1 - x0) * (unsigned)ld * 2u) + 16 * piece;
-  };
+  // Blocks c = 0, 1, .. of a stage, in the order they have in memory: row of blocks by row of blocks, step by step, part by part.  This wavefront
+  // loads every WAVES-th, each lane the 16 bytes it will read.
+  constexpr int PER = T::P * T::STEPS;
+  unsigned sa[T::CA], sb[T::CB];
+  const long rowa = (long)(A.K / 16) * T::P * 1024, rowb = (long)(B.K / 16) * T::P * 1024;
 #pragma unroll
-  for (int c = 0; c < T::CA; c++) va[c] = offset((c * T::WAVES + wave) * T::RPC + lane / T::PPR, m0, M, A.ld);
+  for (int c = 0; c < T::CA; c++) {
+    const int at = c * T::WAVES + wave;
+    sa[c] = (unsigned)min(at / PER, (M - 1 - m0) / 32) * (unsigned)rowa + at % PER * 1024;
+  }
 #pragma unroll
-  for (int c = 0; c < T::CB; c++) vb[c] = offset((c * T::WAVES + wave) * T::RPC + lane / T::PPR, n0, N, B.ld);
-  [[maybe_unused]] const u16 *pa = A.p + (long)m0 * A.ld + kbeg, *pb = B.p + (long)n0 * B.ld + kbeg;
+  for (int c = 0; c < T::CB; c++) {
+    const int at = c * T::WAVES + wave;
+    sb[c] = (unsigned)min(at / PER, (N - 1 - n0) / 32) * (unsigned)rowb + at % PER * 1024;
+  }
+  [[maybe_unused]] const char *pa = reinterpret_cast<const char *>(A.p) + m0 / 32 * rowa + (long)(kbeg / 16) * (T::P * 1024);
+  [[maybe_unused]] const char *pb = reinterpret_cast<const char *>(B.p) + n0 / 32 * rowb + (long)(kbeg / 16) * (T::P * 1024);
 
   auto fetch = [&](int kt, char *to) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass knows no such load)
-    const unsigned off = (unsigned)kt * T::ROWB;
+    const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pa), 0, 0xffffffffu, 0x00020000);
+    const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pb), 0, 0xffffffffu, 0x00020000);
+    const unsigned off = (unsigned)kt * (PER * 1024);
 #pragma unroll
-    for (int p = 0; p < T::P; p++) {
-      const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16 *>(pa + p * A.plane), 0, 0xffffffffu, 0x00020000);
-      const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16 *>(pb + p * B.plane), 0, 0xffffffffu, 0x00020000);
+    for (int c = 0; c < T::CA; c++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void *)(to + (c * T::WAVES + wave) * 1024), 16, 16 * lane, sa[c] + off, 0, 0);
 #pragma unroll
-      for (int c = 0; c < T::CA; c++)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void *)(to + p * (T::PA + T::PB) + (c * T::WAVES + wave) * 1024), 16,
-                                                 va[c], off, 0, 0);
-#pragma unroll
-      for (int c = 0; c < T::CB; c++)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void *)(to + p * (T::PA + T::PB) + T::PA + (c * T::WAVES + wave) * 1024),
-                                                 16, vb[c], off, 0, 0);
-    }
+    for (int c = 0; c < T::CB; c++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void *)(to + T::PA + (c * T::WAVES + wave) * 1024), 16, 16 * lane, sb[c] + off,
+                                               0, 0);
 #endif
   };
-  // where this lane's first piece of either operand lies; that of step s is at the address with s in its bits 5 and up (rows are
-  // multiples of ROWB, their order of pieces repeats within 32 rows)
-  const int half = lane >> 5, a0 = nt_at<T>(wm * T::WM + (lane & 31), half), b0 = T::PA + nt_at<T>(wn * T::WN + (lane & 31), half);
-  auto multiply = [&](const char *from) {
+  const int a0 = wm * (T::WM / 32) * T::ROWB + 16 * lane, b0 = T::PA + wn * (T::WN / 32) * T::ROWB + 16 * lane;
+  struct Pieces {
+    bf16x8 a[T::TM][T::P], b[T::TN][T::P];
+  };
+  auto read = [&](Pieces &f, const char *from, int s) {
 #pragma unroll
-    for (int s = 0; s < T::BK / 16; s++) {
-      bf16x8 a[T::TM][T::P], b[T::TN][T::P];
+    for (int p = 0; p < T::P; p++) {
 #pragma unroll
-      for (int p = 0; p < T::P; p++) {
+      for (int i = 0; i < T::TM; i++) f.a[i][p] = *reinterpret_cast<const bf16x8 *>(from + a0 + (i * T::ROWB + (s * T::P + p) * 1024));
 #pragma unroll
-        for (int i = 0; i < T::TM; i++) a[i][p] = *reinterpret_cast<const bf16x8 *>(from + (a0 ^ (32 * s)) + (p * (T::PA + T::PB) + 32 * i * T::ROWB));
-#pragma unroll
-        for (int j = 0; j < T::TN; j++) b[j][p] = *reinterpret_cast<const bf16x8 *>(from + (b0 ^ (32 * s)) + (p * (T::PA + T::PB) + 32 * j * T::ROWB));
-      }
-#pragma unroll
-      for (int w = T::P - 1; w >= 0; w--)  // the parts' weights, the small products first
-#pragma unroll
-        for (int p = 0; p <= w; p++)
-#pragma unroll
-          for (int i = 0; i < T::TM; i++)
-#pragma unroll
-            for (int j = 0; j < T::TN; j++)
-              acc[w ? T::ACC - 1 : 0][i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i][p], b[j][w - p], acc[w ? T::ACC - 1 : 0][i][j], 0, 0, 0);
+      for (int j = 0; j < T::TN; j++) f.b[j][p] = *reinterpret_cast<const bf16x8 *>(from + b0 + (j * T::ROWB + (s * T::P + p) * 1024));
     }
   };
+  auto multiply = [&](const Pieces &f) {
+#pragma unroll
+    for (int w = T::P - 1; w >= 0; w--)  // the parts' weights, the small products first
+#pragma unroll
+      for (int p = 0; p <= w; p++)
+#pragma unroll
+        for (int i = 0; i < T::TM; i++)
+#pragma unroll
+          for (int j = 0; j < T::TN; j++)
+            acc[w ? T::ACC - 1 : 0][i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a[i][p], f.b[j][w - p], acc[w ? T::ACC - 1 : 0][i][j], 0, 0, 0);
+  };
   const int nk = (kend - kbeg) / T::BK;
-  if (nk > 0) fetch(0, S);
+#pragma unroll
+  for (int q = 0; q < T::NS - 1; q++)
+    if (q < nk) fetch(q, S + q * T::STAGE);
   int at = 0;
-  for (int kt = 0; kt < nk; kt++) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a barrier by itself need not wait for loads that go to LDS)
-    __syncthreads();
-    if (kt + 1 < nk) fetch(kt + 1, S + (T::STAGE - at));
-    multiply(S + at);
-    at = T::STAGE - at;
+  auto behind = [](int x) { return x == (T::NS - 1) * T::STAGE ? 0 : x + T::STAGE; };
+  constexpr int STEPS = T::STEPS;
+  if constexpr (!T::RA) {
+    for (int kt = 0; kt < nk; kt++) {
+      if (kt + T::NS - 2 < nk) nt_arrive<(T::NS - 2) * T::LOADS>();
+      else nt_arrive<0>();
+      if (kt + T::NS - 1 < nk) fetch(kt + T::NS - 1, S + (at == 0 ? (T::NS - 1) * T::STAGE : at - T::STAGE));
+#pragma unroll
+      for (int s = 0; s < STEPS; s++) {
+        Pieces f;
+        read(f, S + at, s);
+        multiply(f);
+      }
+      at = behind(at);
+    }
+  } else {
+    Pieces f[2];
+    if (nk > 0) {
+      if (nk >= T::NS - 1) nt_arrive<(T::NS - 2) * T::LOADS>();
+      else nt_arrive<0>();
+      read(f[0], S, 0);
+    }
+    for (int kt = 0; kt < nk; kt++) {
+      if (kt + T::NS - 2 < nk) nt_arrive<(T::NS - 3) * T::LOADS>();
+      else nt_arrive<0>();
+      if (kt + T::NS - 1 < nk) fetch(kt + T::NS - 1, S + (at == 0 ? (T::NS - 1) * T::STAGE : at - T::STAGE));
+      const int next = behind(at);
+#pragma unroll
+      for (int s = 0; s < STEPS; s++) {
+        if (s + 1 < STEPS) read(f[(s + 1) & 1], S + at, s + 1);
+        else if (kt + 1 < nk) read(f[STEPS & 1], S + next, 0);
+        multiply(f[s & 1]);
+      }
+      if constexpr (STEPS & 1) f[0] = f[1];
+      at = next;
+    }
   }
-  __syncthreads();  // (LDS is free for what follows)
+  nt_arrive<0>();  // (LDS is free for what follows)
 }
 
 // The tiles of a launch over tilesM x tilesN: eight tiles of A at a time, down each tile of B, the tiles that one XCD runs together reading
@@ -161,32 +215,75 @@ __device__ inline void nt_tile_of(int block, int tilesM, int tilesN, int *tm, in
   *tn = in / high;
 }
 
-// Four neighbouring values of a row: x[0..3] to o[0..3], `left` of them (4 or more: all), as one store where the row allows it.
-__device__ inline void store4(float *o, const float (&x)[4], int left, bool vec) {
-  if (vec && left >= 4) {
-    *reinterpret_cast<float4 *>(o) = make_float4(x[0], x[1], x[2], x[3]);
-  } else {
+// The 32 x 32 values a wavefront holds of an accumulator (lane l, element r: c = l % 32, r' = 8 (r / 4) + 4 (l / 32) + r % 4), as parts, into a
+// packed operand: with x = c, k = r' ("rows", 16-byte pieces of two halves), or with x = r', k = c ("columns", by way of LDS: kTurn bytes
+// of the wavefront's own).  xb, kb: the block of 32 rows, of 32 k.
+constexpr int kTurn = 4 * 528;
+template <int P>
+struct Parts16 {
+  u16 v[16][P];
+};
+template <int P>
+__device__ inline void put_rows(const PackedOut &o, int xb, int kb, const Parts16<P> &t, int lane) {
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-      if (k < left) o[k] = x[k];
+  for (int p = 0; p < P; p++)
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+      *reinterpret_cast<uint2 *>(o.p + (((long)xb * (o.K / 16) + 2 * kb + (q >> 1)) * P + p) * 512 + ((lane & 31) + 32 * (q & 1)) * 8 + 4 * (lane >> 5)) =
+          make_uint2(t.v[4 * q][p] | (unsigned)t.v[4 * q + 1][p] << 16, t.v[4 * q + 2][p] | (unsigned)t.v[4 * q + 3][p] << 16);
+}
+template <int P>
+__device__ inline void put_columns(const PackedOut &o, int xb, int kb, const Parts16<P> &t, int lane, char *turn) {
+  // eight k of a row are a piece; pieces of the same eight k lie together, 16 bytes further for the next eight so that all banks take part
+  u16 *in = reinterpret_cast<u16 *>(turn + (lane >> 3 & 3) * 528 + (lane >> 5) * 64 + (lane & 7) * 2);
+#pragma unroll
+  for (int p = 0; p < P; p++) {
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int r = 0; r < 16; r++) in[(8 * (r >> 2) + (r & 3)) * 8] = t.v[r][p];
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");  // (a wavefront's own accesses to LDS happen in their order)
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+      *reinterpret_cast<uint4 *>(o.p + (((long)xb * (o.K / 16) + 2 * kb + b) * P + p) * 512 + lane * 8) =
+          *reinterpret_cast<const uint4 *>(turn + (2 * b + (lane >> 5)) * 528 + (lane & 31) * 16);
   }
 }
-__device__ inline void store4(u16 *o, const float (&x)[4], int left, bool vec) {
-  const u16 a = bf16_bits(x[0]), b = bf16_bits(x[1]), c = bf16_bits(x[2]), d = bf16_bits(x[3]);
-  if (vec && left >= 4) {
-    *reinterpret_cast<uint2 *>(o) = make_uint2(a | (unsigned)b << 16, c | (unsigned)d << 16);
-  } else {
-    if (left > 0) o[0] = a;
-    if (left > 1) o[1] = b;
-    if (left > 2) o[2] = c;
-    if (left > 3) o[3] = d;
+
+// 64 x 64 values in LDS as parts, into packed operands: rows r0 .. of `o` with k = k0 .., and rows k0 .. of `t` with k = r0 ..; 256 threads.
+// What lies beyond `rows` and `cols` is zero in the tile.
+typedef float PackTile[64][65];
+template <int P>
+__device__ inline void pack_tile(const PackTile &tile, const PackedOut &o, const PackedOut &t, int r0, int k0, int rows, int cols) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int b = 0; b < 2; b++) {  // a block of 32 rows; the wavefront's 16 k
+    auto put = [&](const PackedOut &to, int row0, int col0, int all, auto &&at) {
+      if (row0 + 32 * b >= all || col0 + 16 * wave >= to.K) return;
+      u16 part[8][P];
+#pragma unroll
+      for (int e = 0; e < 8; e++) parts_of<P>(at(32 * b + x, 16 * wave + 8 * h + e), part[e]);
+#pragma unroll
+      for (int p = 0; p < P; p++)
+        *reinterpret_cast<uint4 *>(to.p + (((long)(row0 / 32 + b) * (to.K / 16) + col0 / 16 + wave) * P + p) * 512 + lane * 8) =
+            make_uint4(part[0][p] | (unsigned)part[1][p] << 16, part[2][p] | (unsigned)part[3][p] << 16, part[4][p] | (unsigned)part[5][p] << 16,
+                       part[6][p] | (unsigned)part[7][p] << 16);
+    };
+    if (o.p) put(o, r0, k0, rows, [&](int r, int k) { return tile[r][k]; });
+    if (t.p) put(t, k0, r0, cols, [&](int r, int k) { return tile[k][r]; });
   }
 }
+
+__device__ inline void store_as(float *o, float x) { *o = x; }
+__device__ inline void store_as(u16 *o, float x) { *o = bf16_bits(x); }
 
 // an operand's element as a float
 __device__ inline float value_of(const float *p) { return *p; }
 __device__ inline float value_of(const u16 *p) { return bf16_float(*p); }
 
 constexpr int ceil_to(int x, int to) { return (x + to - 1) / to * to; }
+inline int tiles_of(int x, int side) { return (x + side - 1) / side; }
+
 
 }  // namespace cavs

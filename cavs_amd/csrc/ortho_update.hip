@@ -3,8 +3,8 @@
 //   M <- mu M + G,  U = G + mu M or M,  X = U / (|U| + eps);  `steps` times  X <- (a I + b A + c A A) X, A = X X^T
 //
 // on the side that is smaller: m x n with m <= n.  Three products a step, each one launch over all matrices: A and a I + b A + c A A are
-// symmetric, so only tiles that reach the diagonal or below are made, and each is stored twice.  What a launch makes is
-// what the next ones read, as planes of bf16 parts (nt_product.h): X by rows (for A) and by columns (for the product
+// symmetric, so only blocks on the diagonal and below are made, and those below are stored twice.  What a launch makes is
+// what the next ones read, packed as bf16 parts (nt_product.h): X by rows (for A) and by columns (for the product
 // with it), A and the polynomial by rows, which are their columns.
 //
 // A singular value next to 0 grows a-fold a step, 485-fold in five, and so does a rounding error made beside it.  With three parts X, A and the
@@ -25,7 +25,7 @@ struct Mat {
   long ldg, ldm, ldw, ldo;
   int rows, cols;      // as the caller has them
   int m, n, mp, np;    // of X, and padded to whole steps
-  u16 *X, *Xt[2], *A, *Q;  // planes: [m, np], [n, mp] (read, written), [m, mp], [m, mp]
+  u16 *X, *Xt[2], *A, *Q;  // packed: [m, np], [n, mp] (read, written), [m, mp], [m, mp]
   float shrink;        // sqrt(max(1, rows / cols))
 };
 
@@ -90,7 +90,7 @@ struct StartArgs {
 };
 template <int P, class Src>
 __global__ __launch_bounds__(256) void start_kernel(StartArgs g) {
-  __shared__ float tile[64][65];
+  __shared__ PackTile tile;
   const Common &c = g.c;
   if (held_back(c)) return;
   int who = 0;
@@ -101,36 +101,15 @@ __global__ __launch_bounds__(256) void start_kernel(StartArgs g) {
   const double by = 1. / (sqrt(sum) + (double)c.eps);
   const bool flat = t.rows <= t.cols;
   const int across = (flat ? t.np : t.mp) / 64, block = blockIdx.x - g.first[who];
-  const int r0 = block / across * 64, k0 = block % across * 64;
-  u16 *o = flat ? t.X : t.Xt[0], *tr = flat ? t.Xt[0] : t.X;
-  const int ldo = flat ? t.np : t.mp, ldt = flat ? t.mp : t.np;
-  const long po = (long)t.rows * ldo, pt = (long)t.cols * ldt;
-  {
-    const int k = threadIdx.x & 63;
-#pragma unroll 4
-    for (int i = threadIdx.x >> 6; i < 64; i += 4) {
-      const int r = r0 + i;
-      float x = 0.f;
-      if (r < t.rows && k0 + k < t.cols) x = (float)((double)update_of<Src>(t, c, r, k0 + k) * by);
-      if (r < t.rows) {
-        u16 part[P];
-        parts_of<P>(x, part);
-#pragma unroll
-        for (int p = 0; p < P; p++) o[p * po + (long)r * ldo + k0 + k] = part[p];
-      }
-      tile[i][k] = x;
-    }
+  const int r0 = block / across * 64, k0 = block % across * 64, k = threadIdx.x & 63;
+#pragma unroll 8
+  for (int i = threadIdx.x >> 6; i < 64; i += 4) {
+    const int r = r0 + i;
+    tile[i][k] = r < t.rows && k0 + k < t.cols ? (float)((double)update_of<Src>(t, c, r, k0 + k) * by) : 0.f;
   }
   __syncthreads();
-  const int i = threadIdx.x & 63;
-#pragma unroll 4
-  for (int k = threadIdx.x >> 6; k < 64; k += 4) {
-    if (k0 + k >= t.cols || r0 + i >= ldt) continue;
-    u16 part[P];
-    parts_of<P>(tile[i][k], part);
-#pragma unroll
-    for (int p = 0; p < P; p++) tr[p * pt + (long)(k0 + k) * ldt + r0 + i] = part[p];
-  }
+  const PackedOut X{t.X, t.np}, Xt{t.Xt[0], t.mp};
+  pack_tile<P>(tile, flat ? X : Xt, flat ? Xt : X, r0, k0, t.rows, t.cols);
 }
 
 enum { GRAM = 0, POLYNOMIAL = 1, APPLY = 2, LAST = 3 };
@@ -166,14 +145,6 @@ int lower_tiles(int m) {
   return all;
 }
 
-// four neighbours of a row of planes
-template <int P>
-__device__ inline void put4(u16 *o, long plane, const u16 (&part)[4][P]) {
-#pragma unroll
-  for (int p = 0; p < P; p++)
-    *reinterpret_cast<uint2 *>(o + p * plane) = make_uint2(part[0][p] | (unsigned)part[1][p] << 16, part[2][p] | (unsigned)part[3][p] << 16);
-}
-
 template <class T, class Src, int STAGE>
 __global__ __launch_bounds__(T::THREADS, T::EU) void ortho_product_kernel(ProductArgs g) {
   __shared__ __attribute__((aligned(16))) char S[T::LDS];
@@ -188,153 +159,132 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void ortho_product_kernel(Produc
   constexpr bool SYM = STAGE == GRAM || STAGE == POLYNOMIAL;
   int tm, tn;
   if constexpr (SYM) lower_tile<T>(xcd_remap(id, tiles), m, &tm, &tn);
-  else nt_tile_of(id, tiles / g.tilesN[who], g.tilesN[who], &tm, &tn);
+  else nt_tile_of(id, tiles / g.tilesN[who], g.tilesN[who], &tm, &tn);  // (the plan's, for this matrix's orientation)
   const int m0 = tm * T::BM, n0 = tn * T::BN;
-  const long px = (long)m * t.np, pt = (long)n * t.mp, pa = (long)m * t.mp;
-  const PlanesRef A = STAGE == GRAM ? PlanesRef{t.X, px, t.np} : STAGE == POLYNOMIAL ? PlanesRef{t.A, pa, t.mp} : PlanesRef{t.Xt[0], pt, t.mp};
-  const PlanesRef B = STAGE == GRAM ? A : STAGE == POLYNOMIAL ? A : PlanesRef{t.Q, pa, t.mp};
+  // The last product is made so that a row of the result is a row of the accumulators, whichever side of X is the longer one in the caller's.
+  const bool turned = STAGE == LAST && t.rows <= t.cols;
+  const PackedRef X{t.X, t.np}, Xt{t.Xt[0], t.mp}, A1{t.A, t.mp}, Q{t.Q, t.mp};
+  const PackedRef &A = STAGE == GRAM ? X : STAGE == POLYNOMIAL ? A1 : turned ? Q : Xt, &B = STAGE == GRAM ? X : STAGE == POLYNOMIAL ? A1 : turned ? Xt : Q;
   const int K = STAGE == GRAM ? t.np : t.mp, kbeg = split * g.chunk[who], kend = min(K, kbeg + g.chunk[who]);
-  const int M = SYM ? m : n, N = m;
+  const int M = SYM || turned ? m : n, N = turned ? n : m;
   floatx16 acc[T::ACC][T::TM][T::TN];
   nt_multiply<T>(A, M, m0, B, N, n0, kbeg, kend, S, acc);
   if constexpr (T::ACC > 1)
 #pragma unroll
     for (int i = 0; i < T::TM; i++)
 #pragma unroll
-      for (int j = 0; j < T::TN; j++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) acc[0][i][j][r] += acc[T::ACC - 1][i][j][r];
+      for (int j = 0; j < T::TN; j++) acc[0][i][j] += acc[T::ACC - 1][i][j];
 
   if (splits > 1) {
-    // Each stretch of K leaves its tile; whoever is the last to arrive adds them up in their order and goes on.  (Past this XCD's L2, as the
-    // others may be anywhere.)
+    // Each stretch of K leaves its tile; whoever is the last to arrive adds them up in their order and goes on.  Past this XCD's L2, as the
+    // others may be anywhere; the count goes up once the stores have arrived.  (Fences instead, which write back and drop all of an L2: 105 us a
+    // launch where this takes 20.)
     float *here = c.part + g.part0[who] + (long)id * splits * (T::BM * T::BN) + threadIdx.x;
+    auto at = [&](int s, int e) { return here + (long)s * (T::BM * T::BN) + e * T::THREADS; };
 #pragma unroll
-    for (int i = 0; i < T::TM; i++)
-#pragma unroll
-      for (int j = 0; j < T::TN; j++)
-#pragma unroll
-        for (int r = 0; r < 16; r++)
-          __hip_atomic_store(here + (long)split * (T::BM * T::BN) + ((i * T::TN + j) * 16 + r) * T::THREADS, acc[0][i][j][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int e = 0; e < T::TM * T::TN * 16; e++)
+      __hip_atomic_store(at(split, e), acc[0][e / 16 / T::TN][e / 16 % T::TN][e % 16], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     int *last = reinterpret_cast<int *>(S);
-    __threadfence();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
       int *counter = c.arrived + g.tiles0[who] + id;
-      const bool all = __hip_atomic_fetch_add(counter, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == splits - 1;
+      const bool all = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == splits - 1;
       if (all) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       *last = all;
     }
     __syncthreads();
     if (!*last) return;
-    __threadfence();
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < T::TM; i++)
 #pragma unroll
-      for (int j = 0; j < T::TN; j++)
+      for (int j = 0; j < T::TN; j++) {
+        float sum[16] = {};
+        for (int s = 0; s < splits; s += 4) {  // four stretches' loads on their way at a time
+          float v[4][16];
 #pragma unroll
-        for (int r = 0; r < 16; r++) acc[0][i][j][r] = 0.f;
-    for (int s = 0; s < splits; s++)
+          for (int k = 0; k < 4; k++)
 #pragma unroll
-      for (int i = 0; i < T::TM; i++)
+            for (int r = 0; r < 16; r++)
+              v[k][r] = __hip_atomic_load(at(s + k < splits ? s + k : s, (i * T::TN + j) * 16 + r), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-        for (int j = 0; j < T::TN; j++)
+          for (int k = 0; k < 4; k++)
 #pragma unroll
-          for (int r = 0; r < 16; r++)
-            acc[0][i][j][r] += __hip_atomic_load(here + (long)s * (T::BM * T::BN) + ((i * T::TN + j) * 16 + r) * T::THREADS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (int r = 0; r < 16; r++) sum[r] += s + k < splits ? v[k][r] : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[0][i][j][r] = sum[r];
+      }
   }
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int rbase = m0 + wave / T::WGN * T::WM + 4 * (lane >> 5), cbase = n0 + wave % T::WGN * T::WN + (lane & 31);
+  char *turn = S + wave * kTurn;
 #pragma unroll
-  for (int j = 0; j < T::TN; j++) {
-    const int col = cbase + 32 * j;
+  for (int i = 0; i < T::TM; i++)
 #pragma unroll
-    for (int i = 0; i < T::TM; i++)
+    for (int j = 0; j < T::TN; j++) {
+      // the block of 32 rows and of 32 columns; this lane's column, the first of its rows
+      const int rb = (m0 + wave / T::WGN * T::WM) / 32 + i, cb = (n0 + wave % T::WGN * T::WN) / 32 + j;
+      const int col = 32 * cb + (lane & 31), row0 = 32 * rb + 4 * (lane >> 5);
+      auto row = [&](int r) { return row0 + 8 * (r >> 2) + (r & 3); };
+      float x[16];
 #pragma unroll
-      for (int q = 0; q < 4; q++) {
-        const int row = rbase + 32 * i + 8 * q;
-        float x[4];
+      for (int r = 0; r < 16; r++) x[r] = acc[0][i][j][r];
+      if constexpr (SYM) {
+        // blocks above the diagonal are the mirror images of those below; of one on it both halves are here
+        if (32 * cb >= m || 32 * rb >= t.mp || rb < cb) continue;
+        if constexpr (STAGE == POLYNOMIAL) {
+          // (A's parts by its columns' rows: A is symmetric)
 #pragma unroll
-        for (int k = 0; k < 4; k++) x[k] = acc[0][i][j][4 * q + k];
-        if constexpr (SYM) {
-          // element (row + k, col) on the diagonal or below, and its mirror image; zero between m and mp
-          if (col >= m || row >= t.mp || row + 3 < col) continue;
-          u16 part[4][T::P];
-          if constexpr (STAGE == POLYNOMIAL) {
-            u16 old[T::P][4];
+          for (int q = 0; q < 4; q++) {
+            float A4[4] = {};
 #pragma unroll
-            for (int p = 0; p < T::P; p++) {
-              const uint2 v = *reinterpret_cast<const uint2 *>(t.A + p * pa + (long)col * t.mp + row);
-              old[p][0] = v.x & 0xffff, old[p][1] = v.x >> 16, old[p][2] = v.y & 0xffff, old[p][3] = v.y >> 16;
+            for (int p = T::P - 1; p >= 0; p--) {
+              const uint2 v = *reinterpret_cast<const uint2 *>(t.A + (((long)cb * (t.mp / 16) + 2 * rb + (q >> 1)) * T::P + p) * 512 +
+                                                               ((lane & 31) + 32 * (q & 1)) * 8 + 4 * (lane >> 5));
+              A4[0] += __uint_as_float(v.x << 16), A4[1] += __uint_as_float(v.x & 0xffff0000u);
+              A4[2] += __uint_as_float(v.y << 16), A4[3] += __uint_as_float(v.y & 0xffff0000u);
             }
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-              float A1 = bf16_float(old[T::P - 1][k]);
-#pragma unroll
-              for (int p = T::P - 2; p >= 0; p--) A1 += bf16_float(old[p][k]);
-              x[k] = fmaf(c.c, x[k], c.b * A1) + (row + k == col ? c.a : 0.f);
-            }
+            for (int k = 0; k < 4; k++) x[4 * q + k] = fmaf(c.c, x[4 * q + k], c.b * A4[k]) + (row(4 * q + k) == col ? c.a : 0.f);
           }
-          u16 *o = STAGE == GRAM ? t.A : t.Q;
+        }
+        Parts16<T::P> e;
 #pragma unroll
-          for (int k = 0; k < 4; k++) parts_of<T::P>(row + k < m ? x[k] : 0.f, part[k]);
-          if (row >= col) {
-            put4<T::P>(o + (long)col * t.mp + row, pa, part);
-          } else {
+        for (int r = 0; r < 16; r++) parts_of<T::P>(row(r) < m ? x[r] : 0.f, e.v[r]);
+        const PackedOut o{STAGE == GRAM ? t.A : t.Q, t.mp};
+        put_rows<T::P>(o, cb, rb, e, lane);
+        if (rb > cb && 32 * rb < m) put_columns<T::P>(o, rb, cb, e, lane, turn);
+      } else if constexpr (STAGE == APPLY) {
+        Parts16<T::P> e;
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-              if (row + k >= col)
+        for (int r = 0; r < 16; r++) parts_of<T::P>(row(r) < n && col < m ? x[r] : 0.f, e.v[r]);
+        if (32 * cb < m && 32 * rb < t.np) put_rows<T::P>(PackedOut{t.X, t.np}, cb, rb, e, lane);
+        if (32 * rb < n && 32 * cb < t.mp) put_columns<T::P>(PackedOut{t.Xt[1], t.mp}, rb, cb, e, lane, turn);
+      } else {
+        if (col >= t.cols) continue;
 #pragma unroll
-                for (int p = 0; p < T::P; p++) o[p * pa + (long)col * t.mp + row + k] = part[k][p];
-          }
-#pragma unroll
-          for (int k = 0; k < 4; k++)
-            if (row + k > col && row + k < m)
-#pragma unroll
-              for (int p = 0; p < T::P; p++) o[p * pa + (long)(row + k) * t.mp + col] = part[k][p];
-        } else if constexpr (STAGE == APPLY) {
-          u16 part[4][T::P];
-#pragma unroll
-          for (int k = 0; k < 4; k++) parts_of<T::P>(row + k < n && col < m ? x[k] : 0.f, part[k]);
-          if (col < m && row < t.np) put4<T::P>(t.X + (long)col * t.np + row, px, part);
-          if (col < t.mp)
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-              if (row + k < n)
-#pragma unroll
-                for (int p = 0; p < T::P; p++) t.Xt[1][p * pt + (long)(row + k) * t.mp + col] = part[k][p];
-        } else {
-          if (col >= m) continue;
-          const bool flat = t.rows <= t.cols;
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            if (row + k >= n) continue;
-            const long r = flat ? col : row + k, cc = flat ? row + k : col;
-            if (t.O) {
-              if constexpr (sizeof(Src) == 4) static_cast<float *>(t.O)[r * t.ldo + cc] = x[k];
-              else static_cast<u16 *>(t.O)[r * t.ldo + cc] = bf16_bits(x[k]);
-            }
-            if (t.W) {
-              float *w = t.W + r * t.ldw + cc;
-              *w = fmaf(1.f - c.lr * c.decay, *w, -c.lr * t.shrink * x[k]);
-            }
+        for (int r = 0; r < 16; r++) {
+          if (row(r) >= t.rows) continue;
+          if (t.O) store_as(static_cast<Src *>(t.O) + row(r) * t.ldo + col, x[r]);
+          if (t.W) {
+            float *w = t.W + row(r) * t.ldw + col;
+            *w = fmaf(1.f - c.lr * c.decay, *w, -c.lr * t.shrink * x[r]);
           }
         }
       }
-  }
+    }
 }
 
 // ------------------------------------------------------------------ what a call consists of
 template <int P> struct Tiles;
 template <> struct Tiles<2> {
-  using L = NtTile<2, 256, 128, 32, 4, 2>;
-  using M = NtTile<2, 128, 128, 32, 2, 2>;
+  using L = NtTile<2, 128, 128, 16, 2, 2, 3>;
   using S = NtTile<2, 64, 64, 32, 2, 2>;
 };
 template <> struct Tiles<3> {
-  using L = NtTile<3, 256, 128, 32, 4, 2>;
-  using M = NtTile<3, 128, 128, 16, 2, 2>;
+  using L = NtTile<3, 128, 128, 16, 2, 2>;
   using S = NtTile<3, 64, 64, 32, 2, 2>;
 };
 
@@ -363,8 +313,9 @@ struct LaunchPlan {
     int own[kMats], K[kMats];
     for (int i = 0; i < count; i++) {
       const Shape s(d[i]);
-      tilesN[i] = (s.m + T::BN - 1) / T::BN;
-      own[i] = stage == GRAM || stage == POLYNOMIAL ? lower_tiles<T>(s.m) : tilesN[i] * ((s.n + T::BM - 1) / T::BM);
+      const bool turned = stage == LAST && d[i].rows <= d[i].cols;
+      tilesN[i] = tiles_of(turned ? s.n : s.m, T::BN);
+      own[i] = stage == GRAM || stage == POLYNOMIAL ? lower_tiles<T>(s.m) : tilesN[i] * tiles_of(turned ? s.m : s.n, T::BM);
       K[i] = stage == GRAM ? s.np : s.mp;
       tiles0[i] = tiles;
       tiles += own[i];
@@ -389,14 +340,13 @@ template <int P, class F>
 auto with_tile(const cavs_ortho_desc *d, int count, int stage, F &&f) {
   using TT = Tiles<P>;
   if (LaunchPlan<typename TT::L>(d, count, stage).tiles >= num_cus() * 3 / 4) return f(typename TT::L{});
-  if (LaunchPlan<typename TT::M>(d, count, stage).tiles >= num_cus() * 3 / 4) return f(typename TT::M{});
   return f(typename TT::S{});
 }
 
-// planes of a matrix: X, two Xt, A and the polynomial
+// what a matrix takes, packed: X, two Xt, A and the polynomial
 template <int P>
-size_t plane_bytes(const Shape &s) {
-  return ((size_t)s.m * s.np + 2 * (size_t)s.n * s.mp + 2 * (size_t)s.m * s.mp) * 2 * P;
+size_t room_of(const Shape &s) {
+  return packed_bytes<P>(s.m, s.np) + 2 * packed_bytes<P>(s.n, s.mp) + 2 * packed_bytes<P>(s.m, s.mp);
 }
 
 template <int P>
@@ -407,9 +357,9 @@ Plan plan_of(const cavs_ortho_desc *d, int count) {
   for (int at = 0; at < count; at += kMats) {  // (batches come one after the other, in the same room)
     const int k = count - at < kMats ? count - at : kMats;
     size_t bytes = 0;
-    for (int i = 0; i < k; i++) bytes += (plane_bytes<P>(Shape(d[at + i])) + 255) & ~(size_t)255;
+    for (int i = 0; i < k; i++) bytes += (room_of<P>(Shape(d[at + i])) + 255) & ~(size_t)255;
     most = bytes > most ? bytes : most;
-    for (int stage = GRAM; stage <= APPLY; stage++)
+    for (int stage = GRAM; stage <= LAST; stage++)
       with_tile<P>(d + at, k, stage, [&](auto t) {
         const LaunchPlan<decltype(t)> l(d + at, k, stage);
         parts = l.parts > parts ? l.parts : parts;
@@ -458,19 +408,19 @@ int run(const cavs_ortho_desc *d, int count, const cavs_ortho_options &o, const 
     char *room = ws;
     for (int i = 0; i < k; i++) {
       const Shape h(b[i]);
-      u16 *at16 = reinterpret_cast<u16 *>(room);
-      auto take = [&](size_t n) {
-        u16 *here = at16;
-        at16 += n * P;
+      char *next = room;
+      auto take = [&](size_t bytes) {
+        u16 *here = reinterpret_cast<u16 *>(next);
+        next += bytes;
         return here;
       };
       Mat t{b[i].G, b[i].M, b[i].W, b[i].O, b[i].ldg, b[i].ldm, b[i].ldw, b[i].ldo, b[i].rows, b[i].cols, h.m, h.n, h.mp, h.np};
-      t.X = take((size_t)h.m * h.np), t.Xt[0] = take((size_t)h.n * h.mp), t.Xt[1] = take((size_t)h.n * h.mp);
-      t.A = take((size_t)h.m * h.mp), t.Q = take((size_t)h.m * h.mp);
+      t.X = take(packed_bytes<P>(h.m, h.np)), t.Xt[0] = take(packed_bytes<P>(h.n, h.mp)), t.Xt[1] = take(packed_bytes<P>(h.n, h.mp));
+      t.A = take(packed_bytes<P>(h.m, h.mp)), t.Q = take(packed_bytes<P>(h.m, h.mp));
       t.shrink = b[i].rows > b[i].cols ? (float)__builtin_sqrt((double)b[i].rows / b[i].cols) : 1.f;
-      room += (plane_bytes<P>(h) + 255) & ~(size_t)255;
+      room += (room_of<P>(h) + 255) & ~(size_t)255;
       s.m[i] = nm.m[i] = t;
-      s.first[i + 1] = s.first[i] + ceil_to(b[i].rows, 64) / 64 * (ceil_to(b[i].cols, 64) / 64);
+      s.first[i + 1] = s.first[i] + tiles_of(b[i].rows, 64) * tiles_of(b[i].cols, 64);
     }
     s.c = nm.c = c;
     launch(norm_kernel<Src>, dim3(kNormBlocks, k), 256, 0, st, nm);

@@ -32,7 +32,7 @@ def _args(**kw):
     (dict(type=2), "neither"), (dict(type=-1), "neither"), (dict(n=-1), "bad shape"), (dict(H=0), "bad shape"), (dict(C=0), "bad shape"),
     (dict(ldx=7), "row stride"), (dict(ldw=7), "row stride"), (dict(lddx=7), "row stride"), (dict(lddw=0), "row stride"),
     (dict(X=None), "null pointer"), (dict(W=None), "null pointer"), (dict(labels=None), "null pointer"),
-    (dict(H=(1 << 16) + 1, ldx=1 << 17, ldw=1 << 17, lddx=1 << 17, lddw=1 << 17), "unsupported shape"), (dict(n=(1 << 22) + 1), "unsupported shape"),
+    (dict(H=(1 << 16) + 1, ldx=1 << 17, ldw=1 << 17, lddx=1 << 17, lddw=1 << 17), "unsupported shape"), (dict(n=(1 << 20) + 1), "unsupported shape"),
     (dict(C=(1 << 23) + 1), "unsupported shape"),
 ])
 def test_refusals(bad, match):
@@ -50,7 +50,7 @@ def test_refusals_of_the_halves():
 def test_shapes_that_are_refused_have_no_workspace():
     ws = hip.lib().cavs_vocab_xent_workspace
     assert ws(2, 4, 8, 8, 1) == 0 and ws(0, 0, 8, 8, 1) == 0 and ws(0, 4, 0, 8, 0) == 0 and ws(0, 4, 8, 0, 0) == 0
-    assert ws(0, (1 << 22) + 1, 8, 8, 0) == 0 and ws(1, 4, (1 << 16) + 1, 8, 0) == 0 and ws(1, 4, 8, (1 << 23) + 1, 0) == 0
+    assert ws(0, (1 << 20) + 1, 8, 8, 0) == 0 and ws(1, 4, (1 << 16) + 1, 8, 0) == 0 and ws(1, 4, 8, (1 << 23) + 1, 0) == 0
 
 
 # ------------------------------------------------------------------ the definition

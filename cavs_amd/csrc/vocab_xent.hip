@@ -15,28 +15,42 @@ namespace cavs {
 namespace {
 
 // ------------------------------------------------------------------ operands, packed
-// src [rows, K] with its columns as k and, for the products that sum over its rows, with its rows as k.  Either may be left out.  A row whose
-// flag says so is zero in the second: 0 times what it holds need not be 0.
-enum { KEEP_ALL = 0, KEEP_NONZERO = 1, KEEP_FINITE = 2 };  // rows with flag != 0; rows whose flag is not -inf
+// src [rows, K] with its columns as k and, for the products that sum over its rows, with its rows as k.  Either may be left out.  A row that
+// takes no part by its flag is zero in the second: 0 times what it holds need not be 0.
+enum { KEEP_ALL = 0, KEEP_LABELLED = 1, KEEP_FINITE = 2 };  // rows whose flag is a class id below `classes`; rows whose flag is not -inf
+__device__ inline bool is_class(float label, int classes) { return label >= 0.f && label < (float)classes; }
+
+struct PackJob {
+  const void *src;
+  long ld;
+  int rows, K;
+  PackedOut o, t;
+  const float *flag;
+  int keep, classes;
+  int across, blocks;  // blocks of 64 columns, of 64 x 64
+};
 
 template <int P, class Src>
-__global__ __launch_bounds__(256) void pack_kernel(const Src *__restrict__ src, long ld, int rows, int K, PackedOut o, PackedOut t, const float *__restrict__ flag,
-                                                   int keep) {
+__global__ __launch_bounds__(256) void pack_kernel(PackJob j0, PackJob j1) {
   __shared__ PackTile tile;
-  const int r0 = blockIdx.y * 64, k0 = blockIdx.x * 64, k = threadIdx.x & 63;
+  const bool second = (int)blockIdx.x >= j0.blocks;
+  const PackJob &g = second ? j1 : j0;
+  const int block = second ? blockIdx.x - j0.blocks : blockIdx.x;
+  const int r0 = block / g.across * 64, k0 = block % g.across * 64, k = threadIdx.x & 63;
+  const Src *src = static_cast<const Src *>(g.src);
 #pragma unroll 8
   for (int i = threadIdx.x >> 6; i < 64; i += 4) {
     const int r = r0 + i;
-    tile[i][k] = r < rows && k0 + k < K ? value_of(src + r * ld + k0 + k) : 0.f;
+    tile[i][k] = r < g.rows && k0 + k < g.K ? value_of(src + r * g.ld + k0 + k) : 0.f;
   }
   __syncthreads();
-  pack_tile<P>(tile, o, keep == KEEP_ALL ? t : PackedOut{}, r0, k0, rows, K);
-  if (!t.p || keep == KEEP_ALL) return;
+  pack_tile<P>(tile, g.o, g.keep == KEEP_ALL ? g.t : PackedOut{}, r0, k0, g.rows, g.K);
+  if (!g.t.p || g.keep == KEEP_ALL) return;
   __syncthreads();
   for (int i = threadIdx.x >> 6; i < 64; i += 4)
-    if (r0 + i < rows && (keep == KEEP_NONZERO ? flag[r0 + i] == 0.f : flag[r0 + i] == -INFINITY)) tile[i][k] = 0.f;
+    if (r0 + i < g.rows && (g.keep == KEEP_LABELLED ? !is_class(g.flag[r0 + i], g.classes) : g.flag[r0 + i] == -INFINITY)) tile[i][k] = 0.f;
   __syncthreads();
-  pack_tile<P>(tile, PackedOut{}, t, r0, k0, rows, K);
+  pack_tile<P>(tile, PackedOut{}, g.t, r0, k0, g.rows, g.K);
 }
 
 // ------------------------------------------------------------------ the tile of z
@@ -151,40 +165,52 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void stats_kernel(TileArgs a, fl
 }
 
 // What a row's tiles come to: lse, loss and the weight of its gradient (zero for a row without a class, or without any class that is not
-// masked).  Sixteen rows to a workgroup, sixteen lanes to a row's tiles.
-__global__ __launch_bounds__(256) void rows_kernel(const float2 *__restrict__ stats, int tiles, const float *__restrict__ zlabel, const float *__restrict__ labels,
-                                                   int n, int C, float *__restrict__ loss, float *__restrict__ lse) {
-  __shared__ float2 part[16][17];
-  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, row = blockIdx.x * 16 + x;
+// masked).  Sixteen lanes to a row, or all of a workgroup where rows are few.
+struct RowArgs {
+  const float2 *stats;
+  int tiles, n, C;
+  const float *zlabel, *labels, *dloss;
+  float *loss, *lse, *weight;
+};
+__device__ inline float2 joined(float2 a, float2 b) {
+  const float top = fmaxf(a.x, b.x), from = top == -INFINITY ? 0.f : top;
+  return make_float2(top, a.y * __expf(a.x - from) + b.y * __expf(b.x - from));
+}
+__device__ inline float weight_of(float label, float lse, const float *dloss, int row, int C) {
+  return is_class(label, C) && lse != -INFINITY ? dloss ? dloss[row] : 1.f : 0.f;
+}
+template <int ROWS>
+__global__ __launch_bounds__(256) void rows_kernel(RowArgs a) {
+  constexpr int LANES = 256 / ROWS;
+  __shared__ float2 part[LANES][ROWS];
+  const int x = threadIdx.x % ROWS, y = threadIdx.x / ROWS, row = blockIdx.x * ROWS + x;
   float2 s = make_float2(-INFINITY, 0.f);
-  if (row < n)
-    for (int t = y; t < tiles; t += 16) {
-      const float2 o = stats[(long)t * n + row];
-      const float top = fmaxf(s.x, o.x), from = top == -INFINITY ? 0.f : top;
-      s = make_float2(top, s.y * __expf(s.x - from) + o.y * __expf(o.x - from));
+  if (row < a.n)
+    for (int t = y; t < a.tiles; t += 4 * LANES) {
+      float2 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) v[k] = t + k * LANES < a.tiles ? a.stats[(long)(t + k * LANES) * a.n + row] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int k = 0; k < 4; k++) s = joined(s, v[k]);
     }
   part[y][x] = s;
-  __syncthreads();
-  if (y != 0 || row >= n) return;
-  float top = s.x;
-  for (int q = 1; q < 16; q++) top = fmaxf(top, part[q][x].x);
-  const float from = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int q = 0; q < 16; q++) sum += part[q][x].y * expf(part[q][x].x - from);
-  const float all = from + logf(sum), label = labels[row];
-  const bool has = label >= 0.f && label < (float)C;
-  if (lse) lse[row] = all;
+  for (int half = LANES / 2; half > 0; half >>= 1) {
+    __syncthreads();
+    if (y < half) part[y][x] = joined(part[y][x], part[y + half][x]);
+  }
+  if (y != 0 || row >= a.n) return;
+  s = part[0][x];
+  const float all = (s.x == -INFINITY ? 0.f : s.x) + logf(s.y), label = a.labels[row];
+  if (a.lse) a.lse[row] = all;
   // (no class left: an infinite loss, not the NaN of -inf - -inf)
-  if (loss) loss[row] = !has ? 0.f : all == -INFINITY ? INFINITY : all - zlabel[row];
+  if (a.loss) a.loss[row] = !is_class(label, a.C) ? 0.f : all == -INFINITY ? INFINITY : all - a.zlabel[row];
+  if (a.weight) a.weight[row] = weight_of(label, all, a.dloss, row, a.C);
 }
 
 __global__ __launch_bounds__(256) void weights_kernel(const float *__restrict__ labels, const float *__restrict__ lse, const float *__restrict__ dloss, int n,
                                                       int C, float *__restrict__ weight) {
   const int row = blockIdx.x * 256 + threadIdx.x;
-  if (row >= n) return;
-  const float label = labels[row];
-  const bool has = label >= 0.f && label < (float)C && lse[row] != -INFINITY;
-  weight[row] = has ? dloss ? dloss[row] : 1.f : 0.f;
+  if (row < n) weight[row] = weight_of(labels[row], lse[row], dloss, row, C);
 }
 
 // d of a tile: e = p - [label] for the product with W, by token, and e times the token's weight for that with X, by class (zero between the last
@@ -193,7 +219,7 @@ __global__ __launch_bounds__(256) void weights_kernel(const float *__restrict__ 
 // holds well, while any factor in it is a rounding error that all of its kind share.
 template <class T>
 __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, const float *__restrict__ lse, const float *__restrict__ weight, PackedOut d,
-                                                                    PackedOut t, float *__restrict__ sums, int ld_sums) {
+                                                                    PackedOut t, float *__restrict__ sums, int ld_sums, float sums_scale) {
   __shared__ __attribute__((aligned(16))) char S[T::LDS];
   int tm, tn;
   nt_tile_of(blockIdx.x, a.tilesM, a.tilesN, &tm, &tn);
@@ -260,12 +286,12 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, 
     float s = part[x];
 #pragma unroll
     for (int q = 1; q < T::WGN; q++) s += part[q * T::BM + x];
-    sums[(long)tn * ld_sums + m0 + x] = s;
+    sums[(long)tn * ld_sums + m0 + x] = sums_scale * s;
   }
 }
 
 // ------------------------------------------------------------------ the products with d
-// out[row, col] = scale * A B^T.  K in `splits` stretches of kchunk, each with sums of its own (unscaled) at part + split * M * N; part null:
+// out[row, col] = scale * factor[row] * A B^T.  K in `splits` stretches of kchunk, each with sums of its own (unscaled) at part + split * M * N; part null:
 // straight to out.
 template <class Out>
 struct ProductJob {
@@ -276,6 +302,7 @@ struct ProductJob {
   Out *out;
   long ldo;
   float scale;
+  const float *factor;  // of out's rows, or null
 };
 
 template <class T, class Out>
@@ -307,23 +334,46 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void product_kernel(ProductJob<O
           float *o = part + (long)row * g.N + col;
           *o = g.add ? *o + x : x;
         } else {
-          store_as(g.out + row * g.ldo + col, g.scale * x);
+          store_as(g.out + row * g.ldo + col, (g.factor ? g.scale * g.factor[row] : g.scale) * x);
         }
       }
   }
 }
 
 // out[r, 0 .. w) = scale * factor[r] * sum of `parts` pieces, in their order
+struct SumJob {
+  const float *part;
+  int parts, rows, w;
+  const float *factor;
+  void *out;
+  long ldo;
+  int blocks;
+};
 template <class Out>
-__global__ __launch_bounds__(256) void parts_kernel(const float *__restrict__ part, int parts, int rows, int w, float scale, const float *__restrict__ factor,
-                                                    Out *__restrict__ out, long ldo) {
-  const long total = (long)rows * w;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-    float s = parts > 0 ? part[i] : 0.f;
-    for (int p = 1; p < parts; p++) s += part[p * total + i];
-    const long r = i / w;
-    store_as(out + r * ldo + (i - r * w), (factor ? scale * factor[r] : scale) * s);
+__device__ inline void sum_parts(const SumJob &g, float scale, int block) {
+  const long total = (long)g.rows * g.w;
+  Out *out = static_cast<Out *>(g.out);
+  for (long i = (long)block * 256 + threadIdx.x; i < total; i += (long)g.blocks * 256) {
+    float s = 0.f;
+    for (int p = 0; p < g.parts; p += 4) {  // (four loads on their way at a time)
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) v[k] = p + k < g.parts ? g.part[(p + k) * total + i] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; k++) s += v[k];
+    }
+    const long r = i / g.w;
+    store_as(out + r * g.ldo + (i - r * g.w), (g.factor ? scale * g.factor[r] : scale) * s);
   }
+}
+// d X, d W and d b (fp32) of what the launches before left in parts
+template <class Out>
+__global__ __launch_bounds__(256) void sums_kernel(SumJob x, SumJob w, SumJob b, float scale) {
+  int block = blockIdx.x;
+  if (block < x.blocks) return sum_parts<Out>(x, scale, block);
+  block -= x.blocks;
+  if (block < w.blocks) return sum_parts<Out>(w, scale, block);
+  sum_parts<float>(b, scale, block - w.blocks);
 }
 
 // ------------------------------------------------------------------ what a call consists of
@@ -439,9 +489,21 @@ Plan plan_of(int n, int H, int C, int grads) {
   return p;
 }
 
+inline PackJob pack_job(const void *src, long ld, int rows, int K, PackedOut o, PackedOut t, const float *flag, int keep, int classes) {
+  const int across = tiles_of(K, 64);
+  return {src, ld, rows, K, o, t, flag, keep, classes, across, o.p || t.p ? across * tiles_of(rows, 64) : 0};
+}
 template <int P, class Src>
-void pack(const void *src, long ld, int rows, int K, PackedOut o, PackedOut t, const float *flag, int keep, hipStream_t st) {
-  launch(pack_kernel<P, Src>, dim3(tiles_of(K, 64), tiles_of(rows, 64)), 256, 0, st, static_cast<const Src *>(src), ld, rows, K, o, t, flag, keep);
+void pack(const PackJob &a, const PackJob &b, hipStream_t st) {
+  if (a.blocks + b.blocks > 0) launch(pack_kernel<P, Src>, a.blocks + b.blocks, 256, 0, st, a, b);
+}
+template <class Out>
+void sums(SumJob x, SumJob w, SumJob b, float scale, hipStream_t st) {
+  for (SumJob *j : {&x, &w, &b}) {
+    const long blocks = j->out ? ((long)j->rows * j->w + 255) / 256 : 0;
+    j->blocks = (int)(blocks > 2048 ? 2048 : blocks);
+  }
+  if (x.blocks + w.blocks + b.blocks > 0) launch(sums_kernel<Out>, x.blocks + w.blocks + b.blocks, 256, 0, st, x, w, b, scale);
 }
 
 template <int P, class Src>
@@ -451,68 +513,83 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
   auto pl = [&](size_t at) { return reinterpret_cast<u16 *>(ws + at); };
   auto ref = [](const PackedOut &o) { return PackedRef{o.p, o.K}; };
   const PackedOut none{}, X{pl(p.x), p.Hp};
-  const bool keep = p.grads && p.keep;
-  pack<P, Src>(c.X, c.ldx, n, H, X, none, nullptr, KEEP_ALL, st);
-  float *lse = c.lse ? c.lse : f32(p.lse);
+  const bool keep = p.grads && p.keep, one = p.pieces == 1;
+  float *lse = c.lse ? c.lse : f32(p.lse), *weight = f32(p.weight);
   auto piece_w = [&](int c0) { return PackedOut{pl(p.w + (keep ? packed_bytes<P>(c0, p.Hp) : 0)), p.Hp}; };
-  auto source = [&](int c0) { return static_cast<const Src *>(c.W) + (long)c0 * c.ldw; };
-  auto tile_args = [&](int c0, int rows) {
+  auto piece_wt = [&](int rows) { return PackedOut{c.dX ? pl(p.wt) : nullptr, ceil_to(rows, kPlaneAlign)}; };
+  auto rows_of = [&](int c0) { return C - c0 < p.piece ? C - c0 : p.piece; };
+  auto job_w = [&](int c0, bool o, bool t) {
+    const int rows = rows_of(c0);
+    return pack_job(static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, rows, H, o ? piece_w(c0) : none, t && p.grads ? piece_wt(rows) : none,
+                    c.b ? c.b + c0 : nullptr, c.b ? KEEP_FINITE : KEEP_ALL, 0);
+  };
+  const PackedOut xt{p.grads && c.dW ? pl(p.xt) : nullptr, p.np};
+  // X in one launch with what there is of W by then
+  PackJob jx = pack_job(c.X, c.ldx, n, H, X, xt, c.labels, KEEP_LABELLED, C);
+  auto tile_args = [&](int c0) {
+    const int rows = rows_of(c0);
     return TileArgs{ref(piece_w(c0)), ref(X), rows, n, p.Hp, tiles_of(rows, p.bm), tiles_of(n, p.bn), c.b ? c.b + c0 : nullptr, c.labels, c0};
   };
   if (!c.lse_given) {
     for (int c0 = 0; c0 < C; c0 += p.piece) {
-      const int rows = C - c0 < p.piece ? C - c0 : p.piece;
-      pack<P, Src>(source(c0), c.ldw, rows, H, piece_w(c0), none, nullptr, KEEP_ALL, st);
-      const TileArgs a = tile_args(c0, rows);
+      pack<P, Src>(jx, job_w(c0, true, one), st);
+      jx = PackJob{};
+      const TileArgs a = tile_args(c0);
       with_tile<P>(p.size, [&](auto t) {
         using T = decltype(t);
         launch(stats_kernel<T>, a.tilesM * a.tilesN, T::THREADS, 0, st, a, reinterpret_cast<float2 *>(ws + p.stats), f32(p.zlabel));
         return 0;
       });
     }
-    launch(rows_kernel, (n + 15) / 16, 256, 0, st, reinterpret_cast<const float2 *>(ws + p.stats), p.tiles, f32(p.zlabel), c.labels, n, C, c.loss, lse);
+    const RowArgs r{reinterpret_cast<const float2 *>(ws + p.stats), p.tiles, n, C, f32(p.zlabel), c.labels, c.dloss, c.loss, lse, p.grads ? weight : nullptr};
+    if (n <= 1024) launch(rows_kernel<1>, n, 256, 0, st, r);
+    else launch(rows_kernel<16>, (n + 15) / 16, 256, 0, st, r);
+  } else {
+    launch(weights_kernel, (n + 255) / 256, 256, 0, st, c.labels, c.lse_given, c.dloss, n, C, weight);
   }
   if (p.grads) {
     const float *all = c.lse_given ? c.lse_given : lse;
-    float *weight = f32(p.weight);
-    launch(weights_kernel, (n + 255) / 256, 256, 0, st, c.labels, all, c.dloss, n, C, weight);
-    const PackedOut xt{pl(p.xt), p.np};
-    if (c.dW) pack<P, Src>(c.X, c.ldx, n, H, none, xt, weight, KEEP_NONZERO, st);
+    const int token_tiles = tiles_of(n, p.bn);
+    const bool x_parts = !one || p.xsplits > 1, w_parts = p.wsplits > 1, b_parts = token_tiles > 1;
     bool first = true;
     for (int c0 = 0; c0 < C; c0 += p.piece, first = false) {
-      const int rows = C - c0 < p.piece ? C - c0 : p.piece, rp = ceil_to(rows, kPlaneAlign);
-      const PackedOut wt{pl(p.wt), rp};
+      const int rows = rows_of(c0), rp = ceil_to(rows, kPlaneAlign);
       // (what the first pass packed may still be there)
-      const bool make = c.lse_given || (!keep && p.pieces > 1);
-      if (c.dX || make)
-        pack<P, Src>(source(c0), c.ldw, rows, H, make ? piece_w(c0) : none, c.dX ? wt : none, c.b ? c.b + c0 : nullptr, c.b ? KEEP_FINITE : KEEP_ALL, st);
-      const TileArgs a = tile_args(c0, rows);
-      const PackedOut d{c.dX ? pl(p.d) : nullptr, rp}, dt{c.dW ? pl(p.dt) : nullptr, p.np};
-      with_tile<P>(p.size, [&](auto t) {
-        using T = decltype(t);
-        launch(dlogits_kernel<T>, a.tilesM * a.tilesN, T::THREADS, 0, st, a, all, weight, d, dt, c.db ? f32(p.sums) + c0 : nullptr, C);
-        return 0;
-      });
-      auto job = [&](const PackedOut &A, const PackedOut &B, int M, int K, int chunk, float *part, bool add, void *out, long ldo) {
+      const bool here = !c.lse_given && one;
+      if (!here) pack<P, Src>(jx, job_w(c0, c.lse_given || !keep, true), st);
+      jx = PackJob{};
+      const TileArgs a = tile_args(c0);
+      const PackedOut d{c.dX ? pl(p.d) : nullptr, rp}, dt{c.dW ? pl(p.dt) : nullptr, p.np}, wt = piece_wt(rows);
+      if (c.dX || c.dW || c.db)
+        with_tile<P>(p.size, [&](auto t) {
+          using T = decltype(t);
+          launch(dlogits_kernel<T>, a.tilesM * a.tilesN, T::THREADS, 0, st, a, all, weight, d, dt, !c.db ? nullptr : b_parts ? f32(p.sums) + c0 : c.db + c0, C,
+                 b_parts ? 1.f : c.scale);
+          return 0;
+        });
+      auto job = [&](const PackedOut &A, const PackedOut &B, int M, int K, int chunk, float *part, bool add, void *out, long ldo, const float *factor) {
         return ProductJob<Src>{ref(A), ref(B), M, H, K, tiles_of(M, p.pm), tiles_of(H, p.pn), (K + chunk - 1) / chunk, chunk, part, add,
-                               static_cast<Src *>(out), ldo, c.scale};
+                               static_cast<Src *>(out), ldo, c.scale, factor};
       };
-      ProductJob<Src> jx{}, jw{};
+      ProductJob<Src> px{}, pw{};
       // (a last piece shorter than the others fills fewer stretches: those beyond keep what they have)
-      if (c.dX) jx = job(d, wt, n, rp, p.xchunk, f32(p.xpart), !first, nullptr, 0);
+      if (c.dX) px = job(d, wt, n, rp, p.xchunk, x_parts ? f32(p.xpart) : nullptr, !first, c.dX, c.lddx, weight);
       Src *dW = c.dW ? static_cast<Src *>(c.dW) + (long)c0 * c.lddw : nullptr;
-      if (c.dW) jw = job(dt, xt, rows, p.np, p.wchunk, p.wsplits > 1 ? f32(p.wpart) : nullptr, false, dW, c.lddw);
-      const int bx = c.dX ? jx.tilesM * jx.tilesN * jx.splits : 0, bw = c.dW ? jw.tilesM * jw.tilesN * jw.splits : 0;
+      if (c.dW) pw = job(dt, xt, rows, p.np, p.wchunk, w_parts ? f32(p.wpart) : nullptr, false, dW, c.lddw, nullptr);
+      const int bx = c.dX ? px.tilesM * px.tilesN * px.splits : 0, bw = c.dW ? pw.tilesM * pw.tilesN * pw.splits : 0;
       if (bx + bw > 0)
         with_tile<P>(p.psize, [&](auto t) {
           using T = decltype(t);
-          launch(product_kernel<T, Src>, bx + bw, T::THREADS, 0, st, jx, jw, bx);
+          launch(product_kernel<T, Src>, bx + bw, T::THREADS, 0, st, px, pw, bx);
           return 0;
         });
-      if (c.dW && p.wsplits > 1) launch(parts_kernel<Src>, 2048, 256, 0, st, f32(p.wpart), p.wsplits, rows, H, c.scale, nullptr, dW, (long)c.lddw);
+      const bool last = c0 + p.piece >= C;
+      SumJob sx{}, sw{}, sb{};
+      if (last && c.dX && x_parts) sx = {f32(p.xpart), p.xsplits, n, H, weight, c.dX, c.lddx, 0};
+      if (dW && w_parts) sw = {f32(p.wpart), p.wsplits, rows, H, nullptr, dW, c.lddw, 0};
+      if (last && c.db && b_parts) sb = {f32(p.sums), token_tiles, 1, C, nullptr, c.db, C, 0};
+      sums<Src>(sx, sw, sb, c.scale, st);
     }
-    if (c.dX) launch(parts_kernel<Src>, 2048, 256, 0, st, f32(p.xpart), p.xsplits, n, H, c.scale, weight, static_cast<Src *>(c.dX), (long)c.lddx);
-    if (c.db) launch(parts_kernel<float>, 512, 256, 0, st, f32(p.sums), tiles_of(n, p.bn), 1, C, c.scale, nullptr, c.db, (long)C);
   }
   CAVS_LAUNCH_CHECK();
   return CAVS_OK;
@@ -534,9 +611,9 @@ int check_and_run(const char *who, int type, const Call &c, int grads, void *ws,
   CAVS_REQUIRE(c.W && (c.n == 0 || (c.X && c.labels)), "%s: null pointer", who);
   if (c.n == 0) {  // sums over no rows
     hipStream_t st = as_stream(stream);
-    if (c.dW && type == CAVS_F32) launch(parts_kernel<float>, 2048, 256, 0, st, nullptr, 0, c.C, c.H, 0.f, nullptr, static_cast<float *>(c.dW), (long)c.lddw);
-    if (c.dW && type == CAVS_BF16) launch(parts_kernel<u16>, 2048, 256, 0, st, nullptr, 0, c.C, c.H, 0.f, nullptr, static_cast<u16 *>(c.dW), (long)c.lddw);
-    if (c.db) launch(parts_kernel<float>, 64, 256, 0, st, nullptr, 0, 1, c.C, 0.f, nullptr, c.db, (long)c.C);
+    const SumJob w{nullptr, 0, c.C, c.H, nullptr, c.dW, c.lddw, 0}, b{nullptr, 0, 1, c.C, nullptr, c.db, c.C, 0};
+    if (type == CAVS_F32) sums<float>({}, w, b, 0.f, st);
+    else sums<u16>({}, w, b, 0.f, st);
     CAVS_LAUNCH_CHECK();
     return CAVS_OK;
   }

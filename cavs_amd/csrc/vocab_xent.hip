@@ -164,6 +164,167 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void stats_kernel(TileArgs a, fl
   }
 }
 
+__device__ inline float2 joined(float2 a, float2 b) {
+  const float top = fmaxf(a.x, b.x), from = top == -INFINITY ? 0.f : top;
+  return make_float2(top, a.y * __expf(a.x - from) + b.y * __expf(b.x - from));
+}
+// ------------------------------------------------------------------ few tokens
+// Up to 64 tokens: W read where it lies, once; what bounds it is memory.  A workgroup has 32 classes at a time, each of its
+// four wavefronts a quarter of k: 64 lanes with 64 or 128 bytes each under way are what a CU needs to keep memory busy, and a few thousand
+// classes give every CU such wavefronts.  A lane reads 32 k of one row in one go, 64 at a time for its row (a line of memory is used up by one or two
+// lanes one after the other); the instruction does not mind which k it adds up as long as both operands agree.  The four sums of a product
+// meet in LDS.  Up to 32 tokens X is read as W is, and the launch that would pack it is saved; two blocks of 32 come packed, the lane's pieces
+// those of its k (64 tokens, bf16 50000 x 2048: 70 us, as they lie 86).
+// us of a call, this / packed and in tiles (n = 1, 32, 64 / any up to 64):  bf16 32000 x 1024 16, 22, 31 / 55, 50000 x 2048 38 (5.4 TB/s), 56, 70 / 225;
+// fp32 21701 x 300 19, 22, 28 / 28, 50000 x 2048 114, 131, 169 / 442.  Beyond 64 W has to be read again, or wavefronts get few: bf16 32000 x 1024,
+// 96 tokens 55 / 55, 128 61 / 56.
+template <class Src>
+struct RawRow;
+template <>
+struct RawRow<u16> {
+  typedef unsigned four __attribute__((ext_vector_type(4), aligned(2)));
+  four v[4];
+  __device__ inline void load(const u16 *p) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = *reinterpret_cast<const four *>(p + 8 * i);
+  }
+  __device__ inline void load(const u16 *p, int left) {  // 32 values of which `left` are there
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i / 4][i % 4] = (2 * i < left ? p[2 * i] : 0u) | (2 * i + 1 < left ? (unsigned)p[2 * i + 1] << 16 : 0u);
+  }
+  template <int P>
+  __device__ inline void pieces(int s, bf16x8 (&o)[P]) const { o[0] = __builtin_bit_cast(bf16x8, v[s]); }
+};
+template <>
+struct RawRow<float> {
+  typedef float four __attribute__((ext_vector_type(4), aligned(4)));
+  four v[8];
+  __device__ inline void load(const float *p) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = *reinterpret_cast<const four *>(p + 4 * i);
+  }
+  __device__ inline void load(const float *p, int left) {
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i / 4][i % 4] = i < left ? p[i] : 0.f;
+  }
+  template <int P>
+  __device__ inline void pieces(int s, bf16x8 (&o)[P]) const {
+    unsigned short part[8][P];
+#pragma unroll
+    for (int e = 0; e < 8; e++) parts_of<P>(v[2 * s + e / 4][e % 4], part[e]);
+#pragma unroll
+    for (int p = 0; p < P; p++)
+      o[p] = __builtin_bit_cast(bf16x8, make_uint4(part[0][p] | (unsigned)part[1][p] << 16, part[2][p] | (unsigned)part[3][p] << 16,
+                                                   part[4][p] | (unsigned)part[5][p] << 16, part[6][p] | (unsigned)part[7][p] << 16));
+  }
+};
+
+struct DirectArgs {
+  const void *W, *X;
+  long ldw, ldx;
+  PackedRef packed;     // X, where it is packed
+  int H, C, n, blocks;  // blocks: of 32 classes
+  const float *bias, *labels;
+  float2 *stats;  // a row of n for every workgroup
+  float *zlabel;
+};
+template <int P, class Src, int TN, bool PACKED>
+__global__ __launch_bounds__(256, P == 1 ? 4 : 2) void direct_stats_kernel(DirectArgs a) {
+  constexpr int ACC = P > 1 ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) float sums[4][TN * 16][64];
+  __shared__ float2 part[4][32 * TN];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 31, half = lane >> 5;
+  const int chunks = (a.H + 63) / 64, first = chunks * wave / 4, end = chunks * (wave + 1) / 4;
+  auto fetch = [&](RawRow<Src> &r, const Src *row, int chunk) {
+    const int k = 64 * chunk;
+    if (k + 64 <= a.H) r.load(row + k);
+    else r.load(row + k, a.H - k - 32 * half);
+  };
+  const Src *token_row[TN];
+  const u16 *pieces[TN];
+#pragma unroll
+  for (int j = 0; j < TN; j++) {
+    token_row[j] = static_cast<const Src *>(a.X) + min(32 * j + x, a.n - 1) * a.ldx + 32 * half;
+    pieces[j] = a.packed.p + (long)min(j, (a.n - 1) / 32) * (a.packed.K / 16) * P * 512 + (2 * half * P) * 512 + x * 8;
+  }
+  float2 all = make_float2(-INFINITY, 0.f);  // of token threadIdx.x
+  for (int block = blockIdx.x; block < a.blocks; block += gridDim.x) {
+    const Src *row = static_cast<const Src *>(a.W) + (long)min(32 * block + x, a.C - 1) * a.ldw + 32 * half;
+    floatx16 acc[ACC][TN];
+#pragma unroll
+    for (int s = 0; s < ACC; s++)
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[s][j][r] = 0.f;
+    RawRow<Src> now, next, t[TN];
+    if (first < end) fetch(now, row, first);
+    for (int chunk = first; chunk < end; chunk++) {
+      if constexpr (!PACKED)
+#pragma unroll
+        for (int j = 0; j < TN; j++) fetch(t[j], token_row[j], chunk);
+      if (chunk + 1 < end) fetch(next, row, chunk + 1);
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        bf16x8 w[P], u[TN][P];
+#pragma unroll
+        for (int j = 0; j < TN; j++) {
+          if constexpr (PACKED) {
+#pragma unroll
+            for (int p = 0; p < P; p++) u[j][p] = *reinterpret_cast<const bf16x8 *>(pieces[j] + ((4 * chunk + (s >> 1)) * P + p) * 512 + 256 * (s & 1));
+          } else {
+            t[j].template pieces<P>(s, u[j]);
+          }
+        }
+        now.template pieces<P>(s, w);
+#pragma unroll
+        for (int q = P - 1; q >= 0; q--)
+#pragma unroll
+          for (int p = 0; p <= q; p++)
+#pragma unroll
+            for (int j = 0; j < TN; j++) acc[q ? ACC - 1 : 0][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[p], u[j][q - p], acc[q ? ACC - 1 : 0][j], 0, 0, 0);
+      }
+      now = next;
+    }
+    if constexpr (ACC > 1)
+#pragma unroll
+      for (int j = 0; j < TN; j++) acc[0][j] += acc[1][j];
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) sums[wave][16 * j + r][lane] = acc[0][j][r];
+    __syncthreads();
+    // this wavefront's rows of the block: 8 wave + 4 half + 0 .. 3
+    const int c = 32 * block + 8 * wave + 4 * half;
+    float b[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) b[k] = c + k >= a.C ? -INFINITY : a.bias ? a.bias[c + k] : 0.f;
+#pragma unroll
+    for (int j = 0; j < TN; j++) {
+      const int token = 32 * j + x;
+      const float label = token < a.n ? a.labels[token] : -1.f;
+      float z[4], top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int r = 16 * j + 4 * wave + k;
+        z[k] = (sums[0][r][lane] + sums[1][r][lane]) + (sums[2][r][lane] + sums[3][r][lane]);
+        z[k] = b[k] == -INFINITY ? -INFINITY : z[k] + b[k];
+        top = fmaxf(top, z[k]);
+        if (is_class(label, a.C) && (int)label == c + k) a.zlabel[token] = z[k];
+      }
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int k = 0; k < 4; k++) sum += __expf(z[k] - from);
+      sum += __shfl_xor(sum, 32);
+      if (half == 0) part[wave][32 * j + x] = make_float2(top, sum);
+    }
+    __syncthreads();
+    if (threadIdx.x < 32 * TN) all = joined(all, joined(joined(part[0][threadIdx.x], part[1][threadIdx.x]), joined(part[2][threadIdx.x], part[3][threadIdx.x])));
+  }
+  if (threadIdx.x < 32 * TN && (int)threadIdx.x < a.n) a.stats[(long)blockIdx.x * a.n + threadIdx.x] = all;
+}
+
 // What a row's tiles come to: lse, loss and the weight of its gradient (zero for a row without a class, or without any class that is not
 // masked).  Sixteen lanes to a row, or all of a workgroup where rows are few.
 struct RowArgs {
@@ -172,10 +333,6 @@ struct RowArgs {
   const float *zlabel, *labels, *dloss;
   float *loss, *lse, *weight;
 };
-__device__ inline float2 joined(float2 a, float2 b) {
-  const float top = fmaxf(a.x, b.x), from = top == -INFINITY ? 0.f : top;
-  return make_float2(top, a.y * __expf(a.x - from) + b.y * __expf(b.x - from));
-}
 __device__ inline float weight_of(float label, float lse, const float *dloss, int row, int C) {
   return is_class(label, C) && lse != -INFINITY ? dloss ? dloss[row] : 1.f : 0.f;
 }
@@ -427,10 +584,12 @@ struct Call {
 constexpr int kPieceBytes = 256 << 20;  // d of a piece, in both orders
 constexpr size_t kKeepBytes = 512 << 20;  // of W packed: kept from the first pass for the second
 constexpr int kSplits = 8;
+constexpr int kDirectRows = 64;
 
 // Sizes and places of a call's workspace.
 struct Plan {
   int P, size, bm, bn, Hp, np, piece, pieces, tiles;  // tiles: of the whole vocabulary
+  int direct;  // few tokens: W and X read where they lie
   int grads, keep, psize, pm, pn, xsplits, xchunk, wsplits, wchunk;
   size_t stats, zlabel, lse, weight, x, w, xt, wt, d, dt, sums, xpart, wpart, bytes;
 };
@@ -449,6 +608,8 @@ Plan plan_of(int n, int H, int C, int grads) {
   p.size = tile_size<P>(rows, n);
   tile_sides<P>(p.size, &p.bm, &p.bn);
   p.tiles = tiles_of(C, p.bm);
+  p.direct = !grads && n <= kDirectRows;
+  if (p.direct) p.tiles = tiles_of(C, 32) < 4 * num_cus() ? tiles_of(C, 32) : 4 * num_cus();
   p.keep = packed_bytes<P>(C, p.Hp) <= kKeepBytes;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -460,8 +621,8 @@ Plan plan_of(int n, int H, int C, int grads) {
   p.zlabel = take((size_t)n * 4);
   p.lse = take((size_t)n * 4);
   p.weight = take((size_t)n * 4);
-  p.x = take(packed_bytes<P>(n, p.Hp));
-  p.w = take(packed_bytes<P>(grads && p.keep ? C : rows, p.Hp));
+  p.x = take(p.direct && n <= 32 ? 0 : packed_bytes<P>(n, p.Hp));
+  p.w = take(p.direct ? 0 : packed_bytes<P>(grads && p.keep ? C : rows, p.Hp));
   if (grads) {
     const int rp = ceil_to(rows, kPlaneAlign);
     p.psize = tile_size<P>((long)rows + n, H);
@@ -531,7 +692,16 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
     return TileArgs{ref(piece_w(c0)), ref(X), rows, n, p.Hp, tiles_of(rows, p.bm), tiles_of(n, p.bn), c.b ? c.b + c0 : nullptr, c.labels, c0};
   };
   if (!c.lse_given) {
-    for (int c0 = 0; c0 < C; c0 += p.piece) {
+    if (p.direct) {
+      const DirectArgs a{c.W, c.X, c.ldw, c.ldx, ref(X), H, C, n, tiles_of(C, 32), c.b, c.labels, reinterpret_cast<float2 *>(ws + p.stats), f32(p.zlabel)};
+      if (n <= 32) {
+        launch(direct_stats_kernel<P, Src, 1, false>, p.tiles, 256, 0, st, a);
+      } else {
+        pack<P, Src>(jx, PackJob{}, st);
+        launch(direct_stats_kernel<P, Src, 2, true>, p.tiles, 256, 0, st, a);
+      }
+    }
+    for (int c0 = 0; c0 < C && !p.direct; c0 += p.piece) {
       pack<P, Src>(jx, job_w(c0, true, one), st);
       jx = PackJob{};
       const TileArgs a = tile_args(c0);

@@ -358,3 +358,17 @@ def test_the_same_bits_every_time_captured_and_on_another_stream(type_, n, H, C)
             assert torch.equal(got[k][:, :H], o[k][:, :H]), (turn, k)
         if turn != 2:
             assert torch.equal(got["dW"], first["dW"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("pad", [(0, 0, 0, 0), (3, 1, 0, 0), (0, 7, 0, 0)])
+@pytest.mark.parametrize("n,H,C", [(1, 1, 1), (1, 64, 32), (1, 1024, 5000), (2, 300, 33), (5, 31, 1000), (32, 65, 40000), (33, 200, 777), (64, 130, 3001), (65, 63, 4096),
+                                   (96, 283, 1500), (100, 512, 9000), (129, 100, 2000), (200, 33, 300), (256, 96, 5000), (257, 96, 5000)])
+def test_scores(type_, pad, n, H, C):
+    c = Case(n + H + C, type_, n, H, C, ignored=0.2 if n > 1 else 0.0, masked=min(3, C - 1), pad=pad)
+    o, (ws, need) = c.outputs(), c.workspace(0)
+    c.call("cavs_vocab_xent_fwd", o, ws, need)
+    c.check(o, ("loss", "lse"))
+    torch.cuda.synchronize()
+    assert (o["dX"][:, :H] == 7).all() and (o["db"] == 7).all()

@@ -16,7 +16,7 @@ namespace cavs {
 namespace {
 
 constexpr int kMats = 16;       // matrices of a launch
-constexpr int kNormBlocks = 64; // workgroups that add up a matrix's squares
+constexpr int kNormBlocks = 256; // workgroups that add up a matrix's squares
 
 struct Mat {
   const void *G;
@@ -63,15 +63,36 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs g) {
   if (held_back(c)) return;
   const Mat &t = g.m[who];
   double sum = 0.;
-  for (long r = blockIdx.x; r < t.rows; r += gridDim.x)
-    for (int k = threadIdx.x; k < t.cols; k += 256) {
-      if (t.M) {
-        float *m = t.M + r * t.ldm + k;
-        *m = fmaf(c.momentum, *m, value_of(static_cast<const Src *>(t.G) + r * t.ldg + k));
+  // lanes along a row, as many rows at a time as there are lanes left; four values of a lane on their way
+  int across = 64;
+  while (across < 256 && across < t.cols) across *= 2;
+  const int high = 256 / across, x = threadIdx.x % across, y = threadIdx.x / across;
+  for (long r0 = (long)blockIdx.x * high; r0 < t.rows; r0 += (long)gridDim.x * high) {
+    const long r = r0 + y;
+    if (r >= t.rows) continue;
+    const Src *G = static_cast<const Src *>(t.G) + r * t.ldg;
+    float *M = t.M ? t.M + r * t.ldm : nullptr;
+    for (int k0 = x; k0 < t.cols; k0 += 4 * across) {
+      float gr[4], mo[4];
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const int k = k0 + q * across;
+        gr[q] = k < t.cols ? value_of(G + k) : 0.f;
+        mo[q] = M && k < t.cols ? M[k] : 0.f;
       }
-      const double u = update_of<Src>(t, c, r, k);
-      sum += u * u;
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const int k = k0 + q * across;
+        float u = gr[q];
+        if (M) {
+          mo[q] = fmaf(c.momentum, mo[q], gr[q]);
+          if (k < t.cols) M[k] = mo[q];
+          u = c.nesterov ? fmaf(c.momentum, mo[q], gr[q]) : mo[q];
+        }
+        sum += (double)u * u;
+      }
     }
+  }
   __shared__ double s[256];
   s[threadIdx.x] = sum;
   __syncthreads();
@@ -96,9 +117,14 @@ __global__ __launch_bounds__(256) void start_kernel(StartArgs g) {
   int who = 0;
   while (who + 1 < c.count && (int)blockIdx.x >= g.first[who + 1]) who++;
   const Mat &t = g.m[who];
-  double sum = 0.;
-  for (int i = 0; i < kNormBlocks; i++) sum += c.squares[who * kNormBlocks + i];
-  const double by = 1. / (sqrt(sum) + (double)c.eps);
+  __shared__ double s[kNormBlocks];
+  s[threadIdx.x] = c.squares[who * kNormBlocks + threadIdx.x];
+  for (int o = kNormBlocks / 2; o > 0; o >>= 1) {
+    __syncthreads();
+    if ((int)threadIdx.x < o) s[threadIdx.x] += s[threadIdx.x + o];
+  }
+  __syncthreads();
+  const double by = 1. / (sqrt(s[0]) + (double)c.eps);
   const bool flat = t.rows <= t.cols;
   const int across = (flat ? t.np : t.mp) / 64, block = blockIdx.x - g.first[who];
   const int r0 = block / across * 64, k0 = block % across * 64, k = threadIdx.x & 63;
@@ -301,7 +327,7 @@ struct Shape {
   }
 };
 
-// One launch's tiles: the largest that give most compute units one; where there are fewer, K in stretches, none of them short
+// One launch's tiles; where they are few, K in stretches, none of them short
 template <class T>
 struct LaunchPlan {
   int first[kMats + 1], tilesN[kMats], splits[kMats], chunk[kMats], tiles0[kMats];
@@ -321,12 +347,13 @@ struct LaunchPlan {
       tiles += own[i];
       work += (long)own[i] * K[i];
     }
-    const long fits = 2l * num_cus();
-    int step = (int)((work + fits - 1) / fits);
-    step = step < 256 ? 256 : ceil_to(step, kPlaneAlign);
+    // (of 300 x 512 and 512 x 512, four each, 204 tiles: all of K at once 285 us a call, in two stretches 307; of 128 x 512, two, 6 tiles: 159, in
+    // stretches of 256 154, of 128 144)
+    const bool few = 2 * tiles <= num_cus();
+    const int step = ceil_to((int)(work / (2l * num_cus())) + 128, kPlaneAlign);
     first[0] = 0, parts = 0;
     for (int i = 0; i < count; i++) {
-      splits[i] = tiles >= num_cus() || K[i] <= step ? 1 : (K[i] + step - 1) / step;
+      splits[i] = !few || K[i] <= step ? 1 : (K[i] + step - 1) / step;
       chunk[i] = splits[i] == 1 ? K[i] : ceil_to((K[i] + splits[i] - 1) / splits[i], kPlaneAlign);
       splits[i] = (K[i] + chunk[i] - 1) / chunk[i];
       first[i + 1] = first[i] + own[i] * splits[i];
@@ -336,11 +363,15 @@ struct LaunchPlan {
   }
 };
 
+// The tiles with the shorter longest way: as many as the fullest compute unit gets, times what one takes (a small one a third longer for its
+// size).  Eight of 1024 x 1024: 288 large tiles 85 us, 1088 small ones 77; their last product, 512 large tiles 102 us.
 template <int P, class F>
 auto with_tile(const cavs_ortho_desc *d, int count, int stage, F &&f) {
-  using TT = Tiles<P>;
-  if (LaunchPlan<typename TT::L>(d, count, stage).tiles >= num_cus() * 3 / 4) return f(typename TT::L{});
-  return f(typename TT::S{});
+  using L = typename Tiles<P>::L;
+  using S = typename Tiles<P>::S;
+  const int large = LaunchPlan<L>(d, count, stage).tiles, small = LaunchPlan<S>(d, count, stage).tiles;
+  if ((long)tiles_of(large, num_cus()) * L::BM * L::BN * 3 > (long)tiles_of(small, num_cus()) * S::BM * S::BN * 4) return f(S{});
+  return f(L{});
 }
 
 // what a matrix takes, packed: X, two Xt, A and the polynomial

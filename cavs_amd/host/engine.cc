@@ -52,6 +52,11 @@ Engine::Engine(const cavs_session_config &cfg, void *external_stream, std::share
   if (reads_x && (cfg.V <= 0 || E_ <= 0))
     fail(CAVS_EINVAL, "vocabulary and embedding sizes must be positive");
   if (cfg.loss == CAVS_LOSS_SOFTMAX && cfg.C <= 0) fail(CAVS_EINVAL, "class count must be positive");
+  if (cfg.vocab_head < 0 || cfg.vocab_head > 1 || (cfg.vocab_head && cfg.loss != CAVS_LOSS_SOFTMAX))
+    fail(CAVS_EINVAL, "vocab_head is 0 or 1, and 1 goes with the softmax loss");
+  if (cfg.optimizer < 0 || cfg.optimizer > 1 || (cfg.optimizer && cell_)) fail(CAVS_EINVAL, "unknown optimizer");
+  if (!(cfg.ortho_lr >= 0.f) || !(cfg.ortho_momentum < 1.f) || !(cfg.ortho_decay >= 0.f))
+    fail(CAVS_EINVAL, "ortho_lr and ortho_decay are not negative, ortho_momentum is below 1");
   check(cavs_init(cfg.device));
   if (external_stream)
     stream_ = external_stream;
@@ -102,6 +107,7 @@ Engine::Engine(const cavs_session_config &cfg, void *external_stream, std::share
     add_param("Wfc", (size_t)cfg.C * H, 0, rows(cfg.C, h, H));
     add_param("bfc", cfg.C);
   }
+  if (cfg_.optimizer == CAVS_OPTIMIZER_ORTHO) ortho_setup();
   tail_setup();
 }
 
@@ -125,6 +131,52 @@ void Engine::pad_sizes() {
   // the lookup's row offset is id * E in single precision (EmbeddingLookup): where that is not
   // exact for every id, the rows stay where they are
   if (E_ > 0 && (double)cfg_.V * E_ <= (double)(1 << 24)) E_ = (E_ + 3) / 4 * 4;
+}
+
+// The matrices among the weights: a gate's block of "W" or "U" (a child's, of Tree-FC's), as declared -- of padded weights without the
+// padding, whose zeros would be no part of the matrix's shape.
+void Engine::ortho_setup() {
+  const size_t H = cfg_.H;
+  auto momentum = [&](const char *name) {
+    const Param &p = param(name);
+    const std::string key = std::string(name) + ".momentum";
+    add_param(key, p.n, 0, p.blocks, p.user_n);
+    param(key).state = true;
+  };
+  auto blocks = [&](const char *name, size_t at, int n, int rows) {  // n blocks [rows, h] side by side in rows of n H
+    const Param &p = param(name);
+    float *m = cfg_.ortho_momentum < 0.f ? nullptr : param(std::string(name) + ".momentum").w;
+    for (int k = 0; k < n; k++) {
+      const size_t first = at + k * H;
+      ortho_.push_back({rows, uH_, p.g + first, (int)(n * H), m ? m + first : nullptr, (int)(n * H), p.w + first, (int)(n * H), nullptr, 0});
+    }
+  };
+  momentum("W");
+  switch (cfg_.model) {
+    case CAVS_MODEL_TREELSTM:
+      momentum("U");
+      blocks("W", 0, 4, uE_);
+      blocks("U", 0, 3, uH_);
+      blocks("U", 3 * H * H, 1, uH_);
+      break;
+    case CAVS_MODEL_LSTM:
+      blocks("W", 0, 4, uE_);
+      blocks("W", 4 * H * E_, 4, uH_);
+      break;
+    default:
+      blocks("W", 0, 1, uH_);
+      blocks("W", H * H, 1, uH_);
+  }
+  ortho_ws_.reserve(cavs_ortho_update_workspace(CAVS_F32, (int)ortho_.size(), ortho_.data()) / 4 + 1);
+}
+
+void Engine::ortho_update(float lr) {
+  // (coefficients that lift small singular values fast; what comes of five steps lies between 0.7 and 1.2)
+  const cavs_ortho_options o{5, 1, 3.4445f, -4.7750f, 2.0315f, 1e-7f, cfg_.ortho_momentum == 0.f ? 0.95f : std::max(cfg_.ortho_momentum, 0.f),
+                             cfg_.ortho_lr > 0.f ? cfg_.ortho_lr : lr, cfg_.ortho_decay, update_guard()};
+  check(cavs_ortho_update(CAVS_F32, (int)ortho_.size(), ortho_.data(), &o, ortho_ws_.get(), ortho_ws_.capacity() * 4, stream_));
+  c_launches_ += 2 + 3 * o.steps;
+  upk_valid_ = utp_valid_ = false;
 }
 
 const float *Engine::user_rows(const float *src, size_t n, int blocks) {
@@ -397,6 +449,8 @@ bool Engine::wide_head() const {
          cavs_fc_softmax_xent_workspace(1, cfg_.H, cfg_.C) == 0;
 }
 
+bool Engine::vocab_head() const { return cfg_.vocab_head && cavs_fc_softmax_xent_workspace(1, cfg_.H, cfg_.C) == 0; }
+
 bool Engine::update_jobs(float *w, float *g, float lr, std::vector<cavs_task> *out) {
   if (!w || !g) return false;
   if (wide_head() && w == param("Wfc").w && WfcT_.capacity() >= (size_t)cfg_.C * cfg_.H) {
@@ -454,6 +508,7 @@ void Engine::get_param(const std::string &name, float *host, size_t n, bool grad
   Param &p = param(name);
   if (n != p.user_n || !host)
     fail(CAVS_EINVAL, "parameter '" + name + "' has " + std::to_string(p.user_n) + " elements, got " + std::to_string(n));
+  if (grad && p.state) fail(CAVS_EINVAL, "'" + name + "' is the optimizer's and has no gradient");
   aux_join();
   float *src = grad ? p.g : p.w;
   if (!p.blocks.empty()) {
@@ -719,8 +774,10 @@ void Engine::reserve_edges() {
     R(r_dhlr_, rc * H);
   }
   if (cfg_.loss == CAVS_LOSS_SOFTMAX) {
-    R(logits_, cap * cfg_.C);
-    R(dlogits_, cap * cfg_.C);
+    if (!vocab_head()) {
+      R(logits_, cap * cfg_.C);
+      R(dlogits_, cap * cfg_.C);
+    }
     R(loss_, cap);
   } else {
     R(loss_, std::max<size_t>(cap, 2 * H + 2));
@@ -1534,6 +1591,7 @@ void Engine::step(const int *graph, int B, int maxlen, const void *x, const void
       for (auto &kv : params_) {
         Param &p = *kv.second;
         if (std::find(by_job.begin(), by_job.end(), kv.first) != by_job.end()) continue;  // updated by the job that delivers its gradient
+        if (p.state || (!ortho_.empty() && (kv.first == "W" || kv.first == "U"))) continue;
         if (kv.first == "Emb" && emb_dirty_n_ == N) {
           const int E = (int)(p.n / cfg_.V);
           if (emb_stamp_.capacity() < (size_t)cfg_.V) {
@@ -1554,6 +1612,7 @@ void Engine::step(const int *graph, int B, int maxlen, const void *x, const void
         }
         tasks.push_back({CAVS_TASK_SGD, lr, (long long)p.n, 0, 0, p.w, p.g, nullptr, nullptr});
       }
+      if (!ortho_.empty()) ortho_update(lr);
       StepMark &m = marks_[steps_ & 3];
       stamping(m.ev, &end_stamped_, [&] { check(cavs_run_tasks((int)tasks.size(), tasks.data(), stream_)); });
       if (end_stamped_) m.step = steps_;
@@ -2746,6 +2805,19 @@ void Engine::head_forward_backward(bool backward) {
     // FullyConnected + SoftmaxEntropyLoss (cavs/backend/op_impl_fullyconnected_cublas.cc:71-79,
     // op_impl_softmax_entropy_logits_loss.cu:94-140) and their gradients (:150-163, :212-250)
     Param &Wfc = param("Wfc"), &bfc = param("bfc");
+    if (vocab_head()) {
+      const size_t bytes = cavs_vocab_xent_workspace(CAVS_F32, N, H, C, backward);
+      ensure(head_ws_, grow(bytes / 4 + 1, head_ws_.capacity()));
+      ProfScope ps(this, K_GEMM);
+      if (backward)
+        check(cavs_vocab_xent(CAVS_F32, GO_.get(), H, Wfc.w, H, bfc.w, d_labels_, nullptr, 1.f / N, loss_.get(), nullptr, dGO_.get(), H, Wfc.g, H, bfc.g, N, H, C,
+                              head_ws_.get(), bytes, stream_));
+      else
+        check(cavs_vocab_xent_fwd(CAVS_F32, GO_.get(), H, Wfc.w, H, bfc.w, d_labels_, loss_.get(), nullptr, N, H, C, head_ws_.get(), bytes, stream_));
+      c_gemm_flops_ += (backward ? 8.0 : 2.0) * N * C * H;
+      c_launches_ += 1;
+      return;
+    }
     const size_t head_bytes = cavs_fc_softmax_xent_workspace(N, H, C);
     if (head_bytes > 0) {  // few classes: the whole head and its gradients in one launch; the sum of
                            // its weight-gradient partials rides in the launch that opens backward, or in the update's
@@ -2901,7 +2973,7 @@ void Engine::plan_head_chunks(const int *orphans_host) {
   head_chunks_.clear();
   const Schedule &s = *sched_;
   const int R = (int)s.rounds.size(), N = s.N;
-  if (cfg_.head_chunks < 0 || cfg_.model != CAVS_MODEL_LSTM || !wide_head() || !s.batching || !forest_ || cfg_.graph_replay || R < 8 ||
+  if (vocab_head() || cfg_.head_chunks < 0 || cfg_.model != CAVS_MODEL_LSTM || !wide_head() || !s.batching || !forest_ || cfg_.graph_replay || R < 8 ||
       N < 256)
     return;
   // Where the rounds are one launch per direction, chunks cost more than they cover: the backward rounds become

@@ -32,6 +32,7 @@ struct Param {
   // uw when a forward pass begins, ug from g when a backward pass ends
   float *uw = nullptr, *ug = nullptr;
   DeviceArray<float> own_ug;
+  bool state = false;  // the optimizer's: no gradient, not updated by itself
 };
 
 class Engine {
@@ -105,6 +106,10 @@ class Engine {
 
  private:
   Param &param(const std::string &name);
+  void ortho_setup();
+  void ortho_update(float lr);
+  // the head without logits (cfg_.vocab_head; few classes have a head of their own)
+  bool vocab_head() const;
   void add_param(const std::string &name, size_t n, size_t extra_grad = 0, std::vector<PadBlock> blocks = {}, size_t declared = 0);
   void pad_sizes();
   void copy_blocks(const std::vector<cavs_block_copy> &jobs);
@@ -217,6 +222,8 @@ class Engine {
   }
   float parse_ms_ = 0.f, sched_ms_ = 0.f, wait_ms_ = 0.f, host_step_ms_ = 0.f;
   std::map<std::string, std::unique_ptr<Param>> params_;
+  std::vector<cavs_ortho_desc> ortho_;  // the blocks of "W" and "U" the optimizer takes as matrices
+  DeviceArray<float> ortho_ws_, head_ws_;
 
   std::shared_ptr<Schedule> sched_ = std::make_shared<Schedule>();
   std::shared_ptr<Schedule> spare_[3];

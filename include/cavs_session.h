@@ -99,7 +99,18 @@ typedef struct {
    * the head in one piece between the two passes.  The counter "head_chunks" says in how many
    * chunks the last step's head ran (0: in one piece). */
   int head_chunks;
+  /* Softmax loss, more than 8 classes: 1 = the head keeps no [N, C] logits or d logits (cavs_vocab_xent): vertices whose label is no
+   * class (-1) take no part in it then.  0 = the head with logits. */
+  int vocab_head;
+  /* What applies the gradients: 0 = SGD (cavs/backend/op_impl_sgd.cu).  1 = the input and recurrent weights ("W", "U"), each gate's (Tree-FC: each
+   * child's) block a matrix, by their orthogonalised momentum (cavs_ortho_update, Nesterov, five steps), everything else by SGD.
+   * The momentum is the parameter "W.momentum" / "U.momentum" (zero at first; for checkpoints). */
+  int optimizer;
+  float ortho_lr;       /* step size of the orthogonalised updates; 0 = cavs_session_step's lr */
+  float ortho_momentum; /* 0 = 0.95, negative = none */
+  float ortho_decay;    /* weight decay */
 } cavs_session_config;
+enum { CAVS_OPTIMIZER_SGD = 0, CAVS_OPTIMIZER_ORTHO = 1 };
 
 const char *cavs_session_error(void);
 int cavs_session_create(const cavs_session_config *cfg, cavs_session **out);

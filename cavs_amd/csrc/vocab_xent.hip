@@ -8,6 +8,8 @@
 // (packed for its two products, by token and by class), which d X and d W are made of before the next piece overwrites it.
 // Statistics, sums and accumulators are fp32; d is rounded to bf16 where the gradients are (half a unit of 2^-8, as their own
 // rounding), and is three bf16 parts, all of an fp32's bits, where they are fp32.
+#include <type_traits>
+
 #include "nt_product.h"
 #include "wave_reduce.h"
 
@@ -38,11 +40,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackJob j0, PackJob j1) {
   const int block = second ? blockIdx.x - j0.blocks : blockIdx.x;
   const int r0 = block / g.across * 64, k0 = block % g.across * 64, k = threadIdx.x & 63;
   const Src *src = static_cast<const Src *>(g.src);
-#pragma unroll 8
-  for (int i = threadIdx.x >> 6; i < 64; i += 4) {
-    const int r = r0 + i;
-    tile[i][k] = r < g.rows && k0 + k < g.K ? value_of(src + r * g.ld + k0 + k) : 0.f;
-  }
+  load_tile(tile, src, g.ld, r0, k0, g.rows, g.K);
   __syncthreads();
   pack_tile<P>(tile, g.o, g.keep == KEEP_ALL ? g.t : PackedOut{}, r0, k0, g.rows, g.K);
   if (!g.t.p || g.keep == KEEP_ALL) return;
@@ -54,6 +52,131 @@ __global__ __launch_bounds__(256) void pack_kernel(PackJob j0, PackJob j1) {
 }
 
 // ------------------------------------------------------------------ the tile of z
+// 32 values of a row as they lie in memory, as pieces of eight k for the matrix instruction
+template <class Src>
+struct RawRow;
+template <>
+struct RawRow<u16> {
+  typedef unsigned four __attribute__((ext_vector_type(4), aligned(2)));
+  four v[4];
+  __device__ inline void load(const u16 *p) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = *reinterpret_cast<const four *>(p + 8 * i);
+  }
+  __device__ inline void load(const u16 *p, int left) {  // 32 values of which `left` are there
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (8 * i + 8 <= left) v[i] = *reinterpret_cast<const four *>(p + 8 * i);
+      else
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          v[i][e] = (8 * i + 2 * e < left ? p[8 * i + 2 * e] : 0u) | (8 * i + 2 * e + 1 < left ? (unsigned)p[8 * i + 2 * e + 1] << 16 : 0u);
+    }
+  }
+  template <int P>
+  __device__ inline void pieces(int s, bf16x8 (&o)[P]) const { o[0] = __builtin_bit_cast(bf16x8, v[s]); }
+};
+template <>
+struct RawRow<float> {
+  typedef float four __attribute__((ext_vector_type(4), aligned(4)));
+  four v[8];
+  __device__ inline void load(const float *p) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = *reinterpret_cast<const four *>(p + 4 * i);
+  }
+  __device__ inline void load(const float *p, int left) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (4 * i + 4 <= left) v[i] = *reinterpret_cast<const four *>(p + 4 * i);
+      else
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[i][e] = 4 * i + e < left ? p[4 * i + e] : 0.f;
+    }
+  }
+  template <int P>
+  __device__ inline void pieces(int s, bf16x8 (&o)[P]) const {
+    unsigned short part[8][P];
+#pragma unroll
+    for (int e = 0; e < 8; e++) parts_of<P>(v[2 * s + e / 4][e % 4], part[e]);
+#pragma unroll
+    for (int p = 0; p < P; p++)
+      o[p] = __builtin_bit_cast(bf16x8, make_uint4(part[0][p] | (unsigned)part[1][p] << 16, part[2][p] | (unsigned)part[3][p] << 16,
+                                                   part[4][p] | (unsigned)part[5][p] << 16, part[6][p] | (unsigned)part[7][p] << 16));
+  }
+};
+
+// A tile whose rows of W are read where they lie: four wavefronts of 32 classes each, 32 TN tokens.  For tokens so few that packing W, which writes and
+// reads half as much again (bf16) or three times as much (fp32), would be most of the work.
+template <int P_, int TN_>
+struct RawTile {
+  static constexpr bool RAW = true;
+  static constexpr int P = P_, BM = 128, BN = 32 * TN_, WGM = 4, WGN = 1, WAVES = 4, THREADS = 256, WM = 32, WN = BN, TM = 1, TN = TN_;
+  static constexpr int ACC = P > 1 ? 2 : 1, EU = 2, STAGE = TN * 4 * P * 1024, LDS = 2 * STAGE > 16384 ? 2 * STAGE : 16384;
+};
+// acc = the tile's product: 64 k at a time, a lane's 32 k of its class on their way from memory while those before are multiplied; X packed, by way of
+// LDS, two stages.  A lane's k are 32 in a row (see RawRow's users below): its pieces of X are those of its k.
+template <class T, class Src>
+__device__ __forceinline__ void raw_multiply(const Src *W, long ldw, int M, int m0, const PackedRef &X, int n, int n0, int H, char *S,
+                                             floatx16 (&acc)[T::ACC][T::TM][T::TN]) {
+  constexpr int P = T::P;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 31, half = lane >> 5;
+#pragma unroll
+  for (int s = 0; s < T::ACC; s++)
+#pragma unroll
+    for (int j = 0; j < T::TN; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[s][0][j][r] = 0.f;
+  const Src *row = W + min(m0 + 32 * wave + x, M - 1) * ldw + 32 * half;
+  const int chunks = (H + 63) / 64;
+  auto fetch_w = [&](RawRow<Src> &r, int chunk) {
+    if (64 * chunk + 64 <= H) r.load(row + 64 * chunk);
+    else r.load(row + 64 * chunk, H - 64 * chunk - 32 * half);
+  };
+  // this wavefront's blocks of a stage: every fourth of TN x 4 x P
+  auto fetch_x = [&](int chunk, char *to) {
+#ifdef __HIP_DEVICE_COMPILE__
+    const auto rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16 *>(X.p), 0, 0xffffffffu, 0x00020000);
+#pragma unroll
+    for (int c = 0; c < T::TN * P; c++) {
+      const int at = 4 * c + wave, j = at / (4 * P);
+      const unsigned off = (unsigned)(min(n0 / 32 + j, (n - 1) / 32) * (X.K / 16) + 4 * chunk) * (P * 1024) + at % (4 * P) * 1024;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (__attribute__((address_space(3))) void *)(to + at * 1024), 16, 16 * lane, off, 0, 0);
+    }
+#endif
+  };
+  RawRow<Src> now, next;
+  fetch_x(0, S);
+  fetch_w(now, 0);
+  int at = 0;
+  for (int chunk = 0; chunk < chunks; chunk++) {
+    nt_arrive<0>();
+    if (chunk + 1 < chunks) {
+      fetch_x(chunk + 1, S + (T::STAGE - at));
+      fetch_w(next, chunk + 1);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+      bf16x8 w[P], t[T::TN][P];
+#pragma unroll
+      for (int j = 0; j < T::TN; j++)
+#pragma unroll
+        for (int p = 0; p < P; p++)
+          t[j][p] = *reinterpret_cast<const bf16x8 *>(S + at + ((j * 4 + 2 * half + (s >> 1)) * P + p) * 1024 + (x + 32 * (s & 1)) * 16);
+      now.template pieces<P>(s, w);
+#pragma unroll
+      for (int q = P - 1; q >= 0; q--)
+#pragma unroll
+        for (int p = 0; p <= q; p++)
+#pragma unroll
+          for (int j = 0; j < T::TN; j++)
+            acc[q ? T::ACC - 1 : 0][0][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[p], t[j][q - p], acc[q ? T::ACC - 1 : 0][0][j], 0, 0, 0);
+    }
+    now = next;
+    at = T::STAGE - at;
+  }
+  nt_arrive<0>();
+}
+
 // Vocabulary rows are the tile's rows, tokens its columns: a lane holds 16 TM classes of TN tokens, and a token's sums are
 // sums over registers.
 // Coordinates of acc[.][i][j][r]: class nt_class, token nt_token.
@@ -108,16 +231,33 @@ struct TileArgs {
   const float *bias;   // of the piece, or null
   const float *labels;
   int c0;              // first class of the piece
+  const void *raw;     // the piece's rows of W as they lie, and H
+  long ldw;
+  int H;
 };
+// acc and the tile's place
+template <class T>
+__device__ __forceinline__ void product_of_tile(const TileArgs &a, char *S, floatx16 (&acc)[T::ACC][T::TM][T::TN], int *m0, int *n0, int *tn) {
+  int tm;
+  if constexpr (T::RAW) {
+    using Src = std::conditional_t<T::P == 1, u16, float>;
+    const int t = xcd_remap(blockIdx.x, a.tilesM * a.tilesN);
+    tm = t / a.tilesN, *tn = t - tm * a.tilesN;  // (tiles of the same classes together: W comes from memory once)
+    *m0 = tm * T::BM, *n0 = *tn * T::BN;
+    raw_multiply<T, Src>(static_cast<const Src *>(a.raw), a.ldw, a.M, *m0, a.X, a.n, *n0, a.H, S, acc);
+  } else {
+    nt_tile_of(blockIdx.x, a.tilesM, a.tilesN, &tm, tn);
+    *m0 = tm * T::BM, *n0 = *tn * T::BN;
+    nt_multiply<T>(a.W, a.M, *m0, a.X, a.n, *n0, 0, a.K, S, acc);
+  }
+}
 
 template <class T>
 __global__ __launch_bounds__(T::THREADS, T::EU) void stats_kernel(TileArgs a, float2 *__restrict__ stats, float *__restrict__ zlabel) {
   __shared__ __attribute__((aligned(16))) char S[T::LDS];
-  int tm, tn;
-  nt_tile_of(blockIdx.x, a.tilesM, a.tilesN, &tm, &tn);
-  const int m0 = tm * T::BM, n0 = tn * T::BN;
+  int m0, n0, tn;
   floatx16 acc[T::ACC][T::TM][T::TN];
-  nt_multiply<T>(a.W, a.M, m0, a.X, a.n, n0, 0, a.K, S, acc);
+  product_of_tile<T>(a, S, acc, &m0, &n0, &tn);
   float *lb = reinterpret_cast<float *>(S);
   float2 *part = reinterpret_cast<float2 *>(S + T::BM * 4);  // [WGM][BN]
   const Where<T> w;
@@ -160,7 +300,7 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void stats_kernel(TileArgs a, fl
       const float top = fmaxf(s.x, o.x), from = top == -INFINITY ? 0.f : top;
       s = make_float2(top, s.y * __expf(s.x - from) + o.y * __expf(o.x - from));
     }
-    stats[(long)(a.c0 / T::BM + tm) * a.n + n0 + x] = s;
+    stats[(long)((a.c0 + m0) / T::BM) * a.n + n0 + x] = s;
   }
 }
 
@@ -178,47 +318,6 @@ __device__ inline float2 joined(float2 a, float2 b) {
 // us of a call, this / packed and in tiles (n = 1, 32, 64 / any up to 64):  bf16 32000 x 1024 16, 22, 31 / 55, 50000 x 2048 38 (5.4 TB/s), 56, 70 / 225;
 // fp32 21701 x 300 19, 22, 28 / 28, 50000 x 2048 114, 131, 169 / 442.  Beyond 64 W has to be read again, or wavefronts get few: bf16 32000 x 1024,
 // 96 tokens 55 / 55, 128 61 / 56.
-template <class Src>
-struct RawRow;
-template <>
-struct RawRow<u16> {
-  typedef unsigned four __attribute__((ext_vector_type(4), aligned(2)));
-  four v[4];
-  __device__ inline void load(const u16 *p) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = *reinterpret_cast<const four *>(p + 8 * i);
-  }
-  __device__ inline void load(const u16 *p, int left) {  // 32 values of which `left` are there
-#pragma unroll
-    for (int i = 0; i < 16; i++) v[i / 4][i % 4] = (2 * i < left ? p[2 * i] : 0u) | (2 * i + 1 < left ? (unsigned)p[2 * i + 1] << 16 : 0u);
-  }
-  template <int P>
-  __device__ inline void pieces(int s, bf16x8 (&o)[P]) const { o[0] = __builtin_bit_cast(bf16x8, v[s]); }
-};
-template <>
-struct RawRow<float> {
-  typedef float four __attribute__((ext_vector_type(4), aligned(4)));
-  four v[8];
-  __device__ inline void load(const float *p) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = *reinterpret_cast<const four *>(p + 4 * i);
-  }
-  __device__ inline void load(const float *p, int left) {
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i / 4][i % 4] = i < left ? p[i] : 0.f;
-  }
-  template <int P>
-  __device__ inline void pieces(int s, bf16x8 (&o)[P]) const {
-    unsigned short part[8][P];
-#pragma unroll
-    for (int e = 0; e < 8; e++) parts_of<P>(v[2 * s + e / 4][e % 4], part[e]);
-#pragma unroll
-    for (int p = 0; p < P; p++)
-      o[p] = __builtin_bit_cast(bf16x8, make_uint4(part[0][p] | (unsigned)part[1][p] << 16, part[2][p] | (unsigned)part[3][p] << 16,
-                                                   part[4][p] | (unsigned)part[5][p] << 16, part[6][p] | (unsigned)part[7][p] << 16));
-  }
-};
-
 struct DirectArgs {
   const void *W, *X;
   long ldw, ldx;
@@ -378,11 +477,9 @@ template <class T>
 __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, const float *__restrict__ lse, const float *__restrict__ weight, PackedOut d,
                                                                     PackedOut t, float *__restrict__ sums, int ld_sums, float sums_scale) {
   __shared__ __attribute__((aligned(16))) char S[T::LDS];
-  int tm, tn;
-  nt_tile_of(blockIdx.x, a.tilesM, a.tilesN, &tm, &tn);
-  const int m0 = tm * T::BM, n0 = tn * T::BN;
+  int m0, n0, tn;
   floatx16 acc[T::ACC][T::TM][T::TN];
-  nt_multiply<T>(a.W, a.M, m0, a.X, a.n, n0, 0, a.K, S, acc);
+  product_of_tile<T>(a, S, acc, &m0, &n0, &tn);
   float *lb = reinterpret_cast<float *>(S);
   float *part = lb + T::BM;  // [WGN][BM]
   const Where<T> w;
@@ -425,6 +522,10 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, 
 #pragma unroll
         for (int r = 0; r < 16; r++) parts_of<T::P>(x[r], e.v[r]);
         put_columns<T::P>(t, cb, xb, e, w.lane, turn);
+        if (T::BN < kPlaneAlign && 32 * (xb + 1) >= a.n && 32 * (xb + 1) < t.K) {  // (a tile that ends in front of the padding)
+          Parts16<T::P> zero = {};
+          put_columns<T::P>(t, cb, xb + 1, zero, w.lane, turn);
+        }
       }
     }
     if (!sums) continue;
@@ -445,6 +546,156 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, 
     for (int q = 1; q < T::WGN; q++) s += part[q * T::BM + x];
     sums[(long)tn * ld_sums + m0 + x] = sums_scale * s;
   }
+}
+
+// ------------------------------------------------------------------ d X of few tokens
+// Sums over classes of d times W, W's rows read where they lie, once: what bounds it is memory.  A lane has F neighbouring columns of eight classes
+// of a step, a load of 4 F or 2 F bytes each; the instruction takes its eight classes of one column at a time, so those are F operands, of
+// columns F apart, by renaming registers.  A workgroup has 32 F columns, up to 32 TN tokens and a stretch of the classes, of which each wavefront takes
+// every fourth step of sixteen; what they sum up meets in LDS and goes to part [stretch, n, H].  Rows of classes that are masked are zero.
+// (F as large as accumulators leave room for: with loads of 4 bytes a wavefront has 2 KB under way, too little -- one token, bf16 124416 x 2176,
+// 700 us of a call.)
+struct FewArgs {
+  const void *W;
+  long ldw;
+  PackedRef d;  // by token; its k the piece's classes
+  int M, n, H;  // classes of the piece
+  const float *bias;
+  int across, chunk;  // blocks of 32 F columns, classes of a stretch (a multiple of 64)
+  float *part;
+  int add;
+};
+template <int P, int TN>
+constexpr int few_columns() { return (P == 1 ? 8 : 4) / TN; }
+template <int P, class Src, int TN>
+__global__ __launch_bounds__(256, 2) void few_dx_kernel(FewArgs a) {
+  constexpr int ACC = P > 1 ? 2 : 1, F = few_columns<P, TN>();
+  __shared__ __attribute__((aligned(16))) float sums[4][32][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 31, half = lane >> 5;
+  const int h0 = 32 * F * (blockIdx.x % a.across), stretch = blockIdx.x / a.across;
+  const int kend = min(a.d.K, (stretch + 1) * a.chunk);
+  const u16 *dp[TN];
+#pragma unroll
+  for (int j = 0; j < TN; j++) dp[j] = a.d.p + (long)min(j, (a.n - 1) / 32) * (a.d.K / 16) * P * 512 + lane * 8;
+  floatx16 acc[ACC][TN][F];
+#pragma unroll
+  for (int s = 0; s < ACC; s++)
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int f = 0; f < F; f++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[s][j][f][r] = 0.f;
+  // F columns from h0 + F x on, of eight classes (beyond the last column: nothing)
+  const bool whole = h0 + F * x + F <= a.H;  // (this lane's)
+  constexpr int WORDS = F * sizeof(Src) / 4;
+  typedef unsigned words __attribute__((ext_vector_type(WORDS == 1 ? 2 : WORDS), aligned(sizeof(Src))));
+  struct Eight {
+    unsigned v[8][WORDS];
+    bf16x8 d[TN][P];
+    float b[8];
+  };
+  auto fetch = [&](Eight &o, int k0) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const int c = min(k0 + 8 * half + e, a.M - 1);
+      const Src *row = static_cast<const Src *>(a.W) + c * a.ldw + h0 + F * x;
+      o.b[e] = a.bias ? a.bias[c] : 0.f;
+      if (whole) {
+        static_assert(WORDS > 1, "a lane's columns are eight bytes or more");
+        const words v = *reinterpret_cast<const words *>(row);
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) o.v[e][i] = v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) {
+          if constexpr (sizeof(Src) == 4) {
+            o.v[e][i] = h0 + F * x + i < a.H ? __float_as_uint(value_of(row + i)) : 0u;
+          } else {
+            const unsigned lo = h0 + F * x + 2 * i < a.H ? row[2 * i] : 0u, hi = h0 + F * x + 2 * i + 1 < a.H ? row[2 * i + 1] : 0u;
+            o.v[e][i] = lo | hi << 16;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int p = 0; p < P; p++) o.d[j][p] = *reinterpret_cast<const bf16x8 *>(dp[j] + ((long)(k0 / 16) * P + p) * 512);
+  };
+  auto mask = [&](Eight &o, int k0) {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (k0 + 8 * half + e >= a.M || o.b[e] == -INFINITY)
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) o.v[e][i] = 0;
+  };
+  Eight now, next;
+  int k = stretch * a.chunk + 16 * wave;
+  if (k < kend) fetch(now, k);
+  for (; k < kend; k += 64) {
+    if (k + 64 < kend) fetch(next, k + 64);
+    mask(now, k);
+#pragma unroll
+    for (int f = 0; f < F; f++) {
+      bf16x8 w[P];
+      if constexpr (sizeof(Src) == 4) {
+        u16 part[8][P];
+#pragma unroll
+        for (int e = 0; e < 8; e++) parts_of<P>(__uint_as_float(now.v[e][f]), part[e]);
+#pragma unroll
+        for (int p = 0; p < P; p++)
+          w[p] = __builtin_bit_cast(bf16x8, make_uint4(part[0][p] | (unsigned)part[1][p] << 16, part[2][p] | (unsigned)part[3][p] << 16,
+                                                       part[4][p] | (unsigned)part[5][p] << 16, part[6][p] | (unsigned)part[7][p] << 16));
+      } else {
+        unsigned u[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const unsigned lo = now.v[2 * e][f / 2], hi = now.v[2 * e + 1][f / 2];
+          u[e] = f % 2 ? lo >> 16 | (hi & 0xffff0000u) : (lo & 0xffffu) | hi << 16;
+        }
+        w[0] = __builtin_bit_cast(bf16x8, make_uint4(u[0], u[1], u[2], u[3]));
+      }
+#pragma unroll
+      for (int q = P - 1; q >= 0; q--)
+#pragma unroll
+        for (int p = 0; p <= q; p++)
+#pragma unroll
+          for (int j = 0; j < TN; j++)
+            acc[q ? ACC - 1 : 0][j][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(now.d[j][p], w[q - p], acc[q ? ACC - 1 : 0][j][f], 0, 0, 0);
+    }
+    now = next;
+  }
+  float *part = a.part + (long)stretch * a.n * a.H;
+#pragma unroll
+  for (int j = 0; j < TN; j++)
+#pragma unroll
+    for (int f0 = 0; f0 < F; f0 += 2) {
+      __syncthreads();
+#pragma unroll
+      for (int f = 0; f < 2; f++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          float v = acc[0][j][f0 + f][r];
+          if constexpr (ACC > 1) v += acc[1][j][f0 + f][r];
+          sums[wave][16 * f + r][lane] = v;
+        }
+      __syncthreads();
+      // this wavefront's rows of the block: 8 wave + 4 half + 0 .. 3
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int token = 32 * j + 8 * wave + 4 * half + i;
+        if (token >= a.n) continue;
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+          const int r = 16 * f + 4 * wave + i, h = h0 + F * x + f0 + f;
+          if (h >= a.H) continue;
+          float v = (sums[0][r][lane] + sums[1][r][lane]) + (sums[2][r][lane] + sums[3][r][lane]);
+          float *o = part + (long)token * a.H + h;
+          *o = a.add ? *o + v : v;
+        }
+      }
+    }
 }
 
 // ------------------------------------------------------------------ the products with d
@@ -512,12 +763,12 @@ __device__ inline void sum_parts(const SumJob &g, float scale, int block) {
   Out *out = static_cast<Out *>(g.out);
   for (long i = (long)block * 256 + threadIdx.x; i < total; i += (long)g.blocks * 256) {
     float s = 0.f;
-    for (int p = 0; p < g.parts; p += 4) {  // (four loads on their way at a time)
-      float v[4];
+    for (int p = 0; p < g.parts; p += 8) {  // (eight loads on their way at a time)
+      float v[8];
 #pragma unroll
-      for (int k = 0; k < 4; k++) v[k] = p + k < g.parts ? g.part[(p + k) * total + i] : 0.f;
+      for (int k = 0; k < 8; k++) v[k] = p + k < g.parts ? g.part[(p + k) * total + i] : 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; k++) s += v[k];
+      for (int k = 0; k < 8; k++) s += v[k];
     }
     const long r = i / g.w;
     store_as(out + r * g.ldo + (i - r * g.w), (g.factor ? scale * g.factor[r] : scale) * s);
@@ -547,15 +798,27 @@ template <> struct Tiles<3> {
 };
 
 template <int P, class F>
-int with_tile(int size, F &&f) {
+int with_product_tile(int size, F &&f) {
   using TT = Tiles<P>;
   if (size == 2) return f(typename TT::L{});
   if (size == 1) return f(typename TT::M{});
   return f(typename TT::S{});
 }
+// sizes 0 .. 2: packed operands, small to large; 3 .. 5: W as it lies, 32 (fp32), 64 and 128 (bf16, losses alone) tokens
+template <int P, bool GRADS, class F>
+int with_tile(int size, F &&f) {
+  if constexpr (P == 3) {
+    if (size == 3) return f(RawTile<P, 1>{});
+  }
+  if constexpr (P == 1 && !GRADS) {
+    if (size == 5) return f(RawTile<P, 4>{});
+  }
+  if (size >= 3) return f(RawTile<P, 2>{});
+  return with_product_tile<P>(size, f);
+}
 template <int P>
 void tile_sides(int size, int *bm, int *bn) {
-  with_tile<P>(size, [&](auto t) { return *bm = decltype(t)::BM, *bn = decltype(t)::BN, 0; });
+  with_tile<P, false>(size, [&](auto t) { return *bm = decltype(t)::BM, *bn = decltype(t)::BN, 0; });
 }
 // the largest tile that still gives most compute units one
 template <int P>
@@ -583,13 +846,15 @@ struct Call {
 
 constexpr int kPieceBytes = 256 << 20;  // d of a piece, in both orders
 constexpr size_t kKeepBytes = 512 << 20;  // of W packed: kept from the first pass for the second
-constexpr int kSplits = 8;
-constexpr int kDirectRows = 64;
+constexpr int kSplits = 64;
+constexpr int kDirectRows = 64, kFewRows = 64, kRawRows = 256;
 
 // Sizes and places of a call's workspace.
 struct Plan {
   int P, size, bm, bn, Hp, np, piece, pieces, tiles;  // tiles: of the whole vocabulary
   int direct;  // few tokens: W and X read where they lie
+  int raw;      // not many: W read where it lies
+  int facross;  // few_dx_kernel's
   int grads, keep, psize, pm, pn, xsplits, xchunk, wsplits, wchunk;
   size_t stats, zlabel, lse, weight, x, w, xt, wt, d, dt, sums, xpart, wpart, bytes;
 };
@@ -605,7 +870,14 @@ Plan plan_of(int n, int H, int C, int grads) {
   p.piece = ceil_to((C + p.pieces - 1) / p.pieces, 256);
   p.pieces = tiles_of(C, p.piece);
   const int rows = p.piece < C ? p.piece : C;
-  p.size = tile_size<P>(rows, n);
+  // A vocabulary with a tile of 128 classes for every compute unit (for the losses alone, every second) and few tokens: W read where it lies, packing
+  // it would be most of the work.  us packed / as it lies:
+  //   losses, 96 and 256 tokens: bf16 124416 x 2176 361 / 283, 423 / 313, 45376 x 1024 53 / 33, 74 / 42, 21701 x 300 20 / 18, 23 / 19, 10000 x 512
+  //   20 / 20, 23 / 21; fp32 45376 x 1024 171 / 139, 217 / 181, 21701 x 300 31 / 27, 42 / 40, 1000 x 128 13 / 15
+  //   with gradients, 1 and 64 tokens: fp32 45376 x 1024 425 / 235, 443 / 287, 81792 x 72 141 / 105, 160 / 124, 21701 x 300 83 / 88, 90 / 98;
+  //   bf16 124416 x 2176 917 / 679, 924 / 642, 45376 x 1024 181 / 122, 199 / 134, 81792 x 72 99 / 91, 10000 x 512 49 / 54; 96 tokens: as packed
+  p.raw = grads ? n <= kFewRows && C >= 128 * num_cus() : n <= kRawRows && C >= 64 * num_cus();
+  p.size = !p.raw ? tile_size<P>(rows, n) : P == 3 && n <= 32 ? 3 : P == 1 && n > 64 ? 5 : 4;
   tile_sides<P>(p.size, &p.bm, &p.bn);
   p.tiles = tiles_of(C, p.bm);
   p.direct = !grads && n <= kDirectRows;
@@ -622,14 +894,15 @@ Plan plan_of(int n, int H, int C, int grads) {
   p.lse = take((size_t)n * 4);
   p.weight = take((size_t)n * 4);
   p.x = take(p.direct && n <= 32 ? 0 : packed_bytes<P>(n, p.Hp));
-  p.w = take(p.direct ? 0 : packed_bytes<P>(grads && p.keep ? C : rows, p.Hp));
+  p.w = take(p.direct || p.raw ? 0 : packed_bytes<P>(grads && p.keep ? C : rows, p.Hp));
   if (grads) {
     const int rp = ceil_to(rows, kPlaneAlign);
     p.psize = tile_size<P>((long)rows + n, H);
     tile_sides<P>(p.psize, &p.pm, &p.pn);
     // few tiles: K in several stretches, none of them short
     auto split = [&](long tiles, int K, int *chunk) {
-      int s = (int)(num_cus() / (tiles > 0 ? tiles : 1));
+      int s = (int)(2 * num_cus() / (tiles > 0 ? tiles : 1));
+      s = 2 * tiles > num_cus() ? 1 : s;
       s = s > kSplits ? kSplits : s;
       s = s > K / 512 ? K / 512 : s;
       s = s < 1 ? 1 : s;
@@ -638,8 +911,17 @@ Plan plan_of(int n, int H, int C, int grads) {
     };
     p.xsplits = split((long)tiles_of(n, p.pm) * tiles_of(H, p.pn), rp, &p.xchunk);
     p.wsplits = split((long)tiles_of(rows, p.pm) * tiles_of(H, p.pn), p.np, &p.wchunk);
+    if (p.raw) {
+      p.facross = tiles_of(H, 32 * (n <= 32 ? few_columns<P, 1>() : few_columns<P, 2>()));
+      // stretches for three workgroups a compute unit, of 256 classes or more
+      int stretches = 3 * num_cus() / p.facross;
+      stretches = stretches > rp / 256 ? rp / 256 : stretches;
+      stretches = stretches < 1 ? 1 : stretches;
+      p.xchunk = ceil_to((rp + stretches - 1) / stretches, kPlaneAlign);
+      p.xsplits = (rp + p.xchunk - 1) / p.xchunk;
+    }
     p.xt = take(packed_bytes<P>(H, p.np));
-    p.wt = take(packed_bytes<P>(H, rp));
+    p.wt = take(p.raw ? 0 : packed_bytes<P>(H, rp));
     p.d = take(packed_bytes<P>(n, rp));
     p.dt = take(packed_bytes<P>(rows, p.np));
     p.sums = take((size_t)tiles_of(n, p.bn) * C * 4);
@@ -681,7 +963,8 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
   auto rows_of = [&](int c0) { return C - c0 < p.piece ? C - c0 : p.piece; };
   auto job_w = [&](int c0, bool o, bool t) {
     const int rows = rows_of(c0);
-    return pack_job(static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, rows, H, o ? piece_w(c0) : none, t && p.grads ? piece_wt(rows) : none,
+    return pack_job(static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, rows, H, o && !p.raw ? piece_w(c0) : none,
+                    t && p.grads && !p.raw ? piece_wt(rows) : none,
                     c.b ? c.b + c0 : nullptr, c.b ? KEEP_FINITE : KEEP_ALL, 0);
   };
   const PackedOut xt{p.grads && c.dW ? pl(p.xt) : nullptr, p.np};
@@ -689,7 +972,8 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
   PackJob jx = pack_job(c.X, c.ldx, n, H, X, xt, c.labels, KEEP_LABELLED, C);
   auto tile_args = [&](int c0) {
     const int rows = rows_of(c0);
-    return TileArgs{ref(piece_w(c0)), ref(X), rows, n, p.Hp, tiles_of(rows, p.bm), tiles_of(n, p.bn), c.b ? c.b + c0 : nullptr, c.labels, c0};
+    return TileArgs{ref(piece_w(c0)), ref(X), rows, n, p.Hp, tiles_of(rows, p.bm), tiles_of(n, p.bn), c.b ? c.b + c0 : nullptr, c.labels, c0,
+                    static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, H};
   };
   if (!c.lse_given) {
     if (p.direct) {
@@ -705,7 +989,7 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
       pack<P, Src>(jx, job_w(c0, true, one), st);
       jx = PackJob{};
       const TileArgs a = tile_args(c0);
-      with_tile<P>(p.size, [&](auto t) {
+      with_tile<P, false>(p.size, [&](auto t) {
         using T = decltype(t);
         launch(stats_kernel<T>, a.tilesM * a.tilesN, T::THREADS, 0, st, a, reinterpret_cast<float2 *>(ws + p.stats), f32(p.zlabel));
         return 0;
@@ -720,7 +1004,7 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
   if (p.grads) {
     const float *all = c.lse_given ? c.lse_given : lse;
     const int token_tiles = tiles_of(n, p.bn);
-    const bool x_parts = !one || p.xsplits > 1, w_parts = p.wsplits > 1, b_parts = token_tiles > 1;
+    const bool x_parts = p.raw || !one || p.xsplits > 1, w_parts = p.wsplits > 1, b_parts = token_tiles > 1;
     bool first = true;
     for (int c0 = 0; c0 < C; c0 += p.piece, first = false) {
       const int rows = rows_of(c0), rp = ceil_to(rows, kPlaneAlign);
@@ -731,7 +1015,7 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
       const TileArgs a = tile_args(c0);
       const PackedOut d{c.dX ? pl(p.d) : nullptr, rp}, dt{c.dW ? pl(p.dt) : nullptr, p.np}, wt = piece_wt(rows);
       if (c.dX || c.dW || c.db)
-        with_tile<P>(p.size, [&](auto t) {
+        with_tile<P, true>(p.size, [&](auto t) {
           using T = decltype(t);
           launch(dlogits_kernel<T>, a.tilesM * a.tilesN, T::THREADS, 0, st, a, all, weight, d, dt, !c.db ? nullptr : b_parts ? f32(p.sums) + c0 : c.db + c0, C,
                  b_parts ? 1.f : c.scale);
@@ -743,16 +1027,23 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
       };
       ProductJob<Src> px{}, pw{};
       // (a last piece shorter than the others fills fewer stretches: those beyond keep what they have)
-      if (c.dX) px = job(d, wt, n, rp, p.xchunk, x_parts ? f32(p.xpart) : nullptr, !first, c.dX, c.lddx, weight);
+      if (c.dX && !p.raw) px = job(d, wt, n, rp, p.xchunk, x_parts ? f32(p.xpart) : nullptr, !first, c.dX, c.lddx, weight);
       Src *dW = c.dW ? static_cast<Src *>(c.dW) + (long)c0 * c.lddw : nullptr;
       if (c.dW) pw = job(dt, xt, rows, p.np, p.wchunk, w_parts ? f32(p.wpart) : nullptr, false, dW, c.lddw, nullptr);
-      const int bx = c.dX ? px.tilesM * px.tilesN * px.splits : 0, bw = c.dW ? pw.tilesM * pw.tilesN * pw.splits : 0;
+      const int bx = c.dX && !p.raw ? px.tilesM * px.tilesN * px.splits : 0, bw = c.dW ? pw.tilesM * pw.tilesN * pw.splits : 0;
       if (bx + bw > 0)
-        with_tile<P>(p.psize, [&](auto t) {
+        with_product_tile<P>(p.psize, [&](auto t) {
           using T = decltype(t);
           launch(product_kernel<T, Src>, bx + bw, T::THREADS, 0, st, px, pw, bx);
           return 0;
         });
+      if (c.dX && p.raw) {
+        const FewArgs f{static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, ref(d), rows, n, H, c.b ? c.b + c0 : nullptr, p.facross, p.xchunk,
+                        f32(p.xpart), !first};
+        const int grid = p.facross * ((rp + p.xchunk - 1) / p.xchunk);
+        if (n <= 32) launch(few_dx_kernel<P, Src, 1>, grid, 256, 0, st, f);
+        else launch(few_dx_kernel<P, Src, 2>, grid, 256, 0, st, f);
+      }
       const bool last = c0 + p.piece >= C;
       SumJob sx{}, sw{}, sb{};
       if (last && c.dX && x_parts) sx = {f32(p.xpart), p.xsplits, n, H, weight, c.dX, c.lddx, 0};

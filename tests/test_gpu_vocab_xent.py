@@ -170,7 +170,8 @@ def _device(request):
 
 
 SHAPES = [(1, 64, 256), (1, 1, 1), (2, 5, 3), (3, 33, 64), (17, 64, 65), (64, 128, 63), (65, 100, 257), (130, 300, 1000), (33, 16, 2048), (257, 72, 129),
-          (320, 128, 1000), (5, 700, 5001), (1000, 31, 700)]
+          (320, 128, 1000), (5, 700, 5001), (1000, 31, 700), (257, 1, 1), (260, 5, 3), (300, 33, 64), (511, 64, 257), (1025, 700, 130), (100, 66, 4097),
+          (129, 190, 3000), (250, 64, 700)]
 
 
 @pytest.mark.gpu
@@ -194,7 +195,39 @@ def test_large_tiles(type_, n, H, C):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("type_,n,H,C", [("f32", 1100, 40, 50003), ("bf16", 3000, 72, 60001)])
+@pytest.mark.parametrize("type_,n,H,C", [("f32", 1, 300, 33001), ("f32", 31, 530, 33000), ("f32", 33, 217, 40003), ("f32", 64, 96, 90001), ("bf16", 1, 1025, 33003),
+                                         ("bf16", 32, 300, 60001), ("bf16", 40, 700, 35001), ("bf16", 64, 131, 130003)])
+def test_few_tokens_and_a_large_vocabulary(type_, n, H, C):
+    """W read where it lies: with rows without a class, masked classes whose rows hold no numbers, and rows of W and X further apart than H"""
+    c = Case(n + H + C, type_, n, H, C, ignored=0.3 if n > 1 else 0.0, masked=5, weights=True, pad=(1, 3, 2, 1))
+    gone = ~((c.labels >= 0) & (c.labels < C))
+    c.X[gone, ::2] = float("nan")
+    c.W[C - 5:, ::2] = float("inf")
+    c.W[C - 5:, 1::2] = float("nan")
+    o, (ws, need) = c.outputs(), c.workspace(1)
+    c.call("cavs_vocab_xent", o, ws, need)
+    c.check(o)
+    first = {k: v.clone() for k, v in o.items()}
+    ws.fill_(0xff)
+    c.call("cavs_vocab_xent", o, ws, need)
+    torch.cuda.synchronize()
+    for k, v in o.items():  # (lse of a row without a class that holds NaN is NaN)
+        assert torch.equal(first[k][..., :H].nan_to_num(9.0) if k in ("dX", "dW") else first[k].nan_to_num(9.0), v[..., :H].nan_to_num(9.0) if k in ("dX", "dW")
+                           else v.nan_to_num(9.0)), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,n,H,C", [("f32", 65, 100, 40003), ("f32", 200, 515, 17000), ("bf16", 70, 259, 30001), ("bf16", 129, 1030, 17000), ("bf16", 256, 64, 100001)])
+def test_scores_of_more_tokens_and_a_large_vocabulary(type_, n, H, C):
+    c = Case(n + H + C, type_, n, H, C, ignored=0.3, masked=5, pad=(1, 3, 0, 0))
+    c.W[C - 5:, ::2] = float("nan")
+    o, (ws, need) = c.outputs(), c.workspace(0)
+    c.call("cavs_vocab_xent_fwd", o, ws, need)
+    c.check(o, ("loss", "lse"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,n,H,C", [("f32", 1100, 40, 50003), ("bf16", 3000, 72, 60001), ("f32", 60, 24, 400003), ("bf16", 50, 12, 1500001)])
 def test_several_pieces(type_, n, H, C):
     c = Case(n + H, type_, n, H, C, weights=True)
     o, (ws, need) = c.outputs(), c.workspace(1)
@@ -205,7 +238,7 @@ def test_several_pieces(type_, n, H, C):
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", ["f32", "bf16"])
 @pytest.mark.parametrize("pad", [(0, 8, 0, 8), (1, 3, 5, 2), (64, 64, 64, 64)])
-@pytest.mark.parametrize("n,H,C", [(1, 128, 300), (67, 128, 300), (67, 61, 300)])
+@pytest.mark.parametrize("n,H,C", [(1, 128, 300), (67, 128, 300), (67, 61, 300), (300, 61, 300), (300, 128, 301)])
 def test_strides_rows_without_a_class_masked_classes(type_, pad, n, H, C):
     c = Case(5, type_, n, H, C, ignored=0.4, masked=7, weights=True, pad=pad)
     gone = ~((c.labels >= 0) & (c.labels < C))
@@ -221,7 +254,7 @@ def test_strides_rows_without_a_class_masked_classes(type_, pad, n, H, C):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", ["f32", "bf16"])
-@pytest.mark.parametrize("n", [1, 90])
+@pytest.mark.parametrize("n", [1, 90, 300])
 def test_every_class_masked_or_no_row_with_a_class(type_, n):
     c = Case(6, type_, n, 64, 70)
     c.b[:] = -float("inf")
@@ -251,7 +284,7 @@ def test_no_rows(type_):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", ["f32", "bf16"])
-@pytest.mark.parametrize("n,H,C", [(1, 64, 500), (40, 64, 500), (300, 130, 2000)])
+@pytest.mark.parametrize("n,H,C", [(1, 64, 500), (40, 64, 500), (130, 64, 500), (300, 130, 2000)])
 def test_the_halves_are_the_whole(type_, n, H, C):
     """Forward, and backward from its lse, give the whole call's bits; what is not asked for changes nothing else."""
     c = Case(9, type_, n, H, C, ignored=0.2, masked=3, weights=True)

@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256) void start_kernel(StartArgs g) {
     if ((int)threadIdx.x < o) s[threadIdx.x] += s[threadIdx.x + o];
   }
   __syncthreads();
-  const double by = 1. / (sqrt(s[0]) + (double)c.eps);
+  const double by = s[0] == 0. ? 0. : 1. / (sqrt(s[0]) + (double)c.eps);  // (nothing stays nothing, with eps = 0 too)
   const bool flat = t.rows <= t.cols;
   const int across = (flat ? t.np : t.mp) / 64, block = blockIdx.x - g.first[who];
   const int r0 = block / across * 64, k0 = block % across * 64, k = threadIdx.x & 63;

@@ -54,7 +54,8 @@ Engine::Engine(const cavs_session_config &cfg, void *external_stream, std::share
   if (cfg.loss == CAVS_LOSS_SOFTMAX && cfg.C <= 0) fail(CAVS_EINVAL, "class count must be positive");
   if (cfg.vocab_head < 0 || cfg.vocab_head > 1 || (cfg.vocab_head && cfg.loss != CAVS_LOSS_SOFTMAX))
     fail(CAVS_EINVAL, "vocab_head is 0 or 1, and 1 goes with the softmax loss");
-  if (cfg.optimizer < 0 || cfg.optimizer > 1 || (cfg.optimizer && cell_)) fail(CAVS_EINVAL, "unknown optimizer");
+  if (cfg.optimizer < 0 || cfg.optimizer > 1) fail(CAVS_EINVAL, "unknown optimizer");
+  if (cfg.optimizer && cell_) fail(CAVS_EINVAL, "the optimizer of orthogonalised updates goes with the built-in models");
   if (!(cfg.ortho_lr >= 0.f) || !(cfg.ortho_momentum < 1.f) || !(cfg.ortho_decay >= 0.f))
     fail(CAVS_EINVAL, "ortho_lr and ortho_decay are not negative, ortho_momentum is below 1");
   check(cavs_init(cfg.device));

@@ -240,6 +240,25 @@ def test_nothing_and_no_numbers(type_):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("eps", [0.0, 1e-7])
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+def test_no_gradient_and_no_momentum(type_, eps):
+    """U = 0 has no norm to divide by: X is 0, momentum and weights only decay."""
+    c = Case(9, type_, [(40, 70), (1, 1), (70, 40)], momentum=True, weights=True)
+    for i in (0, 1):
+        c.G[i][:] = 0
+        c.M[i][:] = 0
+    W0 = [w.clone() for w in c.W]
+    o = options(eps=eps)
+    c.run(o)
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert (c.O[i] == 0).all() and (c.M[i] == 0).all()
+        assert ((c.W[i].double() - (1 - o.lr * o.weight_decay) * W0[i].double()).abs() <= 2 * U * W0[i].abs().double()).all()
+    assert c.O[2].isfinite().all() and (c.O[2] != 0).any() and c.W[2].isfinite().all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("type_", ["f32", "bf16"])
 def test_in_place_of_the_gradient(type_):
     c = Case(8, type_, [(90, 130), (130, 90)])

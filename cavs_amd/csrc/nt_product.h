@@ -88,10 +88,28 @@ __device__ __forceinline__ void nt_arrive() {
   asm volatile("" ::: "memory");
 }
 
+// A piece (eight k of row l % 32) from where its half blocks of sixteen rows lie, one `parts` half blocks after the other
+__device__ __forceinline__ bf16x8 turned_piece(const char *from, int lane, int parts) {
+  const int group = lane >> 4 & 1, half = lane >> 5;
+  const char *p = from + group * parts * 512 + half * 256 + 8 * (lane & 15);
+#ifdef __HIP_DEVICE_COMPILE__
+  typedef short four __attribute__((ext_vector_type(4)));
+  const four lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) four *)(p + 128 * (half ^ group)));
+  const four hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) four *)(p + 128 * (half ^ group ^ 1)));
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#else
+  return *reinterpret_cast<const bf16x8 *>(p);
+#endif
+}
+
 // acc[ACC][TM][TN] of the tile at rows m0 of A and n0 of B over k in [kbeg, kend), both multiples of BK.  S: T::LDS bytes.
+// TURNED: what is given is A^T, packed with A's rows as its k and with all of A's k as rows (its last block of rows whole, and as many as kend
+// asks for).  A step's half blocks of 16 of its rows by 16 k, 512 bytes, come to LDS row by row, and the transposing load makes of four neighbouring
+// values of four rows, sixteen lanes at a time, four k of sixteen rows of A.  (Bit 7 of a place is turned over by bit 3 of the row and
+// bit 4 of k: of the four groups of lanes no two that could go together meet in a bank.)
 // NS stages in a ring: while one is multiplied the others are on their way from memory; a step's one barrier says that the stage to come
 // has arrived and that nobody reads the one before it any more, so that its place takes the load of the stage NS - 1 ahead.
-template <class T>
+template <class T, bool TURNED = false>
 __device__ __forceinline__ void nt_multiply(const PackedRef &A, int M, int m0, const PackedRef &B, int N, int n0, int kbeg, int kend, char *S,
                                             floatx16 (&acc)[T::ACC][T::TM][T::TN]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -108,29 +126,40 @@ __device__ __forceinline__ void nt_multiply(const PackedRef &A, int M, int m0, c
   // Blocks c = 0, 1, .. of a stage, in the order they have in memory: row of blocks by row of blocks, step by step, part by part.  This wavefront
   // loads every WAVES-th, each lane the 16 bytes it will read.
   constexpr int PER = T::P * T::STEPS;
-  unsigned sa[T::CA], sb[T::CB];
+  unsigned sa[T::CA], sb[T::CB], la[T::CA];
   const long rowa = (long)(A.K / 16) * T::P * 1024, rowb = (long)(B.K / 16) * T::P * 1024;
 #pragma unroll
   for (int c = 0; c < T::CA; c++) {
     const int at = c * T::WAVES + wave;
-    sa[c] = (unsigned)min(at / PER, (M - 1 - m0) / 32) * (unsigned)rowa + at % PER * 1024;
+    if constexpr (!TURNED) {
+      la[c] = 16 * lane;
+      sa[c] = (unsigned)min(at / PER, (M - 1 - m0) / 32) * (unsigned)rowa + at % PER * 1024;
+    } else {
+      constexpr int PAIRS = T::BM / 32 * T::P;  // of half blocks, a step's
+      const int step = at / PAIRS, unit = at % PAIRS * 2 + (lane >> 5), col = unit / T::P, place = lane & 31;
+      const int here = place ^ 8 * ((place >> 4) ^ (col & 1));
+      la[c] = (min(col, A.K / 16 - 1 - m0 / 16) * T::P + unit % T::P) * 1024 + (here & 1) * 512 + (here >> 1) * 16;
+      sa[c] = (step >> 1) * (unsigned)rowa + (step & 1) * 256;
+    }
   }
 #pragma unroll
   for (int c = 0; c < T::CB; c++) {
     const int at = c * T::WAVES + wave;
     sb[c] = (unsigned)min(at / PER, (N - 1 - n0) / 32) * (unsigned)rowb + at % PER * 1024;
   }
-  [[maybe_unused]] const char *pa = reinterpret_cast<const char *>(A.p) + m0 / 32 * rowa + (long)(kbeg / 16) * (T::P * 1024);
+  [[maybe_unused]] const char *pa = reinterpret_cast<const char *>(A.p) + (TURNED ? kbeg / 32 * rowa + (long)(m0 / 16) * (T::P * 1024)
+                                                                                : m0 / 32 * rowa + (long)(kbeg / 16) * (T::P * 1024));
   [[maybe_unused]] const char *pb = reinterpret_cast<const char *>(B.p) + n0 / 32 * rowb + (long)(kbeg / 16) * (T::P * 1024);
 
   auto fetch = [&](int kt, char *to) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass knows no such load)
-    const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pa), 0, 0xffffffffu, 0x00020000);
+    const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(TURNED ? pa + (long)(kt * T::STEPS / 2) * rowa : pa), 0, 0xffffffffu, 0x00020000);
+    const unsigned offa = TURNED ? kt * T::STEPS % 2 * 256 : (unsigned)kt * (PER * 1024);
     const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pb), 0, 0xffffffffu, 0x00020000);
     const unsigned off = (unsigned)kt * (PER * 1024);
 #pragma unroll
     for (int c = 0; c < T::CA; c++)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void *)(to + (c * T::WAVES + wave) * 1024), 16, 16 * lane, sa[c] + off, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void *)(to + (c * T::WAVES + wave) * 1024), 16, la[c], sa[c] + offa, 0, 0);
 #pragma unroll
     for (int c = 0; c < T::CB; c++)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void *)(to + T::PA + (c * T::WAVES + wave) * 1024), 16, 16 * lane, sb[c] + off,
@@ -145,7 +174,10 @@ __device__ __forceinline__ void nt_multiply(const PackedRef &A, int M, int m0, c
 #pragma unroll
     for (int p = 0; p < T::P; p++) {
 #pragma unroll
-      for (int i = 0; i < T::TM; i++) f.a[i][p] = *reinterpret_cast<const bf16x8 *>(from + a0 + (i * T::ROWB + (s * T::P + p) * 1024));
+      for (int i = 0; i < T::TM; i++) {
+        if constexpr (!TURNED) f.a[i][p] = *reinterpret_cast<const bf16x8 *>(from + a0 + (i * T::ROWB + (s * T::P + p) * 1024));
+        else f.a[i][p] = turned_piece(from + (wm * (T::WM / 16) + 2 * i) * T::P * 512 + (s * (T::BM / 16) * T::P + p) * 512, lane, T::P);
+      }
 #pragma unroll
       for (int j = 0; j < T::TN; j++) f.b[j][p] = *reinterpret_cast<const bf16x8 *>(from + b0 + (j * T::ROWB + (s * T::P + p) * 1024));
     }

@@ -469,13 +469,12 @@ __global__ __launch_bounds__(256) void weights_kernel(const float *__restrict__ 
   if (row < n) weight[row] = weight_of(labels[row], lse[row], dloss, row, C);
 }
 
-// d of a tile: e = p - [label] for the product with W, by token, and e times the token's weight for that with X, by class (zero between the last
-// class or token and the end of the steps); and the sums of the latter over the tile's tokens.
-// What multiplies all of a row's d, or all of d, stays out of what is rounded: next to the label, where p is small, e is -1 and a bit, which bf16
-// holds well, while any factor in it is a rounding error that all of its kind share.
+// d of a tile, weight * (p - [label]), packed by token (zero between the last class or token and the end of the steps), and its sums over the
+// tile's tokens.  `scale`, which multiplies all of d, stays out of what is rounded: next to the label, where p is small, p - 1 is -1 and a bit, which bf16
+// holds well, while a factor in it is a rounding error that all of its kind share.
 template <class T>
 __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, const float *__restrict__ lse, const float *__restrict__ weight, PackedOut d,
-                                                                    PackedOut t, float *__restrict__ sums, int ld_sums, float sums_scale) {
+                                                                    float *__restrict__ sums, int ld_sums, float sums_scale) {
   __shared__ __attribute__((aligned(16))) char S[T::LDS];
   int m0, n0, tn;
   floatx16 acc[T::ACC][T::TM][T::TN];
@@ -483,8 +482,8 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, 
   float *lb = reinterpret_cast<float *>(S);
   float *part = lb + T::BM;  // [WGN][BM]
   const Where<T> w;
-  char *turn = S + 4 * T::BM * (1 + T::WGN) + (threadIdx.x >> 6) * kTurn;
-  static_assert(4 * T::BM * (1 + T::WGN) + T::WAVES * kTurn <= T::LDS, "");
+  static_assert(4 * T::BM * (1 + T::WGN) <= T::LDS, "");
+  const int tokens = (a.n + kPlaneAlign - 1) / kPlaneAlign * kPlaneAlign;
   biases_of_tile<T>(acc, a.bias, m0, a.M, lb);
   int at[T::TN];
   float g[T::TN], all[T::TN];
@@ -510,21 +509,17 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, 
 #pragma unroll
         for (int r = 0; r < 16; r++) x[r] -= at[j] == 32 * i + 8 * (r >> 2) + (r & 3) ? 1.f : 0.f;
       }
-      Parts16<T::P> e;
-      if (d.p && 32 * xb < a.n && 32 * cb < d.K) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) x[r] *= g[j], sum[r] += x[r];
+      if (d.p && 32 * xb < tokens && 32 * cb < d.K) {
+        Parts16<T::P> e;
 #pragma unroll
         for (int r = 0; r < 16; r++) parts_of<T::P>(x[r], e.v[r]);
         put_rows<T::P>(d, xb, cb, e, w.lane);
-      }
-#pragma unroll
-      for (int r = 0; r < 16; r++) x[r] *= g[j], sum[r] += x[r];
-      if (t.p && 32 * cb < a.M && 32 * xb < t.K) {
-#pragma unroll
-        for (int r = 0; r < 16; r++) parts_of<T::P>(x[r], e.v[r]);
-        put_columns<T::P>(t, cb, xb, e, w.lane, turn);
-        if (T::BN < kPlaneAlign && 32 * (xb + 1) >= a.n && 32 * (xb + 1) < t.K) {  // (a tile that ends in front of the padding)
-          Parts16<T::P> zero = {};
-          put_columns<T::P>(t, cb, xb + 1, zero, w.lane, turn);
+        asm volatile("" ::: "memory");  // (one block after the other: a lane has no registers for two)
+        if (T::BN < kPlaneAlign && 32 * (xb + 1) >= a.n && 32 * (xb + 1) < tokens) {  // (a tile that ends in front of the padding)
+          const Parts16<T::P> zero = {};
+          put_rows<T::P>(d, xb + 1, cb, zero, w.lane);
         }
       }
     }
@@ -699,8 +694,8 @@ __global__ __launch_bounds__(256, 2) void few_dx_kernel(FewArgs a) {
 }
 
 // ------------------------------------------------------------------ the products with d
-// out[row, col] = scale * factor[row] * A B^T.  K in `splits` stretches of kchunk, each with sums of its own (unscaled) at part + split * M * N; part null:
-// straight to out.
+// out[row, col] = scale * A B^T.  K in `splits` stretches of kchunk, each with sums of its own (unscaled) at part + split * M * N; part null:
+// straight to out.  A launch is d W, d's rows the tile's rows, and d^T X, d's classes the tile's rows and its tokens what is summed over.
 template <class Out>
 struct ProductJob {
   PackedRef A, B;
@@ -710,7 +705,6 @@ struct ProductJob {
   Out *out;
   long ldo;
   float scale;
-  const float *factor;  // of out's rows, or null
 };
 
 template <class T, class Out>
@@ -723,7 +717,8 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void product_kernel(ProductJob<O
   nt_tile_of(block - split * tiles, g.tilesM, g.tilesN, &tm, &tn);
   const int m0 = tm * T::BM, n0 = tn * T::BN, kbeg = split * g.kchunk, kend = min(g.K, kbeg + g.kchunk);
   floatx16 acc[T::ACC][T::TM][T::TN];
-  nt_multiply<T>(g.A, g.M, m0, g.B, g.N, n0, kbeg, kend, S, acc);
+  if (second) nt_multiply<T, true>(g.A, g.M, m0, g.B, g.N, n0, kbeg, kend, S, acc);
+  else nt_multiply<T>(g.A, g.M, m0, g.B, g.N, n0, kbeg, kend, S, acc);
   const Where<T> w;
   float *part = g.part ? g.part + (long)split * g.M * g.N : nullptr;
 #pragma unroll
@@ -742,17 +737,16 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void product_kernel(ProductJob<O
           float *o = part + (long)row * g.N + col;
           *o = g.add ? *o + x : x;
         } else {
-          store_as(g.out + row * g.ldo + col, (g.factor ? g.scale * g.factor[row] : g.scale) * x);
+          store_as(g.out + row * g.ldo + col, g.scale * x);
         }
       }
   }
 }
 
-// out[r, 0 .. w) = scale * factor[r] * sum of `parts` pieces, in their order
+// out[r, 0 .. w) = scale * sum of `parts` pieces, in their order
 struct SumJob {
   const float *part;
   int parts, rows, w;
-  const float *factor;
   void *out;
   long ldo;
   int blocks;
@@ -771,7 +765,7 @@ __device__ inline void sum_parts(const SumJob &g, float scale, int block) {
       for (int k = 0; k < 8; k++) s += v[k];
     }
     const long r = i / g.w;
-    store_as(out + r * g.ldo + (i - r * g.w), (g.factor ? scale * g.factor[r] : scale) * s);
+    store_as(out + r * g.ldo + (i - r * g.w), scale * s);
   }
 }
 // d X, d W and d b (fp32) of what the launches before left in parts
@@ -844,10 +838,40 @@ struct Call {
   int n, H, C;
 };
 
-constexpr int kPieceBytes = 256 << 20;  // d of a piece, in both orders
+constexpr int kPieceBytes = 256 << 20;  // d of a piece, where it is not all of d
+// d at once: W is packed once then, and d W goes without sums from piece to piece (bf16 50000 x 2048, 4096 tokens, 410 MB: 3219 us, in two
+// pieces 3454; fp32 10000 x 512, 7088 tokens, 427 MB: 1592 us, 1622)
+constexpr int kWholeBytes = 512 << 20;
 constexpr size_t kKeepBytes = 512 << 20;  // of W packed: kept from the first pass for the second
 constexpr int kSplits = 64;
 constexpr int kDirectRows = 64, kFewRows = 64, kRawRows = 256;
+
+// What the two products of a piece take, us, with their K in so many stretches.  Workgroups go to the compute unit that is free first, those of d W
+// before those of d^T X; a unit multiplies at one speed whatever it holds, but for the end, where a long workgroup is left alone.  Each
+// costs 256 k more than it multiplies, and what they leave in parts is written and read at the rate of a copy.
+struct Stretches {
+  int tiles, K, chunk, n;
+  void set(int s) { chunk = ceil_to((K + s - 1) / s, kPlaneAlign), n = (K + chunk - 1) / chunk; }
+};
+inline double products_us(const Stretches &x, const Stretches &w, double us_per_k, double part_bytes) {
+  const long cus = num_cus(), nx = (long)x.tiles * x.n, nw = (long)w.tiles * w.n, a = x.chunk + 256, b = w.chunk + 256;
+  const long more = nx % cus, low = nx / cus * a, high = low + a;  // `more` units with one of d W's more than the others
+  long t = nx > 0 && more == 0 ? low : nx > 0 ? high : 0;
+  if (nw > 0) {
+    const long mean = (nx * a + nw * b) / cus;
+    long i = mean > low ? (mean - low) / b : 0, j = mean > high ? (mean - high) / b : 0;
+    for (;;) {  // the first moment by which all of d^T X's have ended
+      const long ti = low + i * b, tj = high + j * b, at = ti < tj ? ti : tj;
+      if (more * (at > high ? (at - high) / b : 0) + (cus - more) * (at > low ? (at - low) / b : 0) >= nw) {
+        t = at > t ? at : t;
+        break;
+      }
+      i += ti == at, j += tj == at;
+    }
+  }
+  const double longest = a > b && nx > 0 ? a : b, alone = longest - (t - longest) / 2;
+  return (t + (alone > 0 ? 1.5 * alone : 0.)) * us_per_k + part_bytes / 4.7e6;
+}
 
 // Sizes and places of a call's workspace.
 struct Plan {
@@ -856,7 +880,7 @@ struct Plan {
   int raw;      // not many: W read where it lies
   int facross;  // few_dx_kernel's
   int grads, keep, psize, pm, pn, xsplits, xchunk, wsplits, wchunk;
-  size_t stats, zlabel, lse, weight, x, w, xt, wt, d, dt, sums, xpart, wpart, bytes;
+  size_t stats, zlabel, lse, weight, x, w, xt, wt, d, sums, xpart, wpart, bytes;
 };
 
 template <int P>
@@ -864,7 +888,7 @@ Plan plan_of(int n, int H, int C, int grads) {
   Plan p{};
   p.P = P, p.grads = grads;
   p.Hp = ceil_to(H, kPlaneAlign), p.np = ceil_to(n, kPlaneAlign);
-  long most = grads ? kPieceBytes / (4l * P * p.np) : (128l << 20) / (2l * P * p.Hp);
+  long most = grads ? ((long)C * 2 * P * p.np <= kWholeBytes ? kWholeBytes : kPieceBytes) / (2l * P * p.np) : (128l << 20) / (2l * P * p.Hp);
   most = most < 1024 ? 1024 : most > 1 << 20 ? 1 << 20 : most;
   p.pieces = (int)((C + most - 1) / most);
   p.piece = ceil_to((C + p.pieces - 1) / p.pieces, 256);
@@ -899,18 +923,28 @@ Plan plan_of(int n, int H, int C, int grads) {
     const int rp = ceil_to(rows, kPlaneAlign);
     p.psize = tile_size<P>((long)rows + n, H);
     tile_sides<P>(p.psize, &p.pm, &p.pn);
-    // few tiles: K in several stretches, none of them short
-    auto split = [&](long tiles, int K, int *chunk) {
-      int s = (int)(2 * num_cus() / (tiles > 0 ? tiles : 1));
-      s = 2 * tiles > num_cus() ? 1 : s;
-      s = s > kSplits ? kSplits : s;
-      s = s > K / 512 ? K / 512 : s;
-      s = s < 1 ? 1 : s;
-      *chunk = ceil_to((K + s - 1) / s, kPlaneAlign);
-      return (K + *chunk - 1) / *chunk;
+    // What the model finds best, of all sizes up to eight workgroups a compute unit.  us of a call, this / all at once, with 2 CUs / tiles
+    // stretches where tiles are fewer than half the CUs: fp32 10000 x 512, 7088 tokens 1628 / 1733; 21701 x 300, 1000 tokens 396 / 419; 8000 x 64, 4000
+    // tokens 194 / 210; 45376 x 1024, 96 tokens 486 / 513; bf16 25040 x 1000, 2371 tokens 614 / 618; 3000 x 128, 7000 tokens 93 / 97.  (The best
+    // of a sweep is up to 3 % faster.)
+    Stretches x{p.raw ? 0 : tiles_of(n, p.pm) * tiles_of(H, p.pn), rp, rp, 1}, w{tiles_of(rows, p.pm) * tiles_of(H, p.pn), p.np, p.np, 1};
+    const double us_per_k = 2. * p.pm * p.pn * (P == 3 ? 6 / 1450e6 : 1 / 1300e6) * num_cus();  // (the pipe's rates that large products reach)
+    auto most_of = [&](const Stretches &g) {
+      const int s = 8 * num_cus() / (g.tiles > 0 ? g.tiles : 8 * num_cus());
+      return s < kSplits ? s : kSplits;
     };
-    p.xsplits = split((long)tiles_of(n, p.pm) * tiles_of(H, p.pn), rp, &p.xchunk);
-    p.wsplits = split((long)tiles_of(rows, p.pm) * tiles_of(H, p.pn), p.np, &p.wchunk);
+    double best = INFINITY;
+    const int sizes[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+    for (int sx : sizes)
+      for (int sw : sizes) {
+        if ((sx > 1 && sx > most_of(x)) || (sw > 1 && sw > most_of(w))) break;
+        x.set(sx), w.set(sw);
+        double bytes = 0.;
+        if (p.pieces > 1 || x.n > 1) bytes += x.n * (4. * n * H) * (1. + (p.pieces > 1) + 1. / p.pieces);
+        if (w.n > 1) bytes += w.n * (8. * rows * H);
+        const double us = products_us(x, w, us_per_k, bytes);
+        if (us < best) best = us, p.xsplits = x.n, p.xchunk = x.chunk, p.wsplits = w.n, p.wchunk = w.chunk;
+      }
     if (p.raw) {
       p.facross = tiles_of(H, 32 * (n <= 32 ? few_columns<P, 1>() : few_columns<P, 2>()));
       // stretches for three workgroups a compute unit, of 256 classes or more
@@ -922,8 +956,7 @@ Plan plan_of(int n, int H, int C, int grads) {
     }
     p.xt = take(packed_bytes<P>(H, p.np));
     p.wt = take(p.raw ? 0 : packed_bytes<P>(H, rp));
-    p.d = take(packed_bytes<P>(n, rp));
-    p.dt = take(packed_bytes<P>(rows, p.np));
+    p.d = take(packed_bytes<P>(p.np, rp));
     p.sums = take((size_t)tiles_of(n, p.bn) * C * 4);
     p.xpart = take((size_t)p.xsplits * n * H * 4);
     p.wpart = take(p.wsplits > 1 ? (size_t)p.wsplits * rows * H * 4 : 0);
@@ -1013,23 +1046,23 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
       if (!here) pack<P, Src>(jx, job_w(c0, c.lse_given || !keep, true), st);
       jx = PackJob{};
       const TileArgs a = tile_args(c0);
-      const PackedOut d{c.dX ? pl(p.d) : nullptr, rp}, dt{c.dW ? pl(p.dt) : nullptr, p.np}, wt = piece_wt(rows);
+      const PackedOut d{c.dX || c.dW ? pl(p.d) : nullptr, rp}, wt = piece_wt(rows);
       if (c.dX || c.dW || c.db)
         with_tile<P, true>(p.size, [&](auto t) {
           using T = decltype(t);
-          launch(dlogits_kernel<T>, a.tilesM * a.tilesN, T::THREADS, 0, st, a, all, weight, d, dt, !c.db ? nullptr : b_parts ? f32(p.sums) + c0 : c.db + c0, C,
+          launch(dlogits_kernel<T>, a.tilesM * a.tilesN, T::THREADS, 0, st, a, all, weight, d, !c.db ? nullptr : b_parts ? f32(p.sums) + c0 : c.db + c0, C,
                  b_parts ? 1.f : c.scale);
           return 0;
         });
-      auto job = [&](const PackedOut &A, const PackedOut &B, int M, int K, int chunk, float *part, bool add, void *out, long ldo, const float *factor) {
+      auto job = [&](const PackedOut &A, const PackedOut &B, int M, int K, int chunk, float *part, bool add, void *out, long ldo) {
         return ProductJob<Src>{ref(A), ref(B), M, H, K, tiles_of(M, p.pm), tiles_of(H, p.pn), (K + chunk - 1) / chunk, chunk, part, add,
-                               static_cast<Src *>(out), ldo, c.scale, factor};
+                               static_cast<Src *>(out), ldo, c.scale};
       };
       ProductJob<Src> px{}, pw{};
       // (a last piece shorter than the others fills fewer stretches: those beyond keep what they have)
-      if (c.dX && !p.raw) px = job(d, wt, n, rp, p.xchunk, x_parts ? f32(p.xpart) : nullptr, !first, c.dX, c.lddx, weight);
+      if (c.dX && !p.raw) px = job(d, wt, n, rp, p.xchunk, x_parts ? f32(p.xpart) : nullptr, !first, c.dX, c.lddx);
       Src *dW = c.dW ? static_cast<Src *>(c.dW) + (long)c0 * c.lddw : nullptr;
-      if (c.dW) pw = job(dt, xt, rows, p.np, p.wchunk, w_parts ? f32(p.wpart) : nullptr, false, dW, c.lddw, nullptr);
+      if (c.dW) pw = job(d, xt, rows, p.np, p.wchunk, w_parts ? f32(p.wpart) : nullptr, false, dW, c.lddw);
       const int bx = c.dX && !p.raw ? px.tilesM * px.tilesN * px.splits : 0, bw = c.dW ? pw.tilesM * pw.tilesN * pw.splits : 0;
       if (bx + bw > 0)
         with_product_tile<P>(p.psize, [&](auto t) {
@@ -1046,9 +1079,9 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
       }
       const bool last = c0 + p.piece >= C;
       SumJob sx{}, sw{}, sb{};
-      if (last && c.dX && x_parts) sx = {f32(p.xpart), p.xsplits, n, H, weight, c.dX, c.lddx, 0};
-      if (dW && w_parts) sw = {f32(p.wpart), p.wsplits, rows, H, nullptr, dW, c.lddw, 0};
-      if (last && c.db && b_parts) sb = {f32(p.sums), token_tiles, 1, C, nullptr, c.db, C, 0};
+      if (last && c.dX && x_parts) sx = {f32(p.xpart), p.xsplits, n, H, c.dX, c.lddx, 0};
+      if (dW && w_parts) sw = {f32(p.wpart), p.wsplits, rows, H, dW, c.lddw, 0};
+      if (last && c.db && b_parts) sb = {f32(p.sums), token_tiles, 1, C, c.db, C, 0};
       sums<Src>(sx, sw, sb, c.scale, st);
     }
   }
@@ -1072,7 +1105,7 @@ int check_and_run(const char *who, int type, const Call &c, int grads, void *ws,
   CAVS_REQUIRE(c.W && (c.n == 0 || (c.X && c.labels)), "%s: null pointer", who);
   if (c.n == 0) {  // sums over no rows
     hipStream_t st = as_stream(stream);
-    const SumJob w{nullptr, 0, c.C, c.H, nullptr, c.dW, c.lddw, 0}, b{nullptr, 0, 1, c.C, nullptr, c.db, c.C, 0};
+    const SumJob w{nullptr, 0, c.C, c.H, c.dW, c.lddw, 0}, b{nullptr, 0, 1, c.C, c.db, c.C, 0};
     if (type == CAVS_F32) sums<float>({}, w, b, 0.f, st);
     else sums<u16>({}, w, b, 0.f, st);
     CAVS_LAUNCH_CHECK();

@@ -341,6 +341,8 @@ __device__ inline void load_tile(PackTile &tile, const Src *src, long ld, int r0
 }
 
 __device__ inline void store_as(float *o, float x) { *o = x; }
+__device__ inline void stream_as(float *o, float x) { __builtin_nontemporal_store(x, o); }
+__device__ inline void stream_as(u16 *o, float x) { __builtin_nontemporal_store(bf16_bits(x), o); }
 __device__ inline void store_as(u16 *o, float x) { *o = bf16_bits(x); }
 
 constexpr int ceil_to(int x, int to) { return (x + to - 1) / to * to; }

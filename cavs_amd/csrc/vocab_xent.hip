@@ -4,8 +4,9 @@
 //   dX = d W,  dW = d^T X,  db = sums of d's columns
 //
 // The vocabulary goes by in pieces.  The first pass over them makes each tile of z in registers and leaves a maximum and a sum of
-// exponentials per row and tile; what they come to together is lse.  The second makes the tile again, d from it, and leaves d of a piece
-// (packed for its two products, by token and by class), which d X and d W are made of before the next piece overwrites it.
+// exponentials per row and tile; what they come to together is lse.  The second makes the tile again, d from it, and leaves d of a piece,
+// packed by token, which d X and d W are made of before the next piece overwrites it.  (d^T is read from the same bytes: packed in both orders, half
+// as many classes to a piece, fp32 10000 x 512 with 7088 tokens took 1869 us, and takes 1608.)
 // Statistics, sums and accumulators are fp32; d is rounded to bf16 where the gradients are (half a unit of 2^-8, as their own
 // rounding), and is three bf16 parts, all of an fp32's bits, where they are fp32.
 #include <type_traits>
@@ -105,8 +106,8 @@ struct RawRow<float> {
   }
 };
 
-// A tile whose rows of W are read where they lie: four wavefronts of 32 classes each, 32 TN tokens.  For tokens so few that packing W, which writes and
-// reads half as much again (bf16) or three times as much (fp32), would be most of the work.
+// A tile whose rows of W are read where they lie: four wavefronts of 32 classes each, 32 TN tokens.  For losses alone, of tokens so few that packing W, which
+// writes and reads half as much again (bf16) or three times as much (fp32), would be most of the work.
 template <int P_, int TN_>
 struct RawTile {
   static constexpr bool RAW = true;
@@ -325,7 +326,7 @@ struct DirectArgs {
   int H, C, n, blocks;  // blocks: of 32 classes
   const float *bias, *labels;
   float2 *stats;  // a row of n for every workgroup
-  float *zlabel;
+  float *zlabel, *z;  // z: null, or all of it for the gradients, block of 32 classes by block of 32 tokens by wavefront by lane
 };
 template <int P, class Src, int TN, bool PACKED>
 __global__ __launch_bounds__(256, P == 1 ? 4 : 2) void direct_stats_kernel(DirectArgs a) {
@@ -411,6 +412,7 @@ __global__ __launch_bounds__(256, P == 1 ? 4 : 2) void direct_stats_kernel(Direc
         top = fmaxf(top, z[k]);
         if (is_class(label, a.C) && (int)label == c + k) a.zlabel[token] = z[k];
       }
+      if (a.z) *reinterpret_cast<float4 *>(a.z + (((long)block * TN + j) * 4 + wave) * 256 + 4 * lane) = make_float4(z[0], z[1], z[2], z[3]);
       top = fmaxf(top, __shfl_xor(top, 32));
       const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
@@ -517,10 +519,6 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, 
         for (int r = 0; r < 16; r++) parts_of<T::P>(x[r], e.v[r]);
         put_rows<T::P>(d, xb, cb, e, w.lane);
         asm volatile("" ::: "memory");  // (one block after the other: a lane has no registers for two)
-        if (T::BN < kPlaneAlign && 32 * (xb + 1) >= a.n && 32 * (xb + 1) < tokens) {  // (a tile that ends in front of the padding)
-          const Parts16<T::P> zero = {};
-          put_rows<T::P>(d, xb + 1, cb, zero, w.lane);
-        }
       }
     }
     if (!sums) continue;
@@ -543,7 +541,61 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, 
   }
 }
 
-// ------------------------------------------------------------------ d X of few tokens
+// ------------------------------------------------------------------ the gradients of few tokens
+// d of up to 64 tokens from the z that direct_stats_kernel left (a float a token and class, beside W's row of H), packed as dlogits_kernel packs it,
+// and its sums over the tokens.  A wavefront has a block of 32 classes.
+struct FewLogitsArgs {
+  const float *z;
+  const float *lse, *weight, *labels;
+  int n, C, c0;
+  PackedOut d;  // null: not wanted; of the piece that begins with class c0
+  int blocks;   // of 32 classes
+  float *sums;  // of the piece, or null
+  float scale;  // of the sums
+};
+template <int P>
+__global__ __launch_bounds__(256) void few_dlogits_kernel(FewLogitsArgs a) {
+  const int lane = threadIdx.x & 63, x = lane & 31, half = lane >> 5, cb = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (cb >= a.blocks) return;
+  const int c = a.c0 + 32 * cb, TN = (a.n + 31) / 32;
+  float sum[16] = {};
+#pragma unroll
+  for (int j = 0; j < kPlaneAlign / 32; j++) {
+    const int token = 32 * j + x;
+    float e[16] = {};
+    if (j < TN && c < a.C) {
+      const bool in = token < a.n;
+      const float g = in ? a.weight[token] : 0.f, all = in ? a.lse[token] : 0.f, label = in ? a.labels[token] : -1.f;
+      const int at = is_class(label, a.C) ? (int)label - c - 4 * half : -1;
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const float4 z = *reinterpret_cast<const float4 *>(a.z + (((long)(c / 32) * TN + j) * 4 + q) * 256 + 4 * lane);
+        const float v[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          e[4 * q + k] = g == 0.f ? 0.f : g * (__expf(v[k] - all) - (at == 8 * q + k ? 1.f : 0.f));
+          sum[4 * q + k] += e[4 * q + k];
+        }
+      }
+    }
+    if (a.d.p) {
+      Parts16<P> o;
+#pragma unroll
+      for (int r = 0; r < 16; r++) parts_of<P>(e[r], o.v[r]);
+      put_rows<P>(a.d, j, cb, o, lane);
+    }
+  }
+  if (!a.sums) return;
+#pragma unroll
+  for (int r = 0; r < 16; r++) {
+    float v = sum[r];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    const int row = 8 * (r >> 2) + 4 * half + (r & 3);
+    if (x == 0 && c + row < a.C) a.sums[32 * cb + row] = a.scale * v;
+  }
+}
+
 // Sums over classes of d times W, W's rows read where they lie, once: what bounds it is memory.  A lane has F neighbouring columns of eight classes
 // of a step, a load of 4 F or 2 F bytes each; the instruction takes its eight classes of one column at a time, so those are F operands, of
 // columns F apart, by renaming registers.  A workgroup has 32 F columns, up to 32 TN tokens and a stretch of the classes, of which each wavefront takes
@@ -707,7 +759,8 @@ struct ProductJob {
   float scale;
 };
 
-template <class T, class Out>
+// STREAM: `out` goes past the caches
+template <class T, class Out, bool STREAM>
 __global__ __launch_bounds__(T::THREADS, T::EU) void product_kernel(ProductJob<Out> j0, ProductJob<Out> j1, int blocks0) {
   __shared__ __attribute__((aligned(16))) char S[T::LDS];
   const bool second = (int)blockIdx.x >= blocks0;
@@ -736,6 +789,8 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void product_kernel(ProductJob<O
         if (part) {
           float *o = part + (long)row * g.N + col;
           *o = g.add ? *o + x : x;
+        } else if constexpr (STREAM) {
+          stream_as(g.out + row * g.ldo + col, g.scale * x);
         } else {
           store_as(g.out + row * g.ldo + col, g.scale * x);
         }
@@ -798,21 +853,15 @@ int with_product_tile(int size, F &&f) {
   if (size == 1) return f(typename TT::M{});
   return f(typename TT::S{});
 }
-// sizes 0 .. 2: packed operands, small to large; 3 .. 5: W as it lies, 32 (fp32), 64 and 128 (bf16, losses alone) tokens
-template <int P, bool GRADS, class F>
+// sizes 0 .. 2: packed operands, small to large; 3: W as it lies
+template <int P, class F>
 int with_tile(int size, F &&f) {
-  if constexpr (P == 3) {
-    if (size == 3) return f(RawTile<P, 1>{});
-  }
-  if constexpr (P == 1 && !GRADS) {
-    if (size == 5) return f(RawTile<P, 4>{});
-  }
-  if (size >= 3) return f(RawTile<P, 2>{});
+  if (size == 3) return f(RawTile<P, P == 1 ? 4 : 2>{});
   return with_product_tile<P>(size, f);
 }
 template <int P>
 void tile_sides(int size, int *bm, int *bn) {
-  with_tile<P, false>(size, [&](auto t) { return *bm = decltype(t)::BM, *bn = decltype(t)::BN, 0; });
+  with_tile<P>(size, [&](auto t) { return *bm = decltype(t)::BM, *bn = decltype(t)::BN, 0; });
 }
 // the largest tile that still gives most compute units one
 template <int P>
@@ -844,7 +893,7 @@ constexpr int kPieceBytes = 256 << 20;  // d of a piece, where it is not all of 
 constexpr int kWholeBytes = 512 << 20;
 constexpr size_t kKeepBytes = 512 << 20;  // of W packed: kept from the first pass for the second
 constexpr int kSplits = 64;
-constexpr int kDirectRows = 64, kFewRows = 64, kRawRows = 256;
+constexpr int kFewRows = 64, kRawRows = 256;
 
 // What the two products of a piece take, us, with their K in so many stretches.  Workgroups go to the compute unit that is free first, those of d W
 // before those of d^T X; a unit multiplies at one speed whatever it holds, but for the end, where a long workgroup is left alone.  Each
@@ -876,11 +925,11 @@ inline double products_us(const Stretches &x, const Stretches &w, double us_per_
 // Sizes and places of a call's workspace.
 struct Plan {
   int P, size, bm, bn, Hp, np, piece, pieces, tiles;  // tiles: of the whole vocabulary
-  int direct;  // few tokens: W and X read where they lie
-  int raw;      // not many: W read where it lies
+  int few;  // tokens: W read where it lies, z kept for the gradients
+  int raw;  // losses of not many tokens: W read where it lies
   int facross;  // few_dx_kernel's
   int grads, keep, psize, pm, pn, xsplits, xchunk, wsplits, wchunk;
-  size_t stats, zlabel, lse, weight, x, w, xt, wt, d, sums, xpart, wpart, bytes;
+  size_t stats, zlabel, lse, weight, z, x, w, xt, wt, d, sums, xpart, wpart, bytes;
 };
 
 template <int P>
@@ -894,18 +943,22 @@ Plan plan_of(int n, int H, int C, int grads) {
   p.piece = ceil_to((C + p.pieces - 1) / p.pieces, 256);
   p.pieces = tiles_of(C, p.piece);
   const int rows = p.piece < C ? p.piece : C;
-  // A vocabulary with a tile of 128 classes for every compute unit (for the losses alone, every second) and few tokens: W read where it lies, packing
-  // it would be most of the work.  us packed / as it lies:
-  //   losses, 96 and 256 tokens: bf16 124416 x 2176 361 / 283, 423 / 313, 45376 x 1024 53 / 33, 74 / 42, 21701 x 300 20 / 18, 23 / 19, 10000 x 512
-  //   20 / 20, 23 / 21; fp32 45376 x 1024 171 / 139, 217 / 181, 21701 x 300 31 / 27, 42 / 40, 1000 x 128 13 / 15
-  //   with gradients, 1 and 64 tokens: fp32 45376 x 1024 425 / 235, 443 / 287, 81792 x 72 141 / 105, 160 / 124, 21701 x 300 83 / 88, 90 / 98;
-  //   bf16 124416 x 2176 917 / 679, 924 / 642, 45376 x 1024 181 / 122, 199 / 134, 81792 x 72 99 / 91, 10000 x 512 49 / 54; 96 tokens: as packed
-  p.raw = grads ? n <= kFewRows && C >= 128 * num_cus() : n <= kRawRows && C >= 64 * num_cus();
-  p.size = !p.raw ? tile_size<P>(rows, n) : P == 3 && n <= 32 ? 3 : P == 1 && n > 64 ? 5 : 4;
+  // Few tokens: W read where it lies and z kept, packing W and making z twice would be most of the work.  Gradients take two launches more that way, which
+  // long rows or many classes pay for.  us with gradients packed / as it lies, 1, 24 and 64 tokens:
+  //   fp32  300 x 1024 55 / 39, 56 / 42, 57 / 47   1000 x 512 41 / 36, 42 / 38, 43 / 43   12000 x 300 61 / 63, 61 / 66, 63 / 70   12000 x 512 74 / 62, 78 / 66,
+  //         79 / 73   32000 x 128 77 / 65, 81 / 72, 82 / 79   45376 x 1024 425 / 200, 443 / 216 (64)   40806 x 4050 1574 / 823 (12)
+  //   bf16  1000 x 512 29 / 30, 30 / 33, 30 / 41   4000 x 1024 52 / 39, 51 / 42, 52 / 54   12000 x 1024 66 / 54, 68 / 64, 71 / 70   32000 x 128 54 / 55, 57 / 62,
+  //         58 / 60   81792 x 72 93 / 82, 96 / 90, 98 / 95   124416 x 2176 915 / 469 (64)
+  const bool many = C >= 128 * num_cus();
+  p.few = n <= kFewRows && (!grads || many || (P == 3 ? H >= 512 : H >= 1024 && (n <= 32 || (long)C * H >= 12000000)));
+  // Losses of up to 256 tokens under a vocabulary with a tile of 128 classes for every second compute unit.  us packed / as it lies, 96 and 256 tokens:
+  //   bf16 124416 x 2176 361 / 283, 423 / 313, 45376 x 1024 53 / 33, 74 / 42, 21701 x 300 20 / 18, 23 / 19, 10000 x 512 20 / 20, 23 / 21; fp32 45376 x 1024
+  //   171 / 139, 217 / 181, 21701 x 300 31 / 27, 42 / 40, 1000 x 128 13 / 15
+  p.raw = !grads && !p.few && n <= kRawRows && C >= 64 * num_cus();
+  p.size = p.raw ? 3 : tile_size<P>(rows, n);
   tile_sides<P>(p.size, &p.bm, &p.bn);
   p.tiles = tiles_of(C, p.bm);
-  p.direct = !grads && n <= kDirectRows;
-  if (p.direct) p.tiles = tiles_of(C, 32) < 4 * num_cus() ? tiles_of(C, 32) : 4 * num_cus();
+  if (p.few) p.tiles = tiles_of(C, 32) < 4 * num_cus() ? tiles_of(C, 32) : 4 * num_cus();
   p.keep = packed_bytes<P>(C, p.Hp) <= kKeepBytes;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -917,8 +970,9 @@ Plan plan_of(int n, int H, int C, int grads) {
   p.zlabel = take((size_t)n * 4);
   p.lse = take((size_t)n * 4);
   p.weight = take((size_t)n * 4);
-  p.x = take(p.direct && n <= 32 ? 0 : packed_bytes<P>(n, p.Hp));
-  p.w = take(p.direct || p.raw ? 0 : packed_bytes<P>(grads && p.keep ? C : rows, p.Hp));
+  p.z = take(p.few && grads ? (size_t)tiles_of(C, 32) * tiles_of(n, 32) * 4096 : 0);
+  p.x = take(p.few && n <= 32 ? 0 : packed_bytes<P>(n, p.Hp));
+  p.w = take(p.few || p.raw ? 0 : packed_bytes<P>(grads && p.keep ? C : rows, p.Hp));
   if (grads) {
     const int rp = ceil_to(rows, kPlaneAlign);
     p.psize = tile_size<P>((long)rows + n, H);
@@ -927,7 +981,7 @@ Plan plan_of(int n, int H, int C, int grads) {
     // stretches where tiles are fewer than half the CUs: fp32 10000 x 512, 7088 tokens 1628 / 1733; 21701 x 300, 1000 tokens 396 / 419; 8000 x 64, 4000
     // tokens 194 / 210; 45376 x 1024, 96 tokens 486 / 513; bf16 25040 x 1000, 2371 tokens 614 / 618; 3000 x 128, 7000 tokens 93 / 97.  (The best
     // of a sweep is up to 3 % faster.)
-    Stretches x{p.raw ? 0 : tiles_of(n, p.pm) * tiles_of(H, p.pn), rp, rp, 1}, w{tiles_of(rows, p.pm) * tiles_of(H, p.pn), p.np, p.np, 1};
+    Stretches x{p.few ? 0 : tiles_of(n, p.pm) * tiles_of(H, p.pn), rp, rp, 1}, w{tiles_of(rows, p.pm) * tiles_of(H, p.pn), p.np, p.np, 1};
     const double us_per_k = 2. * p.pm * p.pn * (P == 3 ? 6 / 1450e6 : 1 / 1300e6) * num_cus();  // (the pipe's rates that large products reach)
     auto most_of = [&](const Stretches &g) {
       const int s = 8 * num_cus() / (g.tiles > 0 ? g.tiles : 8 * num_cus());
@@ -945,17 +999,17 @@ Plan plan_of(int n, int H, int C, int grads) {
         const double us = products_us(x, w, us_per_k, bytes);
         if (us < best) best = us, p.xsplits = x.n, p.xchunk = x.chunk, p.wsplits = w.n, p.wchunk = w.chunk;
       }
-    if (p.raw) {
+    if (p.few) {
       p.facross = tiles_of(H, 32 * (n <= 32 ? few_columns<P, 1>() : few_columns<P, 2>()));
-      // stretches for three workgroups a compute unit, of 256 classes or more
-      int stretches = 3 * num_cus() / p.facross;
-      stretches = stretches > rp / 256 ? rp / 256 : stretches;
+      // stretches for the two workgroups that a compute unit holds, of 128 classes or more (few classes: 64)
+      int stretches = 2 * num_cus() / p.facross, least = rp <= 2048 ? 64 : 128;
+      stretches = stretches > rp / least ? rp / least : stretches;
       stretches = stretches < 1 ? 1 : stretches;
       p.xchunk = ceil_to((rp + stretches - 1) / stretches, kPlaneAlign);
       p.xsplits = (rp + p.xchunk - 1) / p.xchunk;
     }
     p.xt = take(packed_bytes<P>(H, p.np));
-    p.wt = take(p.raw ? 0 : packed_bytes<P>(H, rp));
+    p.wt = take(p.few ? 0 : packed_bytes<P>(H, rp));
     p.d = take(packed_bytes<P>(p.np, rp));
     p.sums = take((size_t)tiles_of(n, p.bn) * C * 4);
     p.xpart = take((size_t)p.xsplits * n * H * 4);
@@ -996,33 +1050,31 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
   auto rows_of = [&](int c0) { return C - c0 < p.piece ? C - c0 : p.piece; };
   auto job_w = [&](int c0, bool o, bool t) {
     const int rows = rows_of(c0);
-    return pack_job(static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, rows, H, o && !p.raw ? piece_w(c0) : none,
-                    t && p.grads && !p.raw ? piece_wt(rows) : none,
+    return pack_job(static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, rows, H, o && !p.raw && !p.few ? piece_w(c0) : none,
+                    t && p.grads && !p.few ? piece_wt(rows) : none,
                     c.b ? c.b + c0 : nullptr, c.b ? KEEP_FINITE : KEEP_ALL, 0);
   };
   const PackedOut xt{p.grads && c.dW ? pl(p.xt) : nullptr, p.np};
   // X in one launch with what there is of W by then
-  PackJob jx = pack_job(c.X, c.ldx, n, H, X, xt, c.labels, KEEP_LABELLED, C);
+  PackJob jx = pack_job(c.X, c.ldx, n, H, p.few && n <= 32 ? none : X, xt, c.labels, KEEP_LABELLED, C);
   auto tile_args = [&](int c0) {
     const int rows = rows_of(c0);
     return TileArgs{ref(piece_w(c0)), ref(X), rows, n, p.Hp, tiles_of(rows, p.bm), tiles_of(n, p.bn), c.b ? c.b + c0 : nullptr, c.labels, c0,
                     static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, H};
   };
+  if (p.few) {
+    pack<P, Src>(jx, PackJob{}, st);
+    const DirectArgs a{c.W, c.X, c.ldw, c.ldx, ref(X), H, C, n, tiles_of(C, 32), c.b, c.labels, reinterpret_cast<float2 *>(ws + p.stats), f32(p.zlabel),
+                       p.grads ? f32(p.z) : nullptr};
+    if (n <= 32) launch(direct_stats_kernel<P, Src, 1, false>, p.tiles, 256, 0, st, a);
+    else launch(direct_stats_kernel<P, Src, 2, true>, p.tiles, 256, 0, st, a);
+  }
   if (!c.lse_given) {
-    if (p.direct) {
-      const DirectArgs a{c.W, c.X, c.ldw, c.ldx, ref(X), H, C, n, tiles_of(C, 32), c.b, c.labels, reinterpret_cast<float2 *>(ws + p.stats), f32(p.zlabel)};
-      if (n <= 32) {
-        launch(direct_stats_kernel<P, Src, 1, false>, p.tiles, 256, 0, st, a);
-      } else {
-        pack<P, Src>(jx, PackJob{}, st);
-        launch(direct_stats_kernel<P, Src, 2, true>, p.tiles, 256, 0, st, a);
-      }
-    }
-    for (int c0 = 0; c0 < C && !p.direct; c0 += p.piece) {
+    for (int c0 = 0; c0 < C && !p.few; c0 += p.piece) {
       pack<P, Src>(jx, job_w(c0, true, one), st);
       jx = PackJob{};
       const TileArgs a = tile_args(c0);
-      with_tile<P, false>(p.size, [&](auto t) {
+      with_tile<P>(p.size, [&](auto t) {
         using T = decltype(t);
         launch(stats_kernel<T>, a.tilesM * a.tilesN, T::THREADS, 0, st, a, reinterpret_cast<float2 *>(ws + p.stats), f32(p.zlabel));
         return 0;
@@ -1037,40 +1089,49 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
   if (p.grads) {
     const float *all = c.lse_given ? c.lse_given : lse;
     const int token_tiles = tiles_of(n, p.bn);
-    const bool x_parts = p.raw || !one || p.xsplits > 1, w_parts = p.wsplits > 1, b_parts = token_tiles > 1;
+    const bool x_parts = p.few || !one || p.xsplits > 1, w_parts = p.wsplits > 1, b_parts = !p.few && token_tiles > 1;
     bool first = true;
     for (int c0 = 0; c0 < C; c0 += p.piece, first = false) {
       const int rows = rows_of(c0), rp = ceil_to(rows, kPlaneAlign);
       // (what the first pass packed may still be there)
       const bool here = !c.lse_given && one;
-      if (!here) pack<P, Src>(jx, job_w(c0, c.lse_given || !keep, true), st);
+      if (!here && !p.few) pack<P, Src>(jx, job_w(c0, c.lse_given || !keep, true), st);
       jx = PackJob{};
       const TileArgs a = tile_args(c0);
       const PackedOut d{c.dX || c.dW ? pl(p.d) : nullptr, rp}, wt = piece_wt(rows);
-      if (c.dX || c.dW || c.db)
-        with_tile<P, true>(p.size, [&](auto t) {
+      if (p.few && (d.p || c.db)) {
+        const FewLogitsArgs f{f32(p.z), all, weight, c.labels, n, C, c0, d, rp / 32, c.db ? c.db + c0 : nullptr, c.scale};
+        launch(few_dlogits_kernel<P>, (rp / 32 + 3) / 4, 256, 0, st, f);
+      } else if (d.p || c.db) {
+        with_product_tile<P>(p.size, [&](auto t) {
           using T = decltype(t);
           launch(dlogits_kernel<T>, a.tilesM * a.tilesN, T::THREADS, 0, st, a, all, weight, d, !c.db ? nullptr : b_parts ? f32(p.sums) + c0 : c.db + c0, C,
                  b_parts ? 1.f : c.scale);
           return 0;
         });
+      }
       auto job = [&](const PackedOut &A, const PackedOut &B, int M, int K, int chunk, float *part, bool add, void *out, long ldo) {
         return ProductJob<Src>{ref(A), ref(B), M, H, K, tiles_of(M, p.pm), tiles_of(H, p.pn), (K + chunk - 1) / chunk, chunk, part, add,
                                static_cast<Src *>(out), ldo, c.scale};
       };
       ProductJob<Src> px{}, pw{};
       // (a last piece shorter than the others fills fewer stretches: those beyond keep what they have)
-      if (c.dX && !p.raw) px = job(d, wt, n, rp, p.xchunk, x_parts ? f32(p.xpart) : nullptr, !first, c.dX, c.lddx);
+      if (c.dX && !p.few) px = job(d, wt, n, rp, p.xchunk, x_parts ? f32(p.xpart) : nullptr, !first, c.dX, c.lddx);
       Src *dW = c.dW ? static_cast<Src *>(c.dW) + (long)c0 * c.lddw : nullptr;
       if (c.dW) pw = job(d, xt, rows, p.np, p.wchunk, w_parts ? f32(p.wpart) : nullptr, false, dW, c.lddw);
-      const int bx = c.dX && !p.raw ? px.tilesM * px.tilesN * px.splits : 0, bw = c.dW ? pw.tilesM * pw.tilesN * pw.splits : 0;
+      // (d W of more than the last cache holds, in whole lines of 128 bytes: bf16 124416 x 2176, 64 tokens 533 us of a call, streaming 469, 81664 x 4096, 12
+      // tokens 544, 456; lines in parts the other way, fp32 40806 x 4050, 12 tokens 823, 940)
+      const bool stream = p.few && c.dW && (size_t)C * H * sizeof(Src) > 256u << 20 && (uintptr_t)c.dW % 128 == 0 && c.lddw * sizeof(Src) % 128 == 0 && H * sizeof(Src) % 128 == 0;
+      const int bx = c.dX && !p.few ? px.tilesM * px.tilesN * px.splits : 0, bw = c.dW ? pw.tilesM * pw.tilesN * pw.splits : 0;
       if (bx + bw > 0)
         with_product_tile<P>(p.psize, [&](auto t) {
           using T = decltype(t);
-          launch(product_kernel<T, Src>, bx + bw, T::THREADS, 0, st, px, pw, bx);
+          if constexpr (std::is_same_v<T, typename Tiles<P>::L>)  // (so large a d W has tiles enough)
+            if (stream) return launch(product_kernel<T, Src, true>, bx + bw, T::THREADS, 0, st, px, pw, bx), 0;
+          launch(product_kernel<T, Src, false>, bx + bw, T::THREADS, 0, st, px, pw, bx);
           return 0;
         });
-      if (c.dX && p.raw) {
+      if (c.dX && p.few) {
         const FewArgs f{static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, ref(d), rows, n, H, c.b ? c.b + c0 : nullptr, p.facross, p.xchunk,
                         f32(p.xpart), !first};
         const int grid = p.facross * ((rp + p.xchunk - 1) / p.xchunk);

@@ -405,3 +405,46 @@ def test_scores(type_, pad, n, H, C):
     c.check(o, ("loss", "lse"))
     torch.cuda.synchronize()
     assert (o["dX"][:, :H] == 7).all() and (o["db"] == 7).all()
+
+
+# ------------------------------------------------------------------ few tokens with long rows or many classes, whose z is kept between the passes
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("n,H,C", [(1, 1030, 33), (2, 1100, 1), (20, 1025, 3000), (32, 1024, 64), (33, 1500, 8100), (64, 40, 33001), (64, 2050, 6001)])
+def test_gradients_of_few_tokens(type_, n, H, C):
+    c = Case(n + H + C, type_, n, H, C, ignored=0.3 if n > 2 else 0.0, masked=min(3, C - 1), weights=True, pad=(3, 1, 2, 5))
+    gone = ~((c.labels >= 0) & (c.labels < C))
+    c.X[gone, ::2] = float("nan")
+    if C > 3:
+        c.W[C - 3:, ::2] = float("nan")
+        c.W[C - 3:, 1::2] = -float("inf")
+    o, (ws, need) = c.outputs(), c.workspace(1)
+    c.call("cavs_vocab_xent", o, ws, need)
+    c.check(o)
+    assert (o["dX"][:, :H][gone] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("n,H,C", [(1, 1030, 300), (20, 1025, 3000), (64, 40, 33001)])
+def test_the_halves_of_few_tokens(type_, n, H, C):
+    test_the_halves_are_the_whole(type_, n, H, C)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,n,H,C", [("f32", 9, 1026, 900), ("bf16", 50, 32, 40000)])
+def test_few_tokens_captured_and_on_another_stream(type_, n, H, C):
+    test_the_same_bits_every_time_captured_and_on_another_stream(type_, n, H, C)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,n,H,C", [("bf16", 5, 1024, 131201), ("f32", 33, 1024, 65700), ("f32", 2, 1027, 65700), ("f32", 3, 8, 1500003)])
+def test_few_tokens_and_gradients_larger_than_a_cache(type_, n, H, C):
+    """dW of more than 256 MB, in whole lines and not, with rows that follow it left as they were; and classes in several pieces"""
+    c = Case(n + C, type_, n, H, C, masked=2)
+    o, (ws, need) = c.outputs(), c.workspace(1)
+    behind = torch.full((C + 1, H), 7.0, dtype=c.t, device="cuda")
+    o["dW"] = behind[:C]
+    c.call("cavs_vocab_xent", o, ws, need)
+    c.check(o)
+    assert (behind[C] == 7).all()

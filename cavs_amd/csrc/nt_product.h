@@ -59,11 +59,11 @@ __device__ inline void parts_of(float x, u16 (&o)[P]) {
   }
 }
 
-// NS: stages in LDS.  RA: the blocks a step begins with are read while the one before it multiplies.
-template <int P_, int BM_, int BN_, int BK_, int WGM_, int WGN_, int NS_ = 2, bool RA_ = false>
+// NS: stages in LDS.
+template <int P_, int BM_, int BN_, int BK_, int WGM_, int WGN_, int NS_ = 2>
 struct NtTile {
   static constexpr int P = P_, BM = BM_, BN = BN_, BK = BK_, WGM = WGM_, WGN = WGN_, NS = NS_;
-  static constexpr bool RA = RA_, RAW = false;  // RAW: an operand of another layout
+  static constexpr bool RAW = false;  // (an operand of another layout)
   static constexpr int WAVES = WGM * WGN, THREADS = 64 * WAVES;
   static constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 32, TN = WN / 32;
   static constexpr int STEPS = BK / 16, ROWB = 1024 * P * STEPS;    // bytes a row of blocks takes of a stage
@@ -75,7 +75,7 @@ struct NtTile {
   static constexpr int EU = GROUPS * WAVES / 4 < 4 ? GROUPS * WAVES / 4 : WM < 64 ? 4 : 3;  // wavefronts a SIMD is to hold
   static_assert(BM / 32 * P * STEPS % WAVES == 0 && BN / 32 * P * STEPS % WAVES == 0, "a tile's loads are the same for every wavefront");
   static_assert(kPlaneAlign % BK == 0, "operands end on a step");
-  static_assert(NS >= (RA ? 3 : 2) && LDS <= 160 * 1024, "stages");
+  static_assert(NS >= 2 && LDS <= 160 * 1024, "stages");
 };
 
 // Until at most N of this wavefront's loads are on their way and all it read from LDS is there; then until every wavefront is here.  (A barrier
@@ -88,10 +88,10 @@ __device__ __forceinline__ void nt_arrive() {
   asm volatile("" ::: "memory");
 }
 
-// A piece (eight k of row l % 32) from where its half blocks of sixteen rows lie, one `parts` half blocks after the other
-__device__ __forceinline__ bf16x8 turned_piece(const char *from, int lane, int parts) {
+// A piece (eight k of row l % 32) from where its two half blocks of sixteen rows lie
+__device__ __forceinline__ bf16x8 turned_piece(const char *from, int lane) {
   const int group = lane >> 4 & 1, half = lane >> 5;
-  const char *p = from + group * parts * 512 + half * 256 + 8 * (lane & 15);
+  const char *p = from + group * 512 + half * 256 + 8 * (lane & 15);
 #ifdef __HIP_DEVICE_COMPILE__
   typedef short four __attribute__((ext_vector_type(4)));
   const four lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) four *)(p + 128 * (half ^ group)));
@@ -135,11 +135,11 @@ __device__ __forceinline__ void nt_multiply(const PackedRef &A, int M, int m0, c
       la[c] = 16 * lane;
       sa[c] = (unsigned)min(at / PER, (M - 1 - m0) / 32) * (unsigned)rowa + at % PER * 1024;
     } else {
-      constexpr int PAIRS = T::BM / 32 * T::P;  // of half blocks, a step's
-      const int step = at / PAIRS, unit = at % PAIRS * 2 + (lane >> 5), col = unit / T::P, place = lane & 31;
-      const int here = place ^ 8 * ((place >> 4) ^ (col & 1));
-      la[c] = (min(col, A.K / 16 - 1 - m0 / 16) * T::P + unit % T::P) * 1024 + (here & 1) * 512 + (here >> 1) * 16;
-      sa[c] = (step >> 1) * (unsigned)rowa + (step & 1) * 256;
+      // two half blocks, of neighbouring sixteens of rows: step by step, part by part, down the tile
+      const int which = at / (T::BM / 32), step = which / T::P, sixteen = at % (T::BM / 32) * 2 + (lane >> 5), place = lane & 31;
+      const int here = place ^ 8 * ((place >> 4) ^ (lane >> 5));
+      la[c] = min(sixteen, A.K / 16 - 1 - m0 / 16) * (T::P * 1024) + (here & 1) * 512 + (here >> 1) * 16;
+      sa[c] = (step >> 1) * (unsigned)rowa + (step & 1) * 256 + which % T::P * 1024;
     }
   }
 #pragma unroll
@@ -167,75 +167,44 @@ __device__ __forceinline__ void nt_multiply(const PackedRef &A, int M, int m0, c
 #endif
   };
   const int a0 = wm * (T::WM / 32) * T::ROWB + 16 * lane, b0 = T::PA + wn * (T::WN / 32) * T::ROWB + 16 * lane;
-  struct Pieces {
-    bf16x8 a[T::TM][T::P], b[T::TN][T::P];
-  };
-  auto read = [&](Pieces &f, const char *from, int s) {
+  // A's parts from the last to the first, each with those of B that it meets: one part of A and what there is of B by then are all that registers hold
+  auto step = [&](const char *from, int s) {
+    bf16x8 b[T::P][T::TN];
 #pragma unroll
-    for (int p = 0; p < T::P; p++) {
+    for (int p = T::P - 1; p >= 0; p--) {
+      bf16x8 a[T::TM];
 #pragma unroll
       for (int i = 0; i < T::TM; i++) {
-        if constexpr (!TURNED) f.a[i][p] = *reinterpret_cast<const bf16x8 *>(from + a0 + (i * T::ROWB + (s * T::P + p) * 1024));
-        else f.a[i][p] = turned_piece(from + (wm * (T::WM / 16) + 2 * i) * T::P * 512 + (s * (T::BM / 16) * T::P + p) * 512, lane, T::P);
+        if constexpr (!TURNED) a[i] = *reinterpret_cast<const bf16x8 *>(from + a0 + (i * T::ROWB + (s * T::P + p) * 1024));
+        else a[i] = turned_piece(from + wm * (T::WM / 32) * 1024 + ((s * T::P + p) * (T::BM / 32) + i) * 1024, lane);
       }
 #pragma unroll
-      for (int j = 0; j < T::TN; j++) f.b[j][p] = *reinterpret_cast<const bf16x8 *>(from + b0 + (j * T::ROWB + (s * T::P + p) * 1024));
-    }
-  };
-  auto multiply = [&](const Pieces &f) {
+      for (int j = 0; j < T::TN; j++) b[T::P - 1 - p][j] = *reinterpret_cast<const bf16x8 *>(from + b0 + (j * T::ROWB + (s * T::P + T::P - 1 - p) * 1024));
 #pragma unroll
-    for (int w = T::P - 1; w >= 0; w--)  // the parts' weights, the small products first
-#pragma unroll
-      for (int p = 0; p <= w; p++)
+      for (int q = T::P - 1 - p; q >= 0; q--)
 #pragma unroll
         for (int i = 0; i < T::TM; i++)
 #pragma unroll
           for (int j = 0; j < T::TN; j++)
-            acc[w ? T::ACC - 1 : 0][i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a[i][p], f.b[j][w - p], acc[w ? T::ACC - 1 : 0][i][j], 0, 0, 0);
+            acc[p + q ? T::ACC - 1 : 0][i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[q][j], acc[p + q ? T::ACC - 1 : 0][i][j], 0, 0, 0);
+    }
   };
   const int nk = (kend - kbeg) / T::BK;
 #pragma unroll
   for (int q = 0; q < T::NS - 1; q++)
     if (q < nk) fetch(q, S + q * T::STAGE);
   int at = 0;
-  auto behind = [](int x) { return x == (T::NS - 1) * T::STAGE ? 0 : x + T::STAGE; };
-  constexpr int STEPS = T::STEPS;
-  if constexpr (!T::RA) {
-    for (int kt = 0; kt < nk; kt++) {
-      if (kt + T::NS - 2 < nk) nt_arrive<(T::NS - 2) * T::LOADS>();
-      else nt_arrive<0>();
-      if (kt + T::NS - 1 < nk) fetch(kt + T::NS - 1, S + (at == 0 ? (T::NS - 1) * T::STAGE : at - T::STAGE));
+  for (int kt = 0; kt < nk; kt++) {
+    if (kt + T::NS - 2 < nk) nt_arrive<(T::NS - 2) * T::LOADS>();
+    else nt_arrive<0>();
+    if (kt + T::NS - 1 < nk) fetch(kt + T::NS - 1, S + (at == 0 ? (T::NS - 1) * T::STAGE : at - T::STAGE));
 #pragma unroll
-      for (int s = 0; s < STEPS; s++) {
-        Pieces f;
-        read(f, S + at, s);
-        multiply(f);
-        // (one part, 256 x 128: the compiler's own pattern for a product's loop, 2.5 % faster; the others are as fast without)
-        if constexpr (T::P == 1 && T::BM == 256) __builtin_amdgcn_iglp_opt(1);
-      }
-      at = behind(at);
+    for (int s = 0; s < T::STEPS; s++) {
+      step(S + at, s);
+      // (one part, 256 x 128: the compiler's own pattern for a product's loop, 2.5 % faster; the others are as fast without)
+      if constexpr (T::P == 1 && T::BM == 256) __builtin_amdgcn_iglp_opt(1);
     }
-  } else {
-    Pieces f[2];
-    if (nk > 0) {
-      if (nk >= T::NS - 1) nt_arrive<(T::NS - 2) * T::LOADS>();
-      else nt_arrive<0>();
-      read(f[0], S, 0);
-    }
-    for (int kt = 0; kt < nk; kt++) {
-      if (kt + T::NS - 2 < nk) nt_arrive<(T::NS - 3) * T::LOADS>();
-      else nt_arrive<0>();
-      if (kt + T::NS - 1 < nk) fetch(kt + T::NS - 1, S + (at == 0 ? (T::NS - 1) * T::STAGE : at - T::STAGE));
-      const int next = behind(at);
-#pragma unroll
-      for (int s = 0; s < STEPS; s++) {
-        if (s + 1 < STEPS) read(f[(s + 1) & 1], S + at, s + 1);
-        else if (kt + 1 < nk) read(f[STEPS & 1], S + next, 0);
-        multiply(f[s & 1]);
-      }
-      if constexpr (STEPS & 1) f[0] = f[1];
-      at = next;
-    }
+    at = at == (T::NS - 1) * T::STAGE ? 0 : at + T::STAGE;
   }
   nt_arrive<0>();  // (LDS is free for what follows)
 }

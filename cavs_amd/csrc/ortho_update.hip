@@ -290,14 +290,15 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void ortho_product_kernel(Produc
         if (32 * rb < n && 32 * cb < t.mp) put_columns<T::P>(PackedOut{t.Xt[1], t.mp}, rb, cb, e, lane, turn);
       } else {
         if (col >= t.cols) continue;
+        float w[16];  // (all of them on their way before the first is stored)
+        if (t.W)
+#pragma unroll
+          for (int r = 0; r < 16; r++) w[r] = row(r) < t.rows ? t.W[row(r) * t.ldw + col] : 0.f;
 #pragma unroll
         for (int r = 0; r < 16; r++) {
           if (row(r) >= t.rows) continue;
           if (t.O) store_as(static_cast<Src *>(t.O) + row(r) * t.ldo + col, x[r]);
-          if (t.W) {
-            float *w = t.W + row(r) * t.ldw + col;
-            *w = fmaf(1.f - c.lr * c.decay, *w, -c.lr * t.shrink * x[r]);
-          }
+          if (t.W) t.W[row(r) * t.ldw + col] = fmaf(1.f - c.lr * c.decay, w[r], -c.lr * t.shrink * x[r]);
         }
       }
     }
@@ -307,11 +308,11 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void ortho_product_kernel(Produc
 template <int P> struct Tiles;
 template <> struct Tiles<2> {
   using L = NtTile<2, 128, 128, 16, 2, 2, 3>;
-  using S = NtTile<2, 64, 64, 32, 2, 2>;
+  using S = NtTile<2, 64, 64, 32, 2, 2, 3>;
 };
 template <> struct Tiles<3> {
   using L = NtTile<3, 128, 128, 16, 2, 2>;
-  using S = NtTile<3, 64, 64, 32, 2, 2>;
+  using S = NtTile<3, 64, 64, 32, 2, 2, 3>;
 };
 
 struct Plan {

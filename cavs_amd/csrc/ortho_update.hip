@@ -41,14 +41,6 @@ struct Common {
 
 __device__ inline bool held_back(const Common &c) { return c.guard && *c.guard != 0; }
 
-template <class Src>
-__device__ inline float update_of(const Mat &t, const Common &c, long r, int k) {
-  const float g = value_of(static_cast<const Src *>(t.G) + r * t.ldg + k);
-  if (!t.M) return g;
-  const float m = t.M[r * t.ldm + k];
-  return c.nesterov ? fmaf(c.momentum, m, g) : m;
-}
-
 // M <- mu M + G, and the squares of U, added up in 64 bits in a fixed order
 struct NormArgs {
   Mat m[kMats];
@@ -117,6 +109,17 @@ __global__ __launch_bounds__(256) void start_kernel(StartArgs g) {
   int who = 0;
   while (who + 1 < c.count && (int)blockIdx.x >= g.first[who + 1]) who++;
   const Mat &t = g.m[who];
+  const bool flat = t.rows <= t.cols;
+  const int across = (flat ? t.np : t.mp) / 64, block = blockIdx.x - g.first[who];
+  const int r0 = block / across * 64, k0 = block % across * 64, k = threadIdx.x & 63;
+  // (all of a lane's values on their way while the norm is made)
+  float gr[16], mo[16];
+  auto in = [&](int i) { return r0 + (int)(threadIdx.x >> 6) + 4 * i < t.rows && k0 + k < t.cols; };
+  auto at = [&](int i, long ld) { return (long)(r0 + (threadIdx.x >> 6) + 4 * i) * ld + k0 + k; };
+#pragma unroll
+  for (int i = 0; i < 16; i++) gr[i] = in(i) ? value_of(static_cast<const Src *>(t.G) + at(i, t.ldg)) : 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; i++) mo[i] = t.M && in(i) ? t.M[at(i, t.ldm)] : 0.f;
   __shared__ double s[kNormBlocks];
   s[threadIdx.x] = c.squares[who * kNormBlocks + threadIdx.x];
   for (int o = kNormBlocks / 2; o > 0; o >>= 1) {
@@ -125,13 +128,10 @@ __global__ __launch_bounds__(256) void start_kernel(StartArgs g) {
   }
   __syncthreads();
   const double by = s[0] == 0. ? 0. : 1. / (sqrt(s[0]) + (double)c.eps);  // (nothing stays nothing, with eps = 0 too)
-  const bool flat = t.rows <= t.cols;
-  const int across = (flat ? t.np : t.mp) / 64, block = blockIdx.x - g.first[who];
-  const int r0 = block / across * 64, k0 = block % across * 64, k = threadIdx.x & 63;
-#pragma unroll 8
-  for (int i = threadIdx.x >> 6; i < 64; i += 4) {
-    const int r = r0 + i;
-    tile[i][k] = r < t.rows && k0 + k < t.cols ? (float)((double)update_of<Src>(t, c, r, k0 + k) * by) : 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const float u = !t.M ? gr[i] : c.nesterov ? fmaf(c.momentum, mo[i], gr[i]) : mo[i];
+    tile[(threadIdx.x >> 6) + 4 * i][k] = in(i) ? (float)((double)u * by) : 0.f;
   }
   __syncthreads();
   const PackedOut X{t.X, t.np}, Xt{t.Xt[0], t.mp};

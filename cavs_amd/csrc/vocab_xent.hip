@@ -19,7 +19,8 @@ namespace {
 
 // ------------------------------------------------------------------ operands, packed
 // src [rows, K] with its columns as k and, for the products that sum over its rows, with its rows as k.  Either may be left out.  A row that
-// takes no part by its flag is zero in the second: 0 times what it holds need not be 0.
+// takes no part by its flag is zero in the second: 0 times what it holds need not be 0.  There a row may come times a weight, rounded once more to
+// the type: in X's elements those roundings are independent of each other, in d each would be one of all of a token's d.
 enum { KEEP_ALL = 0, KEEP_LABELLED = 1, KEEP_FINITE = 2 };  // rows whose flag is a class id below `classes`; rows whose flag is not -inf
 __device__ inline bool is_class(float label, int classes) { return label >= 0.f && label < (float)classes; }
 
@@ -30,7 +31,8 @@ struct PackJob {
   PackedOut o, t;
   const float *flag;
   int keep, classes;
-  int across, blocks;  // blocks of 64 columns, of 64 x 64
+  const float *weight;  // or null
+  int across, blocks;   // blocks of 64 columns, of 64 x 64
 };
 
 template <int P, class Src>
@@ -47,7 +49,10 @@ __global__ __launch_bounds__(256) void pack_kernel(PackJob j0, PackJob j1) {
   if (!g.t.p || g.keep == KEEP_ALL) return;
   __syncthreads();
   for (int i = threadIdx.x >> 6; i < 64; i += 4)
-    if (r0 + i < g.rows && (g.keep == KEEP_LABELLED ? !is_class(g.flag[r0 + i], g.classes) : g.flag[r0 + i] == -INFINITY)) tile[i][k] = 0.f;
+    if (r0 + i < g.rows) {
+      if (g.keep == KEEP_LABELLED ? !is_class(g.flag[r0 + i], g.classes) : g.flag[r0 + i] == -INFINITY) tile[i][k] = 0.f;
+      else if (g.weight) tile[i][k] *= g.weight[r0 + i];
+    }
   __syncthreads();
   pack_tile<P>(tile, PackedOut{}, g.t, r0, k0, g.rows, g.K);
 }
@@ -471,9 +476,10 @@ __global__ __launch_bounds__(256) void weights_kernel(const float *__restrict__ 
   if (row < n) weight[row] = weight_of(labels[row], lse[row], dloss, row, C);
 }
 
-// d of a tile, weight * (p - [label]), packed by token (zero between the last class or token and the end of the steps), and its sums over the
-// tile's tokens.  `scale`, which multiplies all of d, stays out of what is rounded: next to the label, where p is small, p - 1 is -1 and a bit, which bf16
-// holds well, while a factor in it is a rounding error that all of its kind share.
+// e = p - [label] of a tile, packed by token (zero between the last class or token and the end of the steps, and of a token without weight), and the
+// sums of d = weight * e over the tile's tokens.
+// What multiplies all of a row's d, or all of d, stays out of what is rounded: next to the label, where p is small, e is -1 and a bit, which bf16
+// holds well, while any factor in it is a rounding error that all of its kind share.  d W takes the weights as factors of its rows, d^T X with X.
 template <class T>
 __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, const float *__restrict__ lse, const float *__restrict__ weight, PackedOut d,
                                                                     float *__restrict__ sums, int ld_sums, float sums_scale) {
@@ -512,7 +518,7 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, 
         for (int r = 0; r < 16; r++) x[r] -= at[j] == 32 * i + 8 * (r >> 2) + (r & 3) ? 1.f : 0.f;
       }
 #pragma unroll
-      for (int r = 0; r < 16; r++) x[r] *= g[j], sum[r] += x[r];
+      for (int r = 0; r < 16; r++) sum[r] += g[j] * x[r];
       if (d.p && 32 * xb < tokens && 32 * cb < d.K) {
         Parts16<T::P> e;
 #pragma unroll
@@ -542,8 +548,8 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, 
 }
 
 // ------------------------------------------------------------------ the gradients of few tokens
-// d of up to 64 tokens from the z that direct_stats_kernel left (a float a token and class, beside W's row of H), packed as dlogits_kernel packs it,
-// and its sums over the tokens.  A wavefront has a block of 32 classes.
+// e of up to 64 tokens from the z that direct_stats_kernel left (a float a token and class, beside W's row of H), packed as dlogits_kernel packs it,
+// and d's sums over the tokens.  A wavefront has a block of 32 classes.
 struct FewLogitsArgs {
   const float *z;
   const float *lse, *weight, *labels;
@@ -573,8 +579,8 @@ __global__ __launch_bounds__(256) void few_dlogits_kernel(FewLogitsArgs a) {
         const float v[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          e[4 * q + k] = g == 0.f ? 0.f : g * (__expf(v[k] - all) - (at == 8 * q + k ? 1.f : 0.f));
-          sum[4 * q + k] += e[4 * q + k];
+          e[4 * q + k] = g == 0.f ? 0.f : __expf(v[k] - all) - (at == 8 * q + k ? 1.f : 0.f);
+          sum[4 * q + k] += g * e[4 * q + k];
         }
       }
     }
@@ -746,7 +752,7 @@ __global__ __launch_bounds__(256, 2) void few_dx_kernel(FewArgs a) {
 }
 
 // ------------------------------------------------------------------ the products with d
-// out[row, col] = scale * A B^T.  K in `splits` stretches of kchunk, each with sums of its own (unscaled) at part + split * M * N; part null:
+// out[row, col] = scale * factor[row] * A B^T.  K in `splits` stretches of kchunk, each with sums of its own (unscaled) at part + split * M * N; part null:
 // straight to out.  A launch is d W, d's rows the tile's rows, and d^T X, d's classes the tile's rows and its tokens what is summed over.
 template <class Out>
 struct ProductJob {
@@ -757,6 +763,7 @@ struct ProductJob {
   Out *out;
   long ldo;
   float scale;
+  const float *factor;  // of out's rows, or null
 };
 
 // STREAM: `out` goes past the caches
@@ -790,18 +797,19 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void product_kernel(ProductJob<O
           float *o = part + (long)row * g.N + col;
           *o = g.add ? *o + x : x;
         } else if constexpr (STREAM) {
-          stream_as(g.out + row * g.ldo + col, g.scale * x);
+          stream_as(g.out + row * g.ldo + col, (g.factor ? g.scale * g.factor[row] : g.scale) * x);
         } else {
-          store_as(g.out + row * g.ldo + col, g.scale * x);
+          store_as(g.out + row * g.ldo + col, (g.factor ? g.scale * g.factor[row] : g.scale) * x);
         }
       }
   }
 }
 
-// out[r, 0 .. w) = scale * sum of `parts` pieces, in their order
+// out[r, 0 .. w) = scale * factor[r] * sum of `parts` pieces, in their order
 struct SumJob {
   const float *part;
   int parts, rows, w;
+  const float *factor;
   void *out;
   long ldo;
   int blocks;
@@ -820,7 +828,7 @@ __device__ inline void sum_parts(const SumJob &g, float scale, int block) {
       for (int k = 0; k < 8; k++) s += v[k];
     }
     const long r = i / g.w;
-    store_as(out + r * g.ldo + (i - r * g.w), scale * s);
+    store_as(out + r * g.ldo + (i - r * g.w), (g.factor ? scale * g.factor[r] : scale) * s);
   }
 }
 // d X, d W and d b (fp32) of what the launches before left in parts
@@ -1019,9 +1027,9 @@ Plan plan_of(int n, int H, int C, int grads) {
   return p;
 }
 
-inline PackJob pack_job(const void *src, long ld, int rows, int K, PackedOut o, PackedOut t, const float *flag, int keep, int classes) {
+inline PackJob pack_job(const void *src, long ld, int rows, int K, PackedOut o, PackedOut t, const float *flag, int keep, int classes, const float *weight) {
   const int across = tiles_of(K, 64);
-  return {src, ld, rows, K, o, t, flag, keep, classes, across, o.p || t.p ? across * tiles_of(rows, 64) : 0};
+  return {src, ld, rows, K, o, t, flag, keep, classes, weight, across, o.p || t.p ? across * tiles_of(rows, 64) : 0};
 }
 template <int P, class Src>
 void pack(const PackJob &a, const PackJob &b, hipStream_t st) {
@@ -1052,11 +1060,11 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
     const int rows = rows_of(c0);
     return pack_job(static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, rows, H, o && !p.raw && !p.few ? piece_w(c0) : none,
                     t && p.grads && !p.few ? piece_wt(rows) : none,
-                    c.b ? c.b + c0 : nullptr, c.b ? KEEP_FINITE : KEEP_ALL, 0);
+                    c.b ? c.b + c0 : nullptr, c.b ? KEEP_FINITE : KEEP_ALL, 0, nullptr);
   };
   const PackedOut xt{p.grads && c.dW ? pl(p.xt) : nullptr, p.np};
   // X in one launch with what there is of W by then
-  PackJob jx = pack_job(c.X, c.ldx, n, H, p.few && n <= 32 ? none : X, xt, c.labels, KEEP_LABELLED, C);
+  PackJob jx = pack_job(c.X, c.ldx, n, H, p.few && n <= 32 ? none : X, xt, c.labels, KEEP_LABELLED, C, c.dloss);
   auto tile_args = [&](int c0) {
     const int rows = rows_of(c0);
     return TileArgs{ref(piece_w(c0)), ref(X), rows, n, p.Hp, tiles_of(rows, p.bm), tiles_of(n, p.bn), c.b ? c.b + c0 : nullptr, c.labels, c0,
@@ -1110,15 +1118,15 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
           return 0;
         });
       }
-      auto job = [&](const PackedOut &A, const PackedOut &B, int M, int K, int chunk, float *part, bool add, void *out, long ldo) {
+      auto job = [&](const PackedOut &A, const PackedOut &B, int M, int K, int chunk, float *part, bool add, void *out, long ldo, const float *factor) {
         return ProductJob<Src>{ref(A), ref(B), M, H, K, tiles_of(M, p.pm), tiles_of(H, p.pn), (K + chunk - 1) / chunk, chunk, part, add,
-                               static_cast<Src *>(out), ldo, c.scale};
+                               static_cast<Src *>(out), ldo, c.scale, factor};
       };
       ProductJob<Src> px{}, pw{};
       // (a last piece shorter than the others fills fewer stretches: those beyond keep what they have)
-      if (c.dX && !p.few) px = job(d, wt, n, rp, p.xchunk, x_parts ? f32(p.xpart) : nullptr, !first, c.dX, c.lddx);
+      if (c.dX && !p.few) px = job(d, wt, n, rp, p.xchunk, x_parts ? f32(p.xpart) : nullptr, !first, c.dX, c.lddx, weight);
       Src *dW = c.dW ? static_cast<Src *>(c.dW) + (long)c0 * c.lddw : nullptr;
-      if (c.dW) pw = job(d, xt, rows, p.np, p.wchunk, w_parts ? f32(p.wpart) : nullptr, false, dW, c.lddw);
+      if (c.dW) pw = job(d, xt, rows, p.np, p.wchunk, w_parts ? f32(p.wpart) : nullptr, false, dW, c.lddw, nullptr);
       // (d W of more than the last cache holds, in whole lines of 128 bytes: bf16 124416 x 2176, 64 tokens 533 us of a call, streaming 469, 81664 x 4096, 12
       // tokens 544, 456; lines in parts the other way, fp32 40806 x 4050, 12 tokens 823, 940)
       const bool stream = p.few && c.dW && (size_t)C * H * sizeof(Src) > 256u << 20 && (uintptr_t)c.dW % 128 == 0 && c.lddw * sizeof(Src) % 128 == 0 && H * sizeof(Src) % 128 == 0;
@@ -1140,9 +1148,9 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
       }
       const bool last = c0 + p.piece >= C;
       SumJob sx{}, sw{}, sb{};
-      if (last && c.dX && x_parts) sx = {f32(p.xpart), p.xsplits, n, H, c.dX, c.lddx, 0};
-      if (dW && w_parts) sw = {f32(p.wpart), p.wsplits, rows, H, dW, c.lddw, 0};
-      if (last && c.db && b_parts) sb = {f32(p.sums), token_tiles, 1, C, c.db, C, 0};
+      if (last && c.dX && x_parts) sx = {f32(p.xpart), p.xsplits, n, H, weight, c.dX, c.lddx, 0};
+      if (dW && w_parts) sw = {f32(p.wpart), p.wsplits, rows, H, nullptr, dW, c.lddw, 0};
+      if (last && c.db && b_parts) sb = {f32(p.sums), token_tiles, 1, C, nullptr, c.db, C, 0};
       sums<Src>(sx, sw, sb, c.scale, st);
     }
   }
@@ -1166,7 +1174,7 @@ int check_and_run(const char *who, int type, const Call &c, int grads, void *ws,
   CAVS_REQUIRE(c.W && (c.n == 0 || (c.X && c.labels)), "%s: null pointer", who);
   if (c.n == 0) {  // sums over no rows
     hipStream_t st = as_stream(stream);
-    const SumJob w{nullptr, 0, c.C, c.H, c.dW, c.lddw, 0}, b{nullptr, 0, 1, c.C, c.db, c.C, 0};
+    const SumJob w{nullptr, 0, c.C, c.H, nullptr, c.dW, c.lddw, 0}, b{nullptr, 0, 1, c.C, nullptr, c.db, c.C, 0};
     if (type == CAVS_F32) sums<float>({}, w, b, 0.f, st);
     else sums<u16>({}, w, b, 0.f, st);
     CAVS_LAUNCH_CHECK();

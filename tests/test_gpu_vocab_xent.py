@@ -113,7 +113,9 @@ class Case:
         dX, dW, db = d @ W, d.t() @ X, d.sum(0)
         e = dict(lse=elog, loss=elog + ez[rows, at] + U * loss.abs())
         e["dX"] = edr @ W.abs() + (C / 16 + 64) * U * (d.abs() @ W.abs()) + eps * dX.abs() + 2.0 ** -126
-        e["dW"] = edr.t() @ X.abs() + (self.n / 16 + 64) * U * (d.abs().t() @ X.abs()) + eps * dW.abs() + 2.0 ** -126
+        # (d W takes a row's dloss in fp32, d^T X takes it with X, which bf16 rounds once more: (1 + eps)^2 - 1 for the roundings of d and of dloss X)
+        edw = edr if self.dloss is None or self.t == torch.float32 else ed + ((1 + eps) ** 2 - 1) * d.abs()
+        e["dW"] = edw.t() @ X.abs() + (self.n / 16 + 64) * U * (d.abs().t() @ X.abs()) + eps * dW.abs() + 2.0 ** -126
         e["db"] = ed.sum(0) + (self.n / 16 + 16) * U * d.abs().sum(0)
         return dict(loss=loss, lse=lse, dX=dX, dW=dW, db=db), e
 

@@ -55,33 +55,56 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs g) {
   if (held_back(c)) return;
   const Mat &t = g.m[who];
   double sum = 0.;
-  // lanes along a row, as many rows at a time as there are lanes left; four values of a lane on their way
-  int across = 64;
-  while (across < 256 && across < t.cols) across *= 2;
+  // lanes along a row, four neighbouring values each, as many rows at a time as there are lanes left; four loads of a lane on their way.  (One value a
+  // load: bf16 of 8192 x 4096 and 4096 x 4096 184 us, 46 now.)
+  typedef Src four __attribute__((ext_vector_type(4), aligned(sizeof(Src))));
+  typedef float four32 __attribute__((ext_vector_type(4), aligned(4)));
+  int across = 16;
+  while (across < 256 && 16 * across < t.cols) across *= 2;
   const int high = 256 / across, x = threadIdx.x % across, y = threadIdx.x / across;
   for (long r0 = (long)blockIdx.x * high; r0 < t.rows; r0 += (long)gridDim.x * high) {
     const long r = r0 + y;
     if (r >= t.rows) continue;
     const Src *G = static_cast<const Src *>(t.G) + r * t.ldg;
     float *M = t.M ? t.M + r * t.ldm : nullptr;
-    for (int k0 = x; k0 < t.cols; k0 += 4 * across) {
-      float gr[4], mo[4];
+    for (int k0 = 4 * x; k0 < t.cols; k0 += 16 * across) {
+      four gr[4];
+      four32 mo[4];
 #pragma unroll
       for (int q = 0; q < 4; q++) {
-        const int k = k0 + q * across;
-        gr[q] = k < t.cols ? value_of(G + k) : 0.f;
-        mo[q] = M && k < t.cols ? M[k] : 0.f;
+        const int k = k0 + 4 * q * across;
+        if (k + 4 <= t.cols) {
+          gr[q] = *reinterpret_cast<const four *>(G + k);
+          if (M) mo[q] = *reinterpret_cast<const four32 *>(M + k);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            gr[q][e] = k + e < t.cols ? G[k + e] : Src(0);
+            if (M) mo[q][e] = k + e < t.cols ? M[k + e] : 0.f;
+          }
+        }
       }
 #pragma unroll
       for (int q = 0; q < 4; q++) {
-        const int k = k0 + q * across;
-        float u = gr[q];
-        if (M) {
-          mo[q] = fmaf(c.momentum, mo[q], gr[q]);
-          if (k < t.cols) M[k] = mo[q];
-          u = c.nesterov ? fmaf(c.momentum, mo[q], gr[q]) : mo[q];
+        const int k = k0 + 4 * q * across;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const Src one = gr[q][e];
+          const float v = value_of(&one);
+          float u = v;
+          if (M) {
+            mo[q][e] = fmaf(c.momentum, mo[q][e], v);
+            u = c.nesterov ? fmaf(c.momentum, mo[q][e], v) : mo[q][e];
+          }
+          sum += (double)u * u;  // (zero beyond the last column)
         }
-        sum += (double)u * u;
+        if (M && k + 4 <= t.cols) {
+          *reinterpret_cast<four32 *>(M + k) = mo[q];
+        } else if (M) {
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (k + e < t.cols) M[k + e] = mo[q][e];
+        }
       }
     }
   }

@@ -388,7 +388,7 @@ struct LaunchPlan {
 };
 
 // The tiles with the shorter longest way: as many as the fullest compute unit gets, times what one takes (a small one a third longer for its
-// size).  Eight of 1024 x 1024: 288 large tiles 85 us, 1088 small ones 77; their last product, 512 large tiles 102 us.
+// size).  Eight of 1024 x 1024: 288 large tiles 85 us, 1088 small ones 72; their last product, 512 large tiles 112 us.
 template <int P, class F>
 auto with_tile(const cavs_ortho_desc *d, int count, int stage, F &&f) {
   using L = typename Tiles<P>::L;

@@ -606,8 +606,8 @@ __global__ __launch_bounds__(256) void few_dlogits_kernel(FewLogitsArgs a) {
 // of a step, a load of 4 F or 2 F bytes each; the instruction takes its eight classes of one column at a time, so those are F operands, of
 // columns F apart, by renaming registers.  A workgroup has 32 F columns, up to 32 TN tokens and a stretch of the classes, of which each wavefront takes
 // every fourth step of sixteen; what they sum up meets in LDS and goes to part [stretch, n, H].  Rows of classes that are masked are zero.
-// (F as large as accumulators leave room for: with loads of 4 bytes a wavefront has 2 KB under way, too little -- one token, bf16 124416 x 2176,
-// 700 us of a call.)
+// (F as large as accumulators leave room for: with loads of 4 bytes a wavefront has 2 KB under way, too little.  bf16 81664 x 4096, 12 tokens: W's 669 MB in
+// 119 us, 5.6 TB/s; with stretches for one and a half rounds of workgroups 212.)
 struct FewArgs {
   const void *W;
   long ldw;
@@ -639,8 +639,10 @@ __global__ __launch_bounds__(256, 2) void few_dx_kernel(FewArgs a) {
       for (int f = 0; f < F; f++)
 #pragma unroll
         for (int r = 0; r < 16; r++) acc[s][j][f][r] = 0.f;
-  // F columns from h0 + F x on, of eight classes (beyond the last column: nothing)
-  const bool whole = h0 + F * x + F <= a.H;  // (this lane's)
+  // F columns from h0 + F x on, of eight classes.  Towards the end of a row the last F there are, moved down once they have come: what a lane holds beyond the
+  // last column goes nowhere.  (Value by value there, few workgroups kept all the others waiting: fp32 40806 x 4052, 12 tokens 338 us, 218 now.)
+  const bool edge = h0 + 32 * F > a.H, wide = a.H >= F;
+  const int h = h0 + F * x, from = edge ? min(h, a.H - F) : h, beyond = h - from;
   constexpr int WORDS = F * sizeof(Src) / 4;
   typedef unsigned words __attribute__((ext_vector_type(WORDS == 1 ? 2 : WORDS), aligned(sizeof(Src))));
   struct Eight {
@@ -652,20 +654,20 @@ __global__ __launch_bounds__(256, 2) void few_dx_kernel(FewArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       const int c = min(k0 + 8 * half + e, a.M - 1);
-      const Src *row = static_cast<const Src *>(a.W) + c * a.ldw + h0 + F * x;
+      const Src *row = static_cast<const Src *>(a.W) + c * a.ldw;
       o.b[e] = a.bias ? a.bias[c] : 0.f;
-      if (whole) {
+      if (wide) {
         static_assert(WORDS > 1, "a lane's columns are eight bytes or more");
-        const words v = *reinterpret_cast<const words *>(row);
+        const words v = *reinterpret_cast<const words *>(row + from);
 #pragma unroll
         for (int i = 0; i < WORDS; i++) o.v[e][i] = v[i];
       } else {
 #pragma unroll
         for (int i = 0; i < WORDS; i++) {
           if constexpr (sizeof(Src) == 4) {
-            o.v[e][i] = h0 + F * x + i < a.H ? __float_as_uint(value_of(row + i)) : 0u;
+            o.v[e][i] = h + i < a.H ? __float_as_uint(value_of(row + h + i)) : 0u;
           } else {
-            const unsigned lo = h0 + F * x + 2 * i < a.H ? row[2 * i] : 0u, hi = h0 + F * x + 2 * i + 1 < a.H ? row[2 * i + 1] : 0u;
+            const unsigned lo = h + 2 * i < a.H ? row[h + 2 * i] : 0u, hi = h + 2 * i + 1 < a.H ? row[h + 2 * i + 1] : 0u;
             o.v[e][i] = lo | hi << 16;
           }
         }
@@ -677,6 +679,22 @@ __global__ __launch_bounds__(256, 2) void few_dx_kernel(FewArgs a) {
       for (int p = 0; p < P; p++) o.d[j][p] = *reinterpret_cast<const bf16x8 *>(dp[j] + ((long)(k0 / 16) * P + p) * 512);
   };
   auto mask = [&](Eight &o, int k0) {
+    if (edge && wide)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        unsigned(&v)[WORDS] = o.v[e];
+        if constexpr (sizeof(Src) == 2) {
+          if (beyond & 1)
+#pragma unroll
+            for (int i = 0; i < WORDS; i++) v[i] = v[i] >> 16 | (i + 1 < WORDS ? v[i + 1] << 16 : 0u);
+        }
+        const int words_beyond = sizeof(Src) == 2 ? beyond >> 1 : beyond;
+#pragma unroll
+        for (int by = 1; by < WORDS; by *= 2)
+          if (words_beyond & by)
+#pragma unroll
+            for (int i = 0; i + by < WORDS; i++) v[i] = v[i + by];
+      }
 #pragma unroll
     for (int e = 0; e < 8; e++)
       if (k0 + 8 * half + e >= a.M || o.b[e] == -INFINITY)
@@ -953,12 +971,12 @@ Plan plan_of(int n, int H, int C, int grads) {
   const int rows = p.piece < C ? p.piece : C;
   // Few tokens: W read where it lies and z kept, packing W and making z twice would be most of the work.  Gradients take two launches more that way, which
   // long rows or many classes pay for.  us with gradients packed / as it lies, 1, 24 and 64 tokens:
-  //   fp32  300 x 1024 55 / 39, 56 / 42, 57 / 47   1000 x 512 41 / 36, 42 / 38, 43 / 43   12000 x 300 61 / 63, 61 / 66, 63 / 70   12000 x 512 74 / 62, 78 / 66,
-  //         79 / 73   32000 x 128 77 / 65, 81 / 72, 82 / 79   45376 x 1024 425 / 200, 443 / 216 (64)   40806 x 4050 1574 / 823 (12)
-  //   bf16  1000 x 512 29 / 30, 30 / 33, 30 / 41   4000 x 1024 52 / 39, 51 / 42, 52 / 54   12000 x 1024 66 / 54, 68 / 64, 71 / 70   32000 x 128 54 / 55, 57 / 62,
-  //         58 / 60   81792 x 72 93 / 82, 96 / 90, 98 / 95   124416 x 2176 915 / 469 (64)
+  //   fp32  300 x 1024 56 / 39, 57 / 42, 58 / 48   1000 x 512 43 / 36, 43 / 39, 44 / 44   12000 x 300 61 / 58, 63 / 62, 65 / 68   21701 x 300 78 / 73, 84 / 78,
+  //         91 / 85   12000 x 512 76 / 63, 78 / 67, 82 / 72   32000 x 128 79 / 65, 82 / 72, 84 / 79   40806 x 4050 1574 / 681 (12)
+  //   bf16  1000 x 512 31 / 31, 32 / 34, 31 / 42   4000 x 1024 53 / 40, 53 / 44, 53 / 56   12000 x 1024 68 / 56, 71 / 67, 73 / 73   32000 x 128 54 / 52, 57 / 59,
+  //         59 / 63   81792 x 72 95 / 79, 99 / 86, 100 / 94   124416 x 2176 915 / 469 (64)
   const bool many = C >= 128 * num_cus();
-  p.few = n <= kFewRows && (!grads || many || (P == 3 ? H >= 512 : H >= 1024 && (n <= 32 || (long)C * H >= 12000000)));
+  p.few = n <= kFewRows && (!grads || many || (P == 3 ? H >= 512 || (long)C * H >= 5000000 : H >= 1024 && (n <= 32 || (long)C * H >= 12000000)));
   // Losses of up to 256 tokens under a vocabulary with a tile of 128 classes for every second compute unit.  us packed / as it lies, 96 and 256 tokens:
   //   bf16 124416 x 2176 361 / 283, 423 / 313, 45376 x 1024 53 / 33, 74 / 42, 21701 x 300 20 / 18, 23 / 19, 10000 x 512 20 / 20, 23 / 21; fp32 45376 x 1024
   //   171 / 139, 217 / 181, 21701 x 300 31 / 27, 42 / 40, 1000 x 128 13 / 15

@@ -366,7 +366,7 @@ int cavs_softmax_xent_sums(float *loss, float *dlogits, const float *logits, con
  *   cavs_vocab_xent  both in one call
  * The vocabulary goes by in pieces; the logits are computed once for lse and once more for the gradients (up to 64 tokens: once in all).  The
  * workspace (16-byte aligned, of at least cavs_vocab_xent_workspace(type, n, H, C, grads) bytes on this device, grads = 0 for _fwd) holds the
- * d of one piece, all of the vocabulary only where that is 512 MB or less, and W of the piece, packed; it may be reused by the next call on the same stream, not by one that overlaps in time.  At most 2^20 rows,
+ * d of one piece, all of the vocabulary only where that is 512 MB or less, and W of the piece, packed (up to 64 tokens: z); it may be reused by the next call on the same stream, not by one that overlaps in time.  At most 2^20 rows,
  * 2^23 classes, H <= 2^16.  The workspace query returns 0 for a shape or type that is refused. */
 enum { CAVS_F32 = 0, CAVS_BF16 = 1 };
 size_t cavs_vocab_xent_workspace(int type, int n, int H, int C, int grads);

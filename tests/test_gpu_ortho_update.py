@@ -354,3 +354,50 @@ def test_a_workspace_that_is_too_small_or_crooked_is_refused():
             hip.call("cavs_ortho_update", 0, 1, d, options(), at, room, torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()
     assert (c.O[0] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,sizes", [("f32", [(9000, 40), (50, 60)]), ("bf16", [(17000, 30)])])
+def test_rows_far_apart(type_, sizes):
+    """Columns of tables of more than 2^32 bytes: gradients, momentum, weights and results"""
+    Case(21, type_, sizes, momentum=True, weights=True, pad=131000).go(options())
+
+
+@pytest.mark.gpu
+def test_recorded_calls_that_share_a_workspace():
+    """Two recorded updates replayed in turn through one workspace, the stretches' counters among what they share"""
+    cs = [Case(41, "f32", [(128, 512), (128, 512)], momentum=True, weights=True), Case(42, "bf16", [(300, 512), (64, 40)])]
+    o = options()
+    need = max(hip.lib().cavs_ortho_update_workspace(c.code, len(c.sizes), c.descs()) for c in cs)
+    ws = torch.full((need,), 0xff, dtype=torch.uint8, device="cuda")
+    start = [c.state() for c in cs]
+
+    def reset():
+        for c, s in zip(cs, start):
+            for t, v in zip([t for t in c.M + c.W + c.O if t is not None], s):
+                t.copy_(v)
+
+    def call(c):
+        hip.call("cavs_ortho_update", c.code, len(c.sizes), c.descs(), o, hip.ptr(ws), need, torch.cuda.current_stream().cuda_stream)
+
+    want = []
+    for c in cs:
+        call(c)
+        torch.cuda.synchronize()
+        want.append(c.state())
+    graphs = []
+    for c in cs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(c)
+        graphs.append(g)
+    for turn in range(3):
+        reset()
+        for g in graphs if turn != 1 else graphs[::-1]:
+            g.replay()
+        torch.cuda.synchronize()
+        for c, w in zip(cs, want):
+            assert all(torch.equal(a, b) for a, b in zip(c.state(), w)), turn
+        reset()
+        call(cs[turn % 2])
+        torch.cuda.synchronize()

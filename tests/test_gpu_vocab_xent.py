@@ -8,6 +8,8 @@ Every element is held to a bound that is computed for it, in units u = 2^-24 (ha
   sums   each term's error, and a rounding for every sixteen terms of the sum of their magnitudes, two more for stretches and pieces
   gradients   half a step of their type
 """
+import copy
+
 import numpy as np
 import pytest
 
@@ -450,3 +452,69 @@ def test_few_tokens_and_gradients_larger_than_a_cache(type_, n, H, C):
     c.call("cavs_vocab_xent", o, ws, need)
     c.check(o)
     assert (behind[C] == 7).all()
+
+
+# ------------------------------------------------------------------ rows so far apart that offsets pass 32 bits
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,n,C,pad", [("bf16", 5, 70001, 32700), ("bf16", 100, 70001, 32700), ("bf16", 300, 70001, 32700), ("f32", 64, 35001, 32700),
+                                           ("f32", 300, 35001, 32700)])
+def test_rows_of_a_table_far_apart(type_, n, C, pad):
+    """W and dW of more than 2^32 bytes, few columns of them the matrix's: with and without gradients"""
+    H = 61
+    c = Case(n + C, type_, n, H, C, ignored=0.2, masked=3, pad=(7, pad, 9, pad))
+    o, (ws, need) = c.outputs(), c.workspace(1)
+    c.call("cavs_vocab_xent", o, ws, need)
+    c.check(o)
+    h, (w0, need0) = c.outputs(), c.workspace(0)
+    c.call("cavs_vocab_xent_fwd", h, w0, need0)
+    c.check(h, ("loss", "lse"))
+
+
+@pytest.mark.gpu
+def test_a_million_rows():
+    """d of a piece of more than 2^32 bytes.  The definition row block by row block; a block's bounds on sums over rows are its share of all rows'."""
+    c = Case(77, "f32", 1000003, 32, 1030, ignored=0.1, masked=2)
+    o, (ws, need) = c.outputs(), c.workspace(1)
+    c.call("cavs_vocab_xent", o, ws, need)
+    total, bound, step = {}, {}, 125001
+    for r in range(0, c.n, step):
+        part = copy.copy(c)
+        part.X, part.labels = c.X[r:r + step], c.labels[r:r + step]
+        part.n = part.X.shape[0]
+        want, err = part.want()
+        for k in ("loss", "lse", "dX"):
+            got, w, e = (v if k == "loss" else v[(part.labels >= 0) & (part.labels < c.C)] for v in (o[k][r:r + step].double(), want[k], err[k]))
+            assert ((got - w).abs() <= e).all(), (k, r)
+        for k in ("dW", "db"):
+            total[k] = total.get(k, 0.0) + want[k]
+            bound[k] = bound.get(k, 0.0) + err[k] * (c.n / part.n)
+    for k in ("dW", "db"):
+        assert ((o[k].double() - total[k]).abs() <= bound[k]).all(), k
+
+
+@pytest.mark.gpu
+def test_recorded_calls_that_share_a_workspace():
+    """Two recorded calls, one large and one of few tokens, replayed in turn through one workspace with eager work between"""
+    cs = [Case(31, "f32", 500, 70, 900, weights=True), Case(32, "bf16", 20, 1040, 3000, weights=True), Case(33, "bf16", 900, 130, 2000)]
+    outs, need = [c.outputs() for c in cs], max(c.workspace(1)[1] for c in cs)
+    ws = torch.full((need,), 0xff, dtype=torch.uint8, device="cuda")
+    graphs, first = [], []
+    for c, o in zip(cs, outs):
+        c.call("cavs_vocab_xent", o, ws, need)
+        torch.cuda.synchronize()
+        first.append({k: v.clone() for k, v in o.items()})
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.call("cavs_vocab_xent", o, ws, need)
+        graphs.append(g)
+    for turn in range(3):
+        for o in outs:
+            for v in o.values():
+                v.fill_(3.0)
+        for g in graphs if turn != 1 else graphs[::-1]:
+            g.replay()
+        torch.cuda.synchronize()
+        for o, f in zip(outs, first):
+            assert all(torch.equal(o[k], f[k]) for k in o), turn
+        cs[turn].call("cavs_vocab_xent", outs[turn], ws, need)
+        torch.cuda.synchronize()

@@ -103,13 +103,13 @@ __device__ __forceinline__ bf16x8 turned_piece(const char *from, int lane) {
 }
 
 // acc[ACC][TM][TN] of the tile at rows m0 of A and n0 of B over k in [kbeg, kend), both multiples of BK.  S: T::LDS bytes.
-// TURNED: what is given is A^T, packed with A's rows as its k and with all of A's k as rows (its last block of rows whole, and as many as kend
+// TA: what is given is A^T, packed with A's rows as its k and with all of A's k as rows (its last block of rows whole, and as many as kend
 // asks for).  A step's half blocks of 16 of its rows by 16 k, 512 bytes, come to LDS row by row, and the transposing load makes of four neighbouring
 // values of four rows, sixteen lanes at a time, four k of sixteen rows of A.  (Bit 7 of a place is turned over by bit 3 of the row and
-// bit 4 of k: of the four groups of lanes no two that could go together meet in a bank.)
+// bit 4 of k: of the four groups of lanes no two that could go together meet in a bank.)  TB: the same of B.
 // NS stages in a ring: while one is multiplied the others are on their way from memory; a step's one barrier says that the stage to come
 // has arrived and that nobody reads the one before it any more, so that its place takes the load of the stage NS - 1 ahead.
-template <class T, bool TURNED = false>
+template <class T, bool TA = false, bool TB = false>
 __device__ __forceinline__ void nt_multiply(const PackedRef &A, int M, int m0, const PackedRef &B, int N, int n0, int kbeg, int kend, char *S,
                                             floatx16 (&acc)[T::ACC][T::TM][T::TN]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -126,44 +126,40 @@ __device__ __forceinline__ void nt_multiply(const PackedRef &A, int M, int m0, c
   // Blocks c = 0, 1, .. of a stage, in the order they have in memory: row of blocks by row of blocks, step by step, part by part.  This wavefront
   // loads every WAVES-th, each lane the 16 bytes it will read.
   constexpr int PER = T::P * T::STEPS;
-  unsigned sa[T::CA], sb[T::CB], la[T::CA];
+  unsigned sa[T::CA], sb[T::CB], la[T::CA], lb[T::CB];
   const long rowa = (long)(A.K / 16) * T::P * 1024, rowb = (long)(B.K / 16) * T::P * 1024;
-#pragma unroll
-  for (int c = 0; c < T::CA; c++) {
-    const int at = c * T::WAVES + wave;
-    if constexpr (!TURNED) {
-      la[c] = 16 * lane;
-      sa[c] = (unsigned)min(at / PER, (M - 1 - m0) / 32) * (unsigned)rowa + at % PER * 1024;
-    } else {
-      // two half blocks, of neighbouring sixteens of rows: step by step, part by part, down the tile
-      const int which = at / (T::BM / 32), step = which / T::P, sixteen = at % (T::BM / 32) * 2 + (lane >> 5), place = lane & 31;
+  auto source = [&](bool turned, int at, int blocks, int K, int rows, int first, unsigned row, unsigned *of_lane, unsigned *of_wave) {
+    if (!turned) {
+      *of_lane = 16 * lane;
+      *of_wave = (unsigned)min(at / PER, (rows - 1 - first) / 32) * row + at % PER * 1024;
+    } else {  // two half blocks, of neighbouring sixteens of rows: step by step, part by part, down the tile
+      const int which = at / blocks, step = which / T::P, sixteen = at % blocks * 2 + (lane >> 5), place = lane & 31;
       const int here = place ^ 8 * ((place >> 4) ^ (lane >> 5));
-      la[c] = min(sixteen, A.K / 16 - 1 - m0 / 16) * (T::P * 1024) + (here & 1) * 512 + (here >> 1) * 16;
-      sa[c] = (step >> 1) * (unsigned)rowa + (step & 1) * 256 + which % T::P * 1024;
+      *of_lane = min(sixteen, K / 16 - 1 - first / 16) * (T::P * 1024) + (here & 1) * 512 + (here >> 1) * 16;
+      *of_wave = (step >> 1) * row + (step & 1) * 256 + which % T::P * 1024;
     }
-  }
+  };
 #pragma unroll
-  for (int c = 0; c < T::CB; c++) {
-    const int at = c * T::WAVES + wave;
-    sb[c] = (unsigned)min(at / PER, (N - 1 - n0) / 32) * (unsigned)rowb + at % PER * 1024;
-  }
-  [[maybe_unused]] const char *pa = reinterpret_cast<const char *>(A.p) + (TURNED ? kbeg / 32 * rowa + (long)(m0 / 16) * (T::P * 1024)
-                                                                                : m0 / 32 * rowa + (long)(kbeg / 16) * (T::P * 1024));
-  [[maybe_unused]] const char *pb = reinterpret_cast<const char *>(B.p) + n0 / 32 * rowb + (long)(kbeg / 16) * (T::P * 1024);
+  for (int c = 0; c < T::CA; c++) source(TA, c * T::WAVES + wave, T::BM / 32, A.K, M, m0, (unsigned)rowa, &la[c], &sa[c]);
+#pragma unroll
+  for (int c = 0; c < T::CB; c++) source(TB, c * T::WAVES + wave, T::BN / 32, B.K, N, n0, (unsigned)rowb, &lb[c], &sb[c]);
+  auto begin = [&](bool turned, const u16 *p, int first, long row) {
+    return reinterpret_cast<const char *>(p) + (turned ? kbeg / 32 * row + (long)(first / 16) * (T::P * 1024) : first / 32 * row + (long)(kbeg / 16) * (T::P * 1024));
+  };
+  [[maybe_unused]] const char *pa = begin(TA, A.p, m0, rowa), *pb = begin(TB, B.p, n0, rowb);
 
   auto fetch = [&](int kt, char *to) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass knows no such load)
-    const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(TURNED ? pa + (long)(kt * T::STEPS / 2) * rowa : pa), 0, 0xffffffffu, 0x00020000);
-    const unsigned offa = TURNED ? kt * T::STEPS % 2 * 256 : (unsigned)kt * (PER * 1024);
-    const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pb), 0, 0xffffffffu, 0x00020000);
-    const unsigned off = (unsigned)kt * (PER * 1024);
+    const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(TA ? pa + (long)(kt * T::STEPS / 2) * rowa : pa), 0, 0xffffffffu, 0x00020000);
+    const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(TB ? pb + (long)(kt * T::STEPS / 2) * rowb : pb), 0, 0xffffffffu, 0x00020000);
+    const unsigned on = (unsigned)kt * (PER * 1024), half = kt * T::STEPS % 2 * 256;
 #pragma unroll
     for (int c = 0; c < T::CA; c++)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void *)(to + (c * T::WAVES + wave) * 1024), 16, la[c], sa[c] + offa, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void *)(to + (c * T::WAVES + wave) * 1024), 16, la[c], sa[c] + (TA ? half : on), 0, 0);
 #pragma unroll
     for (int c = 0; c < T::CB; c++)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void *)(to + T::PA + (c * T::WAVES + wave) * 1024), 16, 16 * lane, sb[c] + off,
-                                               0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void *)(to + T::PA + (c * T::WAVES + wave) * 1024), 16, lb[c],
+                                               sb[c] + (TB ? half : on), 0, 0);
 #endif
   };
   const int a0 = wm * (T::WM / 32) * T::ROWB + 16 * lane, b0 = T::PA + wn * (T::WN / 32) * T::ROWB + 16 * lane;
@@ -175,11 +171,15 @@ __device__ __forceinline__ void nt_multiply(const PackedRef &A, int M, int m0, c
       bf16x8 a[T::TM];
 #pragma unroll
       for (int i = 0; i < T::TM; i++) {
-        if constexpr (!TURNED) a[i] = *reinterpret_cast<const bf16x8 *>(from + a0 + (i * T::ROWB + (s * T::P + p) * 1024));
+        if constexpr (!TA) a[i] = *reinterpret_cast<const bf16x8 *>(from + a0 + (i * T::ROWB + (s * T::P + p) * 1024));
         else a[i] = turned_piece(from + wm * (T::WM / 32) * 1024 + ((s * T::P + p) * (T::BM / 32) + i) * 1024, lane);
       }
 #pragma unroll
-      for (int j = 0; j < T::TN; j++) b[T::P - 1 - p][j] = *reinterpret_cast<const bf16x8 *>(from + b0 + (j * T::ROWB + (s * T::P + T::P - 1 - p) * 1024));
+      for (int j = 0; j < T::TN; j++) {
+        const int q = T::P - 1 - p;
+        if constexpr (!TB) b[q][j] = *reinterpret_cast<const bf16x8 *>(from + b0 + (j * T::ROWB + (s * T::P + q) * 1024));
+        else b[q][j] = turned_piece(from + T::PA + wn * (T::WN / 32) * 1024 + ((s * T::P + q) * (T::BN / 32) + j) * 1024, lane);
+      }
 #pragma unroll
       for (int q = T::P - 1 - p; q >= 0; q--)
 #pragma unroll

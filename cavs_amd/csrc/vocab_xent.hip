@@ -18,10 +18,10 @@ namespace cavs {
 namespace {
 
 // ------------------------------------------------------------------ operands, packed
-// src [rows, K] with its columns as k and, for the products that sum over its rows, with its rows as k.  Either may be left out.  A row that
-// takes no part by its flag is zero in the second: 0 times what it holds need not be 0.  There a row may come times a weight, rounded once more to
-// the type: in X's elements those roundings are independent of each other, in d each would be one of all of a token's d.
-enum { KEEP_ALL = 0, KEEP_LABELLED = 1, KEEP_FINITE = 2 };  // rows whose flag is a class id below `classes`; rows whose flag is not -inf
+// src [rows, K] with its columns as k and, for a product that sums over them, with its rows as k; either may be left out.  What takes no part is zero
+// where it is summed over, as 0 times what it holds need not be 0: a row whose bias is -inf (its z is -inf whatever is there), and in X's second order a row
+// without a class.  There a row may come times a weight, rounded once more to the type: in X's elements those roundings are independent of each other, in d each would be
+// one of all of a token's d.
 __device__ inline bool is_class(float label, int classes) { return label >= 0.f && label < (float)classes; }
 
 struct PackJob {
@@ -29,10 +29,11 @@ struct PackJob {
   long ld;
   int rows, K;
   PackedOut o, t;
-  const float *flag;
-  int keep, classes;
-  const float *weight;  // or null
-  int across, blocks;   // blocks of 64 columns, of 64 x 64
+  int orows;                      // rows of o, zero beyond those of src
+  const float *bias;              // of rows, or null
+  const float *labels, *weight;   // of rows, for t, or null
+  int classes;
+  int across, blocks;             // blocks of 64 columns, of 64 x 64
 };
 
 template <int P, class Src>
@@ -45,15 +46,22 @@ __global__ __launch_bounds__(256) void pack_kernel(PackJob j0, PackJob j1) {
   const Src *src = static_cast<const Src *>(g.src);
   load_tile(tile, src, g.ld, r0, k0, g.rows, g.K);
   __syncthreads();
-  pack_tile<P>(tile, g.o, g.keep == KEEP_ALL ? g.t : PackedOut{}, r0, k0, g.rows, g.K);
-  if (!g.t.p || g.keep == KEEP_ALL) return;
-  __syncthreads();
-  for (int i = threadIdx.x >> 6; i < 64; i += 4)
-    if (r0 + i < g.rows) {
-      if (g.keep == KEEP_LABELLED ? !is_class(g.flag[r0 + i], g.classes) : g.flag[r0 + i] == -INFINITY) tile[i][k] = 0.f;
-      else if (g.weight) tile[i][k] *= g.weight[r0 + i];
-    }
-  __syncthreads();
+  if (g.bias) {
+    for (int i = threadIdx.x >> 6; i < 64; i += 4)
+      if (r0 + i < g.rows && g.bias[r0 + i] == -INFINITY) tile[i][k] = 0.f;
+    __syncthreads();
+  }
+  pack_tile<P>(tile, g.o, PackedOut{}, r0, k0, g.orows, g.K);
+  if (!g.t.p) return;
+  if (g.labels) {
+    __syncthreads();
+    for (int i = threadIdx.x >> 6; i < 64; i += 4)
+      if (r0 + i < g.rows) {
+        if (!is_class(g.labels[r0 + i], g.classes)) tile[i][k] = 0.f;
+        else if (g.weight) tile[i][k] *= g.weight[r0 + i];
+      }
+    __syncthreads();
+  }
   pack_tile<P>(tile, PackedOut{}, g.t, r0, k0, g.rows, g.K);
 }
 
@@ -784,8 +792,8 @@ struct ProductJob {
   const float *factor;  // of out's rows, or null
 };
 
-// STREAM: `out` goes past the caches
-template <class T, class Out, bool STREAM>
+// STREAM: `out` goes past the caches.  TB: W by class.
+template <class T, class Out, bool STREAM, bool TB>
 __global__ __launch_bounds__(T::THREADS, T::EU) void product_kernel(ProductJob<Out> j0, ProductJob<Out> j1, int blocks0) {
   __shared__ __attribute__((aligned(16))) char S[T::LDS];
   const bool second = (int)blockIdx.x >= blocks0;
@@ -796,7 +804,7 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void product_kernel(ProductJob<O
   const int m0 = tm * T::BM, n0 = tn * T::BN, kbeg = split * g.kchunk, kend = min(g.K, kbeg + g.kchunk);
   floatx16 acc[T::ACC][T::TM][T::TN];
   if (second) nt_multiply<T, true>(g.A, g.M, m0, g.B, g.N, n0, kbeg, kend, S, acc);
-  else nt_multiply<T>(g.A, g.M, m0, g.B, g.N, n0, kbeg, kend, S, acc);
+  else nt_multiply<T, false, TB>(g.A, g.M, m0, g.B, g.N, n0, kbeg, kend, S, acc);
   const Where<T> w;
   float *part = g.part ? g.part + (long)split * g.M * g.N : nullptr;
 #pragma unroll
@@ -954,6 +962,7 @@ struct Plan {
   int few;  // tokens: W read where it lies, z kept for the gradients
   int raw;  // losses of not many tokens: W read where it lies
   int facross;  // few_dx_kernel's
+  int one_order;  // W packed by class alone
   int grads, keep, psize, pm, pn, xsplits, xchunk, wsplits, wchunk;
   size_t stats, zlabel, lse, weight, z, x, w, xt, wt, d, sums, xpart, wpart, bytes;
 };
@@ -998,7 +1007,7 @@ Plan plan_of(int n, int H, int C, int grads) {
   p.weight = take((size_t)n * 4);
   p.z = take(p.few && grads ? (size_t)tiles_of(C, 32) * tiles_of(n, 32) * 4096 : 0);
   p.x = take(p.few && n <= 32 ? 0 : packed_bytes<P>(n, p.Hp));
-  p.w = take(p.few || p.raw ? 0 : packed_bytes<P>(grads && p.keep ? C : rows, p.Hp));
+  p.w = take(p.few || p.raw ? 0 : packed_bytes<P>(ceil_to(grads && p.keep ? C : rows, kPlaneAlign), p.Hp));
   if (grads) {
     const int rp = ceil_to(rows, kPlaneAlign);
     p.psize = tile_size<P>((long)rows + n, H);
@@ -1035,7 +1044,11 @@ Plan plan_of(int n, int H, int C, int grads) {
       p.xsplits = (rp + p.xchunk - 1) / p.xchunk;
     }
     p.xt = take(packed_bytes<P>(H, p.np));
-    p.wt = take(p.few ? 0 : packed_bytes<P>(H, rp));
+    // W in one order, d W reading it by transposing loads, or packed with its classes as k too, whichever costs less.  us of a call, one order / two: bf16
+    // 30000 x 1024 with 512 tokens 243 / 258, 1000 375 / 387, 2000 633 / 631, 3000 899 / 864; 50000 x 2048 with 1000 1042 / 1063, 4096 3317 / 3295; 128000 x
+    // 4096 with 8192 32500 / 31450; 10000 x 512 with 7000 429 / 442; fp32 45376 x 1024 with 96 430 / 480, 10000 x 512 with 7088 1555 / 1556.
+    p.one_order = P == 3 || n <= 2000 || H <= 512 || p.psize == 0;
+    p.wt = take(p.few || p.one_order ? 0 : packed_bytes<P>(H, rp));
     p.d = take(packed_bytes<P>(p.np, rp));
     p.sums = take((size_t)tiles_of(n, p.bn) * C * 4);
     p.xpart = take((size_t)p.xsplits * n * H * 4);
@@ -1045,9 +1058,10 @@ Plan plan_of(int n, int H, int C, int grads) {
   return p;
 }
 
-inline PackJob pack_job(const void *src, long ld, int rows, int K, PackedOut o, PackedOut t, const float *flag, int keep, int classes, const float *weight) {
-  const int across = tiles_of(K, 64);
-  return {src, ld, rows, K, o, t, flag, keep, classes, weight, across, o.p || t.p ? across * tiles_of(rows, 64) : 0};
+inline PackJob packing(PackJob j) {
+  j.across = tiles_of(j.K, 64);
+  j.blocks = j.o.p || j.t.p ? j.across * tiles_of(j.rows, 64) : 0;
+  return j;
 }
 template <int P, class Src>
 void pack(const PackJob &a, const PackJob &b, hipStream_t st) {
@@ -1072,17 +1086,16 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
   const bool keep = p.grads && p.keep, one = p.pieces == 1;
   float *lse = c.lse ? c.lse : f32(p.lse), *weight = f32(p.weight);
   auto piece_w = [&](int c0) { return PackedOut{pl(p.w + (keep ? packed_bytes<P>(c0, p.Hp) : 0)), p.Hp}; };
-  auto piece_wt = [&](int rows) { return PackedOut{c.dX ? pl(p.wt) : nullptr, ceil_to(rows, kPlaneAlign)}; };
   auto rows_of = [&](int c0) { return C - c0 < p.piece ? C - c0 : p.piece; };
+  auto piece_wt = [&](int rows) { return c.dX && !p.one_order ? PackedOut{pl(p.wt), ceil_to(rows, kPlaneAlign)} : none; };
   auto job_w = [&](int c0, bool o, bool t) {
     const int rows = rows_of(c0);
-    return pack_job(static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, rows, H, o && !p.raw && !p.few ? piece_w(c0) : none,
-                    t && p.grads && !p.few ? piece_wt(rows) : none,
-                    c.b ? c.b + c0 : nullptr, c.b ? KEEP_FINITE : KEEP_ALL, 0, nullptr);
+    return packing({static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, rows, H, o && !p.raw ? piece_w(c0) : none, t && p.grads ? piece_wt(rows) : none,
+                    ceil_to(rows, kPlaneAlign), c.b ? c.b + c0 : nullptr, nullptr, nullptr, 0, 0, 0});
   };
   const PackedOut xt{p.grads && c.dW ? pl(p.xt) : nullptr, p.np};
   // X in one launch with what there is of W by then
-  PackJob jx = pack_job(c.X, c.ldx, n, H, p.few && n <= 32 ? none : X, xt, c.labels, KEEP_LABELLED, C, c.dloss);
+  PackJob jx = packing({c.X, c.ldx, n, H, p.few && n <= 32 ? none : X, xt, n, nullptr, c.labels, c.dloss, C, 0, 0});
   auto tile_args = [&](int c0) {
     const int rows = rows_of(c0);
     return TileArgs{ref(piece_w(c0)), ref(X), rows, n, p.Hp, tiles_of(rows, p.bm), tiles_of(n, p.bn), c.b ? c.b + c0 : nullptr, c.labels, c0,
@@ -1120,11 +1133,10 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
     for (int c0 = 0; c0 < C; c0 += p.piece, first = false) {
       const int rows = rows_of(c0), rp = ceil_to(rows, kPlaneAlign);
       // (what the first pass packed may still be there)
-      const bool here = !c.lse_given && one;
-      if (!here && !p.few) pack<P, Src>(jx, job_w(c0, c.lse_given || !keep, true), st);
+      if (!p.few) pack<P, Src>(jx, job_w(c0, c.lse_given || !(keep || one), c.lse_given || !one), st);
       jx = PackJob{};
       const TileArgs a = tile_args(c0);
-      const PackedOut d{c.dX || c.dW ? pl(p.d) : nullptr, rp}, wt = piece_wt(rows);
+      const PackedOut d{c.dX || c.dW ? pl(p.d) : nullptr, rp};
       if (p.few && (d.p || c.db)) {
         const FewLogitsArgs f{f32(p.z), all, weight, c.labels, n, C, c0, d, rp / 32, c.db ? c.db + c0 : nullptr, c.scale};
         launch(few_dlogits_kernel<P>, (rp / 32 + 3) / 4, 256, 0, st, f);
@@ -1142,7 +1154,7 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
       };
       ProductJob<Src> px{}, pw{};
       // (a last piece shorter than the others fills fewer stretches: those beyond keep what they have)
-      if (c.dX && !p.few) px = job(d, wt, n, rp, p.xchunk, x_parts ? f32(p.xpart) : nullptr, !first, c.dX, c.lddx, weight);
+      if (c.dX && !p.few) px = job(d, p.one_order ? piece_w(c0) : piece_wt(rows), n, rp, p.xchunk, x_parts ? f32(p.xpart) : nullptr, !first, c.dX, c.lddx, weight);
       Src *dW = c.dW ? static_cast<Src *>(c.dW) + (long)c0 * c.lddw : nullptr;
       if (c.dW) pw = job(d, xt, rows, p.np, p.wchunk, w_parts ? f32(p.wpart) : nullptr, false, dW, c.lddw, nullptr);
       // (d W of more than the last cache holds, in whole lines of 128 bytes: bf16 124416 x 2176, 64 tokens 533 us of a call, streaming 469, 81664 x 4096, 12
@@ -1153,8 +1165,10 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
         with_product_tile<P>(p.psize, [&](auto t) {
           using T = decltype(t);
           if constexpr (std::is_same_v<T, typename Tiles<P>::L>)  // (so large a d W has tiles enough)
-            if (stream) return launch(product_kernel<T, Src, true>, bx + bw, T::THREADS, 0, st, px, pw, bx), 0;
-          launch(product_kernel<T, Src, false>, bx + bw, T::THREADS, 0, st, px, pw, bx);
+            if (stream) return launch(product_kernel<T, Src, true, true>, bx + bw, T::THREADS, 0, st, px, pw, bx), 0;
+          if constexpr (P == 1 && !std::is_same_v<T, typename Tiles<P>::S>)
+            if (!p.one_order) return launch(product_kernel<T, Src, false, false>, bx + bw, T::THREADS, 0, st, px, pw, bx), 0;
+          launch(product_kernel<T, Src, false, true>, bx + bw, T::THREADS, 0, st, px, pw, bx);
           return 0;
         });
       if (c.dX && p.few) {

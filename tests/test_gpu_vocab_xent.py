@@ -518,3 +518,20 @@ def test_recorded_calls_that_share_a_workspace():
             assert all(torch.equal(o[k], f[k]) for k in o), turn
         cs[turn].call("cavs_vocab_xent", outs[turn], ws, need)
         torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,H,C", [(2001, 513, 40), (2050, 600, 3001), (2100, 515, 9000), (2300, 1030, 300)])
+def test_many_tokens_and_long_rows(n, H, C):
+    """W packed in two orders: with gradients alone, all at once and in halves; masked classes whose rows hold no numbers"""
+    c = Case(n + C, "bf16", n, H, C, ignored=0.2, masked=3, weights=True, pad=(1, 3, 2, 0))
+    c.W[C - 3:, ::2] = float("nan")
+    o, (ws, need) = c.outputs(), c.workspace(1)
+    c.call("cavs_vocab_xent", o, ws, need)
+    c.check(o)
+    h = c.outputs()
+    h["lse"].copy_(o["lse"])
+    ws.fill_(0xff)
+    c.call("cavs_vocab_xent_bwd", h, ws, need)
+    torch.cuda.synchronize()
+    assert all(torch.equal(h[k], o[k]) for k in ("dX", "dW", "db"))

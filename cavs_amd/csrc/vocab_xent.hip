@@ -980,12 +980,12 @@ Plan plan_of(int n, int H, int C, int grads) {
   const int rows = p.piece < C ? p.piece : C;
   // Few tokens: W read where it lies and z kept, packing W and making z twice would be most of the work.  Gradients take two launches more that way, which
   // long rows or many classes pay for.  us with gradients packed / as it lies, 1, 24 and 64 tokens:
-  //   fp32  300 x 1024 56 / 39, 57 / 42, 58 / 48   1000 x 512 43 / 36, 43 / 39, 44 / 44   12000 x 300 61 / 58, 63 / 62, 65 / 68   21701 x 300 78 / 73, 84 / 78,
-  //         91 / 85   12000 x 512 76 / 63, 78 / 67, 82 / 72   32000 x 128 79 / 65, 82 / 72, 84 / 79   40806 x 4050 1574 / 681 (12)
-  //   bf16  1000 x 512 31 / 31, 32 / 34, 31 / 42   4000 x 1024 53 / 40, 53 / 44, 53 / 56   12000 x 1024 68 / 56, 71 / 67, 73 / 73   32000 x 128 54 / 52, 57 / 59,
-  //         59 / 63   81792 x 72 95 / 79, 99 / 86, 100 / 94   124416 x 2176 915 / 469 (64)
+  //   fp32  300 x 1024 53 / 39, 54 / 42, 57 / 47   1000 x 512 41 / 36, 42 / 39, 44 / 43   12000 x 300 58 / 57, 61 / 60, 63 / 66   21701 x 300 79 / 72, 81 / 77,
+  //         87 / 82   12000 x 512 70 / 61, 72 / 65, 77 / 71   32000 x 128 79 / 64, 82 / 71, 84 / 77   40806 x 4050 1417 / 679 (12)
+  //   bf16  1000 x 512 28 / 30, 30 / 33, 31 / 41   4000 x 1024 49 / 39, 48 / 43, 51 / 55   12000 x 1024 63 / 56, 64 / 64, 66 / 71   32000 x 128 54 / 51, 57 / 59,
+  //         59 / 63   81792 x 72 95 / 78, 99 / 85, 100 / 93   124416 x 2176 858 / 475 (64)
   const bool many = C >= 128 * num_cus();
-  p.few = n <= kFewRows && (!grads || many || (P == 3 ? H >= 512 || (long)C * H >= 5000000 : H >= 1024 && (n <= 32 || (long)C * H >= 12000000)));
+  p.few = n <= kFewRows && (!grads || many || (P == 3 ? H >= 512 || (long)C * H >= 5000000 : H >= 1024 && (n <= 32 || (long)C * H >= 16000000)));
   // Losses of up to 256 tokens under a vocabulary with a tile of 128 classes for every second compute unit.  us packed / as it lies, 96 and 256 tokens:
   //   bf16 124416 x 2176 361 / 283, 423 / 313, 45376 x 1024 53 / 33, 74 / 42, 21701 x 300 20 / 18, 23 / 19, 10000 x 512 20 / 20, 23 / 21; fp32 45376 x 1024
   //   171 / 139, 217 / 181, 21701 x 300 31 / 27, 42 / 40, 1000 x 128 13 / 15
@@ -1046,8 +1046,9 @@ Plan plan_of(int n, int H, int C, int grads) {
     p.xt = take(packed_bytes<P>(H, p.np));
     // W in one order, d W reading it by transposing loads, or packed with its classes as k too, whichever costs less.  us of a call, one order / two: bf16
     // 30000 x 1024 with 512 tokens 243 / 258, 1000 375 / 387, 2000 633 / 631, 3000 899 / 864; 50000 x 2048 with 1000 1042 / 1063, 4096 3317 / 3295; 128000 x
-    // 4096 with 8192 32500 / 31450; 10000 x 512 with 7000 429 / 442; fp32 45376 x 1024 with 96 430 / 480, 10000 x 512 with 7088 1555 / 1556.
-    p.one_order = P == 3 || n <= 2000 || H <= 512 || p.psize == 0;
+    // 4096 with 8192 32500 / 31450; 10000 x 512 with 7000 429 / 442; fp32 45376 x 1024 with 96 430 / 480, 10000 x 512 with 7088 1555 / 1556.  Narrow rows and
+    // few tokens, a tile or three of d W, each a long way: fp32 81792 x 72 with 96 177 / 152, 300 276 / 270, 1000 635 / 675; bf16 112 / 103 with 96.
+    p.one_order = (H > 128 || n > 512) && (P == 3 || n <= 2000 || H <= 512);
     p.wt = take(p.few || p.one_order ? 0 : packed_bytes<P>(H, rp));
     p.d = take(packed_bytes<P>(p.np, rp));
     p.sums = take((size_t)tiles_of(n, p.bn) * C * 4);
@@ -1166,9 +1167,8 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
           using T = decltype(t);
           if constexpr (std::is_same_v<T, typename Tiles<P>::L>)  // (so large a d W has tiles enough)
             if (stream) return launch(product_kernel<T, Src, true, true>, bx + bw, T::THREADS, 0, st, px, pw, bx), 0;
-          if constexpr (P == 1 && !std::is_same_v<T, typename Tiles<P>::S>)
-            if (!p.one_order) return launch(product_kernel<T, Src, false, false>, bx + bw, T::THREADS, 0, st, px, pw, bx), 0;
-          launch(product_kernel<T, Src, false, true>, bx + bw, T::THREADS, 0, st, px, pw, bx);
+          if (p.one_order) launch(product_kernel<T, Src, false, true>, bx + bw, T::THREADS, 0, st, px, pw, bx);
+          else launch(product_kernel<T, Src, false, false>, bx + bw, T::THREADS, 0, st, px, pw, bx);
           return 0;
         });
       if (c.dX && p.few) {

@@ -10,14 +10,14 @@
 // A packed operand [rows, K] is blocks of 32 rows by 16 k, 1 KB a part: lane l of a wavefront finds its piece for the 32x32x16 instruction,
 // eight k of row l % 32, at byte 16 l.  Blocks follow each other part by part, then along k, then along the rows.  So a wavefront's load is 1 KB in
 // one piece, and LDS is read in the order it was written.  (Rows of bf16 as they lie in memory, 32 or 128 bytes of each to a tile: the loads of a
-// 128 x 128 x 16 tile alone took 2277 us of 7088 x 4096 x 3584, all of it takes 836 now.)  K is padded with zeros to whole steps: the loops
+// 128 x 128 x 16 tile alone took 2277 us of 7088 x 4096 x 3584, all of it takes 865 now.)  K is padded with zeros to whole steps: the loops
 // below know no k that is not there.  Blocks of rows beyond the last read the last one again; what comes of them is not stored.
 //
 // A workgroup is four wavefronts and its LDS two stages, so that a CU holds three of them that know nothing of each other: while one waits
 // for its loads the others multiply.  TFLOP/s of the bf16 pipe, random operands (power holds the clock at 1.9 GHz):
-//   one part     8192 x 8192 x 4096   256 x 128 x 32 1287    256 x 256 x 32, eight wavefronts, five stages 1162    128 x 128 x 32 1240
-//   three parts  7088 x 4096 x 3584   128 x 128 x 16 1493 (249 of the fp32 product)   256 x 128 x 32, eight wavefronts 1329
-//   two parts    4096 x 4096 x 4096   128 x 128 x 16, three stages 1355   256 x 128 x 32, eight wavefronts 1344
+//   one part     8192 x 8192 x 4096   256 x 128 x 32 1342    256 x 256 x 32, eight wavefronts 1349    128 x 128 x 32 1213
+//   three parts  7088 x 4096 x 3584   128 x 128 x 16 1444 (241 of the fp32 product)   256 x 128 x 32, eight wavefronts 1351
+//   two parts    4096 x 4096 x 4096   128 x 128 x 16, three stages 1323   256 x 128 x 32, eight wavefronts 1369 (too few tiles of smaller matrices)
 #pragma once
 #include "gemm_common.h"
 

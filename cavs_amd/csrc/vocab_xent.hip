@@ -6,7 +6,7 @@
 // The vocabulary goes by in pieces.  The first pass over them makes each tile of z in registers and leaves a maximum and a sum of
 // exponentials per row and tile; what they come to together is lse.  The second makes the tile again, d from it, and leaves d of a piece,
 // packed by token, which d X and d W are made of before the next piece overwrites it.  (d^T is read from the same bytes: packed in both orders, half
-// as many classes to a piece, fp32 10000 x 512 with 7088 tokens took 1869 us, and takes 1608.)
+// as many classes to a piece, fp32 10000 x 512 with 7088 tokens took 1869 us, and takes 1520.)
 // Statistics, sums and accumulators are fp32; d is rounded to bf16 where the gradients are (half a unit of 2^-8, as their own
 // rounding), and is three bf16 parts, all of an fp32's bits, where they are fp32.
 #include <type_traits>
@@ -20,8 +20,8 @@ namespace {
 // ------------------------------------------------------------------ operands, packed
 // src [rows, K] with its columns as k and, for a product that sums over them, with its rows as k; either may be left out.  What takes no part is zero
 // where it is summed over, as 0 times what it holds need not be 0: a row whose bias is -inf (its z is -inf whatever is there), and in X's second order a row
-// without a class.  There a row may come times a weight, rounded once more to the type: in X's elements those roundings are independent of each other, in d each would be
-// one of all of a token's d.
+// without a class.
+// `weight`: up to 64 bf16 rows come times their weights as two parts, the second behind the first along k (see dlogits_kernel).
 __device__ inline bool is_class(float label, int classes) { return label >= 0.f && label < (float)classes; }
 
 struct PackJob {
@@ -63,6 +63,16 @@ __global__ __launch_bounds__(256) void pack_kernel(PackJob j0, PackJob j1) {
     __syncthreads();
   }
   pack_tile<P>(tile, PackedOut{}, g.t, r0, k0, g.rows, g.K);
+  if constexpr (P == 1) {
+    if (!g.weight) return;
+    __syncthreads();
+    for (int i = threadIdx.x >> 6; i < 64; i += 4) {
+      const float rest = tile[i][k] - bf16_float(bf16_bits(tile[i][k]));
+      tile[i][k] = fabsf(rest) < INFINITY ? rest : 0.f;
+    }
+    __syncthreads();
+    pack_tile<P>(tile, PackedOut{}, g.t, r0 + 64, k0, g.rows, g.K);
+  }
 }
 
 // ------------------------------------------------------------------ the tile of z
@@ -484,13 +494,13 @@ __global__ __launch_bounds__(256) void weights_kernel(const float *__restrict__ 
   if (row < n) weight[row] = weight_of(labels[row], lse[row], dloss, row, C);
 }
 
-// e = p - [label] of a tile, packed by token (zero between the last class or token and the end of the steps, and of a token without weight), and the
-// sums of d = weight * e over the tile's tokens.
-// What multiplies all of a row's d, or all of d, stays out of what is rounded: next to the label, where p is small, e is -1 and a bit, which bf16
-// holds well, while any factor in it is a rounding error that all of its kind share.  d W takes the weights as factors of its rows, d^T X with X.
+// d = weight * (p - [label]) of a tile, packed by token (zero between the last class or token and the end of the steps), and its sums over the tile's
+// tokens.  `scale`, which multiplies all of d, stays out of what is rounded: next to the label, where p is small, p - 1 is -1 and a bit, which bf16 holds
+// well, while a factor in it is a rounding error that all of its kind share.  So is a token's weight for that token, which many tokens average out: of up to 64
+// bf16 ones (`beside`) it stays out as well.  d W has it as a factor of its rows then, and d^T X with X, in two parts, for which d is there twice.
 template <class T>
 __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, const float *__restrict__ lse, const float *__restrict__ weight, PackedOut d,
-                                                                    float *__restrict__ sums, int ld_sums, float sums_scale) {
+                                                                    float *__restrict__ sums, int ld_sums, float sums_scale, int beside) {
   __shared__ __attribute__((aligned(16))) char S[T::LDS];
   int m0, n0, tn;
   floatx16 acc[T::ACC][T::TM][T::TN];
@@ -526,12 +536,17 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, 
         for (int r = 0; r < 16; r++) x[r] -= at[j] == 32 * i + 8 * (r >> 2) + (r & 3) ? 1.f : 0.f;
       }
 #pragma unroll
-      for (int r = 0; r < 16; r++) sum[r] += g[j] * x[r];
+      for (int r = 0; r < 16; r++) {
+        const float v = g[j] * x[r];
+        sum[r] += v;
+        if (T::P > 1 || !beside) x[r] = v;
+      }
       if (d.p && 32 * xb < tokens && 32 * cb < d.K) {
         Parts16<T::P> e;
 #pragma unroll
         for (int r = 0; r < 16; r++) parts_of<T::P>(x[r], e.v[r]);
         put_rows<T::P>(d, xb, cb, e, w.lane);
+        if (T::P == 1 && beside) put_rows<T::P>(d, xb + 2, cb, e, w.lane);
         asm volatile("" ::: "memory");  // (one block after the other: a lane has no registers for two)
       }
     }
@@ -556,8 +571,8 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, 
 }
 
 // ------------------------------------------------------------------ the gradients of few tokens
-// e of up to 64 tokens from the z that direct_stats_kernel left (a float a token and class, beside W's row of H), packed as dlogits_kernel packs it,
-// and d's sums over the tokens.  A wavefront has a block of 32 classes.
+// d of up to 64 tokens from the z that direct_stats_kernel left (a float a token and class, beside W's row of H), packed as dlogits_kernel packs it,
+// and its sums over the tokens.  A wavefront has a block of 32 classes.
 struct FewLogitsArgs {
   const float *z;
   const float *lse, *weight, *labels;
@@ -566,6 +581,7 @@ struct FewLogitsArgs {
   int blocks;   // of 32 classes
   float *sums;  // of the piece, or null
   float scale;  // of the sums
+  int beside;   // as dlogits_kernel's
 };
 template <int P>
 __global__ __launch_bounds__(256) void few_dlogits_kernel(FewLogitsArgs a) {
@@ -587,8 +603,9 @@ __global__ __launch_bounds__(256) void few_dlogits_kernel(FewLogitsArgs a) {
         const float v[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          e[4 * q + k] = g == 0.f ? 0.f : __expf(v[k] - all) - (at == 8 * q + k ? 1.f : 0.f);
-          sum[4 * q + k] += g * e[4 * q + k];
+          const float x = g == 0.f ? 0.f : __expf(v[k] - all) - (at == 8 * q + k ? 1.f : 0.f), gx = g * x;
+          sum[4 * q + k] += gx;
+          e[4 * q + k] = P == 1 && a.beside ? x : gx;
         }
       }
     }
@@ -597,6 +614,7 @@ __global__ __launch_bounds__(256) void few_dlogits_kernel(FewLogitsArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; r++) parts_of<P>(e[r], o.v[r]);
       put_rows<P>(a.d, j, cb, o, lane);
+      if (P == 1 && a.beside) put_rows<P>(a.d, j + 2, cb, o, lane);
     }
   }
   if (!a.sums) return;
@@ -1043,14 +1061,15 @@ Plan plan_of(int n, int H, int C, int grads) {
       p.xchunk = ceil_to((rp + stretches - 1) / stretches, kPlaneAlign);
       p.xsplits = (rp + p.xchunk - 1) / p.xchunk;
     }
-    p.xt = take(packed_bytes<P>(H, p.np));
+    const int twice = P == 1 && n <= kFewRows ? 2 : 1;  // (see dlogits_kernel)
+    p.xt = take(packed_bytes<P>(H, twice * p.np));
     // W in one order, d W reading it by transposing loads, or packed with its classes as k too, whichever costs less.  us of a call, one order / two: bf16
     // 30000 x 1024 with 512 tokens 243 / 258, 1000 375 / 387, 2000 633 / 631, 3000 899 / 864; 50000 x 2048 with 1000 1042 / 1063, 4096 3317 / 3295; 128000 x
     // 4096 with 8192 32500 / 31450; 10000 x 512 with 7000 429 / 442; fp32 45376 x 1024 with 96 430 / 480, 10000 x 512 with 7088 1555 / 1556.  Narrow rows and
     // few tokens, a tile or three of d W, each a long way: fp32 81792 x 72 with 96 177 / 152, 300 276 / 270, 1000 635 / 675; bf16 112 / 103 with 96.
     p.one_order = (H > 128 || n > 512) && (P == 3 || n <= 2000 || H <= 512);
     p.wt = take(p.few || p.one_order ? 0 : packed_bytes<P>(H, rp));
-    p.d = take(packed_bytes<P>(p.np, rp));
+    p.d = take(packed_bytes<P>(twice * p.np, rp));
     p.sums = take((size_t)tiles_of(n, p.bn) * C * 4);
     p.xpart = take((size_t)p.xsplits * n * H * 4);
     p.wpart = take(p.wsplits > 1 ? (size_t)p.wsplits * rows * H * 4 : 0);
@@ -1094,9 +1113,11 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
     return packing({static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, rows, H, o && !p.raw ? piece_w(c0) : none, t && p.grads ? piece_wt(rows) : none,
                     ceil_to(rows, kPlaneAlign), c.b ? c.b + c0 : nullptr, nullptr, nullptr, 0, 0, 0});
   };
-  const PackedOut xt{p.grads && c.dW ? pl(p.xt) : nullptr, p.np};
+  const bool beside = P == 1 && c.dloss && n <= kFewRows;  // weights are not in d
+  const int wk = beside ? 2 * p.np : p.np;                  // what d^T X sums over
+  const PackedOut xt{p.grads && c.dW ? pl(p.xt) : nullptr, wk};
   // X in one launch with what there is of W by then
-  PackJob jx = packing({c.X, c.ldx, n, H, p.few && n <= 32 ? none : X, xt, n, nullptr, c.labels, c.dloss, C, 0, 0});
+  PackJob jx = packing({c.X, c.ldx, n, H, p.few && n <= 32 ? none : X, xt, n, nullptr, c.labels, beside ? c.dloss : nullptr, C, 0, 0});
   auto tile_args = [&](int c0) {
     const int rows = rows_of(c0);
     return TileArgs{ref(piece_w(c0)), ref(X), rows, n, p.Hp, tiles_of(rows, p.bm), tiles_of(n, p.bn), c.b ? c.b + c0 : nullptr, c.labels, c0,
@@ -1139,13 +1160,13 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
       const TileArgs a = tile_args(c0);
       const PackedOut d{c.dX || c.dW ? pl(p.d) : nullptr, rp};
       if (p.few && (d.p || c.db)) {
-        const FewLogitsArgs f{f32(p.z), all, weight, c.labels, n, C, c0, d, rp / 32, c.db ? c.db + c0 : nullptr, c.scale};
+        const FewLogitsArgs f{f32(p.z), all, weight, c.labels, n, C, c0, d, rp / 32, c.db ? c.db + c0 : nullptr, c.scale, beside};
         launch(few_dlogits_kernel<P>, (rp / 32 + 3) / 4, 256, 0, st, f);
       } else if (d.p || c.db) {
         with_product_tile<P>(p.size, [&](auto t) {
           using T = decltype(t);
           launch(dlogits_kernel<T>, a.tilesM * a.tilesN, T::THREADS, 0, st, a, all, weight, d, !c.db ? nullptr : b_parts ? f32(p.sums) + c0 : c.db + c0, C,
-                 b_parts ? 1.f : c.scale);
+                 b_parts ? 1.f : c.scale, (int)beside);
           return 0;
         });
       }
@@ -1155,9 +1176,9 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
       };
       ProductJob<Src> px{}, pw{};
       // (a last piece shorter than the others fills fewer stretches: those beyond keep what they have)
-      if (c.dX && !p.few) px = job(d, p.one_order ? piece_w(c0) : piece_wt(rows), n, rp, p.xchunk, x_parts ? f32(p.xpart) : nullptr, !first, c.dX, c.lddx, weight);
+      if (c.dX && !p.few) px = job(d, p.one_order ? piece_w(c0) : piece_wt(rows), n, rp, p.xchunk, x_parts ? f32(p.xpart) : nullptr, !first, c.dX, c.lddx, beside ? weight : nullptr);
       Src *dW = c.dW ? static_cast<Src *>(c.dW) + (long)c0 * c.lddw : nullptr;
-      if (c.dW) pw = job(d, xt, rows, p.np, p.wchunk, w_parts ? f32(p.wpart) : nullptr, false, dW, c.lddw, nullptr);
+      if (c.dW) pw = job(d, xt, rows, wk, beside ? wk : p.wchunk, w_parts ? f32(p.wpart) : nullptr, false, dW, c.lddw, nullptr);
       // (d W of more than the last cache holds, in whole lines of 128 bytes: bf16 124416 x 2176, 64 tokens 533 us of a call, streaming 469, 81664 x 4096, 12
       // tokens 544, 456; lines in parts the other way, fp32 40806 x 4050, 12 tokens 823, 940)
       const bool stream = p.few && c.dW && (size_t)C * H * sizeof(Src) > 256u << 20 && (uintptr_t)c.dW % 128 == 0 && c.lddw * sizeof(Src) % 128 == 0 && H * sizeof(Src) % 128 == 0;
@@ -1180,7 +1201,7 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
       }
       const bool last = c0 + p.piece >= C;
       SumJob sx{}, sw{}, sb{};
-      if (last && c.dX && x_parts) sx = {f32(p.xpart), p.xsplits, n, H, weight, c.dX, c.lddx, 0};
+      if (last && c.dX && x_parts) sx = {f32(p.xpart), p.xsplits, n, H, beside ? weight : nullptr, c.dX, c.lddx, 0};
       if (dW && w_parts) sw = {f32(p.wpart), p.wsplits, rows, H, nullptr, dW, c.lddw, 0};
       if (last && c.db && b_parts) sb = {f32(p.sums), token_tiles, 1, C, nullptr, c.db, C, 0};
       sums<Src>(sx, sw, sb, c.scale, st);

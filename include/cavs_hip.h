@@ -360,7 +360,7 @@ int cavs_softmax_xent_sums(float *loss, float *dlogits, const float *logits, con
  * NaN of the results that depend on it, and so does an infinity, but for logits of -infinity that come of it (CAVS_BF16): probability 0.
  * n = 0 is allowed (dW and db become 0).
  * CAVS_F32: products as sums of bf16 parts in full fp32 precision (the arithmetic of cavs_sgemm); CAVS_BF16: products of bf16 values
- * in fp32 accumulators, d (without scale and dloss) rounded to bf16 between its products, dloss X too for dW, gradients rounded once.  Results are the same on every call.
+ * in fp32 accumulators, d (without scale, of up to 64 tokens without dloss) rounded to bf16 between its products, gradients rounded once.  Results are the same on every call.
  *   _fwd  loss and lse
  *   _bwd  the gradients, from the lse that _fwd (or cavs_vocab_xent) left for the same X, W and b
  *   cavs_vocab_xent  both in one call

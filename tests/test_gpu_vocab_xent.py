@@ -115,9 +115,7 @@ class Case:
         dX, dW, db = d @ W, d.t() @ X, d.sum(0)
         e = dict(lse=elog, loss=elog + ez[rows, at] + U * loss.abs())
         e["dX"] = edr @ W.abs() + (C / 16 + 64) * U * (d.abs() @ W.abs()) + eps * dX.abs() + 2.0 ** -126
-        # (d W takes a row's dloss in fp32, d^T X takes it with X, which bf16 rounds once more: (1 + eps)^2 - 1 for the roundings of d and of dloss X)
-        edw = edr if self.dloss is None or self.t == torch.float32 else ed + ((1 + eps) ** 2 - 1) * d.abs()
-        e["dW"] = edw.t() @ X.abs() + (self.n / 16 + 64) * U * (d.abs().t() @ X.abs()) + eps * dW.abs() + 2.0 ** -126
+        e["dW"] = edr.t() @ X.abs() + (self.n / 16 + 64) * U * (d.abs().t() @ X.abs()) + eps * dW.abs() + 2.0 ** -126
         e["db"] = ed.sum(0) + (self.n / 16 + 16) * U * d.abs().sum(0)
         return dict(loss=loss, lse=lse, dX=dX, dW=dW, db=db), e
 
@@ -535,3 +533,22 @@ def test_many_tokens_and_long_rows(n, H, C):
     c.call("cavs_vocab_xent_bwd", h, ws, need)
     torch.cuda.synchronize()
     assert all(torch.equal(h[k], o[k]) for k in ("dX", "dW", "db"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,H,C", [(1, 96, 300), (1, 1100, 2000), (20, 1500, 3000), (40, 130, 500), (64, 64, 40000)])
+def test_weights_of_few_tokens_are_not_rounded(n, H, C):
+    """bf16, a weight that bf16 would round by all but half a step: rows of dX are the weight times those without one, to the rounding of both results (2 eps,
+    and eps^2); so is dW of one token, but for the 2^-16 that two parts leave of the weighted row."""
+    c = Case(n + H, "bf16", n, H, C, weights=False)
+    one, (ws, need) = c.outputs(), c.workspace(1)
+    c.call("cavs_vocab_xent", one, ws, need)
+    w = 1.0 + 2.0 ** -8 * 0.99
+    c.dloss = torch.full((n,), w, device="cuda")
+    o = c.outputs()
+    c.call("cavs_vocab_xent", o, ws, need)
+    c.check(o)
+    eps = torch.finfo(torch.bfloat16).eps / 2
+    for k in ("dX", "dW")[:2 if n == 1 else 1]:
+        got, want = o[k].double(), w * one[k].double()
+        assert ((got - want).abs() <= ((1 + eps) / (1 - eps) - 1 + (n == 1) * 2.0 ** -15) * want.abs() + 2.0 ** -126).all(), k

@@ -26,7 +26,7 @@ struct Mat {
   int rows, cols;      // as the caller has them
   int m, n, mp, np;    // of X, and padded to whole steps
   u16 *X, *Xt[2], *A, *Q;  // packed: [m, np], [n, mp] (read, written), [m, mp], [m, mp]
-  float shrink;        // sqrt(max(1, rows / cols))
+  float shrink;        // sqrt(max(1, outputs / inputs))
 };
 
 struct Common {
@@ -447,7 +447,7 @@ void product(const cavs_ortho_desc *d, int count, const Mat *m, const Common &c,
 }
 
 template <int P, class Src>
-int run(const cavs_ortho_desc *d, int count, const cavs_ortho_options &o, const Plan &p, char *ws, hipStream_t st) {
+int run(const cavs_ortho_desc *d, int count, const cavs_ortho_options &o, bool in_out, const Plan &p, char *ws, hipStream_t st) {
   Common c{};
   c.nesterov = o.nesterov, c.a = o.a, c.b = o.b, c.c = o.c, c.eps = o.eps, c.momentum = o.momentum, c.lr = o.lr, c.decay = o.weight_decay, c.guard = o.guard;
   c.squares = reinterpret_cast<double *>(ws + p.squares);
@@ -472,7 +472,8 @@ int run(const cavs_ortho_desc *d, int count, const cavs_ortho_options &o, const 
       Mat t{b[i].G, b[i].M, b[i].W, b[i].O, b[i].ldg, b[i].ldm, b[i].ldw, b[i].ldo, b[i].rows, b[i].cols, h.m, h.n, h.mp, h.np};
       t.X = take(packed_bytes<P>(h.m, h.np)), t.Xt[0] = take(packed_bytes<P>(h.n, h.mp)), t.Xt[1] = take(packed_bytes<P>(h.n, h.mp));
       t.A = take(packed_bytes<P>(h.m, h.mp)), t.Q = take(packed_bytes<P>(h.m, h.mp));
-      t.shrink = b[i].rows > b[i].cols ? (float)__builtin_sqrt((double)b[i].rows / b[i].cols) : 1.f;
+      const int outputs = in_out ? b[i].cols : b[i].rows, inputs = in_out ? b[i].rows : b[i].cols;
+      t.shrink = outputs > inputs ? (float)__builtin_sqrt((double)outputs / inputs) : 1.f;
       room += (room_of<P>(h) + 255) & ~(size_t)255;
       s.m[i] = nm.m[i] = t;
       s.first[i + 1] = s.first[i] + tiles_of(b[i].rows, 64) * tiles_of(b[i].cols, 64);
@@ -511,6 +512,32 @@ bool sizes_ok(int type, int count, const cavs_ortho_desc *d) {
   return true;
 }
 
+int check_and_run(const char *who, int type, int count, const cavs_ortho_desc *d, const cavs_ortho_options *o, bool in_out, void *workspace, size_t workspace_bytes,
+                  void *stream) {
+  CAVS_REQUIRE(type == CAVS_F32 || type == CAVS_BF16, "%s: type %d is neither CAVS_F32 nor CAVS_BF16", who, type);
+  CAVS_REQUIRE(count >= 0 && (count == 0 || d) && o, "%s: bad count %d or null pointer", who, count);
+  CAVS_REQUIRE(o->steps >= 1 && o->steps <= 64, "%s: %d steps (1 to 64)", who, o->steps);
+  CAVS_REQUIRE(o->eps >= 0.f, "%s: eps is negative or not a number", who);
+  for (int i = 0; i < count; i++) {
+    const cavs_ortho_desc &e = d[i];
+    CAVS_REQUIRE(e.rows > 0 && e.cols > 0 && e.rows <= kMostSide && e.cols <= kMostSide, "%s: matrix %d: unsupported shape %d x %d (1 to 2^16)", who, i,
+                 e.rows, e.cols);
+    CAVS_REQUIRE(e.G, "%s: matrix %d: null pointer", who, i);
+    CAVS_REQUIRE(e.O || e.W, "%s: matrix %d: neither O nor W is wanted", who, i);
+    CAVS_REQUIRE(e.ldg >= e.cols && (!e.M || e.ldm >= e.cols) && (!e.W || e.ldw >= e.cols) && (!e.O || e.ldo >= e.cols),
+                 "%s: matrix %d: a row stride is below its %d columns", who, i, e.cols);
+  }
+  if (count == 0) return CAVS_OK;
+  const bool two = two_parts(type, count, d);
+  const Plan p = two ? plan_of<2>(d, count) : plan_of<3>(d, count);
+  CAVS_REQUIRE(workspace && workspace_bytes >= p.bytes, "%s: workspace of %zu bytes needed, %zu given", who, p.bytes, workspace_bytes);
+  CAVS_REQUIRE(aligned16(workspace), "%s: the workspace must be 16-byte aligned", who);
+  char *ws = static_cast<char *>(workspace);
+  hipStream_t st = as_stream(stream);
+  if (type == CAVS_F32) return run<3, float>(d, count, *o, in_out, p, ws, st);
+  return two ? run<2, u16>(d, count, *o, in_out, p, ws, st) : run<3, u16>(d, count, *o, in_out, p, ws, st);
+}
+
 }  // namespace
 }  // namespace cavs
 
@@ -524,28 +551,11 @@ size_t cavs_ortho_update_workspace(int type, int count, const cavs_ortho_desc *d
 }
 
 int cavs_ortho_update(int type, int count, const cavs_ortho_desc *d, const cavs_ortho_options *o, void *workspace, size_t workspace_bytes, void *stream) {
-  CAVS_REQUIRE(type == CAVS_F32 || type == CAVS_BF16, "cavs_ortho_update: type %d is neither CAVS_F32 nor CAVS_BF16", type);
-  CAVS_REQUIRE(count >= 0 && (count == 0 || d) && o, "cavs_ortho_update: bad count %d or null pointer", count);
-  CAVS_REQUIRE(o->steps >= 1 && o->steps <= 64, "cavs_ortho_update: %d steps (1 to 64)", o->steps);
-  CAVS_REQUIRE(o->eps >= 0.f, "cavs_ortho_update: eps is negative or not a number");
-  for (int i = 0; i < count; i++) {
-    const cavs_ortho_desc &e = d[i];
-    CAVS_REQUIRE(e.rows > 0 && e.cols > 0 && e.rows <= kMostSide && e.cols <= kMostSide, "cavs_ortho_update: matrix %d: unsupported shape %d x %d (1 to 2^16)", i,
-                 e.rows, e.cols);
-    CAVS_REQUIRE(e.G, "cavs_ortho_update: matrix %d: null pointer", i);
-    CAVS_REQUIRE(e.O || e.W, "cavs_ortho_update: matrix %d: neither O nor W is wanted", i);
-    CAVS_REQUIRE(e.ldg >= e.cols && (!e.M || e.ldm >= e.cols) && (!e.W || e.ldw >= e.cols) && (!e.O || e.ldo >= e.cols),
-                 "cavs_ortho_update: matrix %d: a row stride is below its %d columns", i, e.cols);
-  }
-  if (count == 0) return CAVS_OK;
-  const bool two = two_parts(type, count, d);
-  const Plan p = two ? plan_of<2>(d, count) : plan_of<3>(d, count);
-  CAVS_REQUIRE(workspace && workspace_bytes >= p.bytes, "cavs_ortho_update: workspace of %zu bytes needed, %zu given", p.bytes, workspace_bytes);
-  CAVS_REQUIRE(aligned16(workspace), "cavs_ortho_update: the workspace must be 16-byte aligned");
-  char *ws = static_cast<char *>(workspace);
-  hipStream_t st = as_stream(stream);
-  if (type == CAVS_F32) return run<3, float>(d, count, *o, p, ws, st);
-  return two ? run<2, u16>(d, count, *o, p, ws, st) : run<3, u16>(d, count, *o, p, ws, st);
+  return check_and_run("cavs_ortho_update", type, count, d, o, false, workspace, workspace_bytes, stream);
+}
+
+int cavs_ortho_update_in_out(int type, int count, const cavs_ortho_desc *d, const cavs_ortho_options *o, void *workspace, size_t workspace_bytes, void *stream) {
+  return check_and_run("cavs_ortho_update_in_out", type, count, d, o, true, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

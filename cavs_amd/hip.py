@@ -142,6 +142,7 @@ _SIGS = {
     "cavs_vocab_xent": [_I, _P, _I, _P, _I, _P, _P, _P, _F, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _P, _Z, _P],
     "cavs_sgd": [_P, _P, _F, _Z, _P],
     "cavs_ortho_update": [_I, _I, C.POINTER(OrthoDesc), C.POINTER(OrthoOptions), _P, _Z, _P],
+    "cavs_ortho_update_in_out": [_I, _I, C.POINTER(OrthoDesc), C.POINTER(OrthoOptions), _P, _Z, _P],
     "cavs_ew_binary": [_I, _P, _P, _Z, _P, _Z, _Z, _I, _P],
     "cavs_ew_unary": [_I, _P, _P, _Z, _I, _P],
     "cavs_scale": [_P, _P, _F, _Z, _P],

@@ -175,7 +175,8 @@ void Engine::ortho_update(float lr) {
   // (coefficients that lift small singular values fast; what comes of five steps lies between 0.7 and 1.2)
   const cavs_ortho_options o{5, 1, 3.4445f, -4.7750f, 2.0315f, 1e-7f, cfg_.ortho_momentum == 0.f ? 0.95f : std::max(cfg_.ortho_momentum, 0.f),
                              cfg_.ortho_lr > 0.f ? cfg_.ortho_lr : lr, cfg_.ortho_decay, update_guard()};
-  check(cavs_ortho_update(CAVS_F32, (int)ortho_.size(), ortho_.data(), &o, ortho_ws_.get(), ortho_ws_.capacity() * 4, stream_));
+  // (weights here are stored [inputs, outputs]: x W, h U)
+  check(cavs_ortho_update_in_out(CAVS_F32, (int)ortho_.size(), ortho_.data(), &o, ortho_ws_.get(), ortho_ws_.capacity() * 4, stream_));
   c_launches_ += 2 + 3 * o.steps;
   upk_valid_ = utp_valid_ = false;
 }

@@ -476,7 +476,9 @@ int cavs_sgd_multi(int count, float *const *w, const float *const *g, const size
  * every direction of the update gets about the same size).  For each of `count` matrices:
  *   M <- momentum M + G;  U = nesterov ? G + momentum M : M  (M NULL: U = G)
  *   X = U / (|U| + eps), |U| the Frobenius norm;  `steps` times: A = X X^T, X <- a X + (b A + c A A) X  (rows > cols: of the transpose)
- *   O = X (NULL: not wanted);  W <- (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) X (NULL: no weights)
+ *   O = X (NULL: not wanted);  W <- (1 - lr weight_decay) W - lr sqrt(max(1, outputs / inputs)) X (NULL: no weights)
+ * cavs_ortho_update takes matrices stored [outputs, inputs] (y = W x, or Y = X W^T): outputs / inputs is rows / cols.  cavs_ortho_update_in_out takes
+ * those stored [inputs, outputs] (Y = X W, as the models' gates here): cols / rows.  They differ in nothing else.
  * G and O are of `type`, M and W fp32; row strides in elements.  A matrix may be a block of a larger one (a gate's columns of a weight matrix);
  * columns between `cols` and a row's stride are not touched.  O may be G; otherwise what is written may overlap nothing else.  U = 0 gives
  * X = 0.  An infinity or a NaN in a matrix's G or M makes all of its X NaN.
@@ -506,6 +508,8 @@ typedef struct {
 size_t cavs_ortho_update_workspace(int type, int count, const cavs_ortho_desc *d);
 int cavs_ortho_update(int type, int count, const cavs_ortho_desc *d, const cavs_ortho_options *options, void *workspace,
                       size_t workspace_bytes, void *stream);
+int cavs_ortho_update_in_out(int type, int count, const cavs_ortho_desc *d, const cavs_ortho_options *options, void *workspace,
+                             size_t workspace_bytes, void *stream);
 /* Clip (cavs/backend/op_impl_clip.cu:26-50): scales every gradient in place by
  * clip / max(sum_i ||g_i||_2, clip) -- the sum of the tensors' 2-norms, as the reference adds
  * them; at most 8 non-empty tensors per call; the arrays are host arrays.  After the call

@@ -103,7 +103,8 @@ typedef struct {
    * class (-1) take no part in it then.  0 = the head with logits. */
   int vocab_head;
   /* What applies the gradients: 0 = SGD (cavs/backend/op_impl_sgd.cu).  1 = the input and recurrent weights ("W", "U"), each gate's (Tree-FC: each
-   * child's) block a matrix, by their orthogonalised momentum (cavs_ortho_update, Nesterov, five steps), everything else by SGD.
+   * child's) block a matrix, by their orthogonalised momentum (cavs_ortho_update_in_out, Nesterov, five steps: a block of "W" takes E inputs to H outputs,
+   * all others H to H), everything else by SGD.
    * The momentum is the parameter "W.momentum" / "U.momentum" (zero at first; for checkpoints). */
   int optimizer;
   float ortho_lr;       /* step size of the orthogonalised updates; 0 = cavs_session_step's lr */

@@ -8,8 +8,10 @@
 // with it), A and the polynomial by rows, which are their columns.
 //
 // A singular value next to 0 grows a-fold a step, 485-fold in five, and so does a rounding error made beside it.  With three parts X, A and the
-// polynomial keep an fp32's bits and the result is as far off as in fp32.  Where the result is rounded to bf16, two parts will do: what
-// they leave off, 2^-17 of the largest, is 2^-8 then.  (One part, 2^-9, would come out as large as the result.)
+// polynomial keep an fp32's bits and the result is as far off as in fp32.  Where nothing but a result rounded to bf16 is wanted, two parts do for as long as
+// what they leave off, 2^-17 of the largest, has grown to no more than half a step of bf16, 2^-8.  (Error of the result, a bf16 gradient of
+// rank 3 to the last bit, 96 x 160, two / three parts: 5 steps 0.0020 / 0.0017 of its norm, 6 steps 0.0028 / 0.0017, 8 steps 0.042 / 0.0018, 10 steps
+// 0.48 / 0.0083; rounding alone 0.0017.  One part, 2^-9, would come out as large as the result.)
 #include "nt_product.h"
 
 namespace cavs {
@@ -498,11 +500,26 @@ int run(const cavs_ortho_desc *d, int count, const cavs_ortho_options &o, bool i
 
 constexpr int kMostSide = 1 << 16;
 
-// two parts where nothing but a bf16 result is wanted
-bool two_parts(int type, int count, const cavs_ortho_desc *d) {
+// How far the steps carry an error of X: the largest slope of their map at singular values up to 1 (with coefficients that orthogonalise, a^steps, at 0)
+double growth(const cavs_ortho_options &o) {
+  double most = 1.;
+  for (int i = 0; i <= 16; i++) {
+    double x = i / 16., slope = 1.;
+    for (int step = 0; step < o.steps; step++) {
+      const double s = x * x;
+      slope *= o.a + s * (3. * o.b + s * 5. * o.c);
+      x *= o.a + s * (o.b + s * o.c);
+      if (!(fabs(slope) <= most)) most = fabs(slope);
+    }
+  }
+  return most;
+}
+
+// whether two parts hold what is wanted
+bool two_parts(int type, int count, const cavs_ortho_desc *d, const cavs_ortho_options &o) {
   for (int i = 0; i < count; i++)
     if (d[i].W) return false;
-  return type == CAVS_BF16;
+  return type == CAVS_BF16 && growth(o) <= 512.;  // (2^-8 over 2^-17)
 }
 
 bool sizes_ok(int type, int count, const cavs_ortho_desc *d) {
@@ -528,9 +545,11 @@ int check_and_run(const char *who, int type, int count, const cavs_ortho_desc *d
                  "%s: matrix %d: a row stride is below its %d columns", who, i, e.cols);
   }
   if (count == 0) return CAVS_OK;
-  const bool two = two_parts(type, count, d);
-  const Plan p = two ? plan_of<2>(d, count) : plan_of<3>(d, count);
-  CAVS_REQUIRE(workspace && workspace_bytes >= p.bytes, "%s: workspace of %zu bytes needed, %zu given", who, p.bytes, workspace_bytes);
+  const bool two = two_parts(type, count, d, *o);
+  Plan p = plan_of<3>(d, count);
+  const size_t need = p.bytes;
+  if (two) p = plan_of<2>(d, count);
+  CAVS_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
   CAVS_REQUIRE(aligned16(workspace), "%s: the workspace must be 16-byte aligned", who);
   char *ws = static_cast<char *>(workspace);
   hipStream_t st = as_stream(stream);
@@ -547,7 +566,7 @@ extern "C" {
 
 size_t cavs_ortho_update_workspace(int type, int count, const cavs_ortho_desc *d) {
   if (count <= 0 || !sizes_ok(type, count, d)) return 0;
-  return (two_parts(type, count, d) ? plan_of<2>(d, count) : plan_of<3>(d, count)).bytes;
+  return plan_of<3>(d, count).bytes;  // (two parts take less, whatever the options)
 }
 
 int cavs_ortho_update(int type, int count, const cavs_ortho_desc *d, const cavs_ortho_options *o, void *workspace, size_t workspace_bytes, void *stream) {

@@ -482,12 +482,14 @@ int cavs_sgd_multi(int count, float *const *w, const float *const *g, const size
  * G and O are of `type`, M and W fp32; row strides in elements.  A matrix may be a block of a larger one (a gate's columns of a weight matrix);
  * columns between `cols` and a row's stride are not touched.  O may be G; otherwise what is written may overlap nothing else.  U = 0 gives
  * X = 0.  An infinity or a NaN in a matrix's G or M makes all of its X NaN.
- * Products as sums of bf16 parts: three of them (full fp32 precision) where fp32 results are made, two (16 bits) where
- * nothing but bf16 O are.  Sums of squares in 64 bits.  Results are the same on every call.
+ * Products as sums of bf16 parts: three of them (full fp32 precision), or two (16 bits) where nothing but bf16 O are made and the steps let
+ * what two leave off grow to no more than bf16's own rounding: up to a^steps = 512 (five of those below).  Whatever is 0 but for
+ * rounding grows a-fold a step, in these products as in any of fp32: with those below a gradient of few directions alone comes out to 0.001 of its norm after
+ * eight steps, 0.01 after ten.  Sums of squares in 64 bits.  Results are the same on every call.
  * steps 1 .. 64 (5 with a = 3.4445, b = -4.7750, c = 2.0315 bring singular values above 0.003 of the norm to 0.7 .. 1.2), rows and cols up to 2^16.
  * guard (may be NULL): a device word; while it is not 0 the call leaves M, W and O as they are.
- * The workspace: 16-byte aligned, at least cavs_ortho_update_workspace(type, count, d) bytes on this device (it depends on rows, cols and on
- * which W are NULL; 0: refused, or count is 0); for the next call on the same stream to reuse, not for one that overlaps in time.
+ * The workspace: 16-byte aligned, at least cavs_ortho_update_workspace(type, count, d) bytes on this device (whatever the options; it depends on rows
+ * and cols alone; 0: refused, or count is 0); for the next call on the same stream to reuse, not for one that overlaps in time.
  * The arrays are host arrays. */
 typedef struct {
   int rows, cols;

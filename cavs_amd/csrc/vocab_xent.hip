@@ -20,9 +20,14 @@ namespace {
 // ------------------------------------------------------------------ operands, packed
 // src [rows, K] with its columns as k and, for a product that sums over them, with its rows as k; either may be left out.  What takes no part is zero
 // where it is summed over, as 0 times what it holds need not be 0: a row whose bias is -inf (its z is -inf whatever is there), and in X's second order a row
-// without a class.
+// that sends nothing back.
 // `weight`: up to 64 bf16 rows come times their weights as two parts, the second behind the first along k (see dlogits_kernel).
 __device__ inline bool is_class(float label, int classes) { return label >= 0.f && label < (float)classes; }
+// A label that names a masked class: the loss is infinite and, as it is of a row whose classes are all masked, sends nothing back.  (Without its -1 in d the
+// rest would be no loss's gradient; with it d X would need a row of W that may hold anything.)
+__device__ inline bool is_open_class(float label, const float *bias, int classes) {
+  return is_class(label, classes) && !(bias && bias[(int)label] == -INFINITY);
+}
 
 struct PackJob {
   const void *src;
@@ -32,6 +37,7 @@ struct PackJob {
   int orows;                      // rows of o, zero beyond those of src
   const float *bias;              // of rows, or null
   const float *labels, *weight;   // of rows, for t, or null
+  const float *class_bias;        // of the classes, or null
   int classes;
   int across, blocks;             // blocks of 64 columns, of 64 x 64
 };
@@ -44,6 +50,13 @@ __global__ __launch_bounds__(256) void pack_kernel(PackJob j0, PackJob j1) {
   const int block = second ? blockIdx.x - j0.blocks : blockIdx.x;
   const int r0 = block / g.across * 64, k0 = block % g.across * 64, k = threadIdx.x & 63;
   const Src *src = static_cast<const Src *>(g.src);
+  __shared__ bool open[64];  // (looked up beside the tile's loads: a label, and its class's bias)
+  __shared__ float weight[64];
+  if (g.labels && threadIdx.x < 64) {
+    const int r = r0 + threadIdx.x;
+    open[threadIdx.x] = r < g.rows && is_open_class(g.labels[r], g.class_bias, g.classes);
+    weight[threadIdx.x] = g.weight && r < g.rows ? g.weight[r] : 1.f;
+  }
   load_tile(tile, src, g.ld, r0, k0, g.rows, g.K);
   __syncthreads();
   if (g.bias) {
@@ -55,11 +68,10 @@ __global__ __launch_bounds__(256) void pack_kernel(PackJob j0, PackJob j1) {
   if (!g.t.p) return;
   if (g.labels) {
     __syncthreads();
-    for (int i = threadIdx.x >> 6; i < 64; i += 4)
-      if (r0 + i < g.rows) {
-        if (!is_class(g.labels[r0 + i], g.classes)) tile[i][k] = 0.f;
-        else if (g.weight) tile[i][k] *= g.weight[r0 + i];
-      }
+    for (int i = threadIdx.x >> 6; i < 64; i += 4) {
+      if (!open[i]) tile[i][k] = 0.f;
+      else if (g.weight) tile[i][k] *= weight[i];
+    }
     __syncthreads();
   }
   pack_tile<P>(tile, PackedOut{}, g.t, r0, k0, g.rows, g.K);
@@ -449,16 +461,16 @@ __global__ __launch_bounds__(256, P == 1 ? 4 : 2) void direct_stats_kernel(Direc
   if (threadIdx.x < 32 * TN && (int)threadIdx.x < a.n) a.stats[(long)blockIdx.x * a.n + threadIdx.x] = all;
 }
 
-// What a row's tiles come to: lse, loss and the weight of its gradient (zero for a row without a class, or without any class that is not
+// What a row's tiles come to: lse, loss and the weight of its gradient (zero for a row without a class, or whose class is
 // masked).  Sixteen lanes to a row, or all of a workgroup where rows are few.
 struct RowArgs {
   const float2 *stats;
   int tiles, n, C;
-  const float *zlabel, *labels, *dloss;
+  const float *zlabel, *labels, *bias, *dloss;
   float *loss, *lse, *weight;
 };
-__device__ inline float weight_of(float label, float lse, const float *dloss, int row, int C) {
-  return is_class(label, C) && lse != -INFINITY ? dloss ? dloss[row] : 1.f : 0.f;
+__device__ inline float weight_of(bool open, float lse, const float *dloss, int row) {
+  return open && lse != -INFINITY ? dloss ? dloss[row] : 1.f : 0.f;
 }
 template <int ROWS>
 __global__ __launch_bounds__(256) void rows_kernel(RowArgs a) {
@@ -466,6 +478,8 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs a) {
   __shared__ float2 part[LANES][ROWS];
   const int x = threadIdx.x % ROWS, y = threadIdx.x / ROWS, row = blockIdx.x * ROWS + x;
   float2 s = make_float2(-INFINITY, 0.f);
+  const float label = y == 0 && row < a.n ? a.labels[row] : -1.f;
+  const bool open = is_open_class(label, a.bias, a.C);  // (two loads one after the other, on their way beside the statistics)
   if (row < a.n)
     for (int t = y; t < a.tiles; t += 4 * LANES) {
       float2 v[4];
@@ -481,17 +495,17 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs a) {
   }
   if (y != 0 || row >= a.n) return;
   s = part[0][x];
-  const float all = (s.x == -INFINITY ? 0.f : s.x) + logf(s.y), label = a.labels[row];
+  const float all = (s.x == -INFINITY ? 0.f : s.x) + logf(s.y);
   if (a.lse) a.lse[row] = all;
   // (no class left: an infinite loss, not the NaN of -inf - -inf)
-  if (a.loss) a.loss[row] = !is_class(label, a.C) ? 0.f : all == -INFINITY ? INFINITY : all - a.zlabel[row];
-  if (a.weight) a.weight[row] = weight_of(label, all, a.dloss, row, a.C);
+  if (a.loss) a.loss[row] = !is_class(label, a.C) ? 0.f : all == -INFINITY || !open ? INFINITY : all - a.zlabel[row];
+  if (a.weight) a.weight[row] = weight_of(open, all, a.dloss, row);
 }
 
-__global__ __launch_bounds__(256) void weights_kernel(const float *__restrict__ labels, const float *__restrict__ lse, const float *__restrict__ dloss, int n,
-                                                      int C, float *__restrict__ weight) {
+__global__ __launch_bounds__(256) void weights_kernel(const float *__restrict__ labels, const float *__restrict__ lse, const float *__restrict__ bias,
+                                                      const float *__restrict__ dloss, int n, int C, float *__restrict__ weight) {
   const int row = blockIdx.x * 256 + threadIdx.x;
-  if (row < n) weight[row] = weight_of(labels[row], lse[row], dloss, row, C);
+  if (row < n) weight[row] = weight_of(is_open_class(labels[row], bias, C), lse[row], dloss, row);
 }
 
 // d = weight * (p - [label]) of a tile, packed by token (zero between the last class or token and the end of the steps), and its sums over the tile's
@@ -1111,13 +1125,13 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
   auto job_w = [&](int c0, bool o, bool t) {
     const int rows = rows_of(c0);
     return packing({static_cast<const Src *>(c.W) + (long)c0 * c.ldw, c.ldw, rows, H, o && !p.raw ? piece_w(c0) : none, t && p.grads ? piece_wt(rows) : none,
-                    ceil_to(rows, kPlaneAlign), c.b ? c.b + c0 : nullptr, nullptr, nullptr, 0, 0, 0});
+                    ceil_to(rows, kPlaneAlign), c.b ? c.b + c0 : nullptr, nullptr, nullptr, nullptr, 0, 0, 0});
   };
   const bool beside = P == 1 && c.dloss && n <= kFewRows;  // weights are not in d
   const int wk = beside ? 2 * p.np : p.np;                  // what d^T X sums over
   const PackedOut xt{p.grads && c.dW ? pl(p.xt) : nullptr, wk};
   // X in one launch with what there is of W by then
-  PackJob jx = packing({c.X, c.ldx, n, H, p.few && n <= 32 ? none : X, xt, n, nullptr, c.labels, beside ? c.dloss : nullptr, C, 0, 0});
+  PackJob jx = packing({c.X, c.ldx, n, H, p.few && n <= 32 ? none : X, xt, n, nullptr, c.labels, beside ? c.dloss : nullptr, c.b, C, 0, 0});
   auto tile_args = [&](int c0) {
     const int rows = rows_of(c0);
     return TileArgs{ref(piece_w(c0)), ref(X), rows, n, p.Hp, tiles_of(rows, p.bm), tiles_of(n, p.bn), c.b ? c.b + c0 : nullptr, c.labels, c0,
@@ -1141,11 +1155,11 @@ int run(const Call &c, const Plan &p, char *ws, hipStream_t st) {
         return 0;
       });
     }
-    const RowArgs r{reinterpret_cast<const float2 *>(ws + p.stats), p.tiles, n, C, f32(p.zlabel), c.labels, c.dloss, c.loss, lse, p.grads ? weight : nullptr};
+    const RowArgs r{reinterpret_cast<const float2 *>(ws + p.stats), p.tiles, n, C, f32(p.zlabel), c.labels, c.b, c.dloss, c.loss, lse, p.grads ? weight : nullptr};
     if (n <= 1024) launch(rows_kernel<1>, n, 256, 0, st, r);
     else launch(rows_kernel<16>, (n + 15) / 16, 256, 0, st, r);
   } else {
-    launch(weights_kernel, (n + 255) / 256, 256, 0, st, c.labels, c.lse_given, c.dloss, n, C, weight);
+    launch(weights_kernel, (n + 255) / 256, 256, 0, st, c.labels, c.lse_given, c.b, c.dloss, n, C, weight);
   }
   if (p.grads) {
     const float *all = c.lse_given ? c.lse_given : lse;

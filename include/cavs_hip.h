@@ -356,7 +356,8 @@ int cavs_softmax_xent_sums(float *loss, float *dlogits, const float *logits, con
  * may be NULL.  What is NULL of loss, lse, dX, dW and db is not computed.  Outputs may not overlap inputs or each other.
  * labels are class ids as floats; a row whose label is below 0, not below C or NaN takes no part: its loss is 0, it adds nothing
  * to dW and db and its row of dX is 0, whatever X holds there.  A class with b = -infinity is masked: probability 0, gradient 0, whatever its row
- * of W holds.  A row without any class that is not masked has lse = -infinity, loss = infinity and no gradient.  Otherwise a NaN in X or W makes
+ * of W holds.  A row whose label names a masked class has loss = infinity and no gradient (it adds nothing to dW and db, its row of dX is 0, whatever its
+ * dloss is); one without any class that is not masked has lse = -infinity as well.  Otherwise a NaN in X or W makes
  * NaN of the results that depend on it, and so does an infinity, but for logits of -infinity that come of it (CAVS_BF16): probability 0.
  * n = 0 is allowed (dW and db become 0).
  * CAVS_F32: products as sums of bf16 parts in full fp32 precision (the arithmetic of cavs_sgemm); CAVS_BF16: products of bf16 values

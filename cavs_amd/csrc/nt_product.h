@@ -43,18 +43,20 @@ constexpr size_t packed_bytes(long rows, int K) { return (size_t)((rows + 31) / 
 __device__ inline u16 bf16_bits(float x) { return __builtin_bit_cast(u16, (__bf16)x); }
 __device__ inline float bf16_float(u16 b) { return __uint_as_float((unsigned)b << 16); }
 
-// The parts of x.  Where x has no part (an infinity, a NaN, a finite value that rounds to infinity) the first is what bf16 makes of it and
-// the others are zero.
+// The parts of x.  A finite x that bf16 would round to infinity (above 3.39e38) has bf16's largest value as its first part; what is left are 16 bits, which
+// the other two hold.  Of an infinity or a NaN the last part is NaN, and so is what it is multiplied into.  The one part of type bf16 is what bf16 makes of x.
 template <int P>
 __device__ inline void parts_of(float x, u16 (&o)[P]) {
-  o[0] = bf16_bits(x);
-  if constexpr (P > 1) {
-    float rest = x - bf16_float(o[0]);
-    if (!(fabsf(rest) < INFINITY)) rest = 0.f;
+  if constexpr (P == 1) {
+    o[0] = bf16_bits(x);
+  } else {
+    constexpr float most = 3.38953139e38f;  // (2^128 - 2^120)
+    float rest = x;
+    o[0] = bf16_bits(__builtin_amdgcn_fmed3f(x, -most, most));
 #pragma unroll
     for (int p = 1; p < P; p++) {
+      rest -= bf16_float(o[p - 1]);
       o[p] = bf16_bits(rest);
-      rest -= bf16_float(o[p]);
     }
   }
 }

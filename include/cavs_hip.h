@@ -360,7 +360,8 @@ int cavs_softmax_xent_sums(float *loss, float *dlogits, const float *logits, con
  * dloss is); one without any class that is not masked has lse = -infinity as well.  Otherwise a NaN in X or W makes
  * NaN of the results that depend on it, and so does an infinity, but for logits of -infinity that come of it (CAVS_BF16): probability 0.
  * n = 0 is allowed (dW and db become 0).
- * CAVS_F32: products as sums of bf16 parts in full fp32 precision (the arithmetic of cavs_sgemm); CAVS_BF16: products of bf16 values
+ * CAVS_F32: products as sums of bf16 parts in full fp32 precision, of all finite operands (the arithmetic of cavs_sgemm; of an operand or a d below 2^-110
+ * bits below 2^-133 are lost, and results below 2^-126 may be); sums of products are made before `scale`, so they have to be floats without it.  CAVS_BF16: products of bf16 values
  * in fp32 accumulators, d (without scale, of up to 64 tokens without dloss) rounded to bf16 between its products, gradients rounded once.  Results are the same on every call.
  *   _fwd  loss and lse
  *   _bwd  the gradients, from the lse that _fwd (or cavs_vocab_xent) left for the same X, W and b

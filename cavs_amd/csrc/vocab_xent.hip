@@ -45,9 +45,11 @@ struct PackJob {
 template <int P, class Src>
 __global__ __launch_bounds__(256) void pack_kernel(PackJob j0, PackJob j1) {
   __shared__ PackTile tile;
-  const bool second = (int)blockIdx.x >= j0.blocks;
+  const int at = blockIdx.y * gridDim.x + blockIdx.x;
+  if (at >= j0.blocks + j1.blocks) return;
+  const bool second = at >= j0.blocks;
   const PackJob &g = second ? j1 : j0;
-  const int block = second ? blockIdx.x - j0.blocks : blockIdx.x;
+  const int block = second ? at - j0.blocks : at;
   const int r0 = block / g.across * 64, k0 = block % g.across * 64, k = threadIdx.x & 63;
   const Src *src = static_cast<const Src *>(g.src);
   __shared__ bool open[64];  // (looked up beside the tile's loads: a label, and its class's bias)
@@ -959,6 +961,7 @@ constexpr int kPieceBytes = 256 << 20;  // d of a piece, where it is not all of 
 constexpr int kWholeBytes = 512 << 20;
 constexpr size_t kKeepBytes = 512 << 20;  // of W packed: kept from the first pass for the second
 constexpr int kSplits = 64;
+constexpr int kMostBlocks = (1 << 24) - 1;  // workgroups of 256 along one dimension of a grid, whose threads are to be below 2^32
 constexpr int kFewRows = 64, kRawRows = 256;
 
 // What the two products of a piece take, us, with their K in so many stretches.  Workgroups go to the compute unit that is free first, those of d W
@@ -1008,8 +1011,7 @@ Plan plan_of(int n, int H, int C, int grads) {
   most = most < 1024 ? 1024 : most > 1 << 20 ? 1 << 20 : most;
   p.pieces = (int)((C + most - 1) / most);
   p.piece = ceil_to((C + p.pieces - 1) / p.pieces, 256);
-  p.pieces = tiles_of(C, p.piece);
-  const int rows = p.piece < C ? p.piece : C;
+  int rows = p.piece < C ? p.piece : C;
   // Few tokens: W read where it lies and z kept, packing W and making z twice would be most of the work.  Gradients take two launches more that way, which
   // long rows or many classes pay for.  us with gradients packed / as it lies, 1, 24 and 64 tokens:
   //   fp32  300 x 1024 53 / 39, 54 / 42, 57 / 47   1000 x 512 41 / 36, 42 / 39, 44 / 43   12000 x 300 58 / 57, 61 / 60, 63 / 66   21701 x 300 79 / 72, 81 / 77,
@@ -1024,6 +1026,8 @@ Plan plan_of(int n, int H, int C, int grads) {
   p.raw = !grads && !p.few && n <= kRawRows && C >= 64 * num_cus();
   p.size = p.raw ? 3 : tile_size<P>(rows, n);
   tile_sides<P>(p.size, &p.bm, &p.bn);
+  while ((long)tiles_of(rows, p.bm) * tiles_of(n, p.bn) > kMostBlocks) rows = p.piece = ceil_to(rows / 2, 256);  // (losses alone of a million tokens)
+  p.pieces = tiles_of(C, p.piece);
   p.tiles = tiles_of(C, p.bm);
   if (p.few) p.tiles = tiles_of(C, 32) < 4 * num_cus() ? tiles_of(C, 32) : 4 * num_cus();
   p.keep = packed_bytes<P>(C, p.Hp) <= kKeepBytes;
@@ -1099,7 +1103,8 @@ inline PackJob packing(PackJob j) {
 }
 template <int P, class Src>
 void pack(const PackJob &a, const PackJob &b, hipStream_t st) {
-  if (a.blocks + b.blocks > 0) launch(pack_kernel<P, Src>, a.blocks + b.blocks, 256, 0, st, a, b);
+  const int blocks = a.blocks + b.blocks, high = (blocks + kMostBlocks - 1) / kMostBlocks;
+  if (blocks > 0) launch(pack_kernel<P, Src>, dim3((blocks + high - 1) / high, high), 256, 0, st, a, b);
 }
 template <class Out>
 void sums(SumJob x, SumJob w, SumJob b, float scale, hipStream_t st) {

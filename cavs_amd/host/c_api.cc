@@ -1,6 +1,7 @@
 // extern "C" surface of the host runtime (cavs_session.h): exceptions end here.
 #include <algorithm>
 #include <vector>
+#include <cstddef>
 #include <cstdio>
 #include <cstring>
 #include <string>
@@ -50,11 +51,24 @@ extern "C" {
 
 const char *cavs_session_error(void) { return g_error.c_str(); }
 
-int cavs_session_create(const cavs_session_config *cfg, cavs_session **out) {
+int cavs_session_create_sized(const cavs_session_config *cfg, size_t size, cavs_session **out) {
   if (int rc = need(cfg, "config")) return rc;
   if (int rc = need(out, "out pointer")) return rc;
   *out = nullptr;
-  return guarded([&] { *out = new cavs_session(*cfg); });
+  return guarded([&] {
+    if (size < offsetof(cavs_session_config, fused_round_rows))
+      cavs::fail(CAVS_EINVAL, "a configuration of " + std::to_string(size) + " bytes is smaller than any there has been");
+    const char *bytes = reinterpret_cast<const char *>(cfg);
+    for (size_t i = sizeof(*cfg); i < size; i++)
+      if (bytes[i]) cavs::fail(CAVS_EINVAL, "the configuration sets a field this library does not have");
+    cavs_session_config own{};
+    std::memcpy(&own, bytes, std::min(size, sizeof(own)));
+    *out = new cavs_session(own);
+  });
+}
+
+int(cavs_session_create)(const cavs_session_config *cfg, cavs_session **out) {
+  return cavs_session_create_sized(cfg, offsetof(cavs_session_config, vocab_head), out);
 }
 
 int cavs_session_destroy(cavs_session *s) {

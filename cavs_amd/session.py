@@ -43,7 +43,7 @@ def lib():
         l.cavs_session_stream.argtypes = [C.c_void_p]
         P, I, Z, F = C.c_void_p, C.c_int, C.c_size_t, C.c_float
         sigs = {
-            "cavs_session_create": [C.POINTER(_Config), C.POINTER(P)],
+            "cavs_session_create_sized": [C.POINTER(_Config), Z, C.POINTER(P)],
             "cavs_session_destroy": [P],
             "cavs_session_set_param": [P, C.c_char_p, P, Z],
             "cavs_session_get_param": [P, C.c_char_p, P, Z],
@@ -66,6 +66,7 @@ def lib():
         for k, a in sigs.items():
             fn = getattr(l, k)
             fn.argtypes, fn.restype = a, I
+        l.cavs_session_create = lambda cfg, out: l.cavs_session_create_sized(cfg, C.sizeof(_Config), out)  # (the header's macro)
         _lib = l
     return _lib
 

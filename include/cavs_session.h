@@ -114,7 +114,12 @@ typedef struct {
 enum { CAVS_OPTIMIZER_SGD = 0, CAVS_OPTIMIZER_ORTHO = 1 };
 
 const char *cavs_session_error(void);
+/* size: that of the struct as the caller was compiled with it.  Fields are added at its end and 0 is every field's default: what a smaller struct lacks is 0,
+ * and what a larger one holds beyond this library's has to be 0 (CAVS_EINVAL otherwise). */
+int cavs_session_create_sized(const cavs_session_config *cfg, size_t size, cavs_session **out);
+/* In the library, for programs compiled when there was no size: it reads the fields up to head_chunks. */
 int cavs_session_create(const cavs_session_config *cfg, cavs_session **out);
+#define cavs_session_create(cfg, out) cavs_session_create_sized(cfg, sizeof(cavs_session_config), out)
 int cavs_session_destroy(cavs_session *s);
 
 /* Parameters and their gradients by name: "Emb" "W" "U" "Bv" "Wfc" "bfc"

@@ -145,12 +145,8 @@ void Engine::ortho_setup() {
     param(key).state = true;
   };
   auto blocks = [&](const char *name, size_t at, int n, int rows) {  // n blocks [rows, h] side by side in rows of n H
-    const Param &p = param(name);
-    float *m = cfg_.ortho_momentum < 0.f ? nullptr : param(std::string(name) + ".momentum").w;
-    for (int k = 0; k < n; k++) {
-      const size_t first = at + k * H;
-      ortho_.push_back({rows, uH_, p.g + first, (int)(n * H), m ? m + first : nullptr, (int)(n * H), p.w + first, (int)(n * H), nullptr, 0});
-    }
+    const Param *m = cfg_.ortho_momentum < 0.f ? nullptr : &param(std::string(name) + ".momentum");
+    for (int k = 0; k < n; k++) ortho_.push_back({&param(name), m, at + k * H, rows, (int)(n * H)});
   };
   momentum("W");
   switch (cfg_.model) {
@@ -168,7 +164,16 @@ void Engine::ortho_setup() {
       blocks("W", 0, 1, uH_);
       blocks("W", H * H, 1, uH_);
   }
-  ortho_ws_.reserve(cavs_ortho_update_workspace(CAVS_F32, (int)ortho_.size(), ortho_.data()) / 4 + 1);
+  const std::vector<cavs_ortho_desc> d = ortho_descs();
+  ortho_ws_.reserve(cavs_ortho_update_workspace(CAVS_F32, (int)d.size(), d.data()) / 4 + 1);
+}
+
+// (where the tensors are now: bind_param may have moved them)
+std::vector<cavs_ortho_desc> Engine::ortho_descs() const {
+  std::vector<cavs_ortho_desc> d;
+  for (const OrthoBlock &b : ortho_)
+    d.push_back({b.rows, uH_, b.p->g + b.first, b.ld, b.m ? b.m->w + b.first : nullptr, b.ld, b.p->w + b.first, b.ld, nullptr, 0});
+  return d;
 }
 
 void Engine::ortho_update(float lr) {
@@ -176,7 +181,8 @@ void Engine::ortho_update(float lr) {
   const cavs_ortho_options o{5, 1, 3.4445f, -4.7750f, 2.0315f, 1e-7f, cfg_.ortho_momentum == 0.f ? 0.95f : std::max(cfg_.ortho_momentum, 0.f),
                              cfg_.ortho_lr > 0.f ? cfg_.ortho_lr : lr, cfg_.ortho_decay, update_guard()};
   // (weights here are stored [inputs, outputs]: x W, h U)
-  check(cavs_ortho_update_in_out(CAVS_F32, (int)ortho_.size(), ortho_.data(), &o, ortho_ws_.get(), ortho_ws_.capacity() * 4, stream_));
+  const std::vector<cavs_ortho_desc> d = ortho_descs();
+  check(cavs_ortho_update_in_out(CAVS_F32, (int)d.size(), d.data(), &o, ortho_ws_.get(), ortho_ws_.capacity() * 4, stream_));
   c_launches_ += 2 + 3 * o.steps;
   upk_valid_ = utp_valid_ = false;
 }

@@ -107,6 +107,7 @@ class Engine {
  private:
   Param &param(const std::string &name);
   void ortho_setup();
+  std::vector<cavs_ortho_desc> ortho_descs() const;
   void ortho_update(float lr);
   // the head without logits (cfg_.vocab_head; few classes have a head of their own)
   bool vocab_head() const;
@@ -222,7 +223,12 @@ class Engine {
   }
   float parse_ms_ = 0.f, sched_ms_ = 0.f, wait_ms_ = 0.f, host_step_ms_ = 0.f;
   std::map<std::string, std::unique_ptr<Param>> params_;
-  std::vector<cavs_ortho_desc> ortho_;  // the blocks of "W" and "U" the optimizer takes as matrices
+  struct OrthoBlock {
+    const Param *p, *m;  // m: the momentum, or null
+    size_t first;        // element
+    int rows, ld;
+  };
+  std::vector<OrthoBlock> ortho_;  // the blocks of "W" and "U" the optimizer takes as matrices
   DeviceArray<float> ortho_ws_, head_ws_;
 
   std::shared_ptr<Schedule> sched_ = std::make_shared<Schedule>();

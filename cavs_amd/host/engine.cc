@@ -2822,7 +2822,7 @@ void Engine::head_forward_backward(bool backward) {
                               head_ws_.get(), bytes, stream_));
       else
         check(cavs_vocab_xent_fwd(CAVS_F32, GO_.get(), H, Wfc.w, H, bfc.w, d_labels_, loss_.get(), nullptr, N, H, C, head_ws_.get(), bytes, stream_));
-      c_gemm_flops_ += (backward ? 8.0 : 2.0) * N * C * H;
+      c_gemm_flops_ += (backward ? 6.0 : 2.0) * N * C * H;  // (what the head is asked for; z may be made twice)
       c_launches_ += 1;
       return;
     }

@@ -4,9 +4,9 @@
 //   dX = d W,  dW = d^T X,  db = sums of d's columns
 //
 // The vocabulary goes by in pieces.  The first pass over them makes each tile of z in registers and leaves a maximum and a sum of
-// exponentials per row and tile; what they come to together is lse.  The second makes the tile again, d from it, and leaves d of a piece,
-// packed by token, which d X and d W are made of before the next piece overwrites it.  (d^T is read from the same bytes: packed in both orders, half
-// as many classes to a piece, fp32 10000 x 512 with 7088 tokens took 1869 us, and takes 1520.)
+// exponentials per row and tile; what they come to together is lse.  The second makes the tile again, d from it, and leaves d of a piece (of all classes
+// where that is 512 MB or less), packed by token, which d X and d W are made of before the next piece overwrites it.  (d^T is read from the same bytes: packed in
+// both orders, half as many classes to a piece, fp32 10000 x 512 with 7088 tokens took 1869 us, and takes 1520.)
 // Statistics, sums and accumulators are fp32; d is rounded to bf16 where the gradients are (half a unit of 2^-8, as their own
 // rounding), and is three bf16 parts, all of an fp32's bits, where they are fp32.
 #include <type_traits>
@@ -512,8 +512,10 @@ __global__ __launch_bounds__(256) void weights_kernel(const float *__restrict__ 
 
 // d = weight * (p - [label]) of a tile, packed by token (zero between the last class or token and the end of the steps), and its sums over the tile's
 // tokens.  `scale`, which multiplies all of d, stays out of what is rounded: next to the label, where p is small, p - 1 is -1 and a bit, which bf16 holds
-// well, while a factor in it is a rounding error that all of its kind share.  So is a token's weight for that token, which many tokens average out: of up to 64
-// bf16 ones (`beside`) it stays out as well.  d W has it as a factor of its rows then, and d^T X with X, in two parts, for which d is there twice.
+// well, while a factor in it is a rounding error that all of its kind share.  So is a token's weight for that token: of up to 64 bf16 ones (`beside`) it stays
+// out as well.  d W has it as a factor of its rows then, and d^T X with X, in two parts, for which d is there twice (64 tokens, 25040 x 1000: 123 us a call
+// without weights, 128 with them); of thousands of tokens that would be a quarter more operations and twice the d.  Errors of dX and dW, 25040 x 1000: 64 tokens 0.0019 of their
+// norm, 65 0.0024, 2371 0.0024 and 0.0023; rounding the gradients alone 0.0017.
 template <class T>
 __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, const float *__restrict__ lse, const float *__restrict__ weight, PackedOut d,
                                                                     float *__restrict__ sums, int ld_sums, float sums_scale, int beside) {

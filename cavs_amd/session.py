@@ -197,7 +197,8 @@ class Session:
     """One model bound to the device.  `opt` is the reference's bitmask
     (OPT_BATCHING selects the level-wise batch scheduler).
 
-    vocab_head: the softmax head of more than 8 classes without logits in memory; vertices labelled -1 take no part in it.
+    vocab_head: the softmax head of more than 8 classes without logits in memory; vertices labelled -1 take no part in it.  It saves
+    memory from tens of thousands of classes on; below that the head with logits is as small and a little faster.
     optimizer: "sgd", or "ortho": "W" and "U" by their orthogonalised momentum, block by block, the rest by SGD.  Its state
     is the parameter "W.momentum" / "U.momentum" (`param`, `set_params`); ortho_lr 0 is step's lr, ortho_momentum 0 is 0.95,
     negative none."""

@@ -360,16 +360,21 @@ int cavs_softmax_xent_sums(float *loss, float *dlogits, const float *logits, con
  * dloss is); one without any class that is not masked has lse = -infinity as well.  Otherwise a NaN in X or W makes
  * NaN of the results that depend on it, and so does an infinity, but for logits of -infinity that come of it (CAVS_BF16): probability 0.
  * n = 0 is allowed (dW and db become 0).
- * CAVS_F32: products as sums of bf16 parts in full fp32 precision, of all finite operands (the arithmetic of cavs_sgemm; of an operand or a d below 2^-110
- * bits below 2^-133 are lost, and results below 2^-126 may be); sums of products are made before `scale`, so they have to be floats without it.  CAVS_BF16: products of bf16 values
- * in fp32 accumulators, d (without scale, of up to 64 tokens without dloss) rounded to bf16 between its products, gradients rounded once.  Results are the same on every call.
+ * CAVS_F32: products as sums of bf16 parts in full fp32 precision, of all finite operands (the arithmetic of cavs_sgemm; of an operand or a d below
+ * 2^-110 bits below 2^-133 are lost, and results below 2^-126 may be).  CAVS_BF16: products of bf16 values in fp32 accumulators, d (without scale, of up to 64
+ * tokens without dloss too) rounded to bf16 between its products, gradients rounded once.  Sums of products are made before `scale`, so they have to be
+ * floats without it.  Results are the same on every call.
  *   _fwd  loss and lse
  *   _bwd  the gradients, from the lse that _fwd (or cavs_vocab_xent) left for the same X, W and b
  *   cavs_vocab_xent  both in one call
- * The vocabulary goes by in pieces; the logits are computed once for lse and once more for the gradients (up to 64 tokens: once in all).  The
- * workspace (16-byte aligned, of at least cavs_vocab_xent_workspace(type, n, H, C, grads) bytes on this device, grads = 0 for _fwd) holds the
- * d of one piece, all of the vocabulary only where that is 512 MB or less, and W of the piece, packed (up to 64 tokens: z); it may be reused by the next call on the same stream, not by one that overlaps in time.  At most 2^20 rows,
- * 2^23 classes, H <= 2^16.  The workspace query returns 0 for a shape or type that is refused. */
+ * The vocabulary goes by in pieces; the logits are computed once for lse and once more for the gradients (of up to 64 tokens with long rows or many classes
+ * once in all).  At most 2^20 rows, 2^23 classes, H <= 2^16.
+ * The workspace: 16-byte aligned, at least cavs_vocab_xent_workspace(type, n, H, C, grads) bytes on this device (grads = 0 for _fwd; 0: the shape or type is
+ * refused); for the next call on the same stream to reuse, not for one that overlaps in time.  It holds X and W packed (fp32: 6 bytes a value; of W
+ * the piece at hand, 128 MB, or with gradients all of it up to 512 MB; W once more where both orders are faster) and 8 bytes a token and 64 to 256 classes;
+ * with gradients d (2 bytes a token and class, fp32: 6) of all the vocabulary up to 512 MB and of a piece of 256 MB beyond, and what products leave in parts
+ * (up to 64 times dX and a piece's dW, in fp32); of those few tokens, instead of W, one float a token and class.  So it does not grow with n C, but of
+ * 7088 x 512 x 10000 in fp32 (609 MB) it is as large as logits and d logits would be. */
 enum { CAVS_F32 = 0, CAVS_BF16 = 1 };
 size_t cavs_vocab_xent_workspace(int type, int n, int H, int C, int grads);
 int cavs_vocab_xent_fwd(int type, const void *X, int ldx, const void *W, int ldw, const float *b, const float *labels, float *loss,

@@ -100,7 +100,9 @@ typedef struct {
    * chunks the last step's head ran (0: in one piece). */
   int head_chunks;
   /* Softmax loss, more than 8 classes: 1 = the head keeps no [N, C] logits or d logits (cavs_vocab_xent): vertices whose label is no
-   * class (-1) take no part in it then.  0 = the head with logits. */
+   * class (-1) take no part in it then.  0 = the head with logits.  What it saves is memory, of many classes (workspace of cavs_vocab_xent): it makes the
+   * logits twice and runs in one piece.  A chain LSTM of H = 512, 7331 vertices, ms a step and MB of device memory with logits / without: 10 000 classes 2.49 /
+   * 2.72, 1743 / 1703; 40 000 7.71 / 7.99, 4022 / 1642; 100 000 18.13 / 18.08, 8783 / 2166. */
   int vocab_head;
   /* What applies the gradients: 0 = SGD (cavs/backend/op_impl_sgd.cu).  1 = the input and recurrent weights ("W", "U"), each gate's (Tree-FC: each
    * child's) block a matrix, by their orthogonalised momentum (cavs_ortho_update_in_out, Nesterov, five steps: a block of "W" takes E inputs to H outputs,

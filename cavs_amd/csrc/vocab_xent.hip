@@ -514,8 +514,8 @@ __global__ __launch_bounds__(256) void weights_kernel(const float *__restrict__ 
 // tokens.  `scale`, which multiplies all of d, stays out of what is rounded: next to the label, where p is small, p - 1 is -1 and a bit, which bf16 holds
 // well, while a factor in it is a rounding error that all of its kind share.  So is a token's weight for that token: of up to 64 bf16 ones (`beside`) it stays
 // out as well.  d W has it as a factor of its rows then, and d^T X with X, in two parts, for which d is there twice (64 tokens, 25040 x 1000: 123 us a call
-// without weights, 128 with them); of thousands of tokens that would be a quarter more operations and twice the d.  Errors of dX and dW, 25040 x 1000: 64 tokens 0.0019 of their
-// norm, 65 0.0024, 2371 0.0024 and 0.0023; rounding the gradients alone 0.0017.
+// without weights, 128 with them); of thousands of tokens that would be a quarter more operations and twice the d.  Errors of dX and dW, 25040 x 1000:
+// 64 tokens 0.0019 of their norm, 65 0.0024, 2371 0.0024 and 0.0023; rounding the gradients alone 0.0017.
 template <class T>
 __global__ __launch_bounds__(T::THREADS, T::EU) void dlogits_kernel(TileArgs a, const float *__restrict__ lse, const float *__restrict__ weight, PackedOut d,
                                                                     float *__restrict__ sums, int ld_sums, float sums_scale, int beside) {

@@ -1,0 +1,491 @@
+// Y = R + drop(act(X W^T + b)) and its gradients: products with everything that follows them in their epilogue.
+//
+//   forward   Z = X W^T + b, Y = R + drop(act(Z))
+//   backward  D = drop(dY) . act'(Z), dX = D W, dW = D^T X, db = sums of D's columns
+//
+// Tiles are made of the transposed product, so that a lane of the 32x32 instruction holds neighbouring values of a row of the result: after an
+// exchange with the lane 32 away eight of them, which is what bias, residual and results are read and written in, and what one call of the dropout's
+// generator is for.
+#include <cmath>
+
+#include "dropout.h"
+#include "nt_product.h"
+
+namespace cavs {
+namespace {
+
+// ------------------------------------------------------------------ activations
+__device__ __forceinline__ float act_of(int act, float z) {
+  switch (act) {
+    case CAVS_ACT_RELU: return z < 0.f ? 0.f : z;
+    case CAVS_ACT_TANH: return tanhf(z);
+    case CAVS_ACT_SIGMOID: return 1.f / (1.f + expf(-z));
+    case CAVS_ACT_SILU: return z / (1.f + expf(-z));
+    case CAVS_ACT_GELU: return 0.5f * z * erfcf(-0.70710678f * z);
+    default: return z;
+  }
+}
+__device__ __forceinline__ float slope_of(int act, float z) {
+  switch (act) {
+    case CAVS_ACT_RELU: return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;
+    case CAVS_ACT_TANH: {
+      const float h = tanhf(z);
+      return (1.f - h) * (1.f + h);
+    }
+    case CAVS_ACT_SIGMOID: {
+      const float g = 1.f / (1.f + expf(-fabsf(z)));  // (even in z; 1 - g from the smaller exponential)
+      return g * (1.f - g);
+    }
+    case CAVS_ACT_SILU: {
+      const float g = 1.f / (1.f + expf(-z));
+      return g * (1.f + z * (1.f - g));
+    }
+    case CAVS_ACT_GELU: return 0.5f * erfcf(-0.70710678f * z) + z * (0.39894228f * expf(-0.5f * z * z));
+    default: return 1.f;
+  }
+}
+
+// ------------------------------------------------------------------ epilogues: eight neighbouring values of a row of the result
+template <class T>
+struct Forward {
+  const float *bias;
+  int act;
+  Mask m;
+  const T *R;
+  long ldr;
+  T *Z;
+  long ldz;
+  T *Y;
+  long ldy;
+  __device__ __forceinline__ void operator()(int row, int col, int left, float (&v)[8]) const {
+    if (bias) {
+      Eight<float> b;
+      b.load(bias + col, left);
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] += b[e];
+    }
+    if (Z) Eight<T>::store(Z + row * ldz + col, v, left);
+    if (act) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = act_of(act, v[e]);
+    }
+    if (m.t) drop8(m, draws_of(m, step_of(m), row_id(m, row), col >> 3), v);
+    if (R) {
+      Eight<T> r;
+      r.load(R + row * ldr + col, left);
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] += r[e];
+    }
+    Eight<T>::store(Y + row * ldy + col, v, left);
+  }
+};
+template <class T>
+struct Plain {
+  T *Y;
+  long ldy;
+  __device__ __forceinline__ void operator()(int row, int col, int left, float (&v)[8]) const { Eight<T>::store(Y + row * ldy + col, v, left); }
+};
+
+// ------------------------------------------------------------------ operands, packed (nt_product.h)
+template <class T>
+struct PackJob {
+  const T *src;
+  long ld;
+  int rows, K, orows;  // orows: rows of o, zero beyond those of src
+  PackedOut o;
+  int across, blocks;  // blocks of 64 columns, of 64 x 64
+};
+template <int P, class T>
+__global__ __launch_bounds__(256) void pack_kernel(PackJob<T> j0, PackJob<T> j1) {
+  __shared__ PackTile tile;
+  const int at = blockIdx.y * gridDim.x + blockIdx.x;
+  if (at >= j0.blocks + j1.blocks) return;
+  const bool second = at >= j0.blocks;
+  const PackJob<T> &g = second ? j1 : j0;
+  const int block = second ? at - j0.blocks : at, r0 = block / g.across * 64, k0 = block % g.across * 64;
+  load_tile(tile, g.src, g.ld, r0, k0, g.rows, g.K);
+  __syncthreads();
+  pack_tile<P>(tile, g.o, PackedOut{}, r0, k0, g.orows, g.K);
+}
+
+// D packed, and sums of its columns over 64 rows each [blocks of rows][N]
+template <class T>
+struct GradJob {
+  const T *dY, *Z;
+  long lddy, ldz;
+  int act;
+  Mask m;
+  int n, N, orows, across, blocks;
+  PackedOut o;
+  float *sums;
+};
+template <int P, class T>
+__global__ __launch_bounds__(256) void grad_kernel(GradJob<T> g) {
+  __shared__ PackTile tile;
+  __shared__ float part[4][64];
+  const int block = blockIdx.y * gridDim.x + blockIdx.x;
+  if (block >= g.blocks) return;
+  const int r0 = block / g.across * 64, k0 = block % g.across * 64, piece = threadIdx.x & 7;
+  const unsigned long long step = step_of(g.m);
+#pragma unroll
+  for (int q = 0; q < 2; q++) {
+    const int r = (threadIdx.x >> 3) + 32 * q, row = r0 + r, col = k0 + 8 * piece, left = row < g.n ? g.N - col : 0;
+    Eight<T> d, z;
+    d.zero(), z.zero();
+    if (left > 0) {
+      d.load(g.dY + row * g.lddy + col, left);
+      if (g.act) z.load(g.Z + row * g.ldz + col, left);
+    }
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = d[e];
+    if (g.m.t && left > 0) drop8(g.m, draws_of(g.m, step, row_id(g.m, row), col >> 3), v);
+#pragma unroll
+    for (int e = 0; e < 8; e++) tile[r][8 * piece + e] = e < left ? g.act ? v[e] * slope_of(g.act, z[e]) : v[e] : 0.f;
+  }
+  __syncthreads();
+  if (g.o.p) pack_tile<P>(tile, g.o, PackedOut{}, r0, k0, g.orows, g.N);
+  if (!g.sums) return;
+  const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; i++) s += tile[16 * w + i][c];
+  part[w][c] = s;
+  __syncthreads();
+  if (w == 0 && k0 + c < g.N) g.sums[(long)(r0 / 64) * g.N + k0 + c] = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
+}
+
+// ------------------------------------------------------------------ products of packed operands
+// result[row, col] = sum over k of A[col, k] B[row, k].  K in `splits` stretches of kchunk, each with sums of its own at part + split * rows * cols; part
+// null: straight to the epilogue.
+template <class E>
+struct Product {
+  PackedRef A, B;
+  int cols, rows, K, tilesM, tilesN, splits, kchunk;
+  float *part;
+  E out;
+};
+
+// The eight values of block 8 q of a row, q = 0 .. 3 of the 32 columns of a tile of accumulators: lanes below 32 have q = 2 pair, the others 2 pair + 1
+__device__ __forceinline__ void exchanged(const floatx16 &t, int pair, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(t[8 * pair + i]), __float_as_uint(t[8 * pair + 4 + i]), false, false);
+    v[i] = __uint_as_float(x[0]);
+    v[4 + i] = __uint_as_float(x[1]);
+  }
+}
+
+template <class T, bool TA, bool TB, class E>
+__global__ __launch_bounds__(T::THREADS, T::EU) void packed_product_kernel(Product<E> g) {
+  __shared__ __attribute__((aligned(16))) char S[T::LDS];
+  const int tiles = g.tilesM * g.tilesN, split = blockIdx.x / tiles;
+  int tm, tn;
+  nt_tile_of(blockIdx.x - split * tiles, g.tilesM, g.tilesN, &tm, &tn);
+  const int m0 = tm * T::BM, n0 = tn * T::BN, kbeg = split * g.kchunk, kend = min(g.K, kbeg + g.kchunk);
+  floatx16 acc[T::ACC][T::TM][T::TN];
+  nt_multiply<T, TA, TB>(g.A, g.cols, m0, g.B, g.rows, n0, kbeg, kend, S, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c0 = m0 + wave / T::WGN * T::WM + 8 * (lane >> 5), r0 = n0 + wave % T::WGN * T::WN + (lane & 31);
+#pragma unroll
+  for (int j = 0; j < T::TN; j++) {
+    const int row = r0 + 32 * j;
+    if (row >= g.rows) continue;
+#pragma unroll
+    for (int i = 0; i < T::TM; i++) {
+      if constexpr (T::ACC > 1) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[0][i][j][r] += acc[T::ACC - 1][i][j][r];
+      }
+#pragma unroll
+      for (int pair = 0; pair < 2; pair++) {
+        float v[8];
+        exchanged(acc[0][i][j], pair, v);
+        const int col = c0 + 32 * i + 16 * pair;
+        if (col >= g.cols) continue;
+        if (g.part) Eight<float>::store(g.part + ((long)split * g.rows + row) * g.cols + col, v, g.cols - col);
+        else g.out(row, col, g.cols - col, v);
+      }
+    }
+  }
+}
+
+// what products left in parts, in their order, to the epilogue; pieces of eight columns
+template <class E>
+__global__ __launch_bounds__(256) void parts_kernel(const float *part, int parts, int rows, int cols, E out) {
+  const int pieces = (cols + 7) / 8;
+  const long total = (long)rows * pieces, i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int row = (int)(i / pieces), col = 8 * (int)(i - (long)row * pieces), left = cols - col;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < parts; p += 4) {
+    Eight<float> t[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      t[k].zero();
+      if (p + k < parts) t[k].load(part + ((long)(p + k) * rows + row) * cols + col, left);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] += t[k][e];
+  }
+  out(row, col, left, v);
+}
+
+__global__ __launch_bounds__(256) void column_sums_kernel(const float *part, int parts, int cols, float *out) {
+  __shared__ float each[4][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6, per = (parts + 3) / 4, end = min(parts, (w + 1) * per);
+  float s = 0.f;
+  if (c < cols)
+    for (int p = w * per; p < end; p += 8) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[k] = p + k < end ? part[(long)(p + k) * cols + c] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; k++) s += v[k];
+    }
+  each[w][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (w == 0 && c < cols) out[c] = (each[0][threadIdx.x] + each[1][threadIdx.x]) + (each[2][threadIdx.x] + each[3][threadIdx.x]);
+}
+
+// ------------------------------------------------------------------ what a call consists of
+template <int P> struct Tiles;
+template <> struct Tiles<1> {
+  using L = NtTile<1, 256, 128, 32, 2, 2>;
+  using M = NtTile<1, 128, 128, 32, 2, 2>;
+  using S = NtTile<1, 64, 64, 64, 2, 2, 3>;
+};
+template <> struct Tiles<3> {
+  using L = NtTile<3, 128, 128, 16, 2, 2>;
+  using M = L;
+  using S = NtTile<3, 64, 64, 32, 2, 2>;
+};
+template <int P, class F>
+int with_tile(int size, F &&f) {
+  using TT = Tiles<P>;
+  if (size == 2) return f(typename TT::L{});
+  if (size == 1) return f(typename TT::M{});
+  return f(typename TT::S{});
+}
+
+constexpr int kSplits = 32;
+struct Shape {  // of a product
+  int size, tm, tn, splits, kchunk;
+};
+// the largest tile that still gives most compute units one; K in stretches where tiles are fewer than two a unit
+template <int P>
+Shape shape_of(int cols, int rows, int K) {
+  Shape s{};
+  int bm = 0, bn = 0;
+  for (s.size = 2; s.size >= 0; s.size--) {
+    with_tile<P>(s.size, [&](auto t) { return bm = decltype(t)::BM, bn = decltype(t)::BN, 0; });
+    if (s.size == 0 || (long)tiles_of(cols, bm) * tiles_of(rows, bn) >= num_cus() * 3 / 4) break;
+  }
+  s.tm = tiles_of(cols, bm), s.tn = tiles_of(rows, bn);
+  const long tiles = (long)s.tm * s.tn;
+  int splits = (int)(tiles * 2 <= num_cus() ? 2 * num_cus() / tiles : 1);
+  const int most = K / 256 > 0 ? K / 256 : 1;
+  splits = splits > most ? most : splits;
+  splits = splits > kSplits ? kSplits : splits;
+  s.kchunk = ceil_to((K + splits - 1) / splits, kPlaneAlign);
+  s.splits = (K + s.kchunk - 1) / s.kchunk;
+  return s;
+}
+
+struct Plan {
+  int Kp, Np, np;  // as contraction lengths
+  Shape fwd, dx, dw;
+  size_t x, w, d, part, sums, bytes;
+};
+template <int P>
+Plan plan_of(int n, int K, int N, int back) {
+  Plan p{};
+  p.Kp = ceil_to(K, kPlaneAlign), p.Np = ceil_to(N, kPlaneAlign), p.np = ceil_to(n, kPlaneAlign);
+  size_t at = 0, part = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) & ~(size_t)255;
+    return here;
+  };
+  auto parts = [&](const Shape &s, int rows, int cols) {
+    const size_t b = s.splits > 1 ? (size_t)s.splits * rows * cols * 4 : 0;
+    part = part > b ? part : b;
+  };
+  p.x = take(packed_bytes<P>(p.np, p.Kp));
+  p.w = take(packed_bytes<P>(p.Np, p.Kp));
+  if (!back) {
+    p.fwd = shape_of<P>(N, n, p.Kp);
+    parts(p.fwd, n, N);
+  } else {
+    p.d = take(packed_bytes<P>(p.np, p.Np));
+    p.dx = shape_of<P>(K, n, p.Np);
+    p.dw = shape_of<P>(K, N, p.np);
+    parts(p.dx, n, K), parts(p.dw, N, K);
+    p.sums = take((size_t)(p.np / 64) * N * 4);
+  }
+  p.part = take(part);
+  p.bytes = at;
+  return p;
+}
+
+struct Call {
+  const void *X, *W, *R, *Z, *dY;
+  int ldx, ldw, ldr, ldz, lddy;
+  const float *b;
+  int act;
+  Mask m;
+  void *Zout, *Y, *dX, *dW;
+  int ldy, lddx, lddw;
+  float *db;
+  int n, K, N;
+};
+
+inline dim3 grid_of(long blocks) {
+  const long most = (1 << 24) - 1, high = (blocks + most - 1) / most;
+  return dim3((unsigned)((blocks + high - 1) / high), (unsigned)high);
+}
+template <int P, class T>
+PackJob<T> packing(const void *src, int ld, int rows, int K, int orows, char *o, int Kp) {
+  PackJob<T> j{static_cast<const T *>(src), ld, rows, K, orows, {reinterpret_cast<u16 *>(o), Kp}, Kp / 64, 0};
+  j.blocks = j.across * tiles_of(orows, 64);
+  return j;
+}
+
+template <int P, bool TA, bool TB, class E>
+int product(const Shape &s, const PackedRef &A, int cols, const PackedRef &B, int rows, int K, float *part, const E &out, hipStream_t st) {
+  Product<E> g{A, B, cols, rows, K, s.tm, s.tn, s.splits, s.kchunk, s.splits > 1 ? part : nullptr, out};
+  with_tile<P>(s.size, [&](auto t) {
+    using T = decltype(t);
+    launch(packed_product_kernel<T, TA, TB, E>, s.tm * s.tn * s.splits, T::THREADS, 0, st, g);
+    return 0;
+  });
+  CAVS_LAUNCH_CHECK();
+  if (g.part) {
+    launch(parts_kernel<E>, (unsigned)(((long)rows * ((cols + 7) / 8) + 255) / 256), 256, 0, st, g.part, s.splits, rows, cols, out);
+    CAVS_LAUNCH_CHECK();
+  }
+  return CAVS_OK;
+}
+
+template <int P, class T>
+int run_fwd(const Call &c, char *ws, hipStream_t st) {
+  const Plan p = plan_of<P>(c.n, c.K, c.N, 0);
+  const PackJob<T> x = packing<P, T>(c.X, c.ldx, c.n, c.K, c.n, ws + p.x, p.Kp), w = packing<P, T>(c.W, c.ldw, c.N, c.K, c.N, ws + p.w, p.Kp);
+  launch(pack_kernel<P, T>, grid_of((long)x.blocks + w.blocks), 256, 0, st, x, w);
+  CAVS_LAUNCH_CHECK();
+  const Forward<T> out{c.b, c.act, c.m, static_cast<const T *>(c.R), c.ldr, static_cast<T *>(c.Zout), c.ldz, static_cast<T *>(c.Y), c.ldy};
+  return product<P, false, false>(p.fwd, PackedRef{w.o.p, p.Kp}, c.N, PackedRef{x.o.p, p.Kp}, c.n, p.Kp, reinterpret_cast<float *>(ws + p.part), out, st);
+}
+
+template <int P, class T>
+int run_bwd(const Call &c, char *ws, hipStream_t st) {
+  const Plan p = plan_of<P>(c.n, c.K, c.N, 1);
+  GradJob<T> g{static_cast<const T *>(c.dY), static_cast<const T *>(c.Z), c.lddy, c.ldz, c.act, c.m, c.n, c.N, p.np, p.Np / 64, 0,
+               {c.dX || c.dW ? reinterpret_cast<u16 *>(ws + p.d) : nullptr, p.Np}, c.db ? reinterpret_cast<float *>(ws + p.sums) : nullptr};
+  g.blocks = g.across * (p.np / 64);
+  launch(grad_kernel<P, T>, grid_of(g.blocks), 256, 0, st, g);
+  CAVS_LAUNCH_CHECK();
+  PackJob<T> x = packing<P, T>(c.X, c.ldx, c.n, c.K, p.np, ws + p.x, p.Kp), w = packing<P, T>(c.W, c.ldw, c.N, c.K, p.Np, ws + p.w, p.Kp);
+  const PackedRef X{x.o.p, p.Kp}, W{w.o.p, p.Kp}, D{g.o.p, p.Np};
+  if (!c.dW) x.blocks = 0;
+  if (!c.dX) w.blocks = 0;
+  if (c.dX || c.dW) {
+    launch(pack_kernel<P, T>, grid_of((long)x.blocks + w.blocks), 256, 0, st, x, w);
+    CAVS_LAUNCH_CHECK();
+  }
+  float *part = reinterpret_cast<float *>(ws + p.part);
+  if (c.dX) {
+    if (const int rc = product<P, true, false>(p.dx, W, c.K, D, c.n, p.Np, part, Plain<T>{static_cast<T *>(c.dX), c.lddx}, st)) return rc;
+  }
+  if (c.dW) {
+    if (const int rc = product<P, true, true>(p.dw, X, c.K, D, c.N, p.np, part, Plain<T>{static_cast<T *>(c.dW), c.lddw}, st)) return rc;
+  }
+  if (c.db) {
+    launch(column_sums_kernel, (c.N + 63) / 64, 256, 0, st, g.sums, p.np / 64, c.N, c.db);
+    CAVS_LAUNCH_CHECK();
+  }
+  return CAVS_OK;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void no_rows_kernel(T *dW, long ld, float *db, int N, int K) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (db && i < N) db[i] = 0.f;
+  if (dW)
+    for (long at = i; at < (long)N * K; at += (long)gridDim.x * 256) dW[at / K * ld + at % K] = T(0);
+}
+
+// (offsets within a tile's rows are below 2^32 bytes, and a launch has less than 2^24 tiles)
+constexpr int kMostRows = 1 << 20, kMostK = 1 << 16;
+constexpr long kMostOut = 1l << 36;
+bool shape_ok(int n, int K, int N) { return n <= kMostRows && N <= kMostRows && K <= kMostK && (long)n * N <= kMostOut && (long)N * K <= kMostOut; }
+
+int check(const char *who, int type, const Call &c, const cavs_dropout_mask *mask, Mask *m) {
+  CAVS_REQUIRE(type == CAVS_F32 || type == CAVS_BF16, "%s: type %d is neither CAVS_F32 nor CAVS_BF16", who, type);
+  CAVS_REQUIRE(c.n >= 0 && c.K > 0 && c.N > 0, "%s: bad shape n=%d K=%d N=%d", who, c.n, c.K, c.N);
+  CAVS_REQUIRE(shape_ok(c.n, c.K, c.N), "%s: unsupported shape n=%d K=%d N=%d (at most 2^20, 2^16, 2^20; n N and N K 2^36)", who, c.n, c.K, c.N);
+  CAVS_REQUIRE(c.act >= CAVS_ACT_NONE && c.act <= CAVS_ACT_GELU, "%s: unknown activation %d", who, c.act);
+  CAVS_REQUIRE(c.ldx >= c.K && c.ldw >= c.K, "%s: a row stride is below K=%d", who, c.K);
+  CAVS_REQUIRE(mask_of(mask, m), "%s: p is not in [0, 1)", who);
+  return CAVS_OK;
+}
+int check_workspace(const char *who, const void *ws, size_t bytes, size_t need) {
+  CAVS_REQUIRE(ws && bytes >= need, "%s: workspace of %zu bytes needed, %zu given", who, need, bytes);
+  CAVS_REQUIRE(aligned16(ws), "%s: the workspace must be 16-byte aligned", who);
+  return CAVS_OK;
+}
+
+}  // namespace
+}  // namespace cavs
+
+using namespace cavs;
+
+extern "C" {
+
+size_t cavs_linear_workspace(int type, int n, int K, int N, int back) {
+  if (n <= 0 || K <= 0 || N <= 0 || !shape_ok(n, K, N) || (type != CAVS_F32 && type != CAVS_BF16)) return 0;
+  return (type == CAVS_F32 ? plan_of<3>(n, K, N, back) : plan_of<1>(n, K, N, back)).bytes;
+}
+
+int cavs_linear_fwd(int type, const void *X, int ldx, const void *W, int ldw, const float *b, int act, const cavs_dropout_mask *mask, const void *R, int ldr,
+                    void *Z, int ldz, void *Y, int ldy, int n, int K, int N, void *workspace, size_t workspace_bytes, void *stream) {
+  const char *who = "cavs_linear_fwd";
+  Call c{};
+  c.X = X, c.ldx = ldx, c.W = W, c.ldw = ldw, c.b = b, c.act = act, c.R = R, c.ldr = ldr, c.Zout = Z, c.ldz = ldz, c.Y = Y, c.ldy = ldy, c.n = n, c.K = K, c.N = N;
+  if (const int rc = check(who, type, c, mask, &c.m)) return rc;
+  CAVS_REQUIRE(ldy >= N && (!R || ldr >= N) && (!Z || ldz >= N), "%s: a row stride is below N=%d", who, N);
+  if (n == 0) return CAVS_OK;
+  CAVS_REQUIRE(X && W && Y, "%s: null pointer", who);
+  if (const int rc = check_workspace(who, workspace, workspace_bytes, cavs_linear_workspace(type, n, K, N, 0))) return rc;
+  char *w = static_cast<char *>(workspace);
+  return type == CAVS_F32 ? run_fwd<3, float>(c, w, as_stream(stream)) : run_fwd<1, u16>(c, w, as_stream(stream));
+}
+
+int cavs_linear_bwd(int type, const void *X, int ldx, const void *W, int ldw, const void *Z, int ldz, int act, const cavs_dropout_mask *mask, const void *dY,
+                    int lddy, void *dX, int lddx, void *dW, int lddw, float *db, int n, int K, int N, void *workspace, size_t workspace_bytes,
+                    void *stream) {
+  const char *who = "cavs_linear_bwd";
+  Call c{};
+  c.X = X, c.ldx = ldx, c.W = W, c.ldw = ldw, c.Z = Z, c.ldz = ldz, c.act = act, c.dY = dY, c.lddy = lddy, c.dX = dX, c.lddx = lddx, c.dW = dW, c.lddw = lddw;
+  c.db = db, c.n = n, c.K = K, c.N = N;
+  if (const int rc = check(who, type, c, mask, &c.m)) return rc;
+  CAVS_REQUIRE(lddy >= N && (!act || ldz >= N) && (!dX || lddx >= K) && (!dW || lddw >= K), "%s: a row stride is below its width", who);
+  hipStream_t st = as_stream(stream);
+  if (!dX && !dW && !db) return CAVS_OK;
+  if (n == 0) {  // sums over no rows
+    if (!dW && !db) return CAVS_OK;
+    const unsigned groups = (unsigned)((N + 255) / 256);
+    if (type == CAVS_F32) launch(no_rows_kernel<float>, groups, 256, 0, st, static_cast<float *>(dW), (long)lddw, db, N, K);
+    else launch(no_rows_kernel<u16>, groups, 256, 0, st, static_cast<u16 *>(dW), (long)lddw, db, N, K);
+    CAVS_LAUNCH_CHECK();
+    return CAVS_OK;
+  }
+  CAVS_REQUIRE(dY && (!act || Z) && (!dW || X) && (!dX || W), "%s: null pointer", who);
+  if (const int rc = check_workspace(who, workspace, workspace_bytes, cavs_linear_workspace(type, n, K, N, 1))) return rc;
+  char *w = static_cast<char *>(workspace);
+  return type == CAVS_F32 ? run_bwd<3, float>(c, w, st) : run_bwd<1, u16>(c, w, st);
+}
+
+}  // extern "C"

@@ -68,6 +68,26 @@ class OrthoOptions(C.Structure):
                 ("guard", _P)]
 
 
+class DropoutMask(C.Structure):
+    """cavs_dropout_mask"""
+    _fields_ = [("p", _F), ("seed", C.c_ulonglong), ("step", C.c_ulonglong), ("step_word", _P), ("ids", _P)]
+
+
+class NormDesc(C.Structure):
+    """cavs_norm_desc"""
+    _fields_ = [("n", _I), ("w", _I), ("y", _P), ("ldy", _I), ("r", _P), ("ldr", _I), ("gate_rows", _P), ("ldg", _I), ("gate", _P), ("scale", _F),
+                ("post", _I), ("post_w", _P), ("post_b", _P), ("pre", _I), ("pre_w", _P), ("pre_b", _P), ("eps", _F)]
+
+
+class NormGrads(C.Structure):
+    """cavs_norm_grads"""
+    _fields_ = [("dy", _P), ("lddy", _I), ("dr", _P), ("lddr", _I), ("dgate_rows", _P), ("lddg", _I), ("dgate", _P), ("dpost_w", _P), ("dpost_b", _P),
+                ("dpre_w", _P), ("dpre_b", _P)]
+
+
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+ACT = dict(none=0, relu=1, tanh=2, sigmoid=3, silu=4, gelu=5)
+
 GEMM_C_UNUSED, GEMM_A_ZERO, GEMM_B_ZERO = 1, 2, 3
 
 
@@ -143,6 +163,12 @@ _SIGS = {
     "cavs_sgd": [_P, _P, _F, _Z, _P],
     "cavs_ortho_update": [_I, _I, C.POINTER(OrthoDesc), C.POINTER(OrthoOptions), _P, _Z, _P],
     "cavs_ortho_update_in_out": [_I, _I, C.POINTER(OrthoDesc), C.POINTER(OrthoOptions), _P, _Z, _P],
+    "cavs_dropout": [_I, _P, _I, _P, _I, _P, _I, _I, _I, C.POINTER(DropoutMask), _P],
+    "cavs_dropout_advance": [_P, C.c_ulonglong, _P],
+    "cavs_norm_residual_fwd": [_I, C.POINTER(NormDesc), _P, _I, _P, _I, _P],
+    "cavs_norm_residual_bwd": [_I, C.POINTER(NormDesc), _P, _I, _P, _I, _P, _I, C.POINTER(NormGrads), _P, _Z, _P],
+    "cavs_linear_fwd": [_I, _P, _I, _P, _I, _P, _I, C.POINTER(DropoutMask), _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _Z, _P],
+    "cavs_linear_bwd": [_I, _P, _I, _P, _I, _P, _I, _I, C.POINTER(DropoutMask), _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _P, _Z, _P],
     "cavs_ew_binary": [_I, _P, _P, _Z, _P, _Z, _Z, _I, _P],
     "cavs_ew_unary": [_I, _P, _P, _Z, _I, _P],
     "cavs_scale": [_P, _P, _F, _Z, _P],
@@ -217,7 +243,8 @@ _RESTYPE = {"cavs_last_error": C.c_char_p, "cavs_abi_version": _I, "cavs_sgemm_s
             "cavs_group_rounds_ok": _I, "cavs_group_max_groups": _I, "cavs_group_rows": _I, "cavs_tail_rounds_ok": _I, "cavs_tail_max_rounds": _I, "cavs_tail_max_groups": _I, "cavs_tail_sync_bytes": _Z,
             "cavs_sgemm_splitk_static_max_bytes": _Z,
             "cavs_embed_index_ints": _Z, "cavs_embed_index_workspace": _Z, "cavs_gather_sums_workspace": _Z,
-            "cavs_schedule_arena_scratch": _Z, "cavs_vocab_xent_workspace": _Z, "cavs_ortho_update_workspace": _Z}
+            "cavs_schedule_arena_scratch": _Z, "cavs_vocab_xent_workspace": _Z, "cavs_ortho_update_workspace": _Z,
+            "cavs_norm_residual_workspace": _Z, "cavs_linear_workspace": _Z}
 _NOCHECK = {"cavs_last_error": [], "cavs_abi_version": [], "cavs_sgemm_splitk_workspace": [_I, _I, _I],
             "cavs_fc_softmax_xent_workspace": [_I, _I, _I], "cavs_colsum_blocks_workspace": [_I, _I, _I],
             "cavs_clip_grads_workspace": [_I], "cavs_sgemm_group_workspace": [_I, C.POINTER(GemmDesc)],
@@ -226,7 +253,8 @@ _NOCHECK = {"cavs_last_error": [], "cavs_abi_version": [], "cavs_sgemm_splitk_wo
             "cavs_group_rounds_ok": [_I], "cavs_group_max_groups": [_I], "cavs_group_rows": [], "cavs_tail_rounds_ok": [_I, _I], "cavs_tail_max_rounds": [], "cavs_tail_max_groups": [], "cavs_tail_sync_bytes": [],
             "cavs_embed_index_ints": [_I], "cavs_embed_index_workspace": [_I], "cavs_gather_sums_workspace": [_I, _I],
             "cavs_schedule_arena_scratch": [_I, _I], "cavs_vocab_xent_workspace": [_I, _I, _I, _I, _I],
-            "cavs_ortho_update_workspace": [_I, _I, C.POINTER(OrthoDesc)]}
+            "cavs_ortho_update_workspace": [_I, _I, C.POINTER(OrthoDesc)], "cavs_norm_residual_workspace": [_I, _I],
+            "cavs_linear_workspace": [_I, _I, _I, _I, _I]}
 
 EW_BINARY = dict(add=0, sub=1, mul=2, div=3, sigmoid_grad=4, tanh_grad=5, relu_grad=6, equal=7)
 EW_UNARY = dict(assign=0, neg=1, abs=2, square=3, sigmoid=4, tanh=5, relu=6)

@@ -388,6 +388,95 @@ int cavs_vocab_xent(int type, const void *X, int ldx, const void *W, int ldw, co
 /* SGD (cavs/backend/op_impl_sgd.cu): w -= lr * g */
 int cavs_sgd(float *w, const float *g, float lr, size_t n, void *stream);
 
+/* ------------------------------------------------------------------ residual block
+ * What today's models put between their states and the head (no counterpart in the reference): dropout, norms with a gate and a residual scale, and
+ * products with everything that follows them in their epilogue.  For a block  u = drop(act(norm(h) W1^T + b1));  y = h + drop(u W2^T + b2)  forward is
+ * cavs_norm_residual_fwd and two cavs_linear_fwd, backward two cavs_linear_bwd and cavs_norm_residual_bwd, whose `ds` is d y.
+ * Matrices are of `type` (CAVS_F32 or CAVS_BF16), row strides in elements, any of at least the width; biases, norms' weights, a gate of one value a column
+ * and all of their gradients are fp32.  Nothing but an element's own alignment is asked for, unless said.  Results are the same on every call. */
+
+/* Which elements a dropout keeps, from a counter-based generator (Philox4x32 of seven rounds, Salmon et al. 2011): nothing is stored, and whoever passes the
+ * same p, seed and step gets the same mask, the backward pass among them.  Element (i, j) is kept if its draw, 16 bits, is at least t = round(65536 p)
+ * (p to the nearest 2^-16; at most 65535); kept elements are multiplied by 65536 / (65536 - t), dropped ones are 0, whatever they were.
+ * Draw (i, j): key = seed (low word first); counter = (j / 8, ids ? ids[i] : i, low word, high word of step + *step_word); of the four words the
+ * (j % 8) / 2-th, its low half where j is even. */
+typedef struct {
+  float p;                             /* in [0, 1) */
+  unsigned long long seed, step;       /* different places of a model: different seeds; different steps of training: different steps */
+  const unsigned long long *step_word; /* device, 8-byte aligned, or NULL: is added to `step` as the call runs, so that a captured call draws anew (cavs_dropout_advance) */
+  const int *ids;                      /* device, a row's number in the generator, or NULL: its place.  With vertex ids a vertex's mask does not depend on the schedule */
+} cavs_dropout_mask;
+/* y = r + drop(x) for n rows of w; r NULL: 0.  y may be x or r, with their row stride; otherwise it may overlap neither.  The gradient of x is the same
+ * call on d y (without r, or with r = y = what to add it to); the gradient of r is d y. */
+int cavs_dropout(int type, void *y, int ldy, const void *x, int ldx, const void *r, int ldr, int n, int w, const cavs_dropout_mask *mask,
+                 void *stream);
+/* *step_word += by, on the stream */
+int cavs_dropout_advance(unsigned long long *step_word, unsigned long long by, void *stream);
+
+/* Norms after and before a block, its gate and the residual's scale, rows of w values:
+ *   z = post(y);  s = r + scale * gate . z;  x = pre(s)
+ * post, pre: CAVS_NORM_NONE (the values themselves), _RMS ((v / sqrt(mean v^2 + eps)) . weight + bias), _LAYER (((v - mean) / sqrt(var + eps)) . weight
+ * + bias; var without a correction for the mean).  Weights [w] NULL: ones, biases [w] NULL: zeros, r NULL: zeros, gate: a row of values
+ * [w], a matrix gate_rows [n, w], or neither: ones.  A norm alone: y, pre, scale 1 and r, gate, s NULL.
+ *   _fwd  s and x (either may be NULL), x from s before it is rounded.  s or x may be y, r or gate_rows, with their row stride, not each other.
+ *   _bwd  from s as _fwd left it (read if pre is a norm and dx given), ds (the gradient of s from elsewhere) and dx (of x), either of which may be NULL:
+ *         D = ds + d<pre(s), dx>/ds;  dr = D;  dgate = scale z . D (of a row of values the sum over rows);  dy, dpost_w, dpost_b through
+ *         dz = scale gate . D;  dpre_w, dpre_b: sums over rows.  What is NULL is not computed; r and, where nothing needs it, y are not read.
+ *         dr may be ds, dx or s, dy may be y, dgate_rows may be gate_rows, with their row stride; otherwise what is written may overlap nothing else.
+ * Sums of a row, and its mean, variance and their like, in 64 bits; sums over rows in fp32, per workgroup and then across them.  w <= 16384, n < 2^22.
+ * n = 0 is allowed (gradients that are sums become 0).  An infinity or a NaN in a row makes NaN of what depends on the row.
+ * The workspace of _bwd: 16-byte aligned, at least cavs_norm_residual_workspace(n, w) bytes on this device (not read where no sums over rows are wanted);
+ * for the next call on the same stream to reuse, not for one that overlaps in time. */
+enum { CAVS_NORM_NONE = 0, CAVS_NORM_RMS = 1, CAVS_NORM_LAYER = 2 };
+typedef struct {
+  int n, w;
+  const void *y;
+  int ldy;
+  const void *r;
+  int ldr;
+  const void *gate_rows;
+  int ldg;
+  const float *gate;
+  float scale;
+  int post;
+  const float *post_w, *post_b;
+  int pre;
+  const float *pre_w, *pre_b;
+  float eps; /* above 0; of both norms */
+} cavs_norm_desc;
+typedef struct {
+  void *dy;
+  int lddy;
+  void *dr;
+  int lddr;
+  void *dgate_rows;
+  int lddg;
+  float *dgate, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+} cavs_norm_grads;
+size_t cavs_norm_residual_workspace(int n, int w);
+int cavs_norm_residual_fwd(int type, const cavs_norm_desc *d, void *s, int lds, void *x, int ldx, void *stream);
+int cavs_norm_residual_bwd(int type, const cavs_norm_desc *d, const void *s, int lds, const void *ds, int ldds, const void *dx, int lddx,
+                           const cavs_norm_grads *grads, void *workspace, size_t workspace_bytes, void *stream);
+
+/* FullyConnected (cavs/backend/op_impl_fullyconnected_cublas.cc:71-79, gradients :150-163) with what follows it:
+ *   Z = X W^T + b;  Y = R + drop(act(Z))            X [n,K], W [N,K], b [N], Z and R and Y [n,N]
+ *   D = drop(dY) . act'(Z);  dX = D W;  dW = D^T X;  db = sum of D's rows;  the gradient of R is dY
+ * b, R and mask may be NULL; Z NULL: not kept (_bwd reads it unless act is CAVS_ACT_NONE, _fwd writes it; Y is made of Z before it is rounded).  What is
+ * NULL of dX, dW and db is not computed.  Y may be R, with its row stride; otherwise outputs may overlap neither inputs nor each other.
+ * CAVS_F32: products as sums of bf16 parts in full fp32 precision (the arithmetic of cavs_sgemm).  CAVS_BF16: products of bf16 values in fp32 accumulators; D
+ * is rounded to bf16 between its products (not in db), results once.
+ * At most 2^20 rows, N <= 2^20, K <= 2^16, n N and N K <= 2^36.  n = 0 is allowed (dW and db become 0).
+ * The workspace: 16-byte aligned, at least cavs_linear_workspace(type, n, K, N, back) bytes on this device (back: 0 for _fwd; 0: the shape or type is
+ * refused); for the next call on the same stream to reuse, not for one that overlaps in time. */
+enum { CAVS_ACT_NONE = 0, CAVS_ACT_RELU = 1, CAVS_ACT_TANH = 2, CAVS_ACT_SIGMOID = 3, CAVS_ACT_SILU = 4, CAVS_ACT_GELU = 5 /* z Phi(z) */ };
+size_t cavs_linear_workspace(int type, int n, int K, int N, int back);
+int cavs_linear_fwd(int type, const void *X, int ldx, const void *W, int ldw, const float *b, int act, const cavs_dropout_mask *mask,
+                    const void *R, int ldr, void *Z, int ldz, void *Y, int ldy, int n, int K, int N, void *workspace,
+                    size_t workspace_bytes, void *stream);
+int cavs_linear_bwd(int type, const void *X, int ldx, const void *W, int ldw, const void *Z, int ldz, int act,
+                    const cavs_dropout_mask *mask, const void *dY, int lddy, void *dX, int lddx, void *dW, int lddw, float *db, int n,
+                    int K, int N, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------------------------ elementwise
  * The un-fused elementwise family (cavs/backend/op_impl_elementwise.{cu,cuh},
  * functor_elementwise.h, op_impl_activation_cudnn.cu).  Operands are read as

@@ -8,8 +8,8 @@
 // generator is for.
 #include <cmath>
 
+#include "direct_product.h"
 #include "dropout.h"
-#include "nt_product.h"
 
 namespace cavs {
 namespace {
@@ -210,6 +210,91 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void packed_product_kernel(Produ
   }
 }
 
+// ------------------------------------------------------------------ products of operands as they lie (direct_product.h)
+template <class E>
+struct DirectJob {
+  DirectRef A, B;
+  int cols, rows, K, tilesM, tilesN, kchunk;
+  float *part;
+  E out;
+};
+template <class T, bool TA, bool TB, class E>
+__global__ __launch_bounds__(T::THREADS, T::EU) void direct_product_kernel(DirectJob<E> g) {
+  __shared__ __attribute__((aligned(16))) char S[T::LDS];
+  const int tiles = g.tilesM * g.tilesN, split = blockIdx.x / tiles;
+  int tm, tn;
+  nt_tile_of(blockIdx.x - split * tiles, g.tilesM, g.tilesN, &tm, &tn);
+  const int m0 = tm * T::BM, n0 = tn * T::BN, kbeg = split * g.kchunk, kend = min(g.K, kbeg + g.kchunk);
+  floatx4 acc[T::I][2 * T::J];
+  direct_multiply<TA, TB>(T{}, g.A, g.cols, m0, g.B, g.rows, n0, kbeg, kend, S, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int j = 0; j < T::J; j++) {
+    const int row = n0 + T::row(wave, lane, j);
+#pragma unroll
+    for (int i = 0; i < T::I; i++) {
+      float v[8];
+      eight_columns(acc[i][2 * j], acc[i][2 * j + 1], v);
+      const int col = m0 + T::col(wave, lane, i);
+      if (row >= g.rows || col >= g.cols) continue;
+      if (g.part) Eight<float>::store(g.part + ((long)split * g.rows + row) * g.cols + col, v, g.cols - col);
+      else g.out(row, col, g.cols - col, v);
+    }
+  }
+}
+
+// D as it lies (write: bf16, rows of N), and sums of its columns over 64 rows each [stretches of rows][N]; 256 columns a workgroup
+__global__ __launch_bounds__(256) void grad_rows_kernel(GradJob<u16> g, u16 *D) {
+  __shared__ float part[8][256];
+  const int block = blockIdx.y * gridDim.x + blockIdx.x;
+  if (block >= g.blocks) return;
+  const int piece = threadIdx.x & 31, line = threadIdx.x >> 5, r0 = block / g.across * 64, col = block % g.across * 256 + 8 * piece;
+  const int left = g.N - col;
+  const unsigned long long step = step_of(g.m);
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (left > 0) {
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      Eight<u16> d[4], z[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int row = r0 + line + 8 * (4 * q + i);
+        d[i].zero(), z[i].zero();
+        if (row < g.n) {
+          d[i].load(g.dY + row * g.lddy + col, left);
+          if (g.act) z[i].load(g.Z + row * g.ldz + col, left);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int row = r0 + line + 8 * (4 * q + i);
+        if (row >= g.n) break;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = d[i][e];
+        if (g.m.t) drop8(g.m, draws_of(g.m, step, row_id(g.m, row), col >> 3), v);
+        if (g.act) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) v[e] *= slope_of(g.act, z[i][e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) s[e] += v[e];
+        if (D) Eight<u16>::store(D + (long)row * g.N + col, v, left);
+      }
+    }
+  }
+  if (!g.sums) return;
+#pragma unroll
+  for (int e = 0; e < 8; e++) part[line][8 * piece + e] = s[e];
+  __syncthreads();
+  const int c = block % g.across * 256 + threadIdx.x;
+  if (c >= g.N) return;
+  float t = part[0][threadIdx.x];
+#pragma unroll
+  for (int i = 1; i < 8; i++) t += part[i][threadIdx.x];
+  g.sums[(long)(r0 / 64) * g.N + c] = t;
+}
+
 // what products left in parts, in their order, to the epilogue; pieces of eight columns
 template <class E>
 __global__ __launch_bounds__(256) void parts_kernel(const float *part, int parts, int rows, int cols, E out) {
@@ -294,6 +379,33 @@ Shape shape_of(int cols, int rows, int K) {
   return s;
 }
 
+// Of operands as they lie: the tile and the stretches of K that a model of the launch finds best.  us a k of a round of tiles, one a compute unit of the wide
+// ones (0.0245 with the chip full, 0.0195 with half of it idle: power), two of the narrow (0.0140; one 0.0090); each workgroup costs 256 k more than it
+// multiplies, and what products leave in parts is written and read at the rate of a copy, by a launch more.
+Shape direct_shape_of(int cols, int rows, int K) {
+  Shape best{};
+  double least = INFINITY;
+  const int cus = num_cus();
+  for (int wide = 0; wide < 2; wide++) {
+    Shape s{};
+    s.size = wide;
+    const int side = wide ? WideTile::BM : NarrowTile::BM;
+    s.tm = tiles_of(cols, side), s.tn = tiles_of(rows, side);
+    for (int splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (splits > 1 && K / splits < 256) break;
+      s.kchunk = ceil_to((K + splits - 1) / splits, 64);
+      s.splits = (K + s.kchunk - 1) / s.kchunk;
+      const long groups = (long)s.tm * s.tn * s.splits, full = wide ? groups / cus : groups / (2 * cus), rest = groups - full * (wide ? cus : 2 * cus);
+      const double k = s.kchunk + 256.;
+      double us = full * k * (wide ? 0.0245 : 0.0140);
+      if (rest > 0) us += k * (wide ? (full > 0 || rest > cus / 2 ? 0.0225 : 0.0195) : (rest > cus ? 0.0140 : 0.0090));
+      if (s.splits > 1) us += 5. + s.splits * (8. * rows * cols) / 4.7e6;
+      if (us < least) least = us, best = s;
+    }
+  }
+  return best;
+}
+
 struct Plan {
   int Kp, Np, np;  // as contraction lengths
   Shape fwd, dx, dw;
@@ -329,6 +441,32 @@ Plan plan_of(int n, int K, int N, int back) {
   p.bytes = at;
   return p;
 }
+Plan direct_plan_of(int n, int K, int N, int back) {
+  Plan p{};
+  size_t at = 0, part = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) & ~(size_t)255;
+    return here;
+  };
+  auto parts = [&](const Shape &s, int rows, int cols) {
+    const size_t b = s.splits > 1 ? (size_t)s.splits * rows * cols * 4 : 0;
+    part = part > b ? part : b;
+  };
+  if (!back) {
+    p.fwd = direct_shape_of(N, n, K);
+    parts(p.fwd, n, N);
+  } else {
+    p.d = take((size_t)n * N * 2);
+    p.dx = direct_shape_of(K, n, N);
+    p.dw = direct_shape_of(K, N, n);
+    parts(p.dx, n, K), parts(p.dw, N, K);
+    p.sums = take((size_t)tiles_of(n, 64) * N * 4);
+  }
+  p.part = take(part);
+  p.bytes = at;
+  return p;
+}
 
 struct Call {
   const void *X, *W, *R, *Z, *dY;
@@ -353,6 +491,12 @@ PackJob<T> packing(const void *src, int ld, int rows, int K, int orows, char *o,
   return j;
 }
 
+template <class E>
+int join_parts(const float *part, const Shape &s, int rows, int cols, const E &out, hipStream_t st) {
+  launch(parts_kernel<E>, (unsigned)(((long)rows * ((cols + 7) / 8) + 255) / 256), 256, 0, st, part, s.splits, rows, cols, out);
+  CAVS_LAUNCH_CHECK();
+  return CAVS_OK;
+}
 template <int P, bool TA, bool TB, class E>
 int product(const Shape &s, const PackedRef &A, int cols, const PackedRef &B, int rows, int K, float *part, const E &out, hipStream_t st) {
   Product<E> g{A, B, cols, rows, K, s.tm, s.tn, s.splits, s.kchunk, s.splits > 1 ? part : nullptr, out};
@@ -362,8 +506,50 @@ int product(const Shape &s, const PackedRef &A, int cols, const PackedRef &B, in
     return 0;
   });
   CAVS_LAUNCH_CHECK();
-  if (g.part) {
-    launch(parts_kernel<E>, (unsigned)(((long)rows * ((cols + 7) / 8) + 255) / 256), 256, 0, st, g.part, s.splits, rows, cols, out);
+  return g.part ? join_parts(part, s, rows, cols, out, st) : (int)CAVS_OK;
+}
+
+template <bool TA, bool TB, class E>
+int direct_product(const Shape &s, const DirectRef &A, int cols, const DirectRef &B, int rows, int K, float *part, const E &out, hipStream_t st) {
+  DirectJob<E> g{A, B, cols, rows, K, s.tm, s.tn, s.kchunk, s.splits > 1 ? part : nullptr, out};
+  const unsigned groups = (unsigned)(s.tm * s.tn * s.splits);
+  if (s.size) launch(direct_product_kernel<WideTile, TA, TB, E>, groups, WideTile::THREADS, 0, st, g);
+  else launch(direct_product_kernel<NarrowTile, TA, TB, E>, groups, NarrowTile::THREADS, 0, st, g);
+  CAVS_LAUNCH_CHECK();
+  return g.part ? join_parts(part, s, rows, cols, out, st) : (int)CAVS_OK;
+}
+
+// rows that begin on 16 bytes and are whole pieces of eight, in reach of 32 bits from the first of a tile
+bool lies_well(const void *p, long ld, int w) { return aligned16(p) && ld % 8 == 0 && w % 8 == 0 && ld <= 1 << 22; }
+
+int run_direct_fwd(const Call &c, char *ws, hipStream_t st) {
+  const Plan p = direct_plan_of(c.n, c.K, c.N, 0);
+  const Forward<u16> out{c.b, c.act, c.m, static_cast<const u16 *>(c.R), c.ldr, static_cast<u16 *>(c.Zout), c.ldz, static_cast<u16 *>(c.Y), c.ldy};
+  return direct_product<false, false>(p.fwd, DirectRef{static_cast<const u16 *>(c.W), c.ldw}, c.N, DirectRef{static_cast<const u16 *>(c.X), c.ldx}, c.n, c.K,
+                                      reinterpret_cast<float *>(ws + p.part), out, st);
+}
+
+int run_direct_bwd(const Call &c, char *ws, hipStream_t st) {
+  const Plan p = direct_plan_of(c.n, c.K, c.N, 1);
+  const bool as_is = !c.act && !c.m.t && lies_well(c.dY, c.lddy, c.N);
+  GradJob<u16> g{static_cast<const u16 *>(c.dY), static_cast<const u16 *>(c.Z), c.lddy, c.ldz, c.act, c.m, c.n, c.N, c.n, tiles_of(c.N, 256), 0,
+                 {}, c.db ? reinterpret_cast<float *>(ws + p.sums) : nullptr};
+  g.blocks = g.across * tiles_of(c.n, 64);
+  u16 *made = !as_is && (c.dX || c.dW) ? reinterpret_cast<u16 *>(ws + p.d) : nullptr;
+  if (made || c.db) {
+    launch(grad_rows_kernel, grid_of(g.blocks), 256, 0, st, g, made);
+    CAVS_LAUNCH_CHECK();
+  }
+  const DirectRef D{made ? made : g.dY, made ? (long)c.N : c.lddy}, X{static_cast<const u16 *>(c.X), c.ldx}, W{static_cast<const u16 *>(c.W), c.ldw};
+  float *part = reinterpret_cast<float *>(ws + p.part);
+  if (c.dX) {
+    if (const int rc = direct_product<true, false>(p.dx, W, c.K, D, c.n, c.N, part, Plain<u16>{static_cast<u16 *>(c.dX), c.lddx}, st)) return rc;
+  }
+  if (c.dW) {
+    if (const int rc = direct_product<true, true>(p.dw, X, c.K, D, c.N, c.n, part, Plain<u16>{static_cast<u16 *>(c.dW), c.lddw}, st)) return rc;
+  }
+  if (c.db) {
+    launch(column_sums_kernel, (c.N + 63) / 64, 256, 0, st, g.sums, tiles_of(c.n, 64), c.N, c.db);
     CAVS_LAUNCH_CHECK();
   }
   return CAVS_OK;
@@ -446,7 +632,9 @@ extern "C" {
 
 size_t cavs_linear_workspace(int type, int n, int K, int N, int back) {
   if (n <= 0 || K <= 0 || N <= 0 || !shape_ok(n, K, N) || (type != CAVS_F32 && type != CAVS_BF16)) return 0;
-  return (type == CAVS_F32 ? plan_of<3>(n, K, N, back) : plan_of<1>(n, K, N, back)).bytes;
+  if (type == CAVS_F32) return plan_of<3>(n, K, N, back).bytes;
+  const size_t packed = plan_of<1>(n, K, N, back).bytes, direct = K % 8 == 0 && (!back || N % 8 == 0) ? direct_plan_of(n, K, N, back).bytes : 0;
+  return packed > direct ? packed : direct;
 }
 
 int cavs_linear_fwd(int type, const void *X, int ldx, const void *W, int ldw, const float *b, int act, const cavs_dropout_mask *mask, const void *R, int ldr,
@@ -460,7 +648,8 @@ int cavs_linear_fwd(int type, const void *X, int ldx, const void *W, int ldw, co
   CAVS_REQUIRE(X && W && Y, "%s: null pointer", who);
   if (const int rc = check_workspace(who, workspace, workspace_bytes, cavs_linear_workspace(type, n, K, N, 0))) return rc;
   char *w = static_cast<char *>(workspace);
-  return type == CAVS_F32 ? run_fwd<3, float>(c, w, as_stream(stream)) : run_fwd<1, u16>(c, w, as_stream(stream));
+  if (type == CAVS_F32) return run_fwd<3, float>(c, w, as_stream(stream));
+  return lies_well(X, ldx, K) && lies_well(W, ldw, K) ? run_direct_fwd(c, w, as_stream(stream)) : run_fwd<1, u16>(c, w, as_stream(stream));
 }
 
 int cavs_linear_bwd(int type, const void *X, int ldx, const void *W, int ldw, const void *Z, int ldz, int act, const cavs_dropout_mask *mask, const void *dY,
@@ -485,7 +674,9 @@ int cavs_linear_bwd(int type, const void *X, int ldx, const void *W, int ldw, co
   CAVS_REQUIRE(dY && (!act || Z) && (!dW || X) && (!dX || W), "%s: null pointer", who);
   if (const int rc = check_workspace(who, workspace, workspace_bytes, cavs_linear_workspace(type, n, K, N, 1))) return rc;
   char *w = static_cast<char *>(workspace);
-  return type == CAVS_F32 ? run_bwd<3, float>(c, w, st) : run_bwd<1, u16>(c, w, st);
+  if (type == CAVS_F32) return run_bwd<3, float>(c, w, st);
+  const bool direct = N % 8 == 0 && (!dW || lies_well(X, ldx, K)) && (!dX || lies_well(W, ldw, K));
+  return direct && (long)N <= 1 << 22 ? run_direct_bwd(c, w, st) : run_bwd<1, u16>(c, w, st);
 }
 
 }  // extern "C"

@@ -355,28 +355,39 @@ int with_tile(int size, F &&f) {
   return f(typename TT::S{});
 }
 
-constexpr int kSplits = 32;
 struct Shape {  // of a product
   int size, tm, tn, splits, kchunk;
 };
-// the largest tile that still gives most compute units one; K in stretches where tiles are fewer than two a unit
+// The tile and the stretches of K that a model of the launch finds best: ns a k of a compute unit that has one, two or three workgroups of a tile, as
+// measured (fp32, in products of 7088 rows: 128 x 128 at 224, 448 and 672 workgroups, 64 x 64 at 256, 512 and 768); each workgroup costs 200 k more than it multiplies,
+// and what products leave in parts is written and read at the rate of a copy, by a launch more.  us of a call with all workgroups whole / in the stretches this
+// finds: fp32 gradients of 7088 x 512 x 2048 405 / 245.
+template <int P> struct Speeds;
+template <> struct Speeds<3> { static constexpr int SIZES = 2; static constexpr double ns[2][3] = {{26, 26, 29}, {68, 73, 98}}; };
+template <> struct Speeds<1> { static constexpr int SIZES = 3; static constexpr double ns[3][3] = {{6, 6.5, 8}, {14, 15, 20}, {24, 27, 38}}; };
+constexpr int kStretches[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
 template <int P>
 Shape shape_of(int cols, int rows, int K) {
-  Shape s{};
-  int bm = 0, bn = 0;
-  for (s.size = 2; s.size >= 0; s.size--) {
-    with_tile<P>(s.size, [&](auto t) { return bm = decltype(t)::BM, bn = decltype(t)::BN, 0; });
-    if (s.size == 0 || (long)tiles_of(cols, bm) * tiles_of(rows, bn) >= num_cus() * 3 / 4) break;
+  Shape best{};
+  double least = INFINITY;
+  const int cus = num_cus();
+  for (int size = 0; size < Speeds<P>::SIZES; size++) {
+    Shape s{};
+    s.size = size;
+    int bm = 0, bn = 0;
+    with_tile<P>(size, [&](auto t) { return bm = decltype(t)::BM, bn = decltype(t)::BN, 0; });
+    s.tm = tiles_of(cols, bm), s.tn = tiles_of(rows, bn);
+    for (int splits : kStretches) {
+      if (splits > 1 && K / splits < 256) break;
+      s.kchunk = ceil_to((K + splits - 1) / splits, kPlaneAlign);
+      s.splits = (K + s.kchunk - 1) / s.kchunk;
+      const long groups = (long)s.tm * s.tn * s.splits, full = groups / (3 * cus), rest = (groups - full * 3 * cus + cus - 1) / cus;
+      double us = 1e-3 * (s.kchunk + 200) * (full * Speeds<P>::ns[size][2] + (rest > 0 ? Speeds<P>::ns[size][rest - 1] : 0.));
+      if (s.splits > 1) us += 5. + s.splits * (8. * rows * cols) / 4.7e6;
+      if (us < least) least = us, best = s;
+    }
   }
-  s.tm = tiles_of(cols, bm), s.tn = tiles_of(rows, bn);
-  const long tiles = (long)s.tm * s.tn;
-  int splits = (int)(tiles * 2 <= num_cus() ? 2 * num_cus() / tiles : 1);
-  const int most = K / 256 > 0 ? K / 256 : 1;
-  splits = splits > most ? most : splits;
-  splits = splits > kSplits ? kSplits : splits;
-  s.kchunk = ceil_to((K + splits - 1) / splits, kPlaneAlign);
-  s.splits = (K + s.kchunk - 1) / s.kchunk;
-  return s;
+  return best;
 }
 
 // Of operands as they lie: the tile and the stretches of K that a model of the launch finds best.  us a k of a round of tiles, one a compute unit of the wide
@@ -391,7 +402,7 @@ Shape direct_shape_of(int cols, int rows, int K) {
     s.size = wide;
     const int side = wide ? WideTile::BM : NarrowTile::BM;
     s.tm = tiles_of(cols, side), s.tn = tiles_of(rows, side);
-    for (int splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+    for (int splits : kStretches) {
       if (splits > 1 && K / splits < 256) break;
       s.kchunk = ceil_to((K + splits - 1) / splits, 64);
       s.splits = (K + s.kchunk - 1) / s.kchunk;

@@ -31,47 +31,73 @@ struct Norm {  // as cavs_norm_desc
 // ------------------------------------------------------------------ sums over the lanes of a row
 __device__ __forceinline__ double two(unsigned lo, unsigned hi) { return __longlong_as_double((long long)((unsigned long long)hi << 32 | lo)); }
 template <int CTRL>
-__device__ __forceinline__ double rotated(double v) {
+__device__ __forceinline__ double moved(double v) {
   const int lo = __double2loint(v), hi = __double2hiint(v);
   return two(__builtin_amdgcn_update_dpp(0, lo, CTRL, 0xf, 0xf, true), __builtin_amdgcn_update_dpp(0, hi, CTRL, 0xf, 0xf, true));
 }
-__device__ __forceinline__ double crossed32(double v) {
-  const unsigned lo = __double2loint(v), hi = __double2hiint(v);
-  const auto a = __builtin_amdgcn_permlane32_swap(lo, lo, false, false), b = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+// of lanes 32 or 16 apart: v's in the lower half (the even rows of sixteen), w's in the upper
+__device__ __forceinline__ double crossed32(double v, double w) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__double2loint(v), __double2loint(w), false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap(__double2hiint(v), __double2hiint(w), false, false);
   return two(a[0], b[0]) + two(a[1], b[1]);
 }
-__device__ __forceinline__ double crossed16(double v) {
-  const unsigned lo = __double2loint(v), hi = __double2hiint(v);
-  const auto a = __builtin_amdgcn_permlane16_swap(lo, lo, false, false), b = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+__device__ __forceinline__ double crossed16(double v, double w) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__double2loint(v), __double2loint(w), false, false);
+  const auto b = __builtin_amdgcn_permlane16_swap(__double2hiint(v), __double2hiint(w), false, false);
   return two(a[0], b[0]) + two(a[1], b[1]);
 }
-// of sixteen, 32 or 64 neighbouring lanes, every lane with the result
-template <int L>
-__device__ __forceinline__ double lanes_sum(double v) {
-  if constexpr (L >= 64) v = crossed32(v);
-  if constexpr (L >= 32) v = crossed16(v);
-  v += rotated<0x128>(v);  // row_ror:8, 4, 2, 1
-  v += rotated<0x124>(v);
-  v += rotated<0x122>(v);
-  return v + rotated<0x121>(v);
+// over N neighbouring lanes, N up to 16, every lane with the result: its neighbour, the pair beside, the four, the eight
+template <int N>
+__device__ __forceinline__ double near_sum(double v) {
+  if constexpr (N >= 2) v += moved<0xb1>(v);    // quad_perm 1 0 3 2
+  if constexpr (N >= 4) v += moved<0x4e>(v);    // quad_perm 2 3 0 1
+  if constexpr (N >= 8) v += moved<0x141>(v);   // row_half_mirror
+  if constexpr (N >= 16) v += moved<0x140>(v);  // row_mirror
+  return v;
 }
-// K sums of the L lanes of a row.  L above 64: a workgroup is a row; `lds` [K][L / 64] is written here and may be written again after the next barrier but one.
+__device__ __forceinline__ double of_lane(double v, int lane) {
+  return two(__builtin_amdgcn_readlane(__double2loint(v), lane), __builtin_amdgcn_readlane(__double2hiint(v), lane));
+}
+// K sums of the L lanes of a row, every lane with the results.  Of a wavefront up to four sums go down together, a quarter of the lanes to each (crossed),
+// so that they cost one sum's trip.  L above 64: `lds` [groups of the workgroup][K][L / 64], which may be written again after the next barrier but one.
 template <int L, int K>
 __device__ __forceinline__ void row_sums(double (&v)[K], double *lds) {
-#pragma unroll
-  for (int k = 0; k < K; k++) v[k] = lanes_sum<L>(v[k]);
-  if constexpr (L > 64) {
-    constexpr int W = L / 64;
-    if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-      for (int k = 0; k < K; k++) lds[k * W + (threadIdx.x >> 6)] = v[k];
-    }
-    __syncthreads();
+  if constexpr (L < 64) {
 #pragma unroll
     for (int k = 0; k < K; k++) {
-      v[k] = 0.;
+      if constexpr (L == 32) v[k] = crossed16(v[k], v[k]);
+      v[k] = near_sum<16>(v[k]);
+    }
+  } else {
+    constexpr int Q = (K + 3) / 4;
+    double t[Q];
 #pragma unroll
-      for (int i = 0; i < W; i++) v[k] += lds[k * W + i];
+    for (int q = 0; q < Q; q++) {
+      const int k = 4 * q;
+      const double a = crossed32(v[k], k + 1 < K ? v[k + 1 < K ? k + 1 : 0] : 0.), b = k + 2 < K ? crossed32(v[k + 2 < K ? k + 2 : 0], k + 3 < K ? v[k + 3 < K ? k + 3 : 0] : 0.) : 0.;
+      t[q] = near_sum<16>(crossed16(a, b));  // (of sums k, k + 2, k + 1, k + 3: rows of sixteen 0 .. 3)
+    }
+    if constexpr (L == 64) {
+#pragma unroll
+      for (int k = 0; k < K; k++) v[k] = of_lane(t[k / 4], 16 * ((k & 1) * 2 + (k >> 1 & 1)));
+    } else {
+      constexpr int W = L / 64;
+      const int lane = threadIdx.x & 63, wave = threadIdx.x % L / 64, at = (lane >> 5) + (lane >> 4 & 1) * 2;
+      lds += threadIdx.x / L * (K * W);
+#pragma unroll
+      for (int q = 0; q < Q; q++)
+        if ((lane & 15) == 0 && 4 * q + at < K) lds[(4 * q + at) * W + wave] = t[q];
+      __syncthreads();
+      // lane l: of sum l / W the part of wavefront l % W
+      constexpr int ROUNDS = (K * W + 63) / 64;
+#pragma unroll
+      for (int r = 0; r < ROUNDS; r++) {
+        const int i = r * 64 + lane;
+        const double x = near_sum<W>(i < K * W ? lds[i] : 0.);
+#pragma unroll
+        for (int k = 0; k < 64 / W; k++)
+          if (r * (64 / W) + k < K) v[r * (64 / W) + k] = of_lane(x, k * W);
+      }
     }
   }
 }
@@ -79,8 +105,8 @@ __device__ __forceinline__ void row_sums(double (&v)[K], double *lds) {
 // v^ = ((v - mean) - rest) rstd: mean as a float and what it leaves off, so that the difference is a float's own however far the values are from 0
 struct Stats {
   float mean, rest, rstd;
-  __device__ __forceinline__ void of(double sum, double squares, int w, int kind, float eps) {
-    const double inv = 1. / w, m = kind == CAVS_NORM_LAYER ? sum * inv : 0., v = squares * inv - m * m;
+  __device__ __forceinline__ void of(double sum, double squares, int w, bool centred, float eps) {
+    const double inv = 1. / w, m = centred ? sum * inv : 0., v = squares * inv - m * m;
     mean = (float)m;
     rest = (float)(m - (double)mean);
     const double a = (v > 0. ? v : v == v ? 0. : v) + (double)eps;
@@ -91,37 +117,73 @@ struct Stats {
 };
 
 template <int L>
-constexpr int threads_of() { return L > 64 ? L : 256; }
+constexpr int threads_of() { return L > 256 ? L : 256; }
+template <int L>
+constexpr int sums_lds(int k) { return L > 64 ? k * threads_of<L>() / 64 : 1; }
 
-__device__ __forceinline__ void weights8(float (&o)[8], const float *p, int c, int left, float none) {
-  if (!p || left <= 0) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) o[e] = e < left ? none : 0.f;
-    return;
+// A lane's eight columns.  Of the last piece of a row that is no multiple of eight they are the row's last eight, `skip` of which are the lane's before it: a load is
+// always whole and none waits for another (with its end value by value, each array of a row waited for the one before: d of 16384 x 4096 with norms on
+// both sides 272 us, without that wait 180).  SMALL: rows of less than eight values.
+template <bool SMALL>
+struct Place {
+  int col, skip, w;
+  __device__ __forceinline__ void set(int c, int width) {
+    w = width;
+    col = SMALL ? c : min(c, w - 8);
+    skip = SMALL ? (c < w ? 0 : 8) : c - col;
   }
-  Eight<float> t;
-  t.load(p + c, left);
+  __device__ __forceinline__ bool has(int e) const { return SMALL ? col + e < w : e >= skip; }
+  template <class T>
+  __device__ __forceinline__ void load(Eight<T> &o, const T *row) const {
+    if constexpr (SMALL) o.load(row + col, w - col);
+    else o.load(row + col);
+  }
+  template <class T>
+  __device__ __forceinline__ void store(T *row, const float (&v)[8]) const {
+    if (!SMALL && skip == 0) {
+      Eight<T>::store(row + col, v, 8);
+    } else if (skip < 8) {
 #pragma unroll
-  for (int e = 0; e < 8; e++) o[e] = t[e];
-}
+      for (int e = 0; e < 8; e++)
+        if (has(e)) row[col + e] = as<T>(v[e]);
+    }
+  }
+  template <class T>
+  __device__ __forceinline__ static T as(float v) {
+    if constexpr (sizeof(T) == 4) return v;
+    else return (u16)to_bits16(v);
+  }
+  // weights; 0 where a column is not this lane's
+  __device__ __forceinline__ void weights(float (&o)[8], const float *p, float none) const {
+    Eight<float> t;
+    if (p) load(t, p);
+#pragma unroll
+    for (int e = 0; e < 8; e++) o[e] = !has(e) ? 0.f : p ? t[e] : none;
+  }
+};
 
 // ------------------------------------------------------------------ forward
-template <class T, int L, int V>
+template <class T, int L, int V, bool SMALL>
 __global__ __launch_bounds__(threads_of<L>()) void norm_fwd_kernel(Norm a, T *s, long lds_, T *x, long ldx) {
-  __shared__ double part[2][2 * (L > 64 ? L / 64 : 1)];
-  const int lane = threadIdx.x % L, row = blockIdx.x * (threads_of<L>() / L) + threadIdx.x / L;
-  if (row >= a.n) return;  // (a whole workgroup's, where one is a row)
+  __shared__ double part[2][sums_lds<L>(2)];
+  const int lane = threadIdx.x % L, at = blockIdx.x * (threads_of<L>() / L) + threadIdx.x / L, row = min(at, a.n - 1);
+  const bool on = at < a.n;  // (rows of more than a wavefront's lanes go through the barriers together)
+  Place<SMALL> c[V];
   float v[V][8];
   Eight<T> y[V], r[V], g[V];
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    const int c = 8 * (i * L + lane), left = a.w - c;
-    y[i].zero(), r[i].zero(), g[i].zero();
-    if (left > 0) {
-      y[i].load(static_cast<const T *>(a.y) + row * a.ldy + c, left);
-      if (a.r) r[i].load(static_cast<const T *>(a.r) + row * a.ldr + c, left);
-      if (a.gate_rows) g[i].load(static_cast<const T *>(a.gate_rows) + row * a.ldg + c, left);
-    }
+    c[i].set(8 * (i * L + lane), a.w);
+    c[i].load(y[i], static_cast<const T *>(a.y) + row * a.ldy);
+    r[i].zero(), g[i].zero();
+  }
+  if (a.r) {
+#pragma unroll
+    for (int i = 0; i < V; i++) c[i].load(r[i], static_cast<const T *>(a.r) + row * a.ldr);
+  }
+  if (a.gate_rows) {
+#pragma unroll
+    for (int i = 0; i < V; i++) c[i].load(g[i], static_cast<const T *>(a.gate_rows) + row * a.ldg);
   }
   auto stats = [&](int kind, double *lds) {
     double t[2] = {0., 0.};
@@ -129,47 +191,46 @@ __global__ __launch_bounds__(threads_of<L>()) void norm_fwd_kernel(Norm a, T *s,
     for (int i = 0; i < V; i++)
 #pragma unroll
       for (int e = 0; e < 8; e++) t[0] += v[i][e], t[1] += (double)v[i][e] * v[i][e];
-    row_sums<L, 2>(t, lds);
+    row_sums<L>(t, lds);
     Stats o;
-    o.of(t[0], t[1], a.w, kind, a.eps);
+    o.of(t[0], t[1], a.w, kind == CAVS_NORM_LAYER, a.eps);
     return o;
   };
 #pragma unroll
   for (int i = 0; i < V; i++)
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[i][e] = y[i][e];
+    for (int e = 0; e < 8; e++) v[i][e] = c[i].has(e) ? y[i][e] : 0.f;
   Stats post{}, pre{};
   if (a.post) post = stats(a.post, part[0]);
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    const int c = 8 * (i * L + lane), left = a.w - c;
-    float w[8], b[8], gate[8];
+    float w[8], b[8];
     if (a.post) {
-      weights8(w, a.post_w, c, left, 1.f), weights8(b, a.post_b, c, left, 0.f);
+      c[i].weights(w, a.post_w, 1.f), c[i].weights(b, a.post_b, 0.f);
 #pragma unroll
       for (int e = 0; e < 8; e++) v[i][e] = post.hat(v[i][e]) * w[e] + b[e];
     }
-    weights8(gate, a.gate, c, left, 1.f);
+    if (a.gate_rows) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      v[i][e] *= a.scale * (a.gate_rows ? g[i][e] : gate[e]);
-      v[i][e] = 8 * (i * L + lane) + e < a.w ? v[i][e] + r[i][e] : 0.f;
+      for (int e = 0; e < 8; e++) w[e] = g[i][e];
+    } else {
+      c[i].weights(w, a.gate, 1.f);
     }
-    if (s && left > 0) Eight<T>::store(s + row * lds_ + c, v[i], left);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[i][e] = c[i].has(e) ? v[i][e] * (a.scale * w[e]) + r[i][e] : 0.f;
+    if (s && on) c[i].store(s + row * lds_, v[i]);
   }
   if (!x) return;
   if (a.pre) pre = stats(a.pre, part[1]);
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    const int c = 8 * (i * L + lane), left = a.w - c;
-    if (left <= 0) continue;
     float w[8], b[8];
     if (a.pre) {
-      weights8(w, a.pre_w, c, left, 1.f), weights8(b, a.pre_b, c, left, 0.f);
+      c[i].weights(w, a.pre_w, 1.f), c[i].weights(b, a.pre_b, 0.f);
 #pragma unroll
       for (int e = 0; e < 8; e++) v[i][e] = pre.hat(v[i][e]) * w[e] + b[e];
     }
-    Eight<T>::store(x + row * ldx + c, v[i], left);
+    if (on) c[i].store(x + row * ldx, v[i]);
   }
 }
 
@@ -179,128 +240,190 @@ struct Back {
   long lds, ldds, lddx;
   void *dy, *dr, *dg;
   long lddy, lddr, lddg;
-  float *part;  // [workgroups][sums][w]: pre_w, pre_b, gate, post_w, post_b; null: none wanted
-  int sums;     // 3 or 5
+  float *part;  // [workgroups][sums][w]: pre_w, gate, (POST) post_w, (FULL) pre_b, (both) post_b; null: none wanted
 };
 
-// A workgroup takes every gridDim.x-th row (group of rows), its lanes the same columns of each: the sums over rows are in registers until it ends.
-template <class T, int L, int V, bool POST>
-__global__ __launch_bounds__(threads_of<L>()) void norm_bwd_kernel(Norm a, Back b) {
-  constexpr int G = threads_of<L>() / L, S = POST ? 5 : 3;
-  __shared__ double part[2][8 * (L > 64 ? L / 64 : 1)];
-  __shared__ float merged[G > 1 ? G - 1 : 1][G > 1 ? 8 * L * V : 1];
+// A workgroup takes every gridDim.x-th row (group of rows), its lanes the same columns of each: the sums over rows are in registers until it ends. The weights
+// are in LDS (of the widest rows in memory), which leaves registers for two workgroups of 512 a compute unit where there are no more than the sums below:
+// while one waits for a row's sums the other has its loads on their way.
+// what is summed over rows: weights of both norms and the gate, and (FULL) biases.  FULL is for norms that take the mean off, or gradients of biases; what they need
+// besides of a row's sums and of registers is left out otherwise (rms norms on both sides, bf16 16384 x 4096 with / without it
+// 260 / 221 us, and 180 with two workgroups a compute unit then).
+constexpr int back_sums(bool post, bool full) { return full ? (post ? 5 : 3) : (post ? 3 : 2); }
+// One workgroup of 512 a compute unit, with the registers to have its next row on the way while it computes this one, where what it computes leaves no room for two:
+// us of two / of one so: norms on both sides, fp32 2371 x 1001 with biases 41 / 26, bf16 32768 x 512 without 51 / 44; 16384 x 4096 without 180 / 221.
+constexpr bool back_ahead(int lanes, bool post, bool full) { return post && lanes <= 512 && (full || lanes <= 64); }
+template <int L>
+constexpr int back_threads() { return L > 512 ? L : 512; }
+
+template <class T, int L, int V, bool POST, bool FULL, bool SMALL>
+__global__ __launch_bounds__(back_threads<L>(), back_ahead(L, POST, FULL) ? 2 : 4) void norm_bwd_kernel(Norm a, Back b) {
+  typedef float four __attribute__((ext_vector_type(4)));
+  constexpr int THREADS = back_threads<L>(), G = THREADS / L, S = back_sums(POST, FULL), WAVES = L > 64 ? THREADS / 64 : 1, KINDS = POST ? 4 : 2;
+  constexpr int PRE_W = 0, GATE = 1, POST_W = 2, PRE_B = POST ? 3 : 2, POST_B = 4;  // of the sums over rows
+  constexpr int SS = 0, HS = 1, YY = 2, S1 = POST ? 3 : 2, H1 = S1 + 1, Y1 = H1 + 1, K = FULL ? (POST ? 6 : 4) : (POST ? 3 : 2);  // of those of a row
+  constexpr bool KEPT = V == 1, AHEAD = back_ahead(L, POST, FULL);
+  __shared__ double part[2][K * WAVES];
+  __shared__ four kept[KEPT ? KINDS : 1][2][KEPT ? L : 1];  // pre_w, gate, post_w, post_b
+  __shared__ float merged[G > 1 ? (G - 1) * 8 * L * V : 1];
   const int lane = threadIdx.x % L, group = threadIdx.x / L;
-  float acc[S][V][8], pw[V][8], qw[V][8], qb[V][8], gate[V][8];
+  Place<SMALL> c[V];
 #pragma unroll
-  for (int i = 0; i < V; i++) {
-    const int c = 8 * (i * L + lane), left = a.w - c;
-    weights8(pw[i], a.pre_w, c, left, 1.f);
-    if constexpr (POST) weights8(qw[i], a.post_w, c, left, 1.f), weights8(qb[i], a.post_b, c, left, 0.f);
-    weights8(gate[i], a.gate, c, left, 1.f);
+  for (int i = 0; i < V; i++) c[i].set(8 * (i * L + lane), a.w);
+  auto weights = [&](int kind, int i, float (&o)[8]) {
+    if constexpr (KEPT) {
+      const four lo = kept[kind][0][lane], hi = kept[kind][1][lane];
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-#pragma unroll
-      for (int k = 0; k < S; k++) acc[k][i][e] = 0.f;
-  }
-  const double inv = 1. / a.w;
-  for (int first = blockIdx.x * G; first < a.n; first += gridDim.x * G) {
-    const int row = first + group;
-    const bool on = row < a.n;
-    Eight<T> s[V], ds[V], dx[V], y[V], g[V];
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-      const int c = 8 * (i * L + lane), left = on ? a.w - c : 0;
-      s[i].zero(), ds[i].zero(), dx[i].zero(), y[i].zero(), g[i].zero();
-      if (left > 0) {
-        if (a.pre) s[i].load(static_cast<const T *>(b.s) + row * b.lds + c, left);
-        if (b.dx) dx[i].load(static_cast<const T *>(b.dx) + row * b.lddx + c, left);
-        if (b.ds) ds[i].load(static_cast<const T *>(b.ds) + row * b.ldds + c, left);
-        if (a.y) y[i].load(static_cast<const T *>(a.y) + row * a.ldy + c, left);
-        if (a.gate_rows) g[i].load(static_cast<const T *>(a.gate_rows) + row * a.ldg + c, left);
-      }
+      for (int e = 0; e < 4; e++) o[e] = lo[e], o[4 + e] = hi[e];
+    } else {
+      c[i].weights(o, kind == 0 ? a.pre_w : kind == 1 ? a.gate : kind == 2 ? a.post_w : a.post_b, kind == 3 ? 0.f : 1.f);
     }
-    double t[6] = {0., 0., 0., 0., 0., 0.};
+  };
+  if constexpr (KEPT) {
+    for (int k = group; k < KINDS; k += G) {
+      float o[8];
+      c[0].weights(o, k == 0 ? a.pre_w : k == 1 ? a.gate : k == 2 ? a.post_w : a.post_b, k == 3 ? 0.f : 1.f);
+      kept[k][0][lane] = four{o[0], o[1], o[2], o[3]}, kept[k][1][lane] = four{o[4], o[5], o[6], o[7]};
+    }
+    __syncthreads();
+  }
+  float acc[S][V][8];
+#pragma unroll
+  for (int k = 0; k < S; k++)
 #pragma unroll
     for (int i = 0; i < V; i++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const double v = s[i][e], h = dx[i][e] * pw[i][e];
-        t[0] += v, t[1] += v * v, t[2] += h, t[3] += h * v;
-        if constexpr (POST) t[4] += y[i][e], t[5] += (double)y[i][e] * y[i][e];
-      }
-    if constexpr (!POST) {
-      double u[4] = {t[0], t[1], t[2], t[3]};
-      row_sums<L, 4>(u, part[0]);
+      for (int e = 0; e < 8; e++) acc[k][i][e] = 0.f;
+  const double inv = 1. / a.w;
+  const bool whole = a.w == 8 * L * V;
+  int turn = 0;
+  struct Row {
+    Eight<T> s[V], ds[V], dx[V], y[V], g[V];
+  } now;
+  auto fetch = [&](Row &o, int first) {
+    const int row = min(first + group, a.n - 1);  // (a group without a row goes along with the last: nothing of it is stored or added)
 #pragma unroll
-      for (int k = 0; k < 4; k++) t[k] = u[k];
-    } else {
-      row_sums<L, 6>(t, part[0]);
-    }
-    Stats pre{}, post{};
-    float h1 = 0.f, h2 = 0.f;  // means of h and of h s^
-    if (a.pre) {
-      pre.of(t[0], t[1], a.w, a.pre, a.eps);
-      const double m = a.pre == CAVS_NORM_LAYER ? t[0] * inv : 0.;
-      h1 = a.pre == CAVS_NORM_LAYER ? (float)(t[2] * inv) : 0.f;
-      h2 = (float)((t[3] - m * t[2]) * inv * pre.rstd);
-    }
-    if constexpr (POST) post.of(t[4], t[5], a.w, a.post, a.eps);
-    float D[V][8], dz[V][8];
-    double q[2] = {0., 0.};
+    for (int i = 0; i < V; i++) o.s[i].zero(), o.ds[i].zero(), o.dx[i].zero(), o.y[i].zero(), o.g[i].zero();
+    auto load = [&](Eight<T> (&to)[V], const void *p, long ld) {
+      if (!p) return;
+#pragma unroll
+      for (int i = 0; i < V; i++) c[i].load(to[i], static_cast<const T *>(p) + row * ld);
+    };
+    load(o.s, a.pre ? b.s : nullptr, b.lds), load(o.dx, b.dx, b.lddx), load(o.y, a.y, a.ldy), load(o.ds, b.ds, b.ldds), load(o.g, a.gate_rows, a.ldg);
+  };
+  if constexpr (AHEAD) fetch(now, blockIdx.x * G);
+  for (int first = blockIdx.x * G; first < a.n; first += gridDim.x * G, turn ^= 1) {
+    const int row = min(first + group, a.n - 1);
+    const bool on = first + group < a.n;
+    Row next;
+    if constexpr (AHEAD) fetch(next, min(first + (int)gridDim.x * G, a.n - 1));
+    else fetch(now, first);
+    const Eight<T>(&s)[V] = now.s, (&ds)[V] = now.ds, (&dx)[V] = now.dx, (&y)[V] = now.y, (&g)[V] = now.g;
+    double t[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) t[k] = 0.;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      const int c = 8 * (i * L + lane), left = on ? a.w - c : 0;
-      float dgate[8];
+      float pw[8], sv[8], yv[8], hs = 0.f;
+      weights(0, i, pw);
+#pragma unroll
+      for (int e = 0; e < 8; e++) sv[e] = s[i][e], yv[e] = y[i][e];
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (!c[i].has(e)) sv[e] = 0.f, yv[e] = 0.f;
+      }
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        D[i][e] = ds[i][e];
-        if (a.pre) {
-          const float hat = pre.hat(s[i][e]), d = dx[i][e];
-          D[i][e] += pre.rstd * ((d * pw[i][e] - h1) - hat * h2);
-          acc[0][i][e] += d * hat;
-          acc[1][i][e] += d;
-        } else {
-          D[i][e] += dx[i][e];
-        }
-        const float gt = a.gate_rows ? g[i][e] : gate[i][e];
-        float z = y[i][e], zh = 0.f;
+        const double v = sv[e];
+        const float h = dx[i][e] * pw[e];
+        t[SS] += v * v;
+        if constexpr (FULL) t[HS] += h * v, t[S1] += v, t[H1] += h;
+        else hs += h * sv[e];
         if constexpr (POST) {
-          zh = post.hat(z);
-          z = zh * qw[i][e] + qb[i][e];
-        }
-        const float scaled = a.scale * D[i][e];
-        dgate[e] = scaled * z;
-        acc[2][i][e] += dgate[e];
-        dz[i][e] = scaled * gt;
-        if constexpr (POST) {
-          acc[3][i][e] += dz[i][e] * zh;
-          acc[4][i][e] += dz[i][e];
-          const double h = dz[i][e] * qw[i][e];
-          q[0] += h, q[1] += h * y[i][e];
+          const double u = yv[e];
+          t[YY] += u * u;
+          if constexpr (FULL) t[Y1] += u;
         }
       }
-      if (left > 0) {
-        if (b.dr) Eight<T>::store(static_cast<T *>(b.dr) + row * b.lddr + c, D[i], left);
-        if (b.dg) Eight<T>::store(static_cast<T *>(b.dg) + row * b.lddg + c, dgate, left);
-        if constexpr (!POST) {
-          if (b.dy) Eight<T>::store(static_cast<T *>(b.dy) + row * b.lddy + c, dz[i], left);
+      if constexpr (!FULL) t[HS] += hs;
+    }
+    row_sums<L>(t, part[POST ? 0 : turn]);  // (of two calls a row, or one: never the place of the call before)
+    Stats pre{0.f, 0.f, 1.f}, post{};
+    float h1 = 0.f, h2 = 0.f;  // means of h and of h s^ (no norm: s is 0 here, and D = ds + dx)
+    const bool centred = FULL && a.pre == CAVS_NORM_LAYER, post_centred = FULL && POST && a.post == CAVS_NORM_LAYER;
+    if (a.pre) {
+      pre.of(centred ? t[FULL ? S1 : 0] : 0., t[SS], a.w, centred, a.eps);
+      const double m = centred ? t[FULL ? S1 : 0] * inv : 0., hm = centred ? t[FULL ? H1 : 0] * inv : 0.;
+      h1 = (float)hm;
+      h2 = (float)((t[HS] * inv - m * hm) * pre.rstd);
+    }
+    if constexpr (POST) post.of(post_centred ? t[FULL ? Y1 : 0] : 0., t[YY], a.w, post_centred, a.eps);
+    float dz[V][8];
+    double q[FULL ? 2 : 1] = {};
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      float w[8], D[8], qy = 0.f;
+      weights(0, i, w);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float hat = pre.hat(s[i][e]), d = dx[i][e];
+        D[e] = ds[i][e] + pre.rstd * ((d * w[e] - h1) - hat * h2);
+        if (on) {
+          acc[PRE_W][i][e] += d * hat;
+          if constexpr (FULL) acc[PRE_B][i][e] += d;
         }
+      }
+      if (b.dr && on) c[i].store(static_cast<T *>(b.dr) + row * b.lddr, D);
+      if (a.gate_rows) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[e] = g[i][e];
+      } else {
+        weights(1, i, w);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) D[e] *= a.scale, dz[i][e] = D[e] * w[e];
+      if constexpr (POST) {
+        float qb[8];
+        weights(2, i, w), weights(3, i, qb);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float zh = post.hat(y[i][e]);
+          D[e] *= zh * w[e] + qb[e];
+          if (on) {
+            acc[POST_W][i][e] += dz[i][e] * zh;
+            if constexpr (FULL) acc[POST_B][i][e] += dz[i][e];
+          }
+          dz[i][e] *= w[e];
+          if constexpr (FULL) q[0] += (double)dz[i][e] * y[i][e], q[FULL ? 1 : 0] += dz[i][e];
+          else qy += dz[i][e] * y[i][e];
+        }
+        if constexpr (!FULL) q[0] += qy;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) D[e] *= y[i][e];
+        if (b.dy && on) c[i].store(static_cast<T *>(b.dy) + row * b.lddy, dz[i]);
+      }
+      if (b.dg && on) c[i].store(static_cast<T *>(b.dg) + row * b.lddg, D);
+      if (on) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc[GATE][i][e] += D[e];
       }
     }
     if constexpr (POST) {
-      row_sums<L, 2>(q, part[1]);
-      const double m = a.post == CAVS_NORM_LAYER ? t[4] * inv : 0.;
-      const float g1 = a.post == CAVS_NORM_LAYER ? (float)(q[0] * inv) : 0.f, g2 = (float)((q[1] - m * q[0]) * inv * post.rstd);
+      row_sums<L>(q, part[1]);
+      const double m = post_centred ? t[FULL ? Y1 : 0] * inv : 0., gm = post_centred ? q[FULL ? 1 : 0] * inv : 0.;
+      const float g1 = (float)gm, g2 = (float)((q[0] * inv - m * gm) * post.rstd);
+      if (b.dy && on) {
 #pragma unroll
-      for (int i = 0; i < V; i++) {
-        const int c = 8 * (i * L + lane), left = on ? a.w - c : 0;
-        if (left <= 0 || !b.dy) continue;
-        float o[8];
+        for (int i = 0; i < V; i++) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = post.rstd * ((dz[i][e] * qw[i][e] - g1) - post.hat(y[i][e]) * g2);
-        Eight<T>::store(static_cast<T *>(b.dy) + row * b.lddy + c, o, left);
+          for (int e = 0; e < 8; e++) dz[i][e] = post.rstd * ((dz[i][e] - g1) - post.hat(y[i][e]) * g2);
+          c[i].store(static_cast<T *>(b.dy) + row * b.lddy, dz[i]);
+        }
       }
     }
+    if constexpr (AHEAD) now = next;
   }
   if (!b.part) return;
 #pragma unroll
@@ -311,22 +434,19 @@ __global__ __launch_bounds__(threads_of<L>()) void norm_bwd_kernel(Norm a, Back 
 #pragma unroll
         for (int i = 0; i < V; i++)
 #pragma unroll
-          for (int e = 0; e < 8; e++) merged[group - 1][(i * 8 + e) * L + lane] = acc[k][i][e];
+          for (int e = 0; e < 8; e++) merged[((group - 1) * V * 8 + i * 8 + e) * L + lane] = acc[k][i][e];
       }
       __syncthreads();
       if (group > 0) continue;
-#pragma unroll
+#pragma unroll 1
       for (int q = 1; q < G; q++)
 #pragma unroll
         for (int i = 0; i < V; i++)
 #pragma unroll
-          for (int e = 0; e < 8; e++) acc[k][i][e] += merged[q - 1][(i * 8 + e) * L + lane];
+          for (int e = 0; e < 8; e++) acc[k][i][e] += merged[((q - 1) * V * 8 + i * 8 + e) * L + lane];
     }
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-      const int c = 8 * (i * L + lane), left = a.w - c;
-      if (left > 0) Eight<float>::store(b.part + ((long)blockIdx.x * S + k) * a.w + c, acc[k][i], left);
-    }
+    for (int i = 0; i < V; i++) c[i].store(b.part + ((long)blockIdx.x * S + k) * a.w, acc[k][i]);
   }
 }
 
@@ -359,11 +479,12 @@ __global__ __launch_bounds__(1024) void norm_sums_kernel(const float *part, int 
 }
 
 // ------------------------------------------------------------------ what a call consists of
-// lanes of a row: the fewest that hold it eight values each, of 128 values and more as many as leave at most half of them idle
+// lanes of a row: the fewest that hold it eight values each
 template <class F>
 int with_lanes(int w, F &&f) {
+  if (w < 8) return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{}, std::true_type{});
 #define CAVS_NORM_LANES(L, V) \
-  if (w <= 8 * L * V) return f(std::integral_constant<int, L>{}, std::integral_constant<int, V>{});
+  if (w <= 8 * L * V) return f(std::integral_constant<int, L>{}, std::integral_constant<int, V>{}, std::false_type{});
   CAVS_NORM_LANES(16, 1)
   CAVS_NORM_LANES(32, 1)
   CAVS_NORM_LANES(64, 1)
@@ -376,13 +497,13 @@ int with_lanes(int w, F &&f) {
   return CAVS_EUNSUPPORTED;
 }
 
-// workgroups of the backward pass: what the compute units hold at once
-int back_groups(int n, int w) {
+// workgroups of the backward pass: what the compute units hold at once, each the same number of rows but for the last
+int back_groups(int n, int w, bool post, bool full) {
   int groups = 0;
-  with_lanes(w, [&](auto l, auto) {
-    constexpr int L = decltype(l)::value, T = threads_of<L>(), G = T / L;
-    const int most = (1024 / T > 0 ? 1024 / T : 1) * num_cus(), wanted = (int)((n + (long)G - 1) / G);
-    groups = wanted < most ? wanted : most;
+  with_lanes(w, [&](auto l, auto, auto) {
+    constexpr int L = decltype(l)::value, T = back_threads<L>(), G = T / L;
+    const long most = (back_ahead(L, post, full) ? 1 : 1024 / T) * num_cus(), wanted = (n + (long)G - 1) / G, turns = (wanted + most - 1) / most;
+    groups = (int)((wanted + turns - 1) / turns);
     return CAVS_OK;
   });
   return groups;
@@ -390,22 +511,27 @@ int back_groups(int n, int w) {
 
 template <class T>
 int run_fwd(const Norm &a, void *s, int lds, void *x, int ldx, hipStream_t st) {
-  return with_lanes(a.w, [&](auto l, auto v) {
+  return with_lanes(a.w, [&](auto l, auto v, auto small) {
+    constexpr bool SMALL = decltype(small)::value;
     constexpr int L = decltype(l)::value, V = decltype(v)::value, G = threads_of<L>() / L;
-    launch(norm_fwd_kernel<T, L, V>, (unsigned)((a.n + (long)G - 1) / G), threads_of<L>(), 0, st, a, static_cast<T *>(s), (long)lds, static_cast<T *>(x), (long)ldx);
+    launch(norm_fwd_kernel<T, L, V, SMALL>, (unsigned)((a.n + (long)G - 1) / G), threads_of<L>(), 0, st, a, static_cast<T *>(s), (long)lds, static_cast<T *>(x), (long)ldx);
     CAVS_LAUNCH_CHECK();
     return (int)CAVS_OK;
   });
 }
 
 template <class T>
-int run_bwd(const Norm &a, const Back &b, const SumOut &o, int groups, hipStream_t st) {
-  return with_lanes(a.w, [&](auto l, auto v) {
+int run_bwd(const Norm &a, const Back &b, const SumOut &o, bool full, int groups, hipStream_t st) {
+  return with_lanes(a.w, [&](auto l, auto v, auto small) {
+    constexpr bool SMALL = decltype(small)::value;
     constexpr int L = decltype(l)::value, V = decltype(v)::value;
-    launch(a.post ? norm_bwd_kernel<T, L, V, true> : norm_bwd_kernel<T, L, V, false>, groups, threads_of<L>(), 0, st, a, b);
+    const auto kernel = a.post ? (full ? norm_bwd_kernel<T, L, V, true, true, SMALL> : norm_bwd_kernel<T, L, V, true, false, SMALL>)
+                               : (full ? norm_bwd_kernel<T, L, V, false, true, SMALL> : norm_bwd_kernel<T, L, V, false, false, SMALL>);
+    launch(kernel, groups, back_threads<L>(), 0, st, a, b);
     CAVS_LAUNCH_CHECK();
     if (b.part) {
-      launch(norm_sums_kernel, dim3((a.w + 63) / 64, b.sums), 1024, 0, st, b.part, groups, b.sums, a.w, o);
+      const int sums = back_sums(a.post, full);
+      launch(norm_sums_kernel, dim3((a.w + 63) / 64, sums), 1024, 0, st, b.part, groups, sums, a.w, o);
       CAVS_LAUNCH_CHECK();
     }
     return (int)CAVS_OK;
@@ -440,7 +566,7 @@ extern "C" {
 
 size_t cavs_norm_residual_workspace(int n, int w) {
   if (n <= 0 || w <= 0 || w > kMostW || n > (int)most_groups(1024)) return 0;
-  return (size_t)back_groups(n, w) * 5 * w * 4;
+  return (size_t)back_groups(n, w, false, false) * 5 * w * 4;
 }
 
 int cavs_norm_residual_fwd(int type, const cavs_norm_desc *d, void *s, int lds, void *x, int ldx, void *stream) {
@@ -466,7 +592,7 @@ int cavs_norm_residual_bwd(int type, const cavs_norm_desc *d, const void *s, int
   CAVS_REQUIRE(a.pre || (!g->dpre_w && !g->dpre_b), "%s: gradients of a norm that is not there", who);
   CAVS_REQUIRE(a.post || (!g->dpost_w && !g->dpost_b), "%s: gradients of a norm that is not there", who);
   CAVS_REQUIRE((a.gate || !g->dgate) && (a.gate_rows || !g->dgate_rows), "%s: gradients of a gate that is not there", who);
-  const SumOut o{{g->dpre_w, g->dpre_b, g->dgate, g->dpost_w, g->dpost_b}};
+  SumOut o{{g->dpre_w, g->dgate, g->dpost_w, g->dpre_b, g->dpost_b}};
   const bool sums = g->dpre_w || g->dpre_b || g->dgate || g->dpost_w || g->dpost_b;
   hipStream_t st = as_stream(stream);
   if (a.n == 0) {  // sums over no rows
@@ -482,8 +608,10 @@ int cavs_norm_residual_bwd(int type, const cavs_norm_desc *d, const void *s, int
   const bool needs_y = g->dgate || g->dgate_rows || a.post;
   CAVS_REQUIRE(!needs_y || a.y, "%s: null pointer", who);
   if (!dx) a.pre = CAVS_NORM_NONE;  // (nothing comes through it)
-  const int groups = back_groups(a.n, a.w);
-  Back b{s, ds, dx, lds, ldds, lddx, g->dy, g->dr, g->dgate_rows, g->lddy, g->lddr, g->lddg, nullptr, a.post ? 5 : 3};
+  if (!a.post) o.o[2] = o.o[3], o.o[3] = o.o[4] = nullptr;  // (in the order of the sums there are)
+  const bool full = a.pre == CAVS_NORM_LAYER || a.post == CAVS_NORM_LAYER || g->dpre_b || g->dpost_b;
+  const int groups = back_groups(a.n, a.w, a.post, full);
+  Back b{s, ds, dx, lds, ldds, lddx, g->dy, g->dr, g->dgate_rows, g->lddy, g->lddr, g->lddg, nullptr};
   if (!needs_y) a.y = nullptr;  // (not read)
   if (sums) {
     CAVS_REQUIRE(workspace && workspace_bytes >= (size_t)groups * 5 * a.w * 4, "%s: workspace of %zu bytes needed, %zu given", who, (size_t)groups * 5 * a.w * 4,
@@ -491,7 +619,7 @@ int cavs_norm_residual_bwd(int type, const cavs_norm_desc *d, const void *s, int
     CAVS_REQUIRE(aligned16(workspace), "%s: the workspace must be 16-byte aligned", who);
     b.part = static_cast<float *>(workspace);
   }
-  return (type == CAVS_F32 ? run_bwd<float> : run_bwd<u16>)(a, b, o, groups, st);
+  return (type == CAVS_F32 ? run_bwd<float> : run_bwd<u16>)(a, b, o, full, groups, st);
 }
 
 }  // extern "C"

@@ -8,46 +8,18 @@
 // generator is for.
 #include <cmath>
 
+#include "activations.h"
 #include "direct_product.h"
 #include "dropout.h"
 
 namespace cavs {
 namespace {
 
-// ------------------------------------------------------------------ activations
-__device__ __forceinline__ float act_of(int act, float z) {
-  switch (act) {
-    case CAVS_ACT_RELU: return z < 0.f ? 0.f : z;
-    case CAVS_ACT_TANH: return tanhf(z);
-    case CAVS_ACT_SIGMOID: return 1.f / (1.f + expf(-z));
-    case CAVS_ACT_SILU: return z / (1.f + expf(-z));
-    case CAVS_ACT_GELU: return 0.5f * z * erfcf(-0.70710678f * z);
-    default: return z;
-  }
-}
-__device__ __forceinline__ float slope_of(int act, float z) {
-  switch (act) {
-    case CAVS_ACT_RELU: return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;
-    case CAVS_ACT_TANH: {
-      const float h = tanhf(z);
-      return (1.f - h) * (1.f + h);
-    }
-    case CAVS_ACT_SIGMOID: {
-      const float g = 1.f / (1.f + expf(-fabsf(z)));  // (even in z; 1 - g from the smaller exponential)
-      return g * (1.f - g);
-    }
-    case CAVS_ACT_SILU: {
-      const float g = 1.f / (1.f + expf(-z));
-      return g * (1.f + z * (1.f - g));
-    }
-    case CAVS_ACT_GELU: return 0.5f * erfcf(-0.70710678f * z) + z * (0.39894228f * expf(-0.5f * z * z));
-    default: return 1.f;
-  }
-}
-
 // ------------------------------------------------------------------ epilogues: eight neighbouring values of a row of the result
+// What they read of a row is asked for before any of it is made (hold), where the tile lies inside the result without a look at where it ends.
 template <class T>
 struct Forward {
+  static constexpr bool FAST = sizeof(T) == 2;
   const float *bias;
   int act;
   Mask m;
@@ -57,34 +29,95 @@ struct Forward {
   long ldz;
   T *Y;
   long ldy;
-  __device__ __forceinline__ void operator()(int row, int col, int left, float (&v)[8]) const {
-    if (bias) {
-      Eight<float> b;
-      b.load(bias + col, left);
+  typedef Eight<T> Held;
+  __device__ __forceinline__ void hold(Held &r, int row, int col, int left) const {
+    r.zero();
+    if (R) r.load(R + row * ldr + col, left);
+  }
+  __device__ __forceinline__ void hold_whole(Held &r, int row, int col) const {
+    if (R) r.load(R + row * ldr + col);
+    else r.zero();
+  }
+  // bias: of the eight columns, or null
+  __device__ __forceinline__ void finish(unsigned long long step, unsigned id, const float *b, const Held &r, int row, int col, int left, float (&v)[8]) const {
+    if (b) {
 #pragma unroll
       for (int e = 0; e < 8; e++) v[e] += b[e];
     }
     if (Z) Eight<T>::store(Z + row * ldz + col, v, left);
     if (act) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = act_of(act, v[e]);
+      for (int e = 0; e < 8; e++) v[e] = act_of<FAST>(act, v[e]);
     }
-    if (m.t) drop8(m, draws_of(m, step_of(m), row_id(m, row), col >> 3), v);
-    if (R) {
-      Eight<T> r;
-      r.load(R + row * ldr + col, left);
+    if (m.t) drop8(m, draws_of(m, step, id, col >> 3), v);
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[e] += r[e];
-    }
+    for (int e = 0; e < 8; e++) v[e] += r[e];
     Eight<T>::store(Y + row * ldy + col, v, left);
   }
+  __device__ __forceinline__ const float *biases() const { return bias; }
+  __device__ __forceinline__ unsigned long long step() const { return step_of(m); }
+  __device__ __forceinline__ unsigned id(int row) const { return m.t ? row_id(m, row) : 0u; }
 };
 template <class T>
 struct Plain {
   T *Y;
   long ldy;
-  __device__ __forceinline__ void operator()(int row, int col, int left, float (&v)[8]) const { Eight<T>::store(Y + row * ldy + col, v, left); }
+  struct Held {};
+  __device__ __forceinline__ void hold(Held &, int, int, int) const {}
+  __device__ __forceinline__ void hold_whole(Held &, int, int) const {}
+  __device__ __forceinline__ void finish(unsigned long long, unsigned, const float *, const Held &, int row, int col, int left, float (&v)[8]) const {
+    Eight<T>::store(Y + row * ldy + col, v, left);
+  }
+  __device__ __forceinline__ const float *biases() const { return nullptr; }
+  __device__ __forceinline__ unsigned long long step() const { return 0; }
+  __device__ __forceinline__ unsigned id(int) const { return 0; }
 };
+
+// A tile's biases in LDS (of its columns, 0 beyond the last), written before the product and read behind its barriers
+template <int BM, class E>
+__device__ __forceinline__ void keep_biases(const E &out, float *kept, int m0, int cols) {
+  const float *b = out.biases();
+  if (!b) return;
+  for (int i = threadIdx.x; i < BM; i += blockDim.x) kept[i] = m0 + i < cols ? b[m0 + i] : 0.f;
+}
+// pieces i < I, j < J of a wavefront's tile: col(i), row(j) within the tile at m0, n0; values(i, j, v)
+template <int I, int J, int BM, int BN, class E, class Row, class Col, class Values>
+__device__ __forceinline__ void finish_tile(const E &out, const float *kept, int m0, int n0, int cols, int rows, Row &&row, Col &&col, Values &&values) {
+  const float *b = out.biases() ? kept : nullptr;
+  const unsigned long long step = out.step();
+  if (m0 + BM <= cols && n0 + BN <= rows) {
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+      const int r = n0 + row(j);
+      const unsigned id = out.id(r);
+      typename E::Held held[I];
+#pragma unroll
+      for (int i = 0; i < I; i++) out.hold_whole(held[i], r, m0 + col(i));
+#pragma unroll
+      for (int i = 0; i < I; i++) {
+        float v[8];
+        values(i, j, v);
+        out.finish(step, id, b ? b + col(i) : nullptr, held[i], r, m0 + col(i), 8, v);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < J; j++) {
+    const int r = n0 + row(j);
+    const unsigned id = r < rows ? out.id(r) : 0u;
+#pragma unroll
+    for (int i = 0; i < I; i++) {
+      float v[8];
+      values(i, j, v);  // (an exchange between lanes: all of them take part)
+      const int c = m0 + col(i);
+      if (r >= rows || c >= cols) continue;
+      typename E::Held held;
+      out.hold(held, r, c, cols - c);
+      out.finish(step, id, b ? b + col(i) : nullptr, held, r, c, cols - c, v);
+    }
+  }
+}
 
 // ------------------------------------------------------------------ operands, packed (nt_product.h)
 template <class T>
@@ -141,7 +174,7 @@ __global__ __launch_bounds__(256) void grad_kernel(GradJob<T> g) {
     for (int e = 0; e < 8; e++) v[e] = d[e];
     if (g.m.t && left > 0) drop8(g.m, draws_of(g.m, step, row_id(g.m, row), col >> 3), v);
 #pragma unroll
-    for (int e = 0; e < 8; e++) tile[r][8 * piece + e] = e < left ? g.act ? v[e] * slope_of(g.act, z[e]) : v[e] : 0.f;
+    for (int e = 0; e < 8; e++) tile[r][8 * piece + e] = e < left ? g.act ? v[e] * slope_of<P == 1>(g.act, z[e]) : v[e] : 0.f;
   }
   __syncthreads();
   if (g.o.p) pack_tile<P>(tile, g.o, PackedOut{}, r0, k0, g.orows, g.N);
@@ -178,35 +211,33 @@ __device__ __forceinline__ void exchanged(const floatx16 &t, int pair, float (&v
 
 template <class T, bool TA, bool TB, class E>
 __global__ __launch_bounds__(T::THREADS, T::EU) void packed_product_kernel(Product<E> g) {
-  __shared__ __attribute__((aligned(16))) char S[T::LDS];
+  // (one array: of two the compiler no longer knows that the pieces are not what is on its way from memory, and waits: 8192 x 8192 x 4096 924 us, 394 so)
+  __shared__ __attribute__((aligned(16))) char S[T::LDS + T::BM * 4];
+  float *kept = reinterpret_cast<float *>(S + T::LDS);
   const int tiles = g.tilesM * g.tilesN, split = blockIdx.x / tiles;
   int tm, tn;
   nt_tile_of(blockIdx.x - split * tiles, g.tilesM, g.tilesN, &tm, &tn);
   const int m0 = tm * T::BM, n0 = tn * T::BN, kbeg = split * g.kchunk, kend = min(g.K, kbeg + g.kchunk);
   floatx16 acc[T::ACC][T::TM][T::TN];
+  if (!g.part) keep_biases<T::BM>(g.out, kept, m0, g.cols);
   nt_multiply<T, TA, TB>(g.A, g.cols, m0, g.B, g.rows, n0, kbeg, kend, S, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c0 = m0 + wave / T::WGN * T::WM + 8 * (lane >> 5), r0 = n0 + wave % T::WGN * T::WN + (lane & 31);
+  if constexpr (T::ACC > 1) {
 #pragma unroll
-  for (int j = 0; j < T::TN; j++) {
-    const int row = r0 + 32 * j;
-    if (row >= g.rows) continue;
+    for (int i = 0; i < T::TM; i++)
 #pragma unroll
-    for (int i = 0; i < T::TM; i++) {
-      if constexpr (T::ACC > 1) {
+      for (int j = 0; j < T::TN; j++)
 #pragma unroll
         for (int r = 0; r < 16; r++) acc[0][i][j][r] += acc[T::ACC - 1][i][j][r];
-      }
-#pragma unroll
-      for (int pair = 0; pair < 2; pair++) {
-        float v[8];
-        exchanged(acc[0][i][j], pair, v);
-        const int col = c0 + 32 * i + 16 * pair;
-        if (col >= g.cols) continue;
-        if (g.part) Eight<float>::store(g.part + ((long)split * g.rows + row) * g.cols + col, v, g.cols - col);
-        else g.out(row, col, g.cols - col, v);
-      }
-    }
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const auto col = [&](int i) { return wave / T::WGN * T::WM + 16 * i + 8 * (lane >> 5); };
+  const auto row = [&](int j) { return wave % T::WGN * T::WN + 32 * j + (lane & 31); };
+  const auto values = [&](int i, int j, float (&v)[8]) { exchanged(acc[0][i >> 1][j], i & 1, v); };
+  if (g.part) {
+    const Plain<float> part{g.part + (long)split * g.rows * g.cols, g.cols};
+    finish_tile<2 * T::TM, T::TN, T::BM, T::BN>(part, kept, m0, n0, g.cols, g.rows, row, col, values);
+  } else {
+    finish_tile<2 * T::TM, T::TN, T::BM, T::BN>(g.out, kept, m0, n0, g.cols, g.rows, row, col, values);
   }
 }
 
@@ -220,26 +251,25 @@ struct DirectJob {
 };
 template <class T, bool TA, bool TB, class E>
 __global__ __launch_bounds__(T::THREADS, T::EU) void direct_product_kernel(DirectJob<E> g) {
-  __shared__ __attribute__((aligned(16))) char S[T::LDS];
+  // (one array: of two the compiler no longer knows that the pieces are not what is on its way from memory, and waits: 8192 x 8192 x 4096 924 us, 394 so)
+  __shared__ __attribute__((aligned(16))) char S[T::LDS + T::BM * 4];
+  float *kept = reinterpret_cast<float *>(S + T::LDS);
   const int tiles = g.tilesM * g.tilesN, split = blockIdx.x / tiles;
   int tm, tn;
   nt_tile_of(blockIdx.x - split * tiles, g.tilesM, g.tilesN, &tm, &tn);
   const int m0 = tm * T::BM, n0 = tn * T::BN, kbeg = split * g.kchunk, kend = min(g.K, kbeg + g.kchunk);
   floatx4 acc[T::I][2 * T::J];
+  if (!g.part) keep_biases<T::BM>(g.out, kept, m0, g.cols);
   direct_multiply<TA, TB>(T{}, g.A, g.cols, m0, g.B, g.rows, n0, kbeg, kend, S, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int j = 0; j < T::J; j++) {
-    const int row = n0 + T::row(wave, lane, j);
-#pragma unroll
-    for (int i = 0; i < T::I; i++) {
-      float v[8];
-      eight_columns(acc[i][2 * j], acc[i][2 * j + 1], v);
-      const int col = m0 + T::col(wave, lane, i);
-      if (row >= g.rows || col >= g.cols) continue;
-      if (g.part) Eight<float>::store(g.part + ((long)split * g.rows + row) * g.cols + col, v, g.cols - col);
-      else g.out(row, col, g.cols - col, v);
-    }
+  const auto col = [&](int i) { return T::col(wave, lane, i); };
+  const auto row = [&](int j) { return T::row(wave, lane, j); };
+  const auto values = [&](int i, int j, float (&v)[8]) { eight_columns(acc[i][2 * j], acc[i][2 * j + 1], v); };
+  if (g.part) {
+    const Plain<float> part{g.part + (long)split * g.rows * g.cols, g.cols};
+    finish_tile<T::I, T::J, T::BM, T::BN>(part, kept, m0, n0, g.cols, g.rows, row, col, values);
+  } else {
+    finish_tile<T::I, T::J, T::BM, T::BN>(g.out, kept, m0, n0, g.cols, g.rows, row, col, values);
   }
 }
 
@@ -258,12 +288,9 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(GradJob<u16> g, u16 *D) 
       Eight<u16> d[4], z[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const int row = r0 + line + 8 * (4 * q + i);
-        d[i].zero(), z[i].zero();
-        if (row < g.n) {
-          d[i].load(g.dY + row * g.lddy + col, left);
-          if (g.act) z[i].load(g.Z + row * g.ldz + col, left);
-        }
+        const int row = min(r0 + line + 8 * (4 * q + i), g.n - 1);  // (N is whole pieces here)
+        d[i].load(g.dY + row * g.lddy + col);
+        if (g.act) z[i].load(g.Z + row * g.ldz + col);
       }
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -275,11 +302,11 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(GradJob<u16> g, u16 *D) 
         if (g.m.t) drop8(g.m, draws_of(g.m, step, row_id(g.m, row), col >> 3), v);
         if (g.act) {
 #pragma unroll
-          for (int e = 0; e < 8; e++) v[e] *= slope_of(g.act, z[i][e]);
+          for (int e = 0; e < 8; e++) v[e] *= slope_of<true>(g.act, z[i][e]);
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) s[e] += v[e];
-        if (D) Eight<u16>::store(D + (long)row * g.N + col, v, left);
+        if (D) Eight<u16>::store(D + (long)row * g.N + col, v, 8);
       }
     }
   }
@@ -315,7 +342,16 @@ __global__ __launch_bounds__(256) void parts_kernel(const float *part, int parts
 #pragma unroll
       for (int e = 0; e < 8; e++) v[e] += t[k][e];
   }
-  out(row, col, left, v);
+  typename E::Held held;
+  out.hold(held, row, col, left);
+  float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (out.biases()) {
+    Eight<float> t;
+    t.load(out.biases() + col, left);
+#pragma unroll
+    for (int e = 0; e < 8; e++) b[e] = t[e];
+  }
+  out.finish(out.step(), out.id(row), b, held, row, col, left, v);
 }
 
 __global__ __launch_bounds__(256) void column_sums_kernel(const float *part, int parts, int cols, float *out) {

@@ -129,16 +129,18 @@ struct PackJob {
   int across, blocks;  // blocks of 64 columns, of 64 x 64
 };
 template <int P, class T>
-__global__ __launch_bounds__(256) void pack_kernel(PackJob<T> j0, PackJob<T> j1) {
-  __shared__ PackTile tile;
-  const int at = blockIdx.y * gridDim.x + blockIdx.x;
-  if (at >= j0.blocks + j1.blocks) return;
-  const bool second = at >= j0.blocks;
-  const PackJob<T> &g = second ? j1 : j0;
-  const int block = second ? at - j0.blocks : at, r0 = block / g.across * 64, k0 = block % g.across * 64;
+__device__ __forceinline__ void pack_block(const PackJob<T> &g, int block, PackTile &tile) {
+  const int r0 = block / g.across * 64, k0 = block % g.across * 64;
   load_tile(tile, g.src, g.ld, r0, k0, g.rows, g.K);
   __syncthreads();
   pack_tile<P>(tile, g.o, PackedOut{}, r0, k0, g.orows, g.K);
+}
+template <int P, class T>
+__global__ __launch_bounds__(256) void pack_kernel(PackJob<T> j0, PackJob<T> j1) {
+  __shared__ PackTile tile;
+  const int block = blockIdx.y * gridDim.x + blockIdx.x;
+  if (block < j0.blocks) pack_block<P>(j0, block, tile);
+  else if (block < j0.blocks + j1.blocks) pack_block<P>(j1, block - j0.blocks, tile);
 }
 
 // D packed, and sums of its columns over 64 rows each [blocks of rows][N]
@@ -152,12 +154,17 @@ struct GradJob {
   PackedOut o;
   float *sums;
 };
+// and X and W packed, behind it
 template <int P, class T>
-__global__ __launch_bounds__(256) void grad_kernel(GradJob<T> g) {
+__global__ __launch_bounds__(256) void grad_kernel(GradJob<T> g, PackJob<T> x, PackJob<T> w) {
   __shared__ PackTile tile;
   __shared__ float part[4][64];
   const int block = blockIdx.y * gridDim.x + blockIdx.x;
-  if (block >= g.blocks) return;
+  if (block >= g.blocks) {
+    if (block < g.blocks + x.blocks) pack_block<P>(x, block - g.blocks, tile);
+    else if (block < g.blocks + x.blocks + w.blocks) pack_block<P>(w, block - g.blocks - x.blocks, tile);
+    return;
+  }
   const int r0 = block / g.across * 64, k0 = block % g.across * 64, piece = threadIdx.x & 7;
   const unsigned long long step = step_of(g.m);
 #pragma unroll
@@ -179,13 +186,13 @@ __global__ __launch_bounds__(256) void grad_kernel(GradJob<T> g) {
   __syncthreads();
   if (g.o.p) pack_tile<P>(tile, g.o, PackedOut{}, r0, k0, g.orows, g.N);
   if (!g.sums) return;
-  const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int c = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; i++) s += tile[16 * w + i][c];
-  part[w][c] = s;
+  for (int i = 0; i < 16; i++) s += tile[16 * wave + i][c];
+  part[wave][c] = s;
   __syncthreads();
-  if (w == 0 && k0 + c < g.N) g.sums[(long)(r0 / 64) * g.N + k0 + c] = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
+  if (wave == 0 && k0 + c < g.N) g.sums[(long)(r0 / 64) * g.N + k0 + c] = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
 }
 
 // ------------------------------------------------------------------ products of packed operands
@@ -194,7 +201,7 @@ __global__ __launch_bounds__(256) void grad_kernel(GradJob<T> g) {
 template <class E>
 struct Product {
   PackedRef A, B;
-  int cols, rows, K, tilesM, tilesN, splits, kchunk;
+  int cols, rows, K, tilesM, tilesN, kchunk;
   float *part;
   E out;
 };
@@ -209,18 +216,8 @@ __device__ __forceinline__ void exchanged(const floatx16 &t, int pair, float (&v
   }
 }
 
-template <class T, bool TA, bool TB, class E>
-__global__ __launch_bounds__(T::THREADS, T::EU) void packed_product_kernel(Product<E> g) {
-  // (one array: of two the compiler no longer knows that the pieces are not what is on its way from memory, and waits: 8192 x 8192 x 4096 924 us, 394 so)
-  __shared__ __attribute__((aligned(16))) char S[T::LDS + T::BM * 4];
-  float *kept = reinterpret_cast<float *>(S + T::LDS);
-  const int tiles = g.tilesM * g.tilesN, split = blockIdx.x / tiles;
-  int tm, tn;
-  nt_tile_of(blockIdx.x - split * tiles, g.tilesM, g.tilesN, &tm, &tn);
-  const int m0 = tm * T::BM, n0 = tn * T::BN, kbeg = split * g.kchunk, kend = min(g.K, kbeg + g.kchunk);
-  floatx16 acc[T::ACC][T::TM][T::TN];
-  if (!g.part) keep_biases<T::BM>(g.out, kept, m0, g.cols);
-  nt_multiply<T, TA, TB>(g.A, g.cols, m0, g.B, g.rows, n0, kbeg, kend, S, acc);
+template <class T, class E>
+__device__ __forceinline__ void finish_packed(const Product<E> &g, int split, const float *kept, int m0, int n0, floatx16 (&acc)[T::ACC][T::TM][T::TN]) {
   if constexpr (T::ACC > 1) {
 #pragma unroll
     for (int i = 0; i < T::TM; i++)
@@ -240,6 +237,42 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void packed_product_kernel(Produ
     finish_tile<2 * T::TM, T::TN, T::BM, T::BN>(g.out, kept, m0, n0, g.cols, g.rows, row, col, values);
   }
 }
+template <class E>
+__device__ __forceinline__ void tile_at(const Product<E> &g, int block, int bm, int bn, int *split, int *m0, int *n0, int *kbeg, int *kend) {
+  const int tiles = g.tilesM * g.tilesN;
+  *split = block / tiles;
+  nt_tile_of(block - *split * tiles, g.tilesM, g.tilesN, m0, n0);
+  *m0 *= bm, *n0 *= bn;
+  *kbeg = *split * g.kchunk, *kend = min(g.K, *kbeg + g.kchunk);
+}
+
+template <class T, class E>
+__global__ __launch_bounds__(T::THREADS, T::EU) void packed_forward_kernel(Product<E> g) {
+  // (one array: of two the compiler no longer knows that the pieces are not what is on its way from memory, and waits: direct_forward_kernel of
+  // 8192 x 8192 x 4096 924 us, 394 so)
+  __shared__ __attribute__((aligned(16))) char S[T::LDS + T::BM * 4];
+  float *kept = reinterpret_cast<float *>(S + T::LDS);
+  int split, m0, n0, kbeg, kend;
+  tile_at(g, blockIdx.x, T::BM, T::BN, &split, &m0, &n0, &kbeg, &kend);
+  floatx16 acc[T::ACC][T::TM][T::TN];
+  if (!g.part) keep_biases<T::BM>(g.out, kept, m0, g.cols);
+  nt_multiply<T, false, false>(g.A, g.cols, m0, g.B, g.rows, n0, kbeg, kend, S, acc);
+  finish_packed<T>(g, split, kept, m0, n0, acc);
+}
+// Both gradients in a launch, so that the compute units whose last tile of the one has ended go on with the other: dX = D W (its A turned) and dW = D^T X (both
+// turned), `wfirst`: dW is j0.
+template <class T, class E>
+__global__ __launch_bounds__(T::THREADS, T::EU) void packed_back_kernel(Product<E> j0, Product<E> j1, int blocks0, int wfirst) {
+  __shared__ __attribute__((aligned(16))) char S[T::LDS];
+  const bool second = (int)blockIdx.x >= blocks0;
+  const Product<E> &g = second ? j1 : j0;
+  int split, m0, n0, kbeg, kend;
+  tile_at(g, second ? blockIdx.x - blocks0 : blockIdx.x, T::BM, T::BN, &split, &m0, &n0, &kbeg, &kend);
+  floatx16 acc[T::ACC][T::TM][T::TN];
+  if (second != (wfirst != 0)) nt_multiply<T, true, true>(g.A, g.cols, m0, g.B, g.rows, n0, kbeg, kend, S, acc);
+  else nt_multiply<T, true, false>(g.A, g.cols, m0, g.B, g.rows, n0, kbeg, kend, S, acc);
+  finish_packed<T>(g, split, nullptr, m0, n0, acc);
+}
 
 // ------------------------------------------------------------------ products of operands as they lie (direct_product.h)
 template <class E>
@@ -249,18 +282,16 @@ struct DirectJob {
   float *part;
   E out;
 };
-template <class T, bool TA, bool TB, class E>
-__global__ __launch_bounds__(T::THREADS, T::EU) void direct_product_kernel(DirectJob<E> g) {
-  // (one array: of two the compiler no longer knows that the pieces are not what is on its way from memory, and waits: 8192 x 8192 x 4096 924 us, 394 so)
-  __shared__ __attribute__((aligned(16))) char S[T::LDS + T::BM * 4];
-  float *kept = reinterpret_cast<float *>(S + T::LDS);
-  const int tiles = g.tilesM * g.tilesN, split = blockIdx.x / tiles;
-  int tm, tn;
-  nt_tile_of(blockIdx.x - split * tiles, g.tilesM, g.tilesN, &tm, &tn);
-  const int m0 = tm * T::BM, n0 = tn * T::BN, kbeg = split * g.kchunk, kend = min(g.K, kbeg + g.kchunk);
-  floatx4 acc[T::I][2 * T::J];
-  if (!g.part) keep_biases<T::BM>(g.out, kept, m0, g.cols);
-  direct_multiply<TA, TB>(T{}, g.A, g.cols, m0, g.B, g.rows, n0, kbeg, kend, S, acc);
+template <class E>
+__device__ __forceinline__ void tile_at(const DirectJob<E> &g, int block, int bm, int bn, int *split, int *m0, int *n0, int *kbeg, int *kend) {
+  const int tiles = g.tilesM * g.tilesN;
+  *split = block / tiles;
+  nt_tile_of(block - *split * tiles, g.tilesM, g.tilesN, m0, n0);
+  *m0 *= bm, *n0 *= bn;
+  *kbeg = *split * g.kchunk, *kend = min(g.K, *kbeg + g.kchunk);
+}
+template <class T, class E>
+__device__ __forceinline__ void finish_direct(const DirectJob<E> &g, int split, const float *kept, int m0, int n0, const floatx4 (&acc)[T::I][2 * T::J]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const auto col = [&](int i) { return T::col(wave, lane, i); };
   const auto row = [&](int j) { return T::row(wave, lane, j); };
@@ -271,6 +302,30 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void direct_product_kernel(Direc
   } else {
     finish_tile<T::I, T::J, T::BM, T::BN>(g.out, kept, m0, n0, g.cols, g.rows, row, col, values);
   }
+}
+template <class T, class E>
+__global__ __launch_bounds__(T::THREADS, T::EU) void direct_forward_kernel(DirectJob<E> g) {
+  __shared__ __attribute__((aligned(16))) char S[T::LDS + T::BM * 4];
+  float *kept = reinterpret_cast<float *>(S + T::LDS);
+  int split, m0, n0, kbeg, kend;
+  tile_at(g, blockIdx.x, T::BM, T::BN, &split, &m0, &n0, &kbeg, &kend);
+  floatx4 acc[T::I][2 * T::J];
+  if (!g.part) keep_biases<T::BM>(g.out, kept, m0, g.cols);
+  direct_multiply<false, false>(T{}, g.A, g.cols, m0, g.B, g.rows, n0, kbeg, kend, S, acc);
+  finish_direct<T>(g, split, kept, m0, n0, acc);
+}
+// (as packed_back_kernel)
+template <class T, class E>
+__global__ __launch_bounds__(T::THREADS, T::EU) void direct_back_kernel(DirectJob<E> j0, DirectJob<E> j1, int blocks0, int wfirst) {
+  __shared__ __attribute__((aligned(16))) char S[T::LDS];
+  const bool second = (int)blockIdx.x >= blocks0;
+  const DirectJob<E> &g = second ? j1 : j0;
+  int split, m0, n0, kbeg, kend;
+  tile_at(g, second ? blockIdx.x - blocks0 : blockIdx.x, T::BM, T::BN, &split, &m0, &n0, &kbeg, &kend);
+  floatx4 acc[T::I][2 * T::J];
+  if (second != (wfirst != 0)) direct_multiply<true, true>(T{}, g.A, g.cols, m0, g.B, g.rows, n0, kbeg, kend, S, acc);
+  else direct_multiply<true, false>(T{}, g.A, g.cols, m0, g.B, g.rows, n0, kbeg, kend, S, acc);
+  finish_direct<T>(g, split, nullptr, m0, n0, acc);
 }
 
 // D as it lies (write: bf16, rows of N), and sums of its columns over 64 rows each [stretches of rows][N]; 256 columns a workgroup
@@ -322,20 +377,140 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(GradJob<u16> g, u16 *D) 
   g.sums[(long)(r0 / 64) * g.N + c] = t;
 }
 
-// what products left in parts, in their order, to the epilogue; pieces of eight columns
+// ------------------------------------------------------------------ few rows: W read once, where it lies
+// A workgroup makes sixteen columns of the result: eight wavefronts, each a stretch of K, the rows of W and X as pieces of the 16x16x32 instruction straight from memory
+// (fp32: split into parts on the way), 256 k of them asked for at a time.  Their sums meet in LDS.  Sixteen columns, so that W has two workgroups
+// a compute unit from 8192 columns on; each reads all of X.
+template <class T>
+struct FewJob {
+  const T *X, *W;
+  long ldx, ldw;
+  int n, K, N, chunk;  // chunk: k of a wavefront, a multiple of 32
+  Forward<T> out;
+};
+template <int P>
+__device__ __forceinline__ void parts_of_eight(const Eight<float> &v, bf16x8 (&o)[P]) {
+  u16 t[8][P];
+#pragma unroll
+  for (int e = 0; e < 8; e++) parts_of<P>(v[e], t[e]);
+#pragma unroll
+  for (int p = 0; p < P; p++)
+    o[p] = __builtin_bit_cast(bf16x8, make_uint4(t[0][p] | (unsigned)t[1][p] << 16, t[2][p] | (unsigned)t[3][p] << 16, t[4][p] | (unsigned)t[5][p] << 16,
+                                                 t[6][p] | (unsigned)t[7][p] << 16));
+}
+__device__ __forceinline__ void parts_of_eight(const Eight<u16> &v, bf16x8 (&o)[1]) {
+  typedef unsigned four __attribute__((ext_vector_type(4)));
+  o[0] = __builtin_bit_cast(bf16x8, (four)v.a);
+}
+
+constexpr int kFewWaves = 8;
+// TT: blocks of sixteen rows of X
+template <class T, int TT>
+__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(FewJob<T> g) {
+  constexpr int P = sizeof(T) == 4 ? 3 : 1, DEPTH = sizeof(T) == 4 ? (TT > 2 ? 2 : 4) : (TT > 2 ? 4 : 8), ACC = P > 1 ? 2 : 1;
+  __shared__ float sums[kFewWaves][TT][16][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = blockIdx.x * 16, x = lane & 15, piece = 8 * (lane >> 4), r0 = blockIdx.y * 16 * TT;
+  const int kbeg = wave * g.chunk, kend = min(g.K, kbeg + g.chunk);
+  const T *w = g.W + min(c0 + x, g.N - 1) * g.ldw + piece;
+  const T *rows[TT];
+#pragma unroll
+  for (int t = 0; t < TT; t++) rows[t] = g.X + min(r0 + 16 * t + x, g.n - 1) * g.ldx + piece;  // (rows beyond the last: once more the last, not stored)
+  floatx4 acc[ACC][TT];
+#pragma unroll
+  for (int a = 0; a < ACC; a++)
+#pragma unroll
+    for (int t = 0; t < TT; t++) acc[a][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](const Eight<T> &wv, const Eight<T> (&xv)[TT]) {
+    bf16x8 a[P], b[P];
+    parts_of_eight(wv, a);
+#pragma unroll
+    for (int t = 0; t < TT; t++) {
+      parts_of_eight(xv[t], b);
+#pragma unroll
+      for (int p = 0; p < P; p++)
+#pragma unroll
+        for (int q = 0; q < P - p; q++)
+          acc[p + q ? ACC - 1 : 0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[p], b[q], acc[p + q ? ACC - 1 : 0][t], 0, 0, 0);
+    }
+  };
+  int k = kbeg;
+  for (; k + 32 * DEPTH <= kend; k += 32 * DEPTH) {
+    Eight<T> wv[DEPTH], xv[DEPTH][TT];
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++) {
+      wv[d].load(w + k + 32 * d);
+#pragma unroll
+      for (int t = 0; t < TT; t++) xv[d][t].load(rows[t] + k + 32 * d);
+    }
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++) multiply(wv[d], xv[d]);
+  }
+  for (; k < kend; k += 32) {
+    Eight<T> wv, xv[TT];
+    const int left = kend - k - piece;
+    wv.zero();
+    if (left > 0) wv.load(w + k, left);
+#pragma unroll
+    for (int t = 0; t < TT; t++) {
+      xv[t].zero();
+      if (left > 0) xv[t].load(rows[t] + k, left);
+    }
+    multiply(wv, xv);
+  }
+#pragma unroll
+  for (int t = 0; t < TT; t++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      float v = acc[0][t][r];
+      if constexpr (ACC > 1) v += acc[1][t][r];
+      sums[wave][t][x][4 * (lane >> 4) + r] = v;
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < TT * 256; i += 64 * kFewWaves) {
+    const int t = i >> 8, r = i >> 4 & 15, c = i & 15;
+    float v = sums[0][t][r][c];
+#pragma unroll
+    for (int q = 1; q < kFewWaves; q++) v += sums[q][t][r][c];
+    sums[0][t][r][c] = v;  // (nobody else reads this one)
+  }
+  __syncthreads();
+  const int r = threadIdx.x >> 1, row = r0 + r, col = c0 + 8 * (threadIdx.x & 1), left = g.N - col;
+  if (r >= 16 * TT || row >= g.n || left <= 0) return;
+  float v[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = sums[0][r >> 4][r & 15][8 * (threadIdx.x & 1) + e];
+  if (g.out.bias) {
+    Eight<float> t;
+    t.load(g.out.bias + col, left);
+#pragma unroll
+    for (int e = 0; e < 8; e++) b[e] = t[e];
+  }
+  Eight<T> held;
+  g.out.hold(held, row, col, left);
+  g.out.finish(g.out.step(), g.out.id(row), b, held, row, col, left, v);
+}
+
+// what a product left in parts, in their order, to the epilogue; pieces of eight columns
 template <class E>
-__global__ __launch_bounds__(256) void parts_kernel(const float *part, int parts, int rows, int cols, E out) {
-  const int pieces = (cols + 7) / 8;
-  const long total = (long)rows * pieces, i = (long)blockIdx.x * 256 + threadIdx.x;
+struct PartsJob {
+  const float *part;
+  int parts, rows, cols;
+  E out;
+  int blocks;  // 0: none
+};
+template <class E>
+__device__ __forceinline__ void join_block(const PartsJob<E> &g, int block) {
+  const int pieces = (g.cols + 7) / 8;
+  const long total = (long)g.rows * pieces, i = (long)block * 256 + threadIdx.x;
   if (i >= total) return;
-  const int row = (int)(i / pieces), col = 8 * (int)(i - (long)row * pieces), left = cols - col;
+  const int row = (int)(i / pieces), col = 8 * (int)(i - (long)row * pieces), left = g.cols - col;
   float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < parts; p += 4) {
+  for (int p = 0; p < g.parts; p += 4) {
     Eight<float> t[4];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       t[k].zero();
-      if (p + k < parts) t[k].load(part + ((long)(p + k) * rows + row) * cols + col, left);
+      if (p + k < g.parts) t[k].load(g.part + ((long)(p + k) * g.rows + row) * g.cols + col, left);
     }
 #pragma unroll
     for (int k = 0; k < 4; k++)
@@ -343,71 +518,86 @@ __global__ __launch_bounds__(256) void parts_kernel(const float *part, int parts
       for (int e = 0; e < 8; e++) v[e] += t[k][e];
   }
   typename E::Held held;
-  out.hold(held, row, col, left);
+  g.out.hold(held, row, col, left);
   float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (out.biases()) {
+  if (g.out.biases()) {
     Eight<float> t;
-    t.load(out.biases() + col, left);
+    t.load(g.out.biases() + col, left);
 #pragma unroll
     for (int e = 0; e < 8; e++) b[e] = t[e];
   }
-  out.finish(out.step(), out.id(row), b, held, row, col, left, v);
+  g.out.finish(g.out.step(), g.out.id(row), b, held, row, col, left, v);
 }
+template <class E>
+__global__ __launch_bounds__(256) void parts_kernel(PartsJob<E> g) { join_block(g, blockIdx.x); }
 
-__global__ __launch_bounds__(256) void column_sums_kernel(const float *part, int parts, int cols, float *out) {
-  __shared__ float each[4][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6, per = (parts + 3) / 4, end = min(parts, (w + 1) * per);
+// sums of columns that launches before left over 64 rows each, 64 columns a workgroup
+struct ColumnsJob {
+  const float *part;
+  int parts, cols;
+  float *out;
+  int blocks;
+};
+__device__ __forceinline__ void sum_columns(const ColumnsJob &g, int block, float (&each)[4][64]) {
+  const int c = block * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6, per = (g.parts + 3) / 4, end = min(g.parts, (w + 1) * per);
   float s = 0.f;
-  if (c < cols)
+  if (c < g.cols)
     for (int p = w * per; p < end; p += 8) {
       float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; k++) v[k] = p + k < end ? part[(long)(p + k) * cols + c] : 0.f;
+      for (int k = 0; k < 8; k++) v[k] = p + k < end ? g.part[(long)(p + k) * g.cols + c] : 0.f;
 #pragma unroll
       for (int k = 0; k < 8; k++) s += v[k];
     }
   each[w][threadIdx.x & 63] = s;
   __syncthreads();
-  if (w == 0 && c < cols) out[c] = (each[0][threadIdx.x] + each[1][threadIdx.x]) + (each[2][threadIdx.x] + each[3][threadIdx.x]);
+  if (w == 0 && c < g.cols) g.out[c] = (each[0][threadIdx.x] + each[1][threadIdx.x]) + (each[2][threadIdx.x] + each[3][threadIdx.x]);
+}
+// the ends of both gradients and db
+template <class E>
+__global__ __launch_bounds__(256) void back_ends_kernel(PartsJob<E> x, PartsJob<E> w, ColumnsJob b) {
+  __shared__ float each[4][64];
+  const int block = blockIdx.x;
+  if (block < b.blocks) sum_columns(b, block, each);
+  else if (block < b.blocks + x.blocks) join_block(x, block - b.blocks);
+  else if (block < b.blocks + x.blocks + w.blocks) join_block(w, block - b.blocks - x.blocks);
 }
 
 // ------------------------------------------------------------------ what a call consists of
 template <int P> struct Tiles;
 template <> struct Tiles<1> {
-  using L = NtTile<1, 256, 128, 32, 2, 2>;
-  using M = NtTile<1, 128, 128, 32, 2, 2>;
+  using L = NtTile<1, 128, 128, 32, 2, 2>;
   using S = NtTile<1, 64, 64, 64, 2, 2, 3>;
 };
 template <> struct Tiles<3> {
   using L = NtTile<3, 128, 128, 16, 2, 2>;
-  using M = L;
   using S = NtTile<3, 64, 64, 32, 2, 2>;
 };
 template <int P, class F>
 int with_tile(int size, F &&f) {
   using TT = Tiles<P>;
-  if (size == 2) return f(typename TT::L{});
-  if (size == 1) return f(typename TT::M{});
+  if (size) return f(typename TT::L{});
   return f(typename TT::S{});
 }
 
 struct Shape {  // of a product
   int size, tm, tn, splits, kchunk;
+  double us;
 };
 // The tile and the stretches of K that a model of the launch finds best: ns a k of a compute unit that has one, two or three workgroups of a tile, as
 // measured (fp32, in products of 7088 rows: 128 x 128 at 224, 448 and 672 workgroups, 64 x 64 at 256, 512 and 768); each workgroup costs 200 k more than it multiplies,
 // and what products leave in parts is written and read at the rate of a copy, by a launch more.  us of a call with all workgroups whole / in the stretches this
 // finds: fp32 gradients of 7088 x 512 x 2048 405 / 245.
 template <int P> struct Speeds;
-template <> struct Speeds<3> { static constexpr int SIZES = 2; static constexpr double ns[2][3] = {{26, 26, 29}, {68, 73, 98}}; };
-template <> struct Speeds<1> { static constexpr int SIZES = 3; static constexpr double ns[3][3] = {{6, 6.5, 8}, {14, 15, 20}, {24, 27, 38}}; };
+template <> struct Speeds<3> { static constexpr double ns[2][3] = {{26, 26, 29}, {68, 73, 98}}; };
+template <> struct Speeds<1> { static constexpr double ns[2][3] = {{6, 6.5, 8}, {14, 15, 20}}; };
 constexpr int kStretches[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
 template <int P>
 Shape shape_of(int cols, int rows, int K) {
   Shape best{};
   double least = INFINITY;
   const int cus = num_cus();
-  for (int size = 0; size < Speeds<P>::SIZES; size++) {
+  for (int size = 0; size < 2; size++) {
     Shape s{};
     s.size = size;
     int bm = 0, bn = 0;
@@ -420,7 +610,7 @@ Shape shape_of(int cols, int rows, int K) {
       const long groups = (long)s.tm * s.tn * s.splits, full = groups / (3 * cus), rest = (groups - full * 3 * cus + cus - 1) / cus;
       double us = 1e-3 * (s.kchunk + 200) * (full * Speeds<P>::ns[size][2] + (rest > 0 ? Speeds<P>::ns[size][rest - 1] : 0.));
       if (s.splits > 1) us += 5. + s.splits * (8. * rows * cols) / 4.7e6;
-      if (us < least) least = us, best = s;
+      if (us < least) least = us, best = s, best.us = us;
     }
   }
   return best;
@@ -447,73 +637,119 @@ Shape direct_shape_of(int cols, int rows, int K) {
       double us = full * k * (wide ? 0.0245 : 0.0140);
       if (rest > 0) us += k * (wide ? (full > 0 || rest > cus / 2 ? 0.0225 : 0.0195) : (rest > cus ? 0.0140 : 0.0090));
       if (s.splits > 1) us += 5. + s.splits * (8. * rows * cols) / 4.7e6;
-      if (us < least) least = us, best = s;
+      if (us < least) least = us, best = s, best.us = us;
     }
   }
   return best;
 }
 
+// Both gradients in a launch: the same tile, and for each the stretches that bring the longest workgroup and what there is a workgroup's place to the least. `price`:
+// ns a k of a place, and how many a compute unit has, of so many workgroups.
+template <class Price>
+void back_shapes_of(int n, int K, int N, int Kx, int Kw, int align, const Price &price, Shape *dx, Shape *dw) {
+  double least = INFINITY;
+  const int cus = num_cus();
+  for (int size = 0; size < 2; size++) {
+    int bm, bn, places;
+    price(size, 1, &bm, &bn, &places);
+    Shape x{}, w{};
+    x.size = w.size = size;
+    x.tm = w.tm = tiles_of(K, bm), x.tn = tiles_of(n, bn), w.tn = tiles_of(N, bn);
+    auto set = [&](Shape &s, int of, int splits) {
+      s.kchunk = ceil_to((of + splits - 1) / splits, align);
+      s.splits = (of + s.kchunk - 1) / s.kchunk;
+    };
+    for (int sx : kStretches) {
+      if (sx > 1 && Kx / sx < 256) break;
+      set(x, Kx, sx);
+      for (int sw : kStretches) {
+        if (sw > 1 && Kw / sw < 256) break;
+        set(w, Kw, sw);
+        const double gx = (double)x.tm * x.tn * x.splits, gw = (double)w.tm * w.tn * w.splits, kx = x.kchunk + 200., kw = w.kchunk + 200.;
+        const double ns = price(size, gx + gw, &bm, &bn, &places), longest = kx > kw ? kx : kw, shortest = kx > kw ? kw : kx;
+        const double even = (gx * kx + gw * kw) / ((double)places * cus) + 0.35 * shortest;
+        double us = 1e-3 * ns * (longest > even ? longest : even);
+        if (x.splits > 1) us += x.splits * (8. * n * K) / 4.7e6;
+        if (w.splits > 1) us += w.splits * (8. * N * K) / 4.7e6;
+        if (x.splits > 1 || w.splits > 1) us += 5.;
+        if (us < least) least = us, *dx = x, *dw = w;
+      }
+    }
+  }
+}
+
 struct Plan {
   int Kp, Np, np;  // as contraction lengths
   Shape fwd, dx, dw;
-  size_t x, w, d, part, sums, bytes;
+  size_t x, w, d, part, wpart, sums, bytes;
 };
 template <int P>
 Plan plan_of(int n, int K, int N, int back) {
   Plan p{};
   p.Kp = ceil_to(K, kPlaneAlign), p.Np = ceil_to(N, kPlaneAlign), p.np = ceil_to(n, kPlaneAlign);
-  size_t at = 0, part = 0;
+  size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
     at += (bytes + 255) & ~(size_t)255;
     return here;
   };
-  auto parts = [&](const Shape &s, int rows, int cols) {
-    const size_t b = s.splits > 1 ? (size_t)s.splits * rows * cols * 4 : 0;
-    part = part > b ? part : b;
-  };
+  auto parts = [&](const Shape &s, int rows, int cols) { return s.splits > 1 ? (size_t)s.splits * rows * cols * 4 : 0; };
   p.x = take(packed_bytes<P>(p.np, p.Kp));
   p.w = take(packed_bytes<P>(p.Np, p.Kp));
   if (!back) {
     p.fwd = shape_of<P>(N, n, p.Kp);
-    parts(p.fwd, n, N);
+    p.part = take(parts(p.fwd, n, N));
   } else {
     p.d = take(packed_bytes<P>(p.np, p.Np));
-    p.dx = shape_of<P>(K, n, p.Np);
-    p.dw = shape_of<P>(K, N, p.np);
-    parts(p.dx, n, K), parts(p.dw, N, K);
+    back_shapes_of(n, K, N, p.Np, p.np, kPlaneAlign, [](int size, double groups, int *bm, int *bn, int *places) {
+      with_tile<P>(size, [&](auto t) { return *bm = decltype(t)::BM, *bn = decltype(t)::BN, 0; });
+      *places = groups <= num_cus() ? 1 : groups <= 2 * num_cus() ? 2 : 3;
+      return Speeds<P>::ns[size][*places - 1];
+    }, &p.dx, &p.dw);
+    p.part = take(parts(p.dx, n, K)), p.wpart = take(parts(p.dw, N, K));
     p.sums = take((size_t)(p.np / 64) * N * 4);
   }
-  p.part = take(part);
   p.bytes = at;
   return p;
 }
 Plan direct_plan_of(int n, int K, int N, int back) {
   Plan p{};
-  size_t at = 0, part = 0;
+  size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
     at += (bytes + 255) & ~(size_t)255;
     return here;
   };
-  auto parts = [&](const Shape &s, int rows, int cols) {
-    const size_t b = s.splits > 1 ? (size_t)s.splits * rows * cols * 4 : 0;
-    part = part > b ? part : b;
-  };
+  auto parts = [&](const Shape &s, int rows, int cols) { return s.splits > 1 ? (size_t)s.splits * rows * cols * 4 : 0; };
   if (!back) {
     p.fwd = direct_shape_of(N, n, K);
-    parts(p.fwd, n, N);
+    p.part = take(parts(p.fwd, n, N));
   } else {
     p.d = take((size_t)n * N * 2);
-    p.dx = direct_shape_of(K, n, N);
-    p.dw = direct_shape_of(K, N, n);
-    parts(p.dx, n, K), parts(p.dw, N, K);
+    back_shapes_of(n, K, N, N, n, 64, [](int size, double groups, int *bm, int *bn, int *places) {
+      *bm = *bn = size ? WideTile::BM : NarrowTile::BM;
+      *places = size || groups <= num_cus() ? 1 : 2;
+      return size ? (groups > num_cus() / 2 ? 24.5 : 19.5) : *places == 1 ? 9.0 : 14.0;
+    }, &p.dx, &p.dw);
+    p.part = take(parts(p.dx, n, K)), p.wpart = take(parts(p.dw, N, K));
     p.sums = take((size_t)tiles_of(n, 64) * N * 4);
   }
-  p.part = take(part);
   p.bytes = at;
   return p;
 }
+
+// Whether a forward pass reads W where it lies (few_rows_kernel) or goes by tiles.  ns a k of its workgroups, one a compute unit: bf16 1.0 + 0.05 a row of X,
+// fp32 3.0 + 0.04 and 0.0013 a row squared (8192 x 2048 with 1, 16, 32, 64 rows: 1.0 1.6 2.5 4.2, 3.2 3.7 5.6 10.8); tiles cost what their model says, and what packing W and X takes.  us of
+// few rows / of tiles: bf16 2048 x 8192 with 1 row 6.9 / 10.8, 16 9.5 / 11.7, 64 20 / 15.5; 8192 x 2048 with 16 16 / 13.4; 1000 x 1000 with 157 5.8 / 13.6, 512
+// 10.5 / 14.1; 512 x 2048 with 512 12.4 / 8.4; fp32 2048 x 8192 with 1 16 / 46, 32 29 / 48, 64 50 / 48; 300 x 777 with 157 7.1 / 12.3, 512 x 2048 with 256 15.5 / 17.7.
+bool few_rows(int type, int n, int K, int N, double tiles_us) {
+  const double rows = n < 64 ? n : 64, groups = (double)tiles_of(N, 16) * tiles_of(n, 64);
+  const double us = 2.5 + 1e-3 * K * (type == CAVS_F32 ? 3.0 + (0.04 + 0.0013 * rows) * rows : 1.0 + 0.05 * rows) * std::ceil(groups / num_cus());
+  return us < tiles_us;
+}
+template <int P>
+double packed_us(int n, int K, int N) { return 0.8 * (shape_of<P>(N, n, ceil_to(K, kPlaneAlign)).us + 4.5 + (double)K * ((double)n + N) * (P == 3 ? 10 : 4) / 7e6); }
+double direct_us(int n, int K, int N) { return direct_shape_of(N, n, K).us + 1.5; }
 
 struct Call {
   const void *X, *W, *R, *Z, *dY;
@@ -539,31 +775,44 @@ PackJob<T> packing(const void *src, int ld, int rows, int K, int orows, char *o,
 }
 
 template <class E>
+PartsJob<E> parts_of_product(const float *part, const Shape &s, int rows, int cols, const E &out) {
+  const long blocks = ((long)rows * ((cols + 7) / 8) + 255) / 256;
+  return PartsJob<E>{part, s.splits, rows, cols, out, s.splits > 1 ? (int)blocks : 0};
+}
+template <class E>
 int join_parts(const float *part, const Shape &s, int rows, int cols, const E &out, hipStream_t st) {
-  launch(parts_kernel<E>, (unsigned)(((long)rows * ((cols + 7) / 8) + 255) / 256), 256, 0, st, part, s.splits, rows, cols, out);
-  CAVS_LAUNCH_CHECK();
+  const PartsJob<E> g = parts_of_product(part, s, rows, cols, out);
+  if (g.blocks > 0) {
+    launch(parts_kernel<E>, (unsigned)g.blocks, 256, 0, st, g);
+    CAVS_LAUNCH_CHECK();
+  }
   return CAVS_OK;
 }
-template <int P, bool TA, bool TB, class E>
-int product(const Shape &s, const PackedRef &A, int cols, const PackedRef &B, int rows, int K, float *part, const E &out, hipStream_t st) {
-  Product<E> g{A, B, cols, rows, K, s.tm, s.tn, s.splits, s.kchunk, s.splits > 1 ? part : nullptr, out};
-  with_tile<P>(s.size, [&](auto t) {
-    using T = decltype(t);
-    launch(packed_product_kernel<T, TA, TB, E>, s.tm * s.tn * s.splits, T::THREADS, 0, st, g);
-    return 0;
-  });
-  CAVS_LAUNCH_CHECK();
-  return g.part ? join_parts(part, s, rows, cols, out, st) : (int)CAVS_OK;
+// what is wanted of both gradients, the longer workgroups first
+template <class Job>
+struct BackJobs {
+  Job j0, j1;
+  int blocks0, blocks, wfirst;
+};
+template <class Job>
+BackJobs<Job> back_jobs(const Job &x, const Shape &sx, bool wantx, const Job &w, const Shape &sw, bool wantw) {
+  const int bx = wantx ? sx.tm * sx.tn * sx.splits : 0, bw = wantw ? sw.tm * sw.tn * sw.splits : 0;
+  const bool wfirst = sw.kchunk > sx.kchunk;
+  return wfirst ? BackJobs<Job>{w, x, bw, bx + bw, 1} : BackJobs<Job>{x, w, bx, bx + bw, 0};
 }
-
-template <bool TA, bool TB, class E>
-int direct_product(const Shape &s, const DirectRef &A, int cols, const DirectRef &B, int rows, int K, float *part, const E &out, hipStream_t st) {
-  DirectJob<E> g{A, B, cols, rows, K, s.tm, s.tn, s.kchunk, s.splits > 1 ? part : nullptr, out};
-  const unsigned groups = (unsigned)(s.tm * s.tn * s.splits);
-  if (s.size) launch(direct_product_kernel<WideTile, TA, TB, E>, groups, WideTile::THREADS, 0, st, g);
-  else launch(direct_product_kernel<NarrowTile, TA, TB, E>, groups, NarrowTile::THREADS, 0, st, g);
-  CAVS_LAUNCH_CHECK();
-  return g.part ? join_parts(part, s, rows, cols, out, st) : (int)CAVS_OK;
+template <class T>
+int back_ends(const Call &c, const Plan &p, char *ws, int stretches, hipStream_t st) {
+  const Plain<T> ox{static_cast<T *>(c.dX), c.lddx}, ow{static_cast<T *>(c.dW), c.lddw};
+  PartsJob<Plain<T>> x = parts_of_product(reinterpret_cast<float *>(ws + p.part), p.dx, c.n, c.K, ox);
+  PartsJob<Plain<T>> w = parts_of_product(reinterpret_cast<float *>(ws + p.wpart), p.dw, c.N, c.K, ow);
+  if (!c.dX) x.blocks = 0;
+  if (!c.dW) w.blocks = 0;
+  const ColumnsJob b{reinterpret_cast<float *>(ws + p.sums), stretches, c.N, c.db, c.db ? (c.N + 63) / 64 : 0};
+  if (x.blocks + w.blocks + b.blocks > 0) {
+    launch(back_ends_kernel<Plain<T>>, (unsigned)(x.blocks + w.blocks + b.blocks), 256, 0, st, x, w, b);
+    CAVS_LAUNCH_CHECK();
+  }
+  return CAVS_OK;
 }
 
 // rows that begin on 16 bytes and are whole pieces of eight, in reach of 32 bits from the first of a tile
@@ -571,9 +820,15 @@ bool lies_well(const void *p, long ld, int w) { return aligned16(p) && ld % 8 ==
 
 int run_direct_fwd(const Call &c, char *ws, hipStream_t st) {
   const Plan p = direct_plan_of(c.n, c.K, c.N, 0);
+  float *part = reinterpret_cast<float *>(ws + p.part);
   const Forward<u16> out{c.b, c.act, c.m, static_cast<const u16 *>(c.R), c.ldr, static_cast<u16 *>(c.Zout), c.ldz, static_cast<u16 *>(c.Y), c.ldy};
-  return direct_product<false, false>(p.fwd, DirectRef{static_cast<const u16 *>(c.W), c.ldw}, c.N, DirectRef{static_cast<const u16 *>(c.X), c.ldx}, c.n, c.K,
-                                      reinterpret_cast<float *>(ws + p.part), out, st);
+  const DirectJob<Forward<u16>> g{{static_cast<const u16 *>(c.W), c.ldw}, {static_cast<const u16 *>(c.X), c.ldx}, c.N, c.n, c.K, p.fwd.tm, p.fwd.tn, p.fwd.kchunk,
+                                  p.fwd.splits > 1 ? part : nullptr, out};
+  const unsigned groups = (unsigned)(p.fwd.tm * p.fwd.tn * p.fwd.splits);
+  if (p.fwd.size) launch(direct_forward_kernel<WideTile, Forward<u16>>, groups, WideTile::THREADS, 0, st, g);
+  else launch(direct_forward_kernel<NarrowTile, Forward<u16>>, groups, NarrowTile::THREADS, 0, st, g);
+  CAVS_LAUNCH_CHECK();
+  return join_parts(part, p.fwd, c.n, c.N, out, st);
 }
 
 int run_direct_bwd(const Call &c, char *ws, hipStream_t st) {
@@ -587,18 +842,29 @@ int run_direct_bwd(const Call &c, char *ws, hipStream_t st) {
     launch(grad_rows_kernel, grid_of(g.blocks), 256, 0, st, g, made);
     CAVS_LAUNCH_CHECK();
   }
-  const DirectRef D{made ? made : g.dY, made ? (long)c.N : c.lddy}, X{static_cast<const u16 *>(c.X), c.ldx}, W{static_cast<const u16 *>(c.W), c.ldw};
-  float *part = reinterpret_cast<float *>(ws + p.part);
-  if (c.dX) {
-    if (const int rc = direct_product<true, false>(p.dx, W, c.K, D, c.n, c.N, part, Plain<u16>{static_cast<u16 *>(c.dX), c.lddx}, st)) return rc;
-  }
-  if (c.dW) {
-    if (const int rc = direct_product<true, true>(p.dw, X, c.K, D, c.N, c.n, part, Plain<u16>{static_cast<u16 *>(c.dW), c.lddw}, st)) return rc;
-  }
-  if (c.db) {
-    launch(column_sums_kernel, (c.N + 63) / 64, 256, 0, st, g.sums, tiles_of(c.n, 64), c.N, c.db);
+  if (c.dX || c.dW) {
+    typedef Plain<u16> E;
+    const DirectRef D{made ? made : g.dY, made ? (long)c.N : c.lddy}, X{static_cast<const u16 *>(c.X), c.ldx}, W{static_cast<const u16 *>(c.W), c.ldw};
+    float *xpart = reinterpret_cast<float *>(ws + p.part), *wpart = reinterpret_cast<float *>(ws + p.wpart);
+    const DirectJob<E> x{W, D, c.K, c.n, c.N, p.dx.tm, p.dx.tn, p.dx.kchunk, p.dx.splits > 1 ? xpart : nullptr, E{static_cast<u16 *>(c.dX), c.lddx}};
+    const DirectJob<E> w{X, D, c.K, c.N, c.n, p.dw.tm, p.dw.tn, p.dw.kchunk, p.dw.splits > 1 ? wpart : nullptr, E{static_cast<u16 *>(c.dW), c.lddw}};
+    const auto j = back_jobs(x, p.dx, c.dX, w, p.dw, c.dW);
+    if (p.dx.size) launch(direct_back_kernel<WideTile, E>, (unsigned)j.blocks, WideTile::THREADS, 0, st, j.j0, j.j1, j.blocks0, j.wfirst);
+    else launch(direct_back_kernel<NarrowTile, E>, (unsigned)j.blocks, NarrowTile::THREADS, 0, st, j.j0, j.j1, j.blocks0, j.wfirst);
     CAVS_LAUNCH_CHECK();
   }
+  return back_ends<u16>(c, p, ws, tiles_of(c.n, 64), st);
+}
+
+template <class T>
+int run_few(const Call &c, hipStream_t st) {
+  const Forward<T> out{c.b, c.act, c.m, static_cast<const T *>(c.R), c.ldr, static_cast<T *>(c.Zout), c.ldz, static_cast<T *>(c.Y), c.ldy};
+  const FewJob<T> g{static_cast<const T *>(c.X), static_cast<const T *>(c.W), c.ldx, c.ldw, c.n, c.K, c.N, ceil_to((c.K + kFewWaves - 1) / kFewWaves, 32), out};
+  const unsigned groups = (unsigned)tiles_of(c.N, 16);
+  if (c.n <= 16) launch(few_rows_kernel<T, 1>, groups, 64 * kFewWaves, 0, st, g);
+  else if (c.n <= 32) launch(few_rows_kernel<T, 2>, groups, 64 * kFewWaves, 0, st, g);
+  else launch(few_rows_kernel<T, 4>, dim3(groups, (unsigned)tiles_of(c.n, 64)), 64 * kFewWaves, 0, st, g);
+  CAVS_LAUNCH_CHECK();
   return CAVS_OK;
 }
 
@@ -608,8 +874,17 @@ int run_fwd(const Call &c, char *ws, hipStream_t st) {
   const PackJob<T> x = packing<P, T>(c.X, c.ldx, c.n, c.K, c.n, ws + p.x, p.Kp), w = packing<P, T>(c.W, c.ldw, c.N, c.K, c.N, ws + p.w, p.Kp);
   launch(pack_kernel<P, T>, grid_of((long)x.blocks + w.blocks), 256, 0, st, x, w);
   CAVS_LAUNCH_CHECK();
-  const Forward<T> out{c.b, c.act, c.m, static_cast<const T *>(c.R), c.ldr, static_cast<T *>(c.Zout), c.ldz, static_cast<T *>(c.Y), c.ldy};
-  return product<P, false, false>(p.fwd, PackedRef{w.o.p, p.Kp}, c.N, PackedRef{x.o.p, p.Kp}, c.n, p.Kp, reinterpret_cast<float *>(ws + p.part), out, st);
+  typedef Forward<T> E;
+  float *part = reinterpret_cast<float *>(ws + p.part);
+  const E out{c.b, c.act, c.m, static_cast<const T *>(c.R), c.ldr, static_cast<T *>(c.Zout), c.ldz, static_cast<T *>(c.Y), c.ldy};
+  const Product<E> g{{w.o.p, p.Kp}, {x.o.p, p.Kp}, c.N, c.n, p.Kp, p.fwd.tm, p.fwd.tn, p.fwd.kchunk, p.fwd.splits > 1 ? part : nullptr, out};
+  with_tile<P>(p.fwd.size, [&](auto t) {
+    using Tile = decltype(t);
+    launch(packed_forward_kernel<Tile, E>, (unsigned)(p.fwd.tm * p.fwd.tn * p.fwd.splits), Tile::THREADS, 0, st, g);
+    return 0;
+  });
+  CAVS_LAUNCH_CHECK();
+  return join_parts(part, p.fwd, c.n, c.N, out, st);
 }
 
 template <int P, class T>
@@ -618,28 +893,26 @@ int run_bwd(const Call &c, char *ws, hipStream_t st) {
   GradJob<T> g{static_cast<const T *>(c.dY), static_cast<const T *>(c.Z), c.lddy, c.ldz, c.act, c.m, c.n, c.N, p.np, p.Np / 64, 0,
                {c.dX || c.dW ? reinterpret_cast<u16 *>(ws + p.d) : nullptr, p.Np}, c.db ? reinterpret_cast<float *>(ws + p.sums) : nullptr};
   g.blocks = g.across * (p.np / 64);
-  launch(grad_kernel<P, T>, grid_of(g.blocks), 256, 0, st, g);
-  CAVS_LAUNCH_CHECK();
   PackJob<T> x = packing<P, T>(c.X, c.ldx, c.n, c.K, p.np, ws + p.x, p.Kp), w = packing<P, T>(c.W, c.ldw, c.N, c.K, p.Np, ws + p.w, p.Kp);
-  const PackedRef X{x.o.p, p.Kp}, W{w.o.p, p.Kp}, D{g.o.p, p.Np};
   if (!c.dW) x.blocks = 0;
   if (!c.dX) w.blocks = 0;
+  launch(grad_kernel<P, T>, grid_of((long)g.blocks + x.blocks + w.blocks), 256, 0, st, g, x, w);
+  CAVS_LAUNCH_CHECK();
   if (c.dX || c.dW) {
-    launch(pack_kernel<P, T>, grid_of((long)x.blocks + w.blocks), 256, 0, st, x, w);
+    typedef Plain<T> E;
+    const PackedRef X{x.o.p, p.Kp}, W{w.o.p, p.Kp}, D{g.o.p, p.Np};
+    float *xpart = reinterpret_cast<float *>(ws + p.part), *wpart = reinterpret_cast<float *>(ws + p.wpart);
+    const Product<E> jx{W, D, c.K, c.n, p.Np, p.dx.tm, p.dx.tn, p.dx.kchunk, p.dx.splits > 1 ? xpart : nullptr, E{static_cast<T *>(c.dX), c.lddx}};
+    const Product<E> jw{X, D, c.K, c.N, p.np, p.dw.tm, p.dw.tn, p.dw.kchunk, p.dw.splits > 1 ? wpart : nullptr, E{static_cast<T *>(c.dW), c.lddw}};
+    const auto j = back_jobs(jx, p.dx, c.dX, jw, p.dw, c.dW);
+    with_tile<P>(p.dx.size, [&](auto t) {
+      using Tile = decltype(t);
+      launch(packed_back_kernel<Tile, E>, (unsigned)j.blocks, Tile::THREADS, 0, st, j.j0, j.j1, j.blocks0, j.wfirst);
+      return 0;
+    });
     CAVS_LAUNCH_CHECK();
   }
-  float *part = reinterpret_cast<float *>(ws + p.part);
-  if (c.dX) {
-    if (const int rc = product<P, true, false>(p.dx, W, c.K, D, c.n, p.Np, part, Plain<T>{static_cast<T *>(c.dX), c.lddx}, st)) return rc;
-  }
-  if (c.dW) {
-    if (const int rc = product<P, true, true>(p.dw, X, c.K, D, c.N, p.np, part, Plain<T>{static_cast<T *>(c.dW), c.lddw}, st)) return rc;
-  }
-  if (c.db) {
-    launch(column_sums_kernel, (c.N + 63) / 64, 256, 0, st, g.sums, p.np / 64, c.N, c.db);
-    CAVS_LAUNCH_CHECK();
-  }
-  return CAVS_OK;
+  return back_ends<T>(c, p, ws, p.np / 64, st);
 }
 
 template <class T>
@@ -679,9 +952,17 @@ extern "C" {
 
 size_t cavs_linear_workspace(int type, int n, int K, int N, int back) {
   if (n <= 0 || K <= 0 || N <= 0 || !shape_ok(n, K, N) || (type != CAVS_F32 && type != CAVS_BF16)) return 0;
-  if (type == CAVS_F32) return plan_of<3>(n, K, N, back).bytes;
-  const size_t packed = plan_of<1>(n, K, N, back).bytes, direct = K % 8 == 0 && (!back || N % 8 == 0) ? direct_plan_of(n, K, N, back).bytes : 0;
-  return packed > direct ? packed : direct;
+  size_t need = 256;  // (of few rows nothing is used)
+  if (type == CAVS_F32) {
+    if (back || !few_rows(type, n, K, N, packed_us<3>(n, K, N))) need = plan_of<3>(n, K, N, back).bytes;
+    return need;
+  }
+  if (back || !few_rows(type, n, K, N, packed_us<1>(n, K, N))) need = plan_of<1>(n, K, N, back).bytes;
+  if (K % 8 == 0 && (back ? N % 8 == 0 : !few_rows(type, n, K, N, direct_us(n, K, N)))) {
+    const size_t direct = direct_plan_of(n, K, N, back).bytes;
+    need = need > direct ? need : direct;
+  }
+  return need;
 }
 
 int cavs_linear_fwd(int type, const void *X, int ldx, const void *W, int ldw, const float *b, int act, const cavs_dropout_mask *mask, const void *R, int ldr,
@@ -695,8 +976,11 @@ int cavs_linear_fwd(int type, const void *X, int ldx, const void *W, int ldw, co
   CAVS_REQUIRE(X && W && Y, "%s: null pointer", who);
   if (const int rc = check_workspace(who, workspace, workspace_bytes, cavs_linear_workspace(type, n, K, N, 0))) return rc;
   char *w = static_cast<char *>(workspace);
-  if (type == CAVS_F32) return run_fwd<3, float>(c, w, as_stream(stream));
-  return lies_well(X, ldx, K) && lies_well(W, ldw, K) ? run_direct_fwd(c, w, as_stream(stream)) : run_fwd<1, u16>(c, w, as_stream(stream));
+  hipStream_t st = as_stream(stream);
+  if (type == CAVS_F32) return few_rows(type, n, K, N, packed_us<3>(n, K, N)) ? run_few<float>(c, st) : run_fwd<3, float>(c, w, st);
+  const bool direct = lies_well(X, ldx, K) && lies_well(W, ldw, K);
+  if (few_rows(type, n, K, N, direct ? direct_us(n, K, N) : packed_us<1>(n, K, N))) return run_few<u16>(c, st);
+  return direct ? run_direct_fwd(c, w, st) : run_fwd<1, u16>(c, w, st);
 }
 
 int cavs_linear_bwd(int type, const void *X, int ldx, const void *W, int ldw, const void *Z, int ldz, int act, const cavs_dropout_mask *mask, const void *dY,

@@ -591,7 +591,7 @@ struct Shape {  // of a product
 template <int P> struct Speeds;
 template <> struct Speeds<3> { static constexpr double ns[2][3] = {{26, 26, 29}, {68, 73, 98}}; };
 template <> struct Speeds<1> { static constexpr double ns[2][3] = {{6, 6.5, 8}, {14, 15, 20}}; };
-constexpr int kStretches[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+constexpr int kStretches[] = {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32};
 template <int P>
 Shape shape_of(int cols, int rows, int K) {
   Shape best{};
@@ -643,18 +643,22 @@ Shape direct_shape_of(int cols, int rows, int K) {
   return best;
 }
 
-// Both gradients in a launch: the same tile, and for each the stretches that bring the longest workgroup and what there is a workgroup's place to the least. `price`:
-// ns a k of a place, and how many a compute unit has, of so many workgroups.
+// Both gradients in a launch: the same tile, and for each the stretches that a model finds best: what there is to multiply at the measured speed of as many
+// workgroups as a compute unit has, or the longest workgroup by itself; where not all have a place at once, a third of a round for the last; parts as above.
+// us of a call with all workgroups whole / in the stretches this finds, and with the products in launches of their own: fp32 7088 x 512 x 2048 266 / 190, 240;
+// 4096 x 1024 x 1024 148 / 120; bf16 2048 x 1024 x 4096 53 / 47; 8192 x 512 x 2048 87 / 47; 512 x 2048 x 2048 30 / 24.
+struct Places {  // of a compute unit for workgroups of a tile, ns a k of one where all are taken and of the longest
+  int bm, bn, places;
+  double ns, longest;
+};
 template <class Price>
 void back_shapes_of(int n, int K, int N, int Kx, int Kw, int align, const Price &price, Shape *dx, Shape *dw) {
   double least = INFINITY;
-  const int cus = num_cus();
   for (int size = 0; size < 2; size++) {
-    int bm, bn, places;
-    price(size, 1, &bm, &bn, &places);
+    const Places any = price(size, 1.);
     Shape x{}, w{};
     x.size = w.size = size;
-    x.tm = w.tm = tiles_of(K, bm), x.tn = tiles_of(n, bn), w.tn = tiles_of(N, bn);
+    x.tm = w.tm = tiles_of(K, any.bm), x.tn = tiles_of(n, any.bn), w.tn = tiles_of(N, any.bn);
     auto set = [&](Shape &s, int of, int splits) {
       s.kchunk = ceil_to((of + splits - 1) / splits, align);
       s.splits = (of + s.kchunk - 1) / s.kchunk;
@@ -666,9 +670,9 @@ void back_shapes_of(int n, int K, int N, int Kx, int Kw, int align, const Price 
         if (sw > 1 && Kw / sw < 256) break;
         set(w, Kw, sw);
         const double gx = (double)x.tm * x.tn * x.splits, gw = (double)w.tm * w.tn * w.splits, kx = x.kchunk + 200., kw = w.kchunk + 200.;
-        const double ns = price(size, gx + gw, &bm, &bn, &places), longest = kx > kw ? kx : kw, shortest = kx > kw ? kw : kx;
-        const double even = (gx * kx + gw * kw) / ((double)places * cus) + 0.35 * shortest;
-        double us = 1e-3 * ns * (longest > even ? longest : even);
+        const Places at = price(size, gx + gw);
+        const double all = (double)at.places * num_cus(), even = at.ns * ((gx * kx + gw * kw) / all + (gx + gw > all ? 0.35 * std::fmin(kx, kw) : 0.));
+        double us = 1e-3 * std::fmax(even, at.longest * std::fmax(kx, kw));
         if (x.splits > 1) us += x.splits * (8. * n * K) / 4.7e6;
         if (w.splits > 1) us += w.splits * (8. * N * K) / 4.7e6;
         if (x.splits > 1 || w.splits > 1) us += 5.;
@@ -701,10 +705,12 @@ Plan plan_of(int n, int K, int N, int back) {
     p.part = take(parts(p.fwd, n, N));
   } else {
     p.d = take(packed_bytes<P>(p.np, p.Np));
-    back_shapes_of(n, K, N, p.Np, p.np, kPlaneAlign, [](int size, double groups, int *bm, int *bn, int *places) {
-      with_tile<P>(size, [&](auto t) { return *bm = decltype(t)::BM, *bn = decltype(t)::BN, 0; });
-      *places = groups <= num_cus() ? 1 : groups <= 2 * num_cus() ? 2 : 3;
-      return Speeds<P>::ns[size][*places - 1];
+    back_shapes_of(n, K, N, p.Np, p.np, kPlaneAlign, [](int size, double groups) {
+      Places at{};
+      with_tile<P>(size, [&](auto t) { return at.bm = decltype(t)::BM, at.bn = decltype(t)::BN, 0; });
+      at.places = groups <= num_cus() ? 1 : groups <= 2 * num_cus() ? 2 : 3;
+      at.ns = Speeds<P>::ns[size][at.places - 1], at.longest = Speeds<P>::ns[size][0];
+      return at;
     }, &p.dx, &p.dw);
     p.part = take(parts(p.dx, n, K)), p.wpart = take(parts(p.dw, N, K));
     p.sums = take((size_t)(p.np / 64) * N * 4);
@@ -726,10 +732,10 @@ Plan direct_plan_of(int n, int K, int N, int back) {
     p.part = take(parts(p.fwd, n, N));
   } else {
     p.d = take((size_t)n * N * 2);
-    back_shapes_of(n, K, N, N, n, 64, [](int size, double groups, int *bm, int *bn, int *places) {
-      *bm = *bn = size ? WideTile::BM : NarrowTile::BM;
-      *places = size || groups <= num_cus() ? 1 : 2;
-      return size ? (groups > num_cus() / 2 ? 24.5 : 19.5) : *places == 1 ? 9.0 : 14.0;
+    back_shapes_of(n, K, N, N, n, 64, [](int size, double groups) {
+      if (size) return Places{WideTile::BM, WideTile::BN, 1, groups > num_cus() / 2 ? 24.5 : 19.5, groups > num_cus() / 2 ? 24.5 : 19.5};
+      const int places = groups <= num_cus() ? 1 : 2;
+      return Places{NarrowTile::BM, NarrowTile::BN, places, places == 1 ? 9. : 14., places == 1 ? 9. : 14.};
     }, &p.dx, &p.dw);
     p.part = take(parts(p.dx, n, K)), p.wpart = take(parts(p.dw, N, K));
     p.sums = take((size_t)tiles_of(n, 64) * N * 4);

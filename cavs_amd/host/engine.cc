@@ -58,6 +58,8 @@ Engine::Engine(const cavs_session_config &cfg, void *external_stream, std::share
   if (cfg.optimizer && cell_) fail(CAVS_EINVAL, "the optimizer of orthogonalised updates goes with the built-in models");
   if (!(cfg.ortho_lr >= 0.f) || !(cfg.ortho_momentum < 1.f) || !(cfg.ortho_decay >= 0.f))
     fail(CAVS_EINVAL, "ortho_lr and ortho_decay are not negative, ortho_momentum is below 1");
+  if (!(cfg.dropout >= 0.f && cfg.dropout < 1.f) || (cfg.dropout > 0.f && cfg.loss != CAVS_LOSS_SOFTMAX))
+    fail(CAVS_EINVAL, "dropout is in [0, 1), and goes with the softmax loss");
   check(cavs_init(cfg.device));
   if (external_stream)
     stream_ = external_stream;
@@ -109,6 +111,10 @@ Engine::Engine(const cavs_session_config &cfg, void *external_stream, std::share
     add_param("bfc", cfg.C);
   }
   if (cfg_.optimizer == CAVS_OPTIMIZER_ORTHO) ortho_setup();
+  if (cfg_.dropout > 0.f) {
+    drop_step_.reserve(1);
+    check(cavs_zero(drop_step_.get(), sizeof(unsigned long long), stream_));
+  }
   tail_setup();
 }
 
@@ -687,6 +693,7 @@ void Engine::reserve_edges() {
   R(GO_, cap * H);
   if (ensure(dGO_, cap * H) && uH_ != cfg_.H) check(cavs_zero(dGO_.get(), cap * H * 4, stream_));
   R(dret_, cap * H);
+  if (cfg_.dropout > 0.f) R(dropped_, cap * H);
   R(G_, cap * nch_ * mw);
   R(r_dmsg_, rc * mw);
   R(r_dG_, rc * nch_ * mw);
@@ -1377,7 +1384,17 @@ void Engine::run_passes(bool backward) {
   pop_ret(GO_.get());
   if (!capturing_) mark_point(1);
   ev_valid_ = !capturing_;
+  const bool drops = backward && cfg_.dropout > 0.f;
+  // (the columns that padding adds are zeros, dropped or not)
+  const cavs_dropout_mask mask{cfg_.dropout, cfg_.dropout_seed, 0, drop_step_.get(), nullptr};
+  head_in_ = drops ? dropped_.get() : GO_.get();
+  if (drops) check(cavs_dropout(CAVS_F32, dropped_.get(), cfg_.H, GO_.get(), cfg_.H, nullptr, 0, N_, cfg_.H, &mask, stream_));
   head_forward_backward(backward);
+  if (drops) {
+    check(cavs_dropout(CAVS_F32, dGO_.get(), cfg_.H, dGO_.get(), cfg_.H, nullptr, 0, N_, cfg_.H, &mask, stream_));
+    check(cavs_dropout_advance(drop_step_.get(), 1, stream_));
+    c_launches_ += 3;
+  }
   d_dgo_ = dGO_.get();
   did_backward_ = backward;
   ev_bwd_valid_ = false;
@@ -2818,10 +2835,10 @@ void Engine::head_forward_backward(bool backward) {
       ensure(head_ws_, grow(bytes / 4 + 1, head_ws_.capacity()));
       ProfScope ps(this, K_GEMM);
       if (backward)
-        check(cavs_vocab_xent(CAVS_F32, GO_.get(), H, Wfc.w, H, bfc.w, d_labels_, nullptr, 1.f / N, loss_.get(), nullptr, dGO_.get(), H, Wfc.g, H, bfc.g, N, H, C,
+        check(cavs_vocab_xent(CAVS_F32, head_in_, H, Wfc.w, H, bfc.w, d_labels_, nullptr, 1.f / N, loss_.get(), nullptr, dGO_.get(), H, Wfc.g, H, bfc.g, N, H, C,
                               head_ws_.get(), bytes, stream_));
       else
-        check(cavs_vocab_xent_fwd(CAVS_F32, GO_.get(), H, Wfc.w, H, bfc.w, d_labels_, loss_.get(), nullptr, N, H, C, head_ws_.get(), bytes, stream_));
+        check(cavs_vocab_xent_fwd(CAVS_F32, head_in_, H, Wfc.w, H, bfc.w, d_labels_, loss_.get(), nullptr, N, H, C, head_ws_.get(), bytes, stream_));
       c_gemm_flops_ += (backward ? 6.0 : 2.0) * N * C * H;  // (what the head is asked for; z may be made twice)
       c_launches_ += 1;
       return;
@@ -2834,7 +2851,7 @@ void Engine::head_forward_backward(bool backward) {
         head_parts_.reserve(head_bytes / 4 + 1);
       }
       last_launch(2, backward, [&] {
-        check(cavs_fc_softmax_xent(GO_.get(), Wfc.w, bfc.w, d_labels_, loss_.get(), logits_.get(), backward ? dGO_.get() : nullptr,
+        check(cavs_fc_softmax_xent(head_in_, Wfc.w, bfc.w, d_labels_, loss_.get(), logits_.get(), backward ? dGO_.get() : nullptr,
                                    nullptr, nullptr, head_parts_.get(), head_bytes, N, H, C, stream_));
       });
       if (backward)
@@ -2854,9 +2871,9 @@ void Engine::head_forward_backward(bool backward) {
       float *ws = workspace(cavs_sgemm_splitk_workspace(N, C, H));
       ProfScope ps(this, K_GEMM);
       if (wide)
-        check(cavs_sgemm_addrows(0, 0, N, C, H, GO_.get(), H, WfcT_.get(), C, bfc.w, C, 30, logits_.get(), C, ws, ws_.capacity() * 4, stream_));
+        check(cavs_sgemm_addrows(0, 0, N, C, H, head_in_, H, WfcT_.get(), C, bfc.w, C, 30, logits_.get(), C, ws, ws_.capacity() * 4, stream_));
       else
-        check(cavs_sgemm_addrows(0, 1, N, C, H, GO_.get(), H, Wfc.w, H, bfc.w, C, 30, logits_.get(), C, ws, ws_.capacity() * 4, stream_));
+        check(cavs_sgemm_addrows(0, 1, N, C, H, head_in_, H, Wfc.w, H, bfc.w, C, 30, logits_.get(), C, ws, ws_.capacity() * 4, stream_));
       c_gemm_flops_ += 2.0 * N * C * H;
       c_launches_ += 1;
     }
@@ -2872,7 +2889,7 @@ void Engine::head_forward_backward(bool backward) {
     const int biased_rows = sum_rows > 0 ? sum_rows : N;
     c_launches_ += 1;
     if (backward) {
-      const cavs_gemm_desc dWd{1, 0, C, H, N, 1.f, 0.f, dlogits_.get(), C, GO_.get(), H, Wfc.g, H};
+      const cavs_gemm_desc dWd{1, 0, C, H, N, 1.f, 0.f, dlogits_.get(), C, head_in_, H, Wfc.g, H};
       const cavs_gemm_desc dGd = wide ? cavs_gemm_desc{0, 1, N, H, C, 1.f, 0.f, dlogits_.get(), C, WfcT_.get(), C, dGO_.get(), H}
                                       : cavs_gemm_desc{0, 0, N, H, C, 1.f, 0.f, dlogits_.get(), C, Wfc.w, H, dGO_.get(), H};
       // (not in a session that records graphs: on this runtime a capture on the session's stream comes
@@ -2981,7 +2998,7 @@ void Engine::plan_head_chunks(const int *orphans_host) {
   head_chunks_.clear();
   const Schedule &s = *sched_;
   const int R = (int)s.rounds.size(), N = s.N;
-  if (vocab_head() || cfg_.head_chunks < 0 || cfg_.model != CAVS_MODEL_LSTM || !wide_head() || !s.batching || !forest_ || cfg_.graph_replay || R < 8 ||
+  if (vocab_head() || cfg_.dropout > 0.f || cfg_.head_chunks < 0 || cfg_.model != CAVS_MODEL_LSTM || !wide_head() || !s.batching || !forest_ || cfg_.graph_replay || R < 8 ||
       N < 256)
     return;
   // Where the rounds are one launch per direction, chunks cost more than they cover: the backward rounds become

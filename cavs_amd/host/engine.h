@@ -230,6 +230,9 @@ class Engine {
   };
   std::vector<OrthoBlock> ortho_;  // the blocks of "W" and "U" the optimizer takes as matrices
   DeviceArray<float> ortho_ws_, head_ws_;
+  DeviceArray<float> dropped_;  // what the head reads in a step that drops
+  DeviceArray<unsigned long long> drop_step_;
+  const float *head_in_ = nullptr;
 
   std::shared_ptr<Schedule> sched_ = std::make_shared<Schedule>();
   std::shared_ptr<Schedule> spare_[3];

@@ -25,7 +25,7 @@ class _Config(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("model", "loss", "pairing", "opt", "V", "E", "H", "C", "act",
                                       "use_bias", "use_x", "device", "fused_round_rows", "split_backward_rounds",
                                       "schedule_mode", "plan_cache", "tail_rows", "graph_replay", "head_chunks", "vocab_head", "optimizer")] + \
-        [(n, C.c_float) for n in ("ortho_lr", "ortho_momentum", "ortho_decay")]
+        [(n, C.c_float) for n in ("ortho_lr", "ortho_momentum", "ortho_decay", "dropout")] + [("dropout_seed", C.c_uint)]
 
 
 _lib = None
@@ -201,18 +201,22 @@ class Session:
     memory from tens of thousands of classes on; below that the head with logits is as small and a little faster.
     optimizer: "sgd", or "ortho": "W" and "U" by their orthogonalised momentum, block by block, the rest by SGD.  Its state
     is the parameter "W.momentum" / "U.momentum" (`param`, `set_params`); ortho_lr 0 is step's lr, ortho_momentum 0 is 0.95,
-    negative none."""
+    negative none.
+    dropout: the share of what the vertices push that is dropped before the softmax head in steps with a backward pass, drawn from
+    dropout_seed, the number of such steps before this one, the vertex and the column (`cavs_dropout`)."""
 
     def __init__(self, model, *, H, E=0, V=0, C_=0, loss="softmax", pairing="reference",
                  opt=OPT_BATCHING, act=0, use_bias=False, use_x=False, device=0, fused_round_rows=0,
                  split_backward_rounds=False, schedule="host", plan_cache=0, tail_rows=0, graph_replay=False, head_chunks=0,
-                 vocab_head=False, optimizer="sgd", ortho_lr=0.0, ortho_momentum=0.0, ortho_decay=0.0):
+                 vocab_head=False, optimizer="sgd", ortho_lr=0.0, ortho_momentum=0.0, ortho_decay=0.0,
+                 dropout=0.0, dropout_seed=0):
         self.model, self.H, self.E, self.V, self.C, self.loss = model, H, (H if model == "lstm" else E), V, C_, loss
         self.mw = H if model == "treefc" else 2 * H
         cfg = _Config(MODEL[model], LOSS[loss], PAIR[pairing], opt, V, E, H, C_, int(act), int(use_bias),
                       int(use_x), device, int(fused_round_rows), int(split_backward_rounds),
                       {"host": 0, "device": 1}[schedule], int(plan_cache), int(tail_rows), int(graph_replay), int(head_chunks),
-                      int(vocab_head), OPTIMIZER[optimizer], float(ortho_lr), float(ortho_momentum), float(ortho_decay))
+                      int(vocab_head), OPTIMIZER[optimizer], float(ortho_lr), float(ortho_momentum), float(ortho_decay),
+                      float(dropout), int(dropout_seed) & 0xFFFFFFFF)
         self._h = C.c_void_p()
         _check(lib().cavs_session_create(C.byref(cfg), C.byref(self._h)), "cavs_session_create")
         self._keep = None

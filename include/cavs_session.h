@@ -112,6 +112,11 @@ typedef struct {
   float ortho_lr;       /* step size of the orthogonalised updates; 0 = cavs_session_step's lr */
   float ortho_momentum; /* 0 = 0.95, negative = none */
   float ortho_decay;    /* weight decay */
+  /* Softmax loss: the share of what the vertices push that is dropped before the head in steps with a backward pass (cavs_dropout; vertex i, declared column j, p = dropout,
+   * seed = dropout_seed, step = the session's steps with a backward pass before this one).  0 = none, below 1.  "graph_out" is what was pushed, "dgraph_out" its gradient; steps
+   * without a backward pass drop nothing.  The head runs in one piece then (head_chunks). */
+  float dropout;
+  unsigned dropout_seed;
 } cavs_session_config;
 enum { CAVS_OPTIMIZER_SGD = 0, CAVS_OPTIMIZER_ORTHO = 1 };
 

@@ -60,6 +60,8 @@ Engine::Engine(const cavs_session_config &cfg, void *external_stream, std::share
     fail(CAVS_EINVAL, "ortho_lr and ortho_decay are not negative, ortho_momentum is below 1");
   if (!(cfg.dropout >= 0.f && cfg.dropout < 1.f) || (cfg.dropout > 0.f && cfg.loss != CAVS_LOSS_SOFTMAX))
     fail(CAVS_EINVAL, "dropout is in [0, 1), and goes with the softmax loss");
+  if (cfg.block < 0 || cfg.block > 65536 || cfg.block_act < 0 || cfg.block_act > CAVS_ACT_GELU || (cfg.block > 0 && (cfg.loss != CAVS_LOSS_SOFTMAX || cfg.H > 16384)))
+    fail(CAVS_EINVAL, "block is 0 .. 65536, of at most 16384 hidden units, and goes with the softmax loss; block_act is one of CAVS_ACT_*");
   check(cavs_init(cfg.device));
   if (external_stream)
     stream_ = external_stream;
@@ -109,6 +111,13 @@ Engine::Engine(const cavs_session_config &cfg, void *external_stream, std::share
   if (cfg.loss == CAVS_LOSS_SOFTMAX) {
     add_param("Wfc", (size_t)cfg.C * H, 0, rows(cfg.C, h, H));
     add_param("bfc", cfg.C);
+  }
+  if (const size_t F = cfg.block) {  // (as declared: its operators take rows of any width)
+    add_param("gnorm", h);
+    add_param("Wup", F * h);
+    add_param("bup", F);
+    add_param("Wdown", h * F);
+    add_param("bdown", h);
   }
   if (cfg_.optimizer == CAVS_OPTIMIZER_ORTHO) ortho_setup();
   if (cfg_.dropout > 0.f) {
@@ -693,7 +702,17 @@ void Engine::reserve_edges() {
   R(GO_, cap * H);
   if (ensure(dGO_, cap * H) && uH_ != cfg_.H) check(cavs_zero(dGO_.get(), cap * H * 4, stream_));
   R(dret_, cap * H);
-  if (cfg_.dropout > 0.f) R(dropped_, cap * H);
+  if (cfg_.block > 0) {
+    const size_t h = uH_, F = cfg_.block;
+    R(block_x_, cap * h);
+    R(block_z_, cap * F);
+    R(block_a_, cap * F);
+    R(block_da_, cap * F);
+    R(dhead_, cap * H);
+    if (ensure(head_x_, cap * H) && uH_ != cfg_.H) check(cavs_zero(head_x_.get(), cap * H * 4, stream_));
+  } else if (cfg_.dropout > 0.f) {
+    R(head_x_, cap * H);
+  }
   R(G_, cap * nch_ * mw);
   R(r_dmsg_, rc * mw);
   R(r_dG_, rc * nch_ * mw);
@@ -1384,17 +1403,9 @@ void Engine::run_passes(bool backward) {
   pop_ret(GO_.get());
   if (!capturing_) mark_point(1);
   ev_valid_ = !capturing_;
-  const bool drops = backward && cfg_.dropout > 0.f;
-  // (the columns that padding adds are zeros, dropped or not)
-  const cavs_dropout_mask mask{cfg_.dropout, cfg_.dropout_seed, 0, drop_step_.get(), nullptr};
-  head_in_ = drops ? dropped_.get() : GO_.get();
-  if (drops) check(cavs_dropout(CAVS_F32, dropped_.get(), cfg_.H, GO_.get(), cfg_.H, nullptr, 0, N_, cfg_.H, &mask, stream_));
+  before_head(backward);
   head_forward_backward(backward);
-  if (drops) {
-    check(cavs_dropout(CAVS_F32, dGO_.get(), cfg_.H, dGO_.get(), cfg_.H, nullptr, 0, N_, cfg_.H, &mask, stream_));
-    check(cavs_dropout_advance(drop_step_.get(), 1, stream_));
-    c_launches_ += 3;
-  }
+  if (backward) behind_head();
   d_dgo_ = dGO_.get();
   did_backward_ = backward;
   ev_bwd_valid_ = false;
@@ -2820,6 +2831,80 @@ void Engine::embedding_backward_rows() {
 }
 
 // ------------------------------------------------------------------ loss head
+// p of a step's dropout at one of the places that drop: 0 before the head, 1 and 2 in the block
+cavs_dropout_mask Engine::dropout_mask(unsigned long long place) const {
+  return {cfg_.dropout, cfg_.dropout_seed + (place << 32), 0, drop_step_.get(), nullptr};
+}
+
+// From what the vertices push to what the head reads.  (The columns that padding adds are zeros, and stay so.)
+void Engine::before_head(bool backward) {
+  const int N = N_, H = cfg_.H, h = uH_, F = cfg_.block;
+  const bool drops = backward && cfg_.dropout > 0.f;
+  head_in_ = GO_.get(), dhead_in_ = dGO_.get();
+  if (F > 0) {
+    size_t bytes = std::max(cavs_linear_workspace(CAVS_F32, N, h, F, 0), cavs_linear_workspace(CAVS_F32, N, F, h, 0));
+    if (backward)
+      bytes = std::max({bytes, cavs_linear_workspace(CAVS_F32, N, h, F, 1), cavs_linear_workspace(CAVS_F32, N, F, h, 1), cavs_norm_residual_workspace(N, h)});
+    ensure(block_ws_, grow(bytes / 4 + 1, block_ws_.capacity()));
+    const cavs_dropout_mask in = dropout_mask(1), out = dropout_mask(2);
+    const cavs_norm_desc norm = block_norm();
+    check(cavs_norm_residual_fwd(CAVS_F32, &norm, nullptr, 0, block_x_.get(), h, stream_));
+    ProfScope ps(this, K_GEMM);
+    check(cavs_linear_fwd(CAVS_F32, block_x_.get(), h, param("Wup").w, h, param("bup").w, cfg_.block_act, drops ? &in : nullptr, nullptr, 0, block_z_.get(), F,
+                          block_a_.get(), F, N, h, F, block_ws_.get(), block_ws_.capacity() * 4, stream_));
+    check(cavs_linear_fwd(CAVS_F32, block_a_.get(), F, param("Wdown").w, F, param("bdown").w, CAVS_ACT_NONE, drops ? &out : nullptr, GO_.get(), H, nullptr, 0,
+                          head_x_.get(), H, N, F, h, block_ws_.get(), block_ws_.capacity() * 4, stream_));
+    c_gemm_flops_ += 4.0 * N * h * F;
+    c_launches_ += 3;
+    head_in_ = head_x_.get(), dhead_in_ = dhead_.get();
+  } else if (drops) {
+    const cavs_dropout_mask mask = dropout_mask(0);
+    check(cavs_dropout(CAVS_F32, head_x_.get(), H, GO_.get(), H, nullptr, 0, N, H, &mask, stream_));
+    c_launches_ += 1;
+    head_in_ = head_x_.get();
+  }
+}
+
+cavs_norm_desc Engine::block_norm() {
+  cavs_norm_desc d{};
+  d.n = N_, d.w = uH_;
+  d.y = GO_.get(), d.ldy = cfg_.H;
+  d.scale = 1.f, d.eps = 1e-6f;
+  d.pre = CAVS_NORM_RMS, d.pre_w = param("gnorm").w;
+  return d;
+}
+
+// and the gradients back
+void Engine::behind_head() {
+  const int N = N_, H = cfg_.H, h = uH_, F = cfg_.block;
+  const bool drops = cfg_.dropout > 0.f;
+  if (F > 0) {
+    const cavs_dropout_mask in = dropout_mask(1), out = dropout_mask(2);
+    const cavs_norm_desc norm = block_norm();
+    {
+      ProfScope ps(this, K_GEMM);
+      check(cavs_linear_bwd(CAVS_F32, block_a_.get(), F, param("Wdown").w, F, nullptr, 0, CAVS_ACT_NONE, drops ? &out : nullptr, dhead_.get(), H, block_da_.get(), F,
+                            param("Wdown").g, F, param("bdown").g, N, F, h, block_ws_.get(), block_ws_.capacity() * 4, stream_));
+      check(cavs_linear_bwd(CAVS_F32, block_x_.get(), h, param("Wup").w, h, block_z_.get(), F, cfg_.block_act, drops ? &in : nullptr, block_da_.get(), F, dGO_.get(), H,
+                            param("Wup").g, h, param("bup").g, N, h, F, block_ws_.get(), block_ws_.capacity() * 4, stream_));
+    }
+    cavs_norm_grads g{};
+    g.dr = dGO_.get(), g.lddr = H;
+    g.dpre_w = param("gnorm").g;
+    check(cavs_norm_residual_bwd(CAVS_F32, &norm, GO_.get(), H, dhead_.get(), H, dGO_.get(), H, &g, block_ws_.get(), block_ws_.capacity() * 4, stream_));
+    c_gemm_flops_ += 8.0 * N * h * F;
+    c_launches_ += 3;
+  } else if (drops) {
+    const cavs_dropout_mask mask = dropout_mask(0);
+    check(cavs_dropout(CAVS_F32, dGO_.get(), H, dGO_.get(), H, nullptr, 0, N, H, &mask, stream_));
+    c_launches_ += 1;
+  }
+  if (drops) {
+    check(cavs_dropout_advance(drop_step_.get(), 1, stream_));
+    c_launches_ += 1;
+  }
+}
+
 void Engine::head_forward_backward(bool backward) {
   const int N = N_, H = cfg_.H, C = cfg_.C, B = sched_->B;
   if (head_chunked_) {
@@ -2835,7 +2920,7 @@ void Engine::head_forward_backward(bool backward) {
       ensure(head_ws_, grow(bytes / 4 + 1, head_ws_.capacity()));
       ProfScope ps(this, K_GEMM);
       if (backward)
-        check(cavs_vocab_xent(CAVS_F32, head_in_, H, Wfc.w, H, bfc.w, d_labels_, nullptr, 1.f / N, loss_.get(), nullptr, dGO_.get(), H, Wfc.g, H, bfc.g, N, H, C,
+        check(cavs_vocab_xent(CAVS_F32, head_in_, H, Wfc.w, H, bfc.w, d_labels_, nullptr, 1.f / N, loss_.get(), nullptr, dhead_in_, H, Wfc.g, H, bfc.g, N, H, C,
                               head_ws_.get(), bytes, stream_));
       else
         check(cavs_vocab_xent_fwd(CAVS_F32, head_in_, H, Wfc.w, H, bfc.w, d_labels_, loss_.get(), nullptr, N, H, C, head_ws_.get(), bytes, stream_));
@@ -2851,7 +2936,7 @@ void Engine::head_forward_backward(bool backward) {
         head_parts_.reserve(head_bytes / 4 + 1);
       }
       last_launch(2, backward, [&] {
-        check(cavs_fc_softmax_xent(head_in_, Wfc.w, bfc.w, d_labels_, loss_.get(), logits_.get(), backward ? dGO_.get() : nullptr,
+        check(cavs_fc_softmax_xent(head_in_, Wfc.w, bfc.w, d_labels_, loss_.get(), logits_.get(), backward ? dhead_in_ : nullptr,
                                    nullptr, nullptr, head_parts_.get(), head_bytes, N, H, C, stream_));
       });
       if (backward)
@@ -2890,8 +2975,8 @@ void Engine::head_forward_backward(bool backward) {
     c_launches_ += 1;
     if (backward) {
       const cavs_gemm_desc dWd{1, 0, C, H, N, 1.f, 0.f, dlogits_.get(), C, head_in_, H, Wfc.g, H};
-      const cavs_gemm_desc dGd = wide ? cavs_gemm_desc{0, 1, N, H, C, 1.f, 0.f, dlogits_.get(), C, WfcT_.get(), C, dGO_.get(), H}
-                                      : cavs_gemm_desc{0, 0, N, H, C, 1.f, 0.f, dlogits_.get(), C, Wfc.w, H, dGO_.get(), H};
+      const cavs_gemm_desc dGd = wide ? cavs_gemm_desc{0, 1, N, H, C, 1.f, 0.f, dlogits_.get(), C, WfcT_.get(), C, dhead_in_, H}
+                                      : cavs_gemm_desc{0, 0, N, H, C, 1.f, 0.f, dlogits_.get(), C, Wfc.w, H, dhead_in_, H};
       // (not in a session that records graphs: on this runtime a capture on the session's stream comes
       // out invalidated once that stream has waited for an event of another stream)
       if (wide && !profile_ && !cfg_.graph_replay) {
@@ -2998,7 +3083,7 @@ void Engine::plan_head_chunks(const int *orphans_host) {
   head_chunks_.clear();
   const Schedule &s = *sched_;
   const int R = (int)s.rounds.size(), N = s.N;
-  if (vocab_head() || cfg_.dropout > 0.f || cfg_.head_chunks < 0 || cfg_.model != CAVS_MODEL_LSTM || !wide_head() || !s.batching || !forest_ || cfg_.graph_replay || R < 8 ||
+  if (vocab_head() || cfg_.dropout > 0.f || cfg_.block > 0 || cfg_.head_chunks < 0 || cfg_.model != CAVS_MODEL_LSTM || !wide_head() || !s.batching || !forest_ || cfg_.graph_replay || R < 8 ||
       N < 256)
     return;
   // Where the rounds are one launch per direction, chunks cost more than they cover: the backward rounds become

@@ -134,7 +134,11 @@ class Engine {
   void model_backward();
   void pop_ret(float *graph_out);
   void begin_step(const int *graph, int B, int maxlen);
+  void before_head(bool backward);
   void head_forward_backward(bool backward);
+  void behind_head();
+  cavs_dropout_mask dropout_mask(unsigned long long place) const;
+  cavs_norm_desc block_norm();
   // counted wrappers
   float *workspace(size_t bytes);
   void gemm(int tA, int tB, int M, int N, int K, const float *A, int lda, const float *B, int ldb,
@@ -230,9 +234,11 @@ class Engine {
   };
   std::vector<OrthoBlock> ortho_;  // the blocks of "W" and "U" the optimizer takes as matrices
   DeviceArray<float> ortho_ws_, head_ws_;
-  DeviceArray<float> dropped_;  // what the head reads in a step that drops
-  DeviceArray<unsigned long long> drop_step_;
+  // what the head reads and its gradient: GO_ and dGO_, or head_x_ (with a block: and dhead_)
   const float *head_in_ = nullptr;
+  float *dhead_in_ = nullptr;
+  DeviceArray<float> head_x_, dhead_, block_x_, block_z_, block_a_, block_da_, block_ws_;
+  DeviceArray<unsigned long long> drop_step_;
 
   std::shared_ptr<Schedule> sched_ = std::make_shared<Schedule>();
   std::shared_ptr<Schedule> spare_[3];

@@ -25,7 +25,7 @@ class _Config(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("model", "loss", "pairing", "opt", "V", "E", "H", "C", "act",
                                       "use_bias", "use_x", "device", "fused_round_rows", "split_backward_rounds",
                                       "schedule_mode", "plan_cache", "tail_rows", "graph_replay", "head_chunks", "vocab_head", "optimizer")] + \
-        [(n, C.c_float) for n in ("ortho_lr", "ortho_momentum", "ortho_decay", "dropout")] + [("dropout_seed", C.c_uint)]
+        [(n, C.c_float) for n in ("ortho_lr", "ortho_momentum", "ortho_decay", "dropout")] + [("dropout_seed", C.c_uint), ("block", C.c_int), ("block_act", C.c_int)]
 
 
 _lib = None
@@ -203,20 +203,23 @@ class Session:
     is the parameter "W.momentum" / "U.momentum" (`param`, `set_params`); ortho_lr 0 is step's lr, ortho_momentum 0 is 0.95,
     negative none.
     dropout: the share of what the vertices push that is dropped before the softmax head in steps with a backward pass, drawn from
-    dropout_seed, the number of such steps before this one, the vertex and the column (`cavs_dropout`)."""
+    dropout_seed, the number of such steps before this one, the vertex and the column (`cavs_dropout`).
+    block: the inner width of a residual block before the head, h + drop(drop(act(rms(h) Wup^T + bup)) Wdown^T + bdown), with the
+    parameters "gnorm" [H], "Wup" [block, H], "bup", "Wdown" [H, block], "bdown"; dropout is then of the block, not of the head's input."""
 
     def __init__(self, model, *, H, E=0, V=0, C_=0, loss="softmax", pairing="reference",
                  opt=OPT_BATCHING, act=0, use_bias=False, use_x=False, device=0, fused_round_rows=0,
                  split_backward_rounds=False, schedule="host", plan_cache=0, tail_rows=0, graph_replay=False, head_chunks=0,
                  vocab_head=False, optimizer="sgd", ortho_lr=0.0, ortho_momentum=0.0, ortho_decay=0.0,
-                 dropout=0.0, dropout_seed=0):
+                 dropout=0.0, dropout_seed=0, block=0, block_act="gelu"):
         self.model, self.H, self.E, self.V, self.C, self.loss = model, H, (H if model == "lstm" else E), V, C_, loss
+        self.block = block
         self.mw = H if model == "treefc" else 2 * H
         cfg = _Config(MODEL[model], LOSS[loss], PAIR[pairing], opt, V, E, H, C_, int(act), int(use_bias),
                       int(use_x), device, int(fused_round_rows), int(split_backward_rounds),
                       {"host": 0, "device": 1}[schedule], int(plan_cache), int(tail_rows), int(graph_replay), int(head_chunks),
                       int(vocab_head), OPTIMIZER[optimizer], float(ortho_lr), float(ortho_momentum), float(ortho_decay),
-                      float(dropout), int(dropout_seed) & 0xFFFFFFFF)
+                      float(dropout), int(dropout_seed) & 0xFFFFFFFF, int(block), hip.ACT[block_act])
         self._h = C.c_void_p()
         _check(lib().cavs_session_create(C.byref(cfg), C.byref(self._h)), "cavs_session_create")
         self._keep = None
@@ -298,6 +301,10 @@ class Session:
         if self.loss == "softmax":
             out["dWfc"] = self.grad("Wfc", (Cc, H))
             out["dbfc"] = self.grad("bfc", (Cc,))
+        if self.block:
+            F = self.block
+            for k, shape in ("gnorm", (H,)), ("Wup", (F, H)), ("bup", (F,)), ("Wdown", (H, F)), ("bdown", (H,)):
+                out["d" + k] = self.grad(k, shape)
         return out
 
     def schedule_trace(self):

@@ -117,6 +117,13 @@ typedef struct {
    * without a backward pass drop nothing.  The head runs in one piece then (head_chunks). */
   float dropout;
   unsigned dropout_seed;
+  /* Softmax loss: the inner width of a residual block between what the vertices push, h [N, H], and the head, which reads
+   *   h + drop(drop(act(rms(h) Wup^T + bup)) Wdown^T + bdown)
+   * (cavs_norm_residual_*, cavs_linear_*; rms with the weight "gnorm" and eps 1e-6).  Its parameters: "gnorm" [H], "Wup" [block, H], "bup" [block], "Wdown" [H, block],
+   * "bdown" [H], by SGD.  `dropout` is then of the block's two places (seeds dropout_seed + 2^32 and + 2^33) and not of the head's input.  0 = none, at most 65536;
+   * H at most 16384.  The head runs in one piece. */
+  int block;
+  int block_act; /* CAVS_ACT_* of cavs_hip.h: 0 none, 1 relu, 2 tanh, 3 sigmoid, 4 silu, 5 gelu */
 } cavs_session_config;
 enum { CAVS_OPTIMIZER_SGD = 0, CAVS_OPTIMIZER_ORTHO = 1 };
 
@@ -129,7 +136,7 @@ int cavs_session_create(const cavs_session_config *cfg, cavs_session **out);
 #define cavs_session_create(cfg, out) cavs_session_create_sized(cfg, sizeof(cavs_session_config), out)
 int cavs_session_destroy(cavs_session *s);
 
-/* Parameters and their gradients by name: "Emb" "W" "U" "Bv" "Wfc" "bfc"
+/* Parameters and their gradients by name: "Emb" "W" "U" "Bv" "Wfc" "bfc" (with a block its five)
  * (shapes: apps/paper/tree-lstm-cavs.cc:110-126, seq-lstm-cavs.cc:49-59,
  * tree-fc-cavs.cc:24). `n` is the element count and must match. */
 int cavs_session_set_param(cavs_session *s, const char *name, const float *host, size_t n);

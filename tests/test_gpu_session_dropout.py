@@ -1,5 +1,5 @@
-"""A session that drops a share of what the vertices push before its head: losses and all gradients against the 64-bit model under the same mask, over steps, heads,
-schedules and recorded steps."""
+"""Sessions that drop a share of what the vertices push before their head: losses and all gradients against the 64-bit model under the same mask, over steps,
+heads, schedules and recorded steps."""
 import ctypes as C
 
 import numpy as np

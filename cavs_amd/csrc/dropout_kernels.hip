@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropArgs<T> a) {
 
 template <class T>
 int run_dropout(void *y, int ldy, const void *x, int ldx, const void *r, int ldr, int n, int w, const Mask &m, hipStream_t st) {
-  DropArgs<T> a{static_cast<T *>(y), static_cast<const T *>(x), static_cast<const T *>(r), ldy, ldx, ldr, n, w, (w + 7) / 8, 1, m};
+  DropArgs<T> a{static_cast<T *>(y), static_cast<const T *>(x), static_cast<const T *>(r), ldy, ldx, ldr, n, w, (int)(((long)w + 7) / 8), 1, m};
   // (few rows: as many workgroups as there are rows or compute units)
   const long per = ((long)n * a.pieces + num_cus() - 1) / num_cus(), items = per < kItems ? per : kItems;
   const long rows = items / a.pieces, least = (n + (long)most_groups(256) - 1) / most_groups(256);

@@ -591,6 +591,8 @@ struct Shape {  // of a product
 template <int P> struct Speeds;
 template <> struct Speeds<3> { static constexpr double ns[2][3] = {{26, 26, 29}, {68, 73, 98}}; };
 template <> struct Speeds<1> { static constexpr double ns[2][3] = {{6, 6.5, 8}, {14, 15, 20}}; };
+// (a dimension of a grid has less than 2^32 threads, of the launch that joins parts too)
+inline bool too_many(double groups, int threads, int splits, long results) { return groups * threads >= 4294967296. || (splits > 1 && results >= 1l << 33); }
 constexpr int kStretches[] = {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32};
 template <int P>
 Shape shape_of(int cols, int rows, int K) {
@@ -607,6 +609,7 @@ Shape shape_of(int cols, int rows, int K) {
       if (splits > 1 && K / splits < 256) break;
       s.kchunk = ceil_to((K + splits - 1) / splits, kPlaneAlign);
       s.splits = (K + s.kchunk - 1) / s.kchunk;
+      if (too_many((double)s.tm * s.tn * s.splits, 256, s.splits, (long)rows * cols)) continue;
       const long groups = (long)s.tm * s.tn * s.splits, full = groups / (3 * cus), rest = (groups - full * 3 * cus + cus - 1) / cus;
       double us = 1e-3 * (s.kchunk + 200) * (full * Speeds<P>::ns[size][2] + (rest > 0 ? Speeds<P>::ns[size][rest - 1] : 0.));
       if (s.splits > 1) us += 5. + s.splits * (8. * rows * cols) / 4.7e6;
@@ -632,6 +635,7 @@ Shape direct_shape_of(int cols, int rows, int K) {
       if (splits > 1 && K / splits < 256) break;
       s.kchunk = ceil_to((K + splits - 1) / splits, 64);
       s.splits = (K + s.kchunk - 1) / s.kchunk;
+      if (too_many((double)s.tm * s.tn * s.splits, wide ? WideTile::THREADS : NarrowTile::THREADS, s.splits, (long)rows * cols)) continue;
       const long groups = (long)s.tm * s.tn * s.splits, full = wide ? groups / cus : groups / (2 * cus), rest = groups - full * (wide ? cus : 2 * cus);
       const double k = s.kchunk + 256.;
       double us = full * k * (wide ? 0.0245 : 0.0140);
@@ -648,7 +652,7 @@ Shape direct_shape_of(int cols, int rows, int K) {
 // us of a call with all workgroups whole / in the stretches this finds, and with the products in launches of their own: fp32 7088 x 512 x 2048 266 / 190, 240;
 // 4096 x 1024 x 1024 148 / 120; bf16 2048 x 1024 x 4096 53 / 47; 8192 x 512 x 2048 87 / 47; 512 x 2048 x 2048 30 / 24.
 struct Places {  // of a compute unit for workgroups of a tile, ns a k of one where all are taken and of the longest
-  int bm, bn, places;
+  int bm, bn, threads, places;
   double ns, longest;
 };
 template <class Price>
@@ -671,6 +675,7 @@ void back_shapes_of(int n, int K, int N, int Kx, int Kw, int align, const Price 
         set(w, Kw, sw);
         const double gx = (double)x.tm * x.tn * x.splits, gw = (double)w.tm * w.tn * w.splits, kx = x.kchunk + 200., kw = w.kchunk + 200.;
         const Places at = price(size, gx + gw);
+        if (too_many(gx + gw, at.threads, x.splits, (long)n * K) || too_many(gx + gw, at.threads, w.splits, (long)N * K)) continue;
         const double all = (double)at.places * num_cus(), even = at.ns * ((gx * kx + gw * kw) / all + (gx + gw > all ? 0.35 * std::fmin(kx, kw) : 0.));
         double us = 1e-3 * std::fmax(even, at.longest * std::fmax(kx, kw));
         if (x.splits > 1) us += x.splits * (8. * n * K) / 4.7e6;
@@ -707,7 +712,7 @@ Plan plan_of(int n, int K, int N, int back) {
     p.d = take(packed_bytes<P>(p.np, p.Np));
     back_shapes_of(n, K, N, p.Np, p.np, kPlaneAlign, [](int size, double groups) {
       Places at{};
-      with_tile<P>(size, [&](auto t) { return at.bm = decltype(t)::BM, at.bn = decltype(t)::BN, 0; });
+      with_tile<P>(size, [&](auto t) { return at.bm = decltype(t)::BM, at.bn = decltype(t)::BN, at.threads = decltype(t)::THREADS, 0; });
       at.places = groups <= num_cus() ? 1 : groups <= 2 * num_cus() ? 2 : 3;
       at.ns = Speeds<P>::ns[size][at.places - 1], at.longest = Speeds<P>::ns[size][0];
       return at;
@@ -733,9 +738,9 @@ Plan direct_plan_of(int n, int K, int N, int back) {
   } else {
     p.d = take((size_t)n * N * 2);
     back_shapes_of(n, K, N, N, n, 64, [](int size, double groups) {
-      if (size) return Places{WideTile::BM, WideTile::BN, 1, groups > num_cus() / 2 ? 24.5 : 19.5, groups > num_cus() / 2 ? 24.5 : 19.5};
+      if (size) return Places{WideTile::BM, WideTile::BN, WideTile::THREADS, 1, groups > num_cus() / 2 ? 24.5 : 19.5, groups > num_cus() / 2 ? 24.5 : 19.5};
       const int places = groups <= num_cus() ? 1 : 2;
-      return Places{NarrowTile::BM, NarrowTile::BN, places, places == 1 ? 9. : 14., places == 1 ? 9. : 14.};
+      return Places{NarrowTile::BM, NarrowTile::BN, NarrowTile::THREADS, places, places == 1 ? 9. : 14., places == 1 ? 9. : 14.};
     }, &p.dx, &p.dw);
     p.part = take(parts(p.dx, n, K)), p.wpart = take(parts(p.dw, N, K));
     p.sums = take((size_t)tiles_of(n, 64) * N * 4);
@@ -929,7 +934,6 @@ __global__ __launch_bounds__(256) void no_rows_kernel(T *dW, long ld, float *db,
     for (long at = i; at < (long)N * K; at += (long)gridDim.x * 256) dW[at / K * ld + at % K] = T(0);
 }
 
-// (offsets within a tile's rows are below 2^32 bytes, and a launch has less than 2^24 tiles)
 constexpr int kMostRows = 1 << 20, kMostK = 1 << 16;
 constexpr long kMostOut = 1l << 36;
 bool shape_ok(int n, int K, int N) { return n <= kMostRows && N <= kMostRows && K <= kMostK && (long)n * N <= kMostOut && (long)N * K <= kMostOut; }

@@ -369,6 +369,18 @@ def test_operands_past_32_bits(type_):
     assert bool(((Y.double() - want["Y"]).abs() <= err["Y"]).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,n,K,N,act", [("bf16", 4104, 2056, 4096, "gelu"), ("bf16", 2048, 1024, 4096, "none"), ("bf16", 8200, 520, 2056, "silu"),
+                                             ("f32", 7001, 513, 2041, "relu"), ("f32", 1200, 512, 2048, "none"), ("f32", 300, 2041, 4100, "tanh")])
+def test_gradients_of_many_tiles(type_, n, K, N, act):
+    """Both products in a launch, in stretches and whole, either the longer; each by itself the same"""
+    c = Case(type_, n, K, N, act, 0.1)
+    both = c.run(1)
+    c.hold(both, *c.backward())
+    for k in both:
+        assert torch.equal(c.run(1, names={k})[k], both[k]), k
+
+
 # ------------------------------------------------------------------ a block, as it is used
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_,n,H,F", [("f32", 37, 96, 200), ("bf16", 150, 128, 512), ("bf16", 1, 128, 512)])

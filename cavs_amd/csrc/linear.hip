@@ -647,10 +647,12 @@ Shape direct_shape_of(int cols, int rows, int K) {
   return best;
 }
 
-// Both gradients in a launch: the same tile, and for each the stretches that a model finds best: what there is to multiply at the measured speed of as many
-// workgroups as a compute unit has, or the longest workgroup by itself; where not all have a place at once, a third of a round for the last; parts as above.
-// us of a call with all workgroups whole / in the stretches this finds, and with the products in launches of their own: fp32 7088 x 512 x 2048 266 / 190, 240;
-// 4096 x 1024 x 1024 148 / 120; bf16 2048 x 1024 x 4096 53 / 47; 8192 x 512 x 2048 87 / 47; 512 x 2048 x 2048 30 / 24.
+// Both gradients in a launch: the same tile, and for each the stretches that a model finds best.  Where all workgroups have a place at once: the mean of them at the
+// measured speed of as many as the fullest compute unit has; where not, what there is to multiply at the speed of all places, and a third of a round for the last;
+// but no less than the longest by itself.  Parts go through the caches at twice a copy's rate, and take a launch's 5 us.
+// us of a call with all workgroups whole / in the stretches this finds / in the best of them: fp32 7088 x 512 x 2048 266 / 187 / 187 (240 with the products in launches
+// of their own), 4096 x 1024 x 1024 148 / 116 / 110, 157 x 300 x 777 31 / 21 / 21; bf16 2048 x 1024 x 4096 53 / 47 / 47, 8192 x 512 x 2048 87 / 48 / 48, 100 x 4096 x 4096
+// 46 / 29 / 28.
 struct Places {  // of a compute unit for workgroups of a tile, ns a k of one where all are taken and of the longest
   int bm, bn, threads, places;
   double ns, longest;
@@ -658,8 +660,9 @@ struct Places {  // of a compute unit for workgroups of a tile, ns a k of one wh
 template <class Price>
 void back_shapes_of(int n, int K, int N, int Kx, int Kw, int align, const Price &price, Shape *dx, Shape *dw) {
   double least = INFINITY;
+  const int cus = num_cus();
   for (int size = 0; size < 2; size++) {
-    const Places any = price(size, 1.);
+    const Places any = price(size, 1., cus);
     Shape x{}, w{};
     x.size = w.size = size;
     x.tm = w.tm = tiles_of(K, any.bm), x.tn = tiles_of(n, any.bn), w.tn = tiles_of(N, any.bn);
@@ -674,12 +677,13 @@ void back_shapes_of(int n, int K, int N, int Kx, int Kw, int align, const Price 
         if (sw > 1 && Kw / sw < 256) break;
         set(w, Kw, sw);
         const double gx = (double)x.tm * x.tn * x.splits, gw = (double)w.tm * w.tn * w.splits, kx = x.kchunk + 200., kw = w.kchunk + 200.;
-        const Places at = price(size, gx + gw);
+        const Places at = price(size, gx + gw, cus);
         if (too_many(gx + gw, at.threads, x.splits, (long)n * K) || too_many(gx + gw, at.threads, w.splits, (long)N * K)) continue;
-        const double all = (double)at.places * num_cus(), even = at.ns * ((gx * kx + gw * kw) / all + (gx + gw > all ? 0.35 * std::fmin(kx, kw) : 0.));
+        const double groups = gx + gw, all = (double)at.places * cus, work = gx * kx + gw * kw;
+        const double even = at.ns * (groups > all ? work / all + 0.35 * std::fmin(kx, kw) : work / groups);
         double us = 1e-3 * std::fmax(even, at.longest * std::fmax(kx, kw));
-        if (x.splits > 1) us += x.splits * (8. * n * K) / 4.7e6;
-        if (w.splits > 1) us += w.splits * (8. * N * K) / 4.7e6;
+        if (x.splits > 1) us += x.splits * (8. * n * K) / 9e6;
+        if (w.splits > 1) us += w.splits * (8. * N * K) / 9e6;
         if (x.splits > 1 || w.splits > 1) us += 5.;
         if (us < least) least = us, *dx = x, *dw = w;
       }
@@ -710,10 +714,10 @@ Plan plan_of(int n, int K, int N, int back) {
     p.part = take(parts(p.fwd, n, N));
   } else {
     p.d = take(packed_bytes<P>(p.np, p.Np));
-    back_shapes_of(n, K, N, p.Np, p.np, kPlaneAlign, [](int size, double groups) {
+    back_shapes_of(n, K, N, p.Np, p.np, kPlaneAlign, [](int size, double groups, int cus) {
       Places at{};
       with_tile<P>(size, [&](auto t) { return at.bm = decltype(t)::BM, at.bn = decltype(t)::BN, at.threads = decltype(t)::THREADS, 0; });
-      at.places = groups <= num_cus() ? 1 : groups <= 2 * num_cus() ? 2 : 3;
+      at.places = groups <= cus ? 1 : groups <= 2 * cus ? 2 : 3;
       at.ns = Speeds<P>::ns[size][at.places - 1], at.longest = Speeds<P>::ns[size][0];
       return at;
     }, &p.dx, &p.dw);
@@ -737,9 +741,9 @@ Plan direct_plan_of(int n, int K, int N, int back) {
     p.part = take(parts(p.fwd, n, N));
   } else {
     p.d = take((size_t)n * N * 2);
-    back_shapes_of(n, K, N, N, n, 64, [](int size, double groups) {
-      if (size) return Places{WideTile::BM, WideTile::BN, WideTile::THREADS, 1, groups > num_cus() / 2 ? 24.5 : 19.5, groups > num_cus() / 2 ? 24.5 : 19.5};
-      const int places = groups <= num_cus() ? 1 : 2;
+    back_shapes_of(n, K, N, N, n, 64, [](int size, double groups, int cus) {
+      if (size) return Places{WideTile::BM, WideTile::BN, WideTile::THREADS, 1, groups > cus / 2 ? 24.5 : 19.5, groups > cus / 2 ? 24.5 : 19.5};
+      const int places = groups <= cus ? 1 : 2;
       return Places{NarrowTile::BM, NarrowTile::BN, NarrowTile::THREADS, places, places == 1 ? 9. : 14., places == 1 ? 9. : 14.};
     }, &p.dx, &p.dw);
     p.part = take(parts(p.dx, n, K)), p.wpart = take(parts(p.dw, N, K));

@@ -6,19 +6,13 @@
 
 namespace cavs {
 
-// e^x: 2^n of the whole part, the instruction of the rest
-__device__ __forceinline__ float exp_fast(float x) {
-  x = __builtin_amdgcn_fmed3f(x, -110.f, 110.f);
-  const float n = __builtin_rintf(x * 1.44269504f);
-  const float f = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269504f, -n));
-  return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
-}
+// e^x, 0 below 2^-126: the instruction of x log2 e, whose rounding is 2^-24 |x| of the result
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 // 1 / (1 + e^-z)
 template <bool FAST>
 __device__ __forceinline__ float logistic(float z) {
   if constexpr (!FAST) return 1.f / (1.f + expf(-z));
-  const float g = __builtin_amdgcn_rcpf(1.f + exp_fast(-z));
-  return z == z ? g : z;
+  return __builtin_amdgcn_rcpf(1.f + exp_fast(-z));
 }
 // e^-(z^2 / 2) and Phi(-|z|), the normal distribution: e^-(a^2) q(a) / 2, a = |z| / sqrt 2, q(a) = erfc(a) e^(a^2) as a polynomial of 1 / (1 + 0.6 a), fitted to
 // 2e-8 of the value over 0 <= a <= 10.3 by weighted least squares at Chebyshev's points.  (Beyond a float holds nothing of it.)

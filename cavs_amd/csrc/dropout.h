@@ -1,8 +1,8 @@
 // Which elements a dropout keeps, from a counter-based generator: Philox4x32 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", 2011) of
 // seven rounds, the fewest its authors found to pass all their tests.  The key is the seed, the counter (column / 8, the row's id, step): its 128 bits are the
 // draws of eight neighbouring columns, 16 bits each, so that a lane that holds eight values makes one.  An element stays if its draw is at least
-// round(65536 p).  Of 32 bits a draw a lane would need two calls: a wavefront's 512 values of bf16, read and written, are 110 ns of a compute unit's share of a copy's
-// rate (4.74 TB/s), and the 14 products of a call, two instructions of 16 cycles each, 50 ns of its four SIMDs.  Two calls would leave nothing for anything else.
+// round(65536 p).  (With 32 bits a draw eight values would need two calls.  A wavefront's 512 values of bf16, read and written, are 110 ns of a compute unit's share of a
+// copy's rate, 4.74 TB/s; a call is 14 products of 16 cycles and some 45 instructions of 4, 400 cycles of one of its four SIMDs, 45 ns.)
 #pragma once
 #include "rows8.h"
 

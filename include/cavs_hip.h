@@ -467,7 +467,8 @@ int cavs_norm_residual_bwd(int type, const cavs_norm_desc *d, const void *s, int
  * is rounded to bf16 between its products (not in db), results once.
  * At most 2^20 rows, N <= 2^20, K <= 2^16, n N and N K <= 2^36.  n = 0 is allowed (dW and db become 0).
  * The workspace: 16-byte aligned, at least cavs_linear_workspace(type, n, K, N, back) bytes on this device (back: 0 for _fwd; 0: the shape or type is
- * refused); for the next call on the same stream to reuse, not for one that overlaps in time. */
+ * refused; what any alignment and stride of the operands takes, and 256 where a forward pass of few rows takes none); for the next call on the same stream to
+ * reuse, not for one that overlaps in time. */
 enum { CAVS_ACT_NONE = 0, CAVS_ACT_RELU = 1, CAVS_ACT_TANH = 2, CAVS_ACT_SIGMOID = 3, CAVS_ACT_SILU = 4, CAVS_ACT_GELU = 5 /* z Phi(z) */ };
 size_t cavs_linear_workspace(int type, int n, int K, int N, int back);
 int cavs_linear_fwd(int type, const void *X, int ldx, const void *W, int ldw, const float *b, int act, const cavs_dropout_mask *mask,

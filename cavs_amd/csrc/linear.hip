@@ -419,6 +419,18 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(FewJob<T> g) {
   const T *rows[TT];
 #pragma unroll
   for (int t = 0; t < TT; t++) rows[t] = g.X + min(r0 + 16 * t + x, g.n - 1) * g.ldx + piece;  // (rows beyond the last: once more the last, not stored)
+  // what the epilogue reads, two lanes a row, is asked for first
+  const int r = threadIdx.x >> 1, row = r0 + r, col = c0 + 8 * (threadIdx.x & 1), left = r < 16 * TT && row < g.n ? g.N - col : 0;
+  Eight<float> bias;
+  Eight<T> held;
+  bias.zero(), held.zero();
+  unsigned long long step = 0;
+  unsigned id = 0;
+  if (left > 0) {
+    if (g.out.bias) bias.load(g.out.bias + col, left);
+    g.out.hold(held, row, col, left);
+    step = g.out.step(), id = g.out.id(row);
+  }
   floatx4 acc[ACC][TT];
 #pragma unroll
   for (int a = 0; a < ACC; a++)
@@ -478,20 +490,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(FewJob<T> g) {
     sums[0][t][r][c] = v;  // (nobody else reads this one)
   }
   __syncthreads();
-  const int r = threadIdx.x >> 1, row = r0 + r, col = c0 + 8 * (threadIdx.x & 1), left = g.N - col;
-  if (r >= 16 * TT || row >= g.n || left <= 0) return;
-  float v[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (left <= 0) return;
+  float v[8], b[8];
 #pragma unroll
-  for (int e = 0; e < 8; e++) v[e] = sums[0][r >> 4][r & 15][8 * (threadIdx.x & 1) + e];
-  if (g.out.bias) {
-    Eight<float> t;
-    t.load(g.out.bias + col, left);
-#pragma unroll
-    for (int e = 0; e < 8; e++) b[e] = t[e];
-  }
-  Eight<T> held;
-  g.out.hold(held, row, col, left);
-  g.out.finish(g.out.step(), g.out.id(row), b, held, row, col, left, v);
+  for (int e = 0; e < 8; e++) v[e] = sums[0][r >> 4][r & 15][8 * (threadIdx.x & 1) + e], b[e] = bias[e];
+  g.out.finish(step, id, b, held, row, col, left, v);
 }
 
 // what a product left in parts, in their order, to the epilogue; pieces of eight columns

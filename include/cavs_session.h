@@ -121,7 +121,7 @@ typedef struct {
    *   h + drop(drop(act(rms(h) Wup^T + bup)) Wdown^T + bdown)
    * (cavs_norm_residual_*, cavs_linear_*; rms with the weight "gnorm" and eps 1e-6).  Its parameters: "gnorm" [H], "Wup" [block, H], "bup" [block], "Wdown" [H, block],
    * "bdown" [H], by SGD.  `dropout` is then of the block's two places (seeds dropout_seed + 2^32 and + 2^33) and not of the head's input.  0 = none, at most 65536;
-   * H at most 16384.  The head runs in one piece. */
+   * H at most 16384, a step at most 2^20 vertices.  The head runs in one piece. */
   int block;
   int block_act; /* CAVS_ACT_* of cavs_hip.h: 0 none, 1 relu, 2 tanh, 3 sigmoid, 4 silu, 5 gelu */
 } cavs_session_config;

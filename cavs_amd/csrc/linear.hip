@@ -199,6 +199,29 @@ __global__ __launch_bounds__(256) void grad_kernel(GradJob<T> g, PackJob<T> x, P
   if (wave == 0 && k0 + c < g.N) g.sums[(long)(r0 / 64) * g.N + k0 + c] = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
 }
 
+// sums of columns that launches before left over 64 rows each, 64 columns a workgroup, of its first four wavefronts
+struct ColumnsJob {
+  const float *part;
+  int parts, cols;
+  float *out;
+  int blocks;  // 0: none
+};
+__device__ __forceinline__ void sum_columns(const ColumnsJob &g, int block, float (*each)[64]) {
+  const int c = block * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6, per = (g.parts + 3) / 4, end = min(g.parts, (w + 1) * per);
+  float s = 0.f;
+  if (w < 4 && c < g.cols)
+    for (int p = w * per; p < end; p += 8) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[k] = p + k < end ? g.part[(long)(p + k) * g.cols + c] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; k++) s += v[k];
+    }
+  if (w < 4) each[w][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (w == 0 && c < g.cols) g.out[c] = (each[0][threadIdx.x] + each[1][threadIdx.x]) + (each[2][threadIdx.x] + each[3][threadIdx.x]);
+}
+
 // ------------------------------------------------------------------ products of packed operands
 // result[row, col] = sum over k of A[col, k] B[row, k].  K in `splits` stretches of kchunk, each with sums of its own at part + split * rows * cols; part
 // null: straight to the epilogue.
@@ -264,10 +287,14 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void packed_forward_kernel(Produ
   finish_packed<T>(g, split, kept, m0, n0, acc);
 }
 // Both gradients in a launch, so that the compute units whose last tile of the one has ended go on with the other: dX = D W (its A turned) and dW = D^T X (both
-// turned), `wfirst`: dW is j0.
+// turned), `wfirst`: dW is j0.  Behind them db, which waits for no more than they do (in a launch of its own 5 us more).
 template <class T, class E>
-__global__ __launch_bounds__(T::THREADS, T::EU) void packed_back_kernel(Product<E> j0, Product<E> j1, int blocks0, int wfirst) {
+__global__ __launch_bounds__(T::THREADS, T::EU) void packed_back_kernel(Product<E> j0, Product<E> j1, int blocks0, int blocks, int wfirst, ColumnsJob b) {
   __shared__ __attribute__((aligned(16))) char S[T::LDS];
+  if ((int)blockIdx.x >= blocks) {
+    sum_columns(b, blockIdx.x - blocks, reinterpret_cast<float(*)[64]>(S));
+    return;
+  }
   const bool second = (int)blockIdx.x >= blocks0;
   const Product<E> &g = second ? j1 : j0;
   int split, m0, n0, kbeg, kend;
@@ -320,8 +347,12 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void direct_forward_kernel(Direc
 }
 // (as packed_back_kernel)
 template <class T, class E>
-__global__ __launch_bounds__(T::THREADS, T::EU) void direct_back_kernel(DirectJob<E> j0, DirectJob<E> j1, int blocks0, int wfirst) {
+__global__ __launch_bounds__(T::THREADS, T::EU) void direct_back_kernel(DirectJob<E> j0, DirectJob<E> j1, int blocks0, int blocks, int wfirst, ColumnsJob b) {
   __shared__ __attribute__((aligned(16))) char S[T::LDS];
+  if ((int)blockIdx.x >= blocks) {
+    sum_columns(b, blockIdx.x - blocks, reinterpret_cast<float(*)[64]>(S));
+    return;
+  }
   const bool second = (int)blockIdx.x >= blocks0;
   const DirectJob<E> &g = second ? j1 : j0;
   int split, m0, n0, kbeg, kend;
@@ -538,28 +569,6 @@ __device__ __forceinline__ void join_block(const PartsJob<E> &g, int block) {
 template <class E>
 __global__ __launch_bounds__(256) void parts_kernel(PartsJob<E> g) { join_block(g, blockIdx.x); }
 
-// sums of columns that launches before left over 64 rows each, 64 columns a workgroup
-struct ColumnsJob {
-  const float *part;
-  int parts, cols;
-  float *out;
-  int blocks;
-};
-__device__ __forceinline__ void sum_columns(const ColumnsJob &g, int block, float (&each)[4][64]) {
-  const int c = block * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6, per = (g.parts + 3) / 4, end = min(g.parts, (w + 1) * per);
-  float s = 0.f;
-  if (c < g.cols)
-    for (int p = w * per; p < end; p += 8) {
-      float v[8];
-#pragma unroll
-      for (int k = 0; k < 8; k++) v[k] = p + k < end ? g.part[(long)(p + k) * g.cols + c] : 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; k++) s += v[k];
-    }
-  each[w][threadIdx.x & 63] = s;
-  __syncthreads();
-  if (w == 0 && c < g.cols) g.out[c] = (each[0][threadIdx.x] + each[1][threadIdx.x]) + (each[2][threadIdx.x] + each[3][threadIdx.x]);
-}
 // the ends of both gradients and db
 template <class E>
 __global__ __launch_bounds__(256) void back_ends_kernel(PartsJob<E> x, PartsJob<E> w, ColumnsJob b) {
@@ -598,8 +607,8 @@ struct Shape {  // of a product
 template <int P> struct Speeds;
 template <> struct Speeds<3> { static constexpr double ns[2][3] = {{26, 26, 29}, {68, 73, 98}}; };
 template <> struct Speeds<1> { static constexpr double ns[2][3] = {{6, 6.5, 8}, {14, 15, 20}}; };
-// (a dimension of a grid has less than 2^32 threads, of the launch that joins parts too)
-inline bool too_many(double groups, int threads, int splits, long results) { return groups * threads >= 4294967296. || (splits > 1 && results >= 1l << 33); }
+// (a dimension of a grid has less than 2^32 threads, with the workgroups that sum columns and of the launch that joins parts too)
+inline bool too_many(double groups, int threads, int splits, long results) { return (groups + 16384) * threads >= 4294967296. || (splits > 1 && results >= 1l << 33); }
 constexpr int kStretches[] = {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32};
 template <int P>
 Shape shape_of(int cols, int rows, int K) {
@@ -822,14 +831,18 @@ BackJobs<Job> back_jobs(const Job &x, const Shape &sx, bool wantx, const Job &w,
   const bool wfirst = sw.kchunk > sx.kchunk;
   return wfirst ? BackJobs<Job>{w, x, bw, bx + bw, 1} : BackJobs<Job>{x, w, bx, bx + bw, 0};
 }
+// db from sums over 64 rows each
+ColumnsJob columns_of(const Call &c, const Plan &p, char *ws, int stretches) {
+  return ColumnsJob{reinterpret_cast<float *>(ws + p.sums), stretches, c.N, c.db, c.db ? (c.N + 63) / 64 : 0};
+}
+// what the products leave to do, and db if there were none
 template <class T>
-int back_ends(const Call &c, const Plan &p, char *ws, int stretches, hipStream_t st) {
+int back_ends(const Call &c, const Plan &p, char *ws, const ColumnsJob &b, hipStream_t st) {
   const Plain<T> ox{static_cast<T *>(c.dX), c.lddx}, ow{static_cast<T *>(c.dW), c.lddw};
   PartsJob<Plain<T>> x = parts_of_product(reinterpret_cast<float *>(ws + p.part), p.dx, c.n, c.K, ox);
   PartsJob<Plain<T>> w = parts_of_product(reinterpret_cast<float *>(ws + p.wpart), p.dw, c.N, c.K, ow);
   if (!c.dX) x.blocks = 0;
   if (!c.dW) w.blocks = 0;
-  const ColumnsJob b{reinterpret_cast<float *>(ws + p.sums), stretches, c.N, c.db, c.db ? (c.N + 63) / 64 : 0};
   if (x.blocks + w.blocks + b.blocks > 0) {
     launch(back_ends_kernel<Plain<T>>, (unsigned)(x.blocks + w.blocks + b.blocks), 256, 0, st, x, w, b);
     CAVS_LAUNCH_CHECK();
@@ -864,6 +877,7 @@ int run_direct_bwd(const Call &c, char *ws, hipStream_t st) {
     launch(grad_rows_kernel, grid_of(g.blocks), 256, 0, st, g, made);
     CAVS_LAUNCH_CHECK();
   }
+  ColumnsJob b = columns_of(c, p, ws, tiles_of(c.n, 64));
   if (c.dX || c.dW) {
     typedef Plain<u16> E;
     const DirectRef D{made ? made : g.dY, made ? (long)c.N : c.lddy}, X{static_cast<const u16 *>(c.X), c.ldx}, W{static_cast<const u16 *>(c.W), c.ldw};
@@ -871,11 +885,13 @@ int run_direct_bwd(const Call &c, char *ws, hipStream_t st) {
     const DirectJob<E> x{W, D, c.K, c.n, c.N, p.dx.tm, p.dx.tn, p.dx.kchunk, p.dx.splits > 1 ? xpart : nullptr, E{static_cast<u16 *>(c.dX), c.lddx}};
     const DirectJob<E> w{X, D, c.K, c.N, c.n, p.dw.tm, p.dw.tn, p.dw.kchunk, p.dw.splits > 1 ? wpart : nullptr, E{static_cast<u16 *>(c.dW), c.lddw}};
     const auto j = back_jobs(x, p.dx, c.dX, w, p.dw, c.dW);
-    if (p.dx.size) launch(direct_back_kernel<WideTile, E>, (unsigned)j.blocks, WideTile::THREADS, 0, st, j.j0, j.j1, j.blocks0, j.wfirst);
-    else launch(direct_back_kernel<NarrowTile, E>, (unsigned)j.blocks, NarrowTile::THREADS, 0, st, j.j0, j.j1, j.blocks0, j.wfirst);
+    const unsigned groups = (unsigned)(j.blocks + b.blocks);
+    if (p.dx.size) launch(direct_back_kernel<WideTile, E>, groups, WideTile::THREADS, 0, st, j.j0, j.j1, j.blocks0, j.blocks, j.wfirst, b);
+    else launch(direct_back_kernel<NarrowTile, E>, groups, NarrowTile::THREADS, 0, st, j.j0, j.j1, j.blocks0, j.blocks, j.wfirst, b);
     CAVS_LAUNCH_CHECK();
+    b.blocks = 0;
   }
-  return back_ends<u16>(c, p, ws, tiles_of(c.n, 64), st);
+  return back_ends<u16>(c, p, ws, b, st);
 }
 
 template <class T>
@@ -920,6 +936,7 @@ int run_bwd(const Call &c, char *ws, hipStream_t st) {
   if (!c.dX) w.blocks = 0;
   launch(grad_kernel<P, T>, grid_of((long)g.blocks + x.blocks + w.blocks), 256, 0, st, g, x, w);
   CAVS_LAUNCH_CHECK();
+  ColumnsJob b = columns_of(c, p, ws, p.np / 64);
   if (c.dX || c.dW) {
     typedef Plain<T> E;
     const PackedRef X{x.o.p, p.Kp}, W{w.o.p, p.Kp}, D{g.o.p, p.Np};
@@ -929,12 +946,13 @@ int run_bwd(const Call &c, char *ws, hipStream_t st) {
     const auto j = back_jobs(jx, p.dx, c.dX, jw, p.dw, c.dW);
     with_tile<P>(p.dx.size, [&](auto t) {
       using Tile = decltype(t);
-      launch(packed_back_kernel<Tile, E>, (unsigned)j.blocks, Tile::THREADS, 0, st, j.j0, j.j1, j.blocks0, j.wfirst);
+      launch(packed_back_kernel<Tile, E>, (unsigned)(j.blocks + b.blocks), Tile::THREADS, 0, st, j.j0, j.j1, j.blocks0, j.blocks, j.wfirst, b);
       return 0;
     });
     CAVS_LAUNCH_CHECK();
+    b.blocks = 0;
   }
-  return back_ends<T>(c, p, ws, p.np / 64, st);
+  return back_ends<T>(c, p, ws, b, st);
 }
 
 template <class T>

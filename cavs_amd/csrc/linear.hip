@@ -415,7 +415,7 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(GradJob<u16> g, u16 *D) 
 // ------------------------------------------------------------------ few rows: W read once, where it lies
 // A workgroup makes sixteen columns of the result: eight wavefronts, each a stretch of K, the rows of W and X as pieces of the 16x16x32 instruction straight from memory
 // (fp32: split into parts on the way), 256 k of them asked for at a time.  Their sums meet in LDS.  Sixteen columns, so that W has two workgroups
-// a compute unit from 8192 columns on; each reads all of X.
+// a compute unit from 8192 columns on; each reads all of X, or one of 16, 32 or 64 rows each (few_of).
 template <class T>
 struct FewJob {
   const T *X, *W;
@@ -773,11 +773,24 @@ Plan direct_plan_of(int n, int K, int N, int back) {
 // fp32 3.0 + 0.04 and 0.0013 a row squared (8192 x 2048 with 1, 16, 32, 64 rows: 1.0 1.6 2.5 4.2, 3.2 3.7 5.6 10.8); tiles cost what their model says, and what packing W and X takes.  us of
 // few rows / of tiles: bf16 2048 x 8192 with 1 row 6.9 / 10.8, 16 9.5 / 11.7, 64 20 / 15.5; 8192 x 2048 with 16 16 / 13.4; 1000 x 1000 with 157 5.8 / 13.6, 512
 // 10.5 / 14.1; 512 x 2048 with 512 12.4 / 8.4; fp32 2048 x 8192 with 1 16 / 46, 32 29 / 48, 64 50 / 48; 300 x 777 with 157 7.1 / 12.3, 512 x 2048 with 256 15.5 / 17.7.
-bool few_rows(int type, int n, int K, int N, double tiles_us) {
-  const double rows = n < 64 ? n : 64, groups = (double)tiles_of(N, 16) * tiles_of(n, 64);
-  const double us = 2.5 + 1e-3 * K * (type == CAVS_F32 ? 3.0 + (0.04 + 0.0013 * rows) * rows : 1.0 + 0.05 * rows) * std::ceil(groups / num_cus());
-  return us < tiles_us;
+// Rows of a workgroup, 16, 32 or 64, by the same figures: where 64 leave compute units idle W is read by more of them (from the caches).  us of 64 / of what this takes: fp32
+// 157 x 300 x 777 7.1 / 5.6, 98 x 1918 x 352 18 / 9.3, 40 x 2048 x 2048 24 / 16, 32 x 8192 x 2048 50 / 35, bf16 64 x 4096 x 640 11 / 9.
+struct Few {
+  int blocks;  // of sixteen rows of X, of a workgroup: 1, 2 or 4
+  double us;
+};
+Few few_of(int type, int n, int K, int N) {
+  Few best{4, INFINITY};
+  const double cus = num_cus();
+  for (int blocks = 1; blocks <= 4; blocks *= 2) {
+    if (tiles_of(n, 16 * blocks) > 65535) continue;  // (a grid's y)
+    const double rows = n < 16 * blocks ? n : 16 * blocks, groups = (double)tiles_of(N, 16) * tiles_of(n, 16 * blocks);
+    const double us = 2.5 + 1e-3 * K * (type == CAVS_F32 ? 3.0 + (0.04 + 0.0013 * rows) * rows : 1.0 + 0.05 * rows) * std::ceil(groups / cus);
+    if (us < best.us) best = Few{blocks, us};
+  }
+  return best;
 }
+bool few_rows(int type, int n, int K, int N, double tiles_us) { return few_of(type, n, K, N).us < tiles_us; }
 template <int P>
 double packed_us(int n, int K, int N) { return 0.8 * (shape_of<P>(N, n, ceil_to(K, kPlaneAlign)).us + 4.5 + (double)K * ((double)n + N) * (P == 3 ? 10 : 4) / 7e6); }
 double direct_us(int n, int K, int N) { return direct_shape_of(N, n, K).us + 1.5; }
@@ -898,10 +911,9 @@ template <class T>
 int run_few(const Call &c, hipStream_t st) {
   const Forward<T> out{c.b, c.act, c.m, static_cast<const T *>(c.R), c.ldr, static_cast<T *>(c.Zout), c.ldz, static_cast<T *>(c.Y), c.ldy};
   const FewJob<T> g{static_cast<const T *>(c.X), static_cast<const T *>(c.W), c.ldx, c.ldw, c.n, c.K, c.N, ceil_to((c.K + kFewWaves - 1) / kFewWaves, 32), out};
-  const unsigned groups = (unsigned)tiles_of(c.N, 16);
-  if (c.n <= 16) launch(few_rows_kernel<T, 1>, groups, 64 * kFewWaves, 0, st, g);
-  else if (c.n <= 32) launch(few_rows_kernel<T, 2>, groups, 64 * kFewWaves, 0, st, g);
-  else launch(few_rows_kernel<T, 4>, dim3(groups, (unsigned)tiles_of(c.n, 64)), 64 * kFewWaves, 0, st, g);
+  const int blocks = few_of(sizeof(T) == 4 ? CAVS_F32 : CAVS_BF16, c.n, c.K, c.N).blocks;
+  const dim3 groups((unsigned)tiles_of(c.N, 16), (unsigned)tiles_of(c.n, 16 * blocks));
+  launch(blocks == 1 ? few_rows_kernel<T, 1> : blocks == 2 ? few_rows_kernel<T, 2> : few_rows_kernel<T, 4>, groups, 64 * kFewWaves, 0, st, g);
   CAVS_LAUNCH_CHECK();
   return CAVS_OK;
 }

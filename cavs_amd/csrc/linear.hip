@@ -589,6 +589,10 @@ template <> struct Tiles<3> {
   using L = NtTile<3, 128, 128, 16, 2, 2>;
   using S = NtTile<3, 64, 64, 32, 2, 2>;
 };
+template <class T>
+struct Apart : T {
+  static constexpr bool APART = true;
+};
 template <int P, class F>
 int with_tile(int size, F &&f) {
   using TT = Tiles<P>;
@@ -958,7 +962,7 @@ int run_bwd(const Call &c, char *ws, hipStream_t st) {
     const auto j = back_jobs(jx, p.dx, c.dX, jw, p.dw, c.dW);
     with_tile<P>(p.dx.size, [&](auto t) {
       using Tile = decltype(t);
-      launch(packed_back_kernel<Tile, E>, (unsigned)(j.blocks + b.blocks), Tile::THREADS, 0, st, j.j0, j.j1, j.blocks0, j.blocks, j.wfirst, b);
+      launch(packed_back_kernel<Apart<Tile>, E>, (unsigned)(j.blocks + b.blocks), Tile::THREADS, 0, st, j.j0, j.j1, j.blocks0, j.blocks, j.wfirst, b);
       return 0;
     });
     CAVS_LAUNCH_CHECK();

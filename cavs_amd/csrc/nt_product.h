@@ -65,7 +65,8 @@ __device__ inline void parts_of(float x, u16 (&o)[P]) {
 template <int P_, int BM_, int BN_, int BK_, int WGM_, int WGN_, int NS_ = 2>
 struct NtTile {
   static constexpr int P = P_, BM = BM_, BN = BN_, BK = BK_, WGM = WGM_, WGN = WGN_, NS = NS_;
-  static constexpr bool RAW = false;  // (an operand of another layout)
+  static constexpr bool RAW = false;      // (an operand of another layout)
+  static constexpr bool APART = false;    // (turned pieces are read without a wait for what is on its way)
   static constexpr int WAVES = WGM * WGN, THREADS = 64 * WAVES;
   static constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 32, TN = WN / 32;
   static constexpr int STEPS = BK / 16, ROWB = 1024 * P * STEPS;    // bytes a row of blocks takes of a stage
@@ -101,6 +102,61 @@ __device__ __forceinline__ bf16x8 turned_piece(const char *from, int lane) {
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #else
   return *reinterpret_cast<const bf16x8 *>(p);
+#endif
+}
+
+// The same for one or two pieces of A, and of B where both are turned, 1 KB apart, all there when this returns.  The compiler takes the builtin for a reader of
+// whatever is on its way from memory and waits for that first, so that a stage's loads are not behind the stage's products; this is assembly with its own wait.
+__device__ __forceinline__ unsigned lds_place(const char *p) {
+#ifdef __HIP_DEVICE_COMPILE__
+  return (unsigned)(size_t)(__attribute__((address_space(3))) const char *)p;
+#else
+  return 0;
+#endif
+}
+typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ bf16x8 halves(u32x2_t lo, u32x2_t hi) { return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3)); }
+__device__ __forceinline__ void turned_pieces_apart(unsigned lo, unsigned hi, bf16x8 (&o)[1]) {
+#ifdef __HIP_DEVICE_COMPILE__
+  u32x2_t t[2];
+  asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %3\n\ts_waitcnt lgkmcnt(0)" : "=&v"(t[0]), "=&v"(t[1]) : "v"(lo), "v"(hi) : "memory");
+  o[0] = halves(t[0], t[1]);
+#endif
+}
+__device__ __forceinline__ void turned_pieces_apart(unsigned lo, unsigned hi, bf16x8 (&o)[2]) {
+#ifdef __HIP_DEVICE_COMPILE__
+  u32x2_t t[4];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5\n\tds_read_b64_tr_b16 %2, %4 offset:1024\n\tds_read_b64_tr_b16 %3, %5 offset:1024\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]), "=&v"(t[3])
+      : "v"(lo), "v"(hi)
+      : "memory");
+  o[0] = halves(t[0], t[1]), o[1] = halves(t[2], t[3]);
+#endif
+}
+__device__ __forceinline__ void turned_pieces_apart(unsigned alo, unsigned ahi, bf16x8 (&a)[1], unsigned blo, unsigned bhi, bf16x8 (&b)[1]) {
+#ifdef __HIP_DEVICE_COMPILE__
+  u32x2_t t[4];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5\n\tds_read_b64_tr_b16 %2, %6\n\tds_read_b64_tr_b16 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]), "=&v"(t[3])
+      : "v"(alo), "v"(ahi), "v"(blo), "v"(bhi)
+      : "memory");
+  a[0] = halves(t[0], t[1]), b[0] = halves(t[2], t[3]);
+#endif
+}
+__device__ __forceinline__ void turned_pieces_apart(unsigned alo, unsigned ahi, bf16x8 (&a)[2], unsigned blo, unsigned bhi, bf16x8 (&b)[2]) {
+#ifdef __HIP_DEVICE_COMPILE__
+  u32x2_t t[8];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %2, %8 offset:1024\n\tds_read_b64_tr_b16 %3, %9 offset:1024\n\t"
+      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %11\n\tds_read_b64_tr_b16 %6, %10 offset:1024\n\tds_read_b64_tr_b16 %7, %11 offset:1024\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]), "=&v"(t[3]), "=&v"(t[4]), "=&v"(t[5]), "=&v"(t[6]), "=&v"(t[7])
+      : "v"(alo), "v"(ahi), "v"(blo), "v"(bhi)
+      : "memory");
+  a[0] = halves(t[0], t[1]), a[1] = halves(t[2], t[3]), b[0] = halves(t[4], t[5]), b[1] = halves(t[6], t[7]);
 #endif
 }
 
@@ -165,21 +221,36 @@ __device__ __forceinline__ void nt_multiply(const PackedRef &A, int M, int m0, c
 #endif
   };
   const int a0 = wm * (T::WM / 32) * T::ROWB + 16 * lane, b0 = T::PA + wn * (T::WN / 32) * T::ROWB + 16 * lane;
+  const int group = lane >> 4 & 1, half = lane >> 5;
+  [[maybe_unused]] const unsigned lo_lane = group * 512 + half * 256 + 8 * (lane & 15) + 128 * (half ^ group), hi_lane = lo_lane ^ 128;
   // A's parts from the last to the first, each with those of B that it meets: one part of A and what there is of B by then are all that registers hold
   auto step = [&](const char *from, int s) {
     bf16x8 b[T::P][T::TN];
 #pragma unroll
     for (int p = T::P - 1; p >= 0; p--) {
       bf16x8 a[T::TM];
+      if constexpr (T::APART && TA) {
+        static_assert(!T::APART || (T::WM / 32 == T::TM && T::WN / 32 == T::TN), "pieces 1 KB apart");
+        const unsigned at = lds_place(from), ia = at + wm * T::TM * 1024 + (s * T::P + p) * (T::BM / 32) * 1024;
+        const int q = T::P - 1 - p;
+        if constexpr (TB) {
+          const unsigned ib = at + T::PA + wn * T::TN * 1024 + (s * T::P + q) * (T::BN / 32) * 1024;
+          turned_pieces_apart(ia + lo_lane, ia + hi_lane, a, ib + lo_lane, ib + hi_lane, b[q]);
+        } else {
+          turned_pieces_apart(ia + lo_lane, ia + hi_lane, a);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < T::TM; i++) {
-        if constexpr (!TA) a[i] = *reinterpret_cast<const bf16x8 *>(from + a0 + (i * T::ROWB + (s * T::P + p) * 1024));
+        if constexpr (T::APART && TA) break;
+        else if constexpr (!TA) a[i] = *reinterpret_cast<const bf16x8 *>(from + a0 + (i * T::ROWB + (s * T::P + p) * 1024));
         else a[i] = turned_piece(from + wm * (T::WM / 32) * 1024 + ((s * T::P + p) * (T::BM / 32) + i) * 1024, lane);
       }
 #pragma unroll
       for (int j = 0; j < T::TN; j++) {
         const int q = T::P - 1 - p;
-        if constexpr (!TB) b[q][j] = *reinterpret_cast<const bf16x8 *>(from + b0 + (j * T::ROWB + (s * T::P + q) * 1024));
+        if constexpr (T::APART && TA && TB) break;
+        else if constexpr (!TB) b[q][j] = *reinterpret_cast<const bf16x8 *>(from + b0 + (j * T::ROWB + (s * T::P + q) * 1024));
         else b[q][j] = turned_piece(from + T::PA + wn * (T::WN / 32) * 1024 + ((s * T::P + q) * (T::BN / 32) + j) * 1024, lane);
       }
 #pragma unroll

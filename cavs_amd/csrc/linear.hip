@@ -8,7 +8,7 @@
 // generator is for.
 //
 // Measured, whole calls: bf16 8192 x 8192 x 4096 onto a residual with dropout 388 us, 1420 TFLOP/s (matrix pipe 72 % busy at the clock power leaves, 1.83 GHz); gradients of
-// 4096 x 2048 x 8192 through gelu and dropout 247 (products 200, 1370 TFLOP/s; D 50); fp32 gradients of 7088 x 512 x 2048 197 (products 146, 203 TFLOP/s of fp32;
+// 4096 x 2048 x 8192 through gelu and dropout 247 (products 200, 1370 TFLOP/s; D 50); fp32 gradients of 7088 x 512 x 2048 194 (products 143, 208 TFLOP/s of fp32;
 // packing 44; joining parts 12); one token of 2048 x 8192 in bf16 8.6, 3.9 TB/s. Gradients' products are bound by the matrix pipe, D and packing by HBM, few rows by W's bytes.
 #include <cmath>
 

@@ -85,15 +85,6 @@ struct DirectPieces {
   }
 };
 
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ bf16x8 both(u32x2 lo, u32x2 hi) { return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3)); }
-__device__ __forceinline__ unsigned lds_address(const char *p) {
-#ifdef __HIP_DEVICE_COMPILE__
-  return (unsigned)(size_t)(__attribute__((address_space(3))) const char *)p;
-#else
-  return 0;
-#endif
-}
 // turned pieces, all there when this returns (as is all that was read before): two or four blocks of sixteen rows, both steps
 __device__ __forceinline__ void turned_pieces(const char *from, const DirectPieces<2, true> &a, bf16x8 (&o)[2][2]) {
 #ifdef __HIP_DEVICE_COMPILE__

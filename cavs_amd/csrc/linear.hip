@@ -589,6 +589,7 @@ template <> struct Tiles<3> {
   using L = NtTile<3, 128, 128, 16, 2, 2>;
   using S = NtTile<3, 64, 64, 32, 2, 2>;
 };
+// (of the products here that turn operands)
 template <class T>
 struct Apart : T {
   static constexpr bool APART = true;

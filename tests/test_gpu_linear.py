@@ -381,6 +381,13 @@ def test_gradients_of_many_tiles(type_, n, K, N, act):
         assert torch.equal(c.run(1, names={k})[k], both[k]), k
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("n,K,N", [(1 << 20, 8, 8), (1 << 20, 3, 1), (8, 8, 1 << 20), (3, 1 << 16, 5)])
+def test_the_longest_sides(type_, n, K, N):
+    Case(type_, n, K, N, "silu").check()
+
+
 # ------------------------------------------------------------------ a block, as it is used
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_,n,H,F", [("f32", 37, 96, 200), ("bf16", 150, 128, 512), ("bf16", 1, 128, 512)])

@@ -280,6 +280,14 @@ def test_many_rows(n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+def test_the_most_rows(type_):
+    c = Case(type_, (1 << 22) - 1, 12, "rms", "layer", "rows")
+    c.hold(c.run_forward(), *c.forward())
+    c.hold(c.run_backward(c.names()), *c.backward())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("size,offset", [(1e18, 0.0), (1e-12, 0.0), (1.0, 3000.0), (1e25, 0.0)])
 def test_values_far_from_one_and_from_zero(size, offset):
     """squares beyond a float's range; means thousands of deviations from 0; deviations far below sqrt(eps)"""

@@ -363,6 +363,9 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void direct_back_kernel(DirectJo
   finish_direct<T>(g, split, nullptr, m0, n0, acc);
 }
 
+// D is rounded to bf16 before its two products, once (here and in grad_kernel<1>): what bf16 leaves off would be a second part in both, twice the instructions of the
+// matrix pipe, which has 200 of the 247 us of 4096 x 2048 x 8192.  There dX and dW are off by 0.00235 of their norm with it, by 0.00166, their own rounding,
+// without.  db is summed before it.
 // D as it lies (write: bf16, rows of N), and sums of its columns over 64 rows each [stretches of rows][N]; 256 columns a workgroup
 __global__ __launch_bounds__(256) void grad_rows_kernel(GradJob<u16> g, u16 *D) {
   __shared__ float part[8][256];

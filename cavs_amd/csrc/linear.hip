@@ -813,7 +813,13 @@ struct Call {
   int ldy, lddx, lddw;
   float *db;
   int n, K, N;
+  size_t room;  // bytes of the workspace
 };
+// (whoever chose the path and whoever sized the workspace agree, or nothing is launched)
+int check_room(const Call &c, size_t need) {
+  CAVS_REQUIRE(need <= c.room, "cavs_linear: a plan of %zu bytes for n=%d K=%d N=%d, a workspace of %zu", need, c.n, c.K, c.N, c.room);
+  return CAVS_OK;
+}
 
 inline dim3 grid_of(long blocks) {
   const long most = (1 << 24) - 1, high = (blocks + most - 1) / most;
@@ -874,8 +880,12 @@ int back_ends(const Call &c, const Plan &p, char *ws, const ColumnsJob &b, hipSt
 // rows that begin on 16 bytes and are whole pieces of eight, in reach of 32 bits from the first of a tile
 bool lies_well(const void *p, long ld, int w) { return aligned16(p) && ld % 8 == 0 && w % 8 == 0 && ld <= 1 << 22; }
 
+// Whether bf16 operands may lie well at all, whatever their strides and alignment: of what cavs_linear_workspace has room for
+bool may_lie_well(int K, int N, int back) { return K % 8 == 0 && (!back || N % 8 == 0); }
+
 int run_direct_fwd(const Call &c, char *ws, hipStream_t st) {
   const Plan p = direct_plan_of(c.n, c.K, c.N, 0);
+  if (const int rc = check_room(c, p.bytes)) return rc;
   float *part = reinterpret_cast<float *>(ws + p.part);
   const Forward<u16> out{c.b, c.act, c.m, static_cast<const u16 *>(c.R), c.ldr, static_cast<u16 *>(c.Zout), c.ldz, static_cast<u16 *>(c.Y), c.ldy};
   const DirectJob<Forward<u16>> g{{static_cast<const u16 *>(c.W), c.ldw}, {static_cast<const u16 *>(c.X), c.ldx}, c.N, c.n, c.K, p.fwd.tm, p.fwd.tn, p.fwd.kchunk,
@@ -889,6 +899,7 @@ int run_direct_fwd(const Call &c, char *ws, hipStream_t st) {
 
 int run_direct_bwd(const Call &c, char *ws, hipStream_t st) {
   const Plan p = direct_plan_of(c.n, c.K, c.N, 1);
+  if (const int rc = check_room(c, p.bytes)) return rc;
   const bool as_is = !c.act && !c.m.t && lies_well(c.dY, c.lddy, c.N);
   GradJob<u16> g{static_cast<const u16 *>(c.dY), static_cast<const u16 *>(c.Z), c.lddy, c.ldz, c.act, c.m, c.n, c.N, c.n, tiles_of(c.N, 256), 0,
                  {}, c.db ? reinterpret_cast<float *>(ws + p.sums) : nullptr};
@@ -929,6 +940,7 @@ int run_few(const Call &c, hipStream_t st) {
 template <int P, class T>
 int run_fwd(const Call &c, char *ws, hipStream_t st) {
   const Plan p = plan_of<P>(c.n, c.K, c.N, 0);
+  if (const int rc = check_room(c, p.bytes)) return rc;
   const PackJob<T> x = packing<P, T>(c.X, c.ldx, c.n, c.K, c.n, ws + p.x, p.Kp), w = packing<P, T>(c.W, c.ldw, c.N, c.K, c.N, ws + p.w, p.Kp);
   launch(pack_kernel<P, T>, grid_of((long)x.blocks + w.blocks), 256, 0, st, x, w);
   CAVS_LAUNCH_CHECK();
@@ -948,6 +960,7 @@ int run_fwd(const Call &c, char *ws, hipStream_t st) {
 template <int P, class T>
 int run_bwd(const Call &c, char *ws, hipStream_t st) {
   const Plan p = plan_of<P>(c.n, c.K, c.N, 1);
+  if (const int rc = check_room(c, p.bytes)) return rc;
   GradJob<T> g{static_cast<const T *>(c.dY), static_cast<const T *>(c.Z), c.lddy, c.ldz, c.act, c.m, c.n, c.N, p.np, p.Np / 64, 0,
                {c.dX || c.dW ? reinterpret_cast<u16 *>(ws + p.d) : nullptr, p.Np}, c.db ? reinterpret_cast<float *>(ws + p.sums) : nullptr};
   g.blocks = g.across * (p.np / 64);
@@ -1017,7 +1030,7 @@ size_t cavs_linear_workspace(int type, int n, int K, int N, int back) {
     return need;
   }
   if (back || !few_rows(type, n, K, N, packed_us<1>(n, K, N))) need = plan_of<1>(n, K, N, back).bytes;
-  if (K % 8 == 0 && (back ? N % 8 == 0 : !few_rows(type, n, K, N, direct_us(n, K, N)))) {
+  if (may_lie_well(K, N, back) && (back || !few_rows(type, n, K, N, direct_us(n, K, N)))) {
     const size_t direct = direct_plan_of(n, K, N, back).bytes;
     need = need > direct ? need : direct;
   }
@@ -1029,6 +1042,7 @@ int cavs_linear_fwd(int type, const void *X, int ldx, const void *W, int ldw, co
   const char *who = "cavs_linear_fwd";
   Call c{};
   c.X = X, c.ldx = ldx, c.W = W, c.ldw = ldw, c.b = b, c.act = act, c.R = R, c.ldr = ldr, c.Zout = Z, c.ldz = ldz, c.Y = Y, c.ldy = ldy, c.n = n, c.K = K, c.N = N;
+  c.room = workspace_bytes;
   if (const int rc = check(who, type, c, mask, &c.m)) return rc;
   CAVS_REQUIRE(ldy >= N && (!R || ldr >= N) && (!Z || ldz >= N), "%s: a row stride is below N=%d", who, N);
   if (n == 0) return CAVS_OK;
@@ -1037,7 +1051,7 @@ int cavs_linear_fwd(int type, const void *X, int ldx, const void *W, int ldw, co
   char *w = static_cast<char *>(workspace);
   hipStream_t st = as_stream(stream);
   if (type == CAVS_F32) return few_rows(type, n, K, N, packed_us<3>(n, K, N)) ? run_few<float>(c, st) : run_fwd<3, float>(c, w, st);
-  const bool direct = lies_well(X, ldx, K) && lies_well(W, ldw, K);
+  const bool direct = may_lie_well(K, N, 0) && lies_well(X, ldx, K) && lies_well(W, ldw, K);
   if (few_rows(type, n, K, N, direct ? direct_us(n, K, N) : packed_us<1>(n, K, N))) return run_few<u16>(c, st);
   return direct ? run_direct_fwd(c, w, st) : run_fwd<1, u16>(c, w, st);
 }
@@ -1048,7 +1062,7 @@ int cavs_linear_bwd(int type, const void *X, int ldx, const void *W, int ldw, co
   const char *who = "cavs_linear_bwd";
   Call c{};
   c.X = X, c.ldx = ldx, c.W = W, c.ldw = ldw, c.Z = Z, c.ldz = ldz, c.act = act, c.dY = dY, c.lddy = lddy, c.dX = dX, c.lddx = lddx, c.dW = dW, c.lddw = lddw;
-  c.db = db, c.n = n, c.K = K, c.N = N;
+  c.db = db, c.n = n, c.K = K, c.N = N, c.room = workspace_bytes;
   if (const int rc = check(who, type, c, mask, &c.m)) return rc;
   CAVS_REQUIRE(lddy >= N && (!act || ldz >= N) && (!dX || lddx >= K) && (!dW || lddw >= K), "%s: a row stride is below its width", who);
   hipStream_t st = as_stream(stream);
@@ -1065,8 +1079,8 @@ int cavs_linear_bwd(int type, const void *X, int ldx, const void *W, int ldw, co
   if (const int rc = check_workspace(who, workspace, workspace_bytes, cavs_linear_workspace(type, n, K, N, 1))) return rc;
   char *w = static_cast<char *>(workspace);
   if (type == CAVS_F32) return run_bwd<3, float>(c, w, st);
-  const bool direct = N % 8 == 0 && (!dW || lies_well(X, ldx, K)) && (!dX || lies_well(W, ldw, K));
-  return direct && (long)N <= 1 << 22 ? run_direct_bwd(c, w, st) : run_bwd<1, u16>(c, w, st);
+  const bool direct = may_lie_well(K, N, 1) && (!dW || lies_well(X, ldx, K)) && (!dX || lies_well(W, ldw, K));
+  return direct ? run_direct_bwd(c, w, st) : run_bwd<1, u16>(c, w, st);
 }
 
 }  // extern "C"

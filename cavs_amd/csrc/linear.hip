@@ -1005,7 +1005,6 @@ int check(const char *who, int type, const Call &c, const cavs_dropout_mask *mas
   CAVS_REQUIRE(c.n >= 0 && c.K > 0 && c.N > 0, "%s: bad shape n=%d K=%d N=%d", who, c.n, c.K, c.N);
   CAVS_REQUIRE(shape_ok(c.n, c.K, c.N), "%s: unsupported shape n=%d K=%d N=%d (at most 2^20, 2^16, 2^20; n N and N K 2^36)", who, c.n, c.K, c.N);
   CAVS_REQUIRE(c.act >= CAVS_ACT_NONE && c.act <= CAVS_ACT_GELU, "%s: unknown activation %d", who, c.act);
-  CAVS_REQUIRE(c.ldx >= c.K && c.ldw >= c.K, "%s: a row stride is below K=%d", who, c.K);
   CAVS_REQUIRE(mask_of(mask, m), "%s: p is not in [0, 1)", who);
   return CAVS_OK;
 }
@@ -1044,7 +1043,8 @@ int cavs_linear_fwd(int type, const void *X, int ldx, const void *W, int ldw, co
   c.X = X, c.ldx = ldx, c.W = W, c.ldw = ldw, c.b = b, c.act = act, c.R = R, c.ldr = ldr, c.Zout = Z, c.ldz = ldz, c.Y = Y, c.ldy = ldy, c.n = n, c.K = K, c.N = N;
   c.room = workspace_bytes;
   if (const int rc = check(who, type, c, mask, &c.m)) return rc;
-  CAVS_REQUIRE(ldy >= N && (!R || ldr >= N) && (!Z || ldz >= N), "%s: a row stride is below N=%d", who, N);
+  CAVS_REQUIRE((!X || ldx >= K) && (!W || ldw >= K), "%s: a row stride is below K=%d", who, K);
+  CAVS_REQUIRE((!Y || ldy >= N) && (!R || ldr >= N) && (!Z || ldz >= N), "%s: a row stride is below N=%d", who, N);
   if (n == 0) return CAVS_OK;
   CAVS_REQUIRE(X && W && Y, "%s: null pointer", who);
   if (const int rc = check_workspace(who, workspace, workspace_bytes, cavs_linear_workspace(type, n, K, N, 0))) return rc;
@@ -1064,7 +1064,9 @@ int cavs_linear_bwd(int type, const void *X, int ldx, const void *W, int ldw, co
   c.X = X, c.ldx = ldx, c.W = W, c.ldw = ldw, c.Z = Z, c.ldz = ldz, c.act = act, c.dY = dY, c.lddy = lddy, c.dX = dX, c.lddx = lddx, c.dW = dW, c.lddw = lddw;
   c.db = db, c.n = n, c.K = K, c.N = N, c.room = workspace_bytes;
   if (const int rc = check(who, type, c, mask, &c.m)) return rc;
-  CAVS_REQUIRE(lddy >= N && (!act || ldz >= N) && (!dX || lddx >= K) && (!dW || lddw >= K), "%s: a row stride is below its width", who);
+  // (of what is read and written: X for dW, W for dX, Z for the slope)
+  CAVS_REQUIRE((!dY || lddy >= N) && (!act || !Z || ldz >= N) && (!dW || !X || ldx >= K) && (!dX || !W || ldw >= K) && (!dX || lddx >= K) && (!dW || lddw >= K),
+               "%s: a row stride is below its width", who);
   hipStream_t st = as_stream(stream);
   if (!dX && !dW && !db) return CAVS_OK;
   if (n == 0) {  // sums over no rows

@@ -555,6 +555,8 @@ int check(const char *who, int type, const cavs_norm_desc *d, Norm *o) {
   CAVS_REQUIRE(!(d->gate && d->gate_rows), "%s: a gate is a row of values or a matrix, not both", who);
   CAVS_REQUIRE(d->eps > 0.f && d->eps < INFINITY, "%s: eps is not a positive number", who);
   *o = Norm{d->n, d->w, d->y, d->r, d->gate_rows, d->ldy, d->ldr, d->ldg, d->gate, d->scale, d->eps, d->post, d->pre, d->post_w, d->post_b, d->pre_w, d->pre_b};
+  if (!o->post) o->post_w = o->post_b = nullptr;  // (a norm that is not there has no weights, whatever the descriptor holds)
+  if (!o->pre) o->pre_w = o->pre_b = nullptr;
   return CAVS_OK;
 }
 
@@ -608,7 +610,7 @@ int cavs_norm_residual_bwd(int type, const cavs_norm_desc *d, const void *s, int
   if (!g->dy && !g->dgate && !g->dgate_rows && !g->dpost_w && !g->dpost_b) a.post = CAVS_NORM_NONE;  // (nothing behind it is wanted)
   const bool needs_y = g->dgate || g->dgate_rows || a.post;
   CAVS_REQUIRE(!needs_y || a.y, "%s: null pointer", who);
-  if (!dx) a.pre = CAVS_NORM_NONE;  // (nothing comes through it)
+  if (!dx) a.pre = CAVS_NORM_NONE, a.pre_w = nullptr;  // (nothing comes through it)
   if (!a.post) o.o[2] = o.o[3], o.o[3] = o.o[4] = nullptr;  // (in the order of the sums there are)
   const bool full = a.pre == CAVS_NORM_LAYER || a.post == CAVS_NORM_LAYER || g->dpre_b || g->dpost_b;
   const int groups = back_groups(a.n, a.w, a.post, full);

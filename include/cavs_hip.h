@@ -416,7 +416,7 @@ int cavs_dropout_advance(unsigned long long *step_word, unsigned long long by, v
 /* Norms after and before a block, its gate and the residual's scale, rows of w values:
  *   z = post(y);  s = r + scale * gate . z;  x = pre(s)
  * post, pre: CAVS_NORM_NONE (the values themselves), _RMS ((v / sqrt(mean v^2 + eps)) . weight + bias), _LAYER (((v - mean) / sqrt(var + eps)) . weight
- * + bias; var without a correction for the mean).  Weights [w] NULL: ones, biases [w] NULL: zeros, r NULL: zeros, gate: a row of values
+ * + bias; var without a correction for the mean).  Weights [w] NULL: ones, biases [w] NULL: zeros, either of CAVS_NORM_NONE: not read, r NULL: zeros, gate: a row of values
  * [w], a matrix gate_rows [n, w], or neither: ones.  A norm alone: y, pre, scale 1 and r, gate, s NULL.
  *   _fwd  s and x (either may be NULL), x from s before it is rounded.  s or x may be y, r or gate_rows, with their row stride, not each other.
  *   _bwd  from s as _fwd left it (read if pre is a norm and dx given), ds (the gradient of s from elsewhere) and dx (of x), either of which may be NULL:

@@ -67,7 +67,7 @@ __device__ __forceinline__ float slope_of(int act, float z) {
       return z == z ? 4.f * e * r * r : z;
     }
     case CAVS_ACT_SIGMOID: {
-      const float g = logistic<FAST>(fabsf(z));  // (even in z)
+      const float g = logistic<FAST>(-fabsf(z));  // (even in z, and on this side 1 - g loses nothing)
       return g * (1.f - g);
     }
     case CAVS_ACT_SILU: {

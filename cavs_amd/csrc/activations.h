@@ -59,11 +59,8 @@ __device__ __forceinline__ float slope_of(int act, float z) {
   switch (act) {
     case CAVS_ACT_RELU: return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;
     case CAVS_ACT_TANH: {
-      if constexpr (!FAST) {
-        const float h = tanhf(z);
-        return (1.f - h) * (1.f + h);
-      }
-      const float e = exp_fast(-2.f * fabsf(z)), r = __builtin_amdgcn_rcpf(1.f + e);
+      // (1 - tanh^2 = 4 e / (1 + e)^2, e = e^-2|z|: 1 - h of a tanh near 1 has lost what it is made of)
+      const float e = FAST ? exp_fast(-2.f * fabsf(z)) : expf(-2.f * fabsf(z)), r = FAST ? __builtin_amdgcn_rcpf(1.f + e) : 1.f / (1.f + e);
       return z == z ? 4.f * e * r * r : z;
     }
     case CAVS_ACT_SIGMOID: {

@@ -42,3 +42,13 @@ def test_sigmoid(type_):
     bound = 20 * U if type_ == "f32" else (4 * z.abs() + 16) * U
     assert bool(((got - want).abs() <= bound * want + 2.0 ** -122).all()), float(((got - want).abs() / want).max())
 
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+def test_tanh(type_):
+    z, got = _slopes(type_, "tanh", _far())
+    e = torch.exp(-2 * z.abs())
+    want = 4 * e / (1 + e).square()
+    bound = 24 * U if type_ == "f32" else (12 * z.abs() + 16) * U
+    assert bool(((got - want).abs() <= bound * want + 2.0 ** -122).all()), float(((got - want).abs() / want).max())

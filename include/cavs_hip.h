@@ -464,7 +464,8 @@ int cavs_norm_residual_bwd(int type, const cavs_norm_desc *d, const void *s, int
  * b, R and mask may be NULL; Z NULL: not kept (_bwd reads it unless act is CAVS_ACT_NONE, _fwd writes it; Y is made of Z before it is rounded).  What is
  * NULL of dX, dW and db is not computed (_bwd reads X for dW, W for dX).  Y may be R, with its row stride; otherwise outputs may overlap neither inputs nor each other.
  * CAVS_F32: products as sums of bf16 parts in full fp32 precision (the arithmetic of cavs_sgemm).  CAVS_BF16: products of bf16 values in fp32 accumulators; D
- * is rounded to bf16 between its products (not in db), results once.
+ * is rounded to bf16 before its products, results once; db is summed from D before that, whose act' has errors of 2^-19 (far from 0, where it is small, of 2^-22 |z| of
+ * it, gelu's of 2^-22 z^2).
  * At most 2^20 rows, N <= 2^20, K <= 2^16, n N and N K <= 2^36.  n = 0 is allowed (dW and db become 0).
  * The workspace: 16-byte aligned, at least cavs_linear_workspace(type, n, K, N, back) bytes on this device (back: 0 for _fwd; 0: the shape or type is
  * refused; what any alignment and stride of the operands takes, and 256 where a forward pass of few rows takes none); for the next call on the same stream to

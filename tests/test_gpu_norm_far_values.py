@@ -1,0 +1,21 @@
+"""Norms of values near the type's largest (cavs_norm_residual_*): finite rows have finite results, with the bounds of any other row."""
+import pytest
+
+from test_gpu_norm_residual import Case, torch
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("w", [3, 9, 300, 2500])
+def test_values_of_the_largest_size(type_, kind, w):
+    """the largest value on one side of 0 and its negative on the other, few against many: a difference from the mean may be twice the largest value"""
+    c = Case(type_, 6, w, kind, kind, "none", residual=False, scale=1.0, bias=False)
+    most = torch.finfo(c.t).max
+    for v in (c.y, c.s):
+        v[:3], v[0, :], v[1, :], v[2, 1::2], v[2, ::2] = 0.0, -most, most, -most, most
+        v[0, 0], v[1, w // 2] = most, -most
+        v[3, :], v[3, w - 1] = 0.0, -most
+    names = [k for k in c.names() if not k.endswith("_b")]
+    c.hold(c.run_forward(), *c.forward())
+    c.hold(c.run_backward(names), *c.backward())

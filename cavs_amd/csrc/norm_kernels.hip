@@ -331,7 +331,7 @@ __global__ __launch_bounds__(back_threads<L>(), back_ahead(L, POST, FULL) ? 2 : 
     for (int k = 0; k < K; k++) t[k] = 0.;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      float pw[8], sv[8], yv[8], hs = 0.f;
+      float pw[8], sv[8], yv[8];
       weights(0, i, pw);
 #pragma unroll
       for (int e = 0; e < 8; e++) sv[e] = s[i][e], yv[e] = y[i][e];
@@ -344,16 +344,14 @@ __global__ __launch_bounds__(back_threads<L>(), back_ahead(L, POST, FULL) ? 2 : 
       for (int e = 0; e < 8; e++) {
         const double v = sv[e];
         const float h = dx[i][e] * pw[e];
-        t[SS] += v * v;
-        if constexpr (FULL) t[HS] += h * v, t[S1] += v, t[H1] += h;
-        else hs += h * sv[e];
+        t[SS] += v * v, t[HS] += h * v;
+        if constexpr (FULL) t[S1] += v, t[H1] += h;
         if constexpr (POST) {
           const double u = yv[e];
           t[YY] += u * u;
           if constexpr (FULL) t[Y1] += u;
         }
       }
-      if constexpr (!FULL) t[HS] += hs;
     }
     row_sums<L>(t, part[POST ? 0 : turn]);  // (of two calls a row, or one: never the place of the call before)
     Stats pre{0.f, 0.f, 4.f, 1.f}, post{};
@@ -370,7 +368,7 @@ __global__ __launch_bounds__(back_threads<L>(), back_ahead(L, POST, FULL) ? 2 : 
     double q[FULL ? 2 : 1] = {};
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      float w[8], D[8], qy = 0.f;
+      float w[8], D[8];
       weights(0, i, w);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
@@ -402,10 +400,9 @@ __global__ __launch_bounds__(back_threads<L>(), back_ahead(L, POST, FULL) ? 2 : 
             if constexpr (FULL) acc[POST_B][i][e] += dz[i][e];
           }
           dz[i][e] *= w[e];
-          if constexpr (FULL) q[0] += (double)dz[i][e] * y[i][e], q[FULL ? 1 : 0] += dz[i][e];
-          else qy += dz[i][e] * y[i][e];
+          q[0] += (double)dz[i][e] * y[i][e];
+          if constexpr (FULL) q[FULL ? 1 : 0] += dz[i][e];
         }
-        if constexpr (!FULL) q[0] += qy;
       } else {
 #pragma unroll
         for (int e = 0; e < 8; e++) D[e] *= y[i][e];

@@ -19,3 +19,17 @@ def test_values_of_the_largest_size(type_, kind, w):
     names = [k for k in c.names() if not k.endswith("_b")]
     c.hold(c.run_forward(), *c.forward())
     c.hold(c.run_backward(names), *c.backward())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("post,pre", [("none", "rms"), ("rms", "rms"), ("rms", "none")])
+@pytest.mark.parametrize("w", [7, 300, 2048])
+def test_gradients_whose_products_are_beyond_a_float(type_, post, pre, w):
+    """values of 10^25 under gradients of 10^18: their products' sum is part of a row's, their gradient is a float"""
+    c = Case(type_, 11, w, post, pre, "column", size=1e25)
+    c.ds.mul_(1e20), c.dx.mul_(1e20)
+    names = [k for k in c.names() if not k.endswith("_b")]
+    if post == "none":
+        names.remove("dgate")  # (10^25 times 10^18 is no float)
+    c.hold(c.run_backward(names), *c.backward())

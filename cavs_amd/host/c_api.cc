@@ -93,6 +93,17 @@ int cavs_session_get_grad(cavs_session *s, const char *name, float *host, size_t
   return guarded([&] { s->engine.get_param(name, host, n, true); });
 }
 
+int cavs_session_get_dropout_steps(cavs_session *s, unsigned long long *steps) {
+  if (int rc = need(s, "session")) return rc;
+  if (int rc = need(steps, "output")) return rc;
+  return guarded([&] { *steps = s->engine.dropout_steps(); });
+}
+
+int cavs_session_set_dropout_steps(cavs_session *s, unsigned long long steps) {
+  if (int rc = need(s, "session")) return rc;
+  return guarded([&] { s->engine.set_dropout_steps(steps); });
+}
+
 int cavs_session_step(cavs_session *s, const int *graph, int B, int maxlen, const void *x,
                       const void *labels, int inputs_on_device, int backward, float lr) {
   if (int rc = need(s, "session")) return rc;

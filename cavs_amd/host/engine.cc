@@ -2836,6 +2836,21 @@ cavs_dropout_mask Engine::dropout_mask(unsigned long long place) const {
   return {cfg_.dropout, cfg_.dropout_seed + (place << 32), 0, drop_step_.get(), nullptr};
 }
 
+unsigned long long Engine::dropout_steps() {
+  if (cfg_.dropout <= 0.f) fail(CAVS_EINVAL, "the session drops nothing and counts no steps for it");
+  sync();
+  unsigned long long steps = 0;
+  check(cavs_memcpy_d2h(&steps, drop_step_.get(), sizeof steps, stream_));
+  check(cavs_stream_sync(stream_));
+  return steps;
+}
+
+void Engine::set_dropout_steps(unsigned long long steps) {
+  if (cfg_.dropout <= 0.f) fail(CAVS_EINVAL, "the session drops nothing and counts no steps for it");
+  check(cavs_memcpy_h2d(drop_step_.get(), &steps, sizeof steps, stream_));
+  check(cavs_stream_sync(stream_));
+}
+
 // From what the vertices push to what the head reads.  (The columns that padding adds are zeros, and stay so.)
 void Engine::before_head(bool backward) {
   const int N = N_, H = cfg_.H, h = uH_, F = cfg_.block;

@@ -87,6 +87,8 @@ class Engine {
   }
   void set_param(const std::string &name, const float *host, size_t n);
   void get_param(const std::string &name, float *host, size_t n, bool grad);
+  unsigned long long dropout_steps();
+  void set_dropout_steps(unsigned long long steps);
   void step(const int *graph, int B, int maxlen, const void *x, const void *labels,
             bool on_device, bool backward, float lr);
   void sync();

@@ -59,6 +59,8 @@ def lib():
             "cavs_schedule_group_lists": [P, I, I, I, I, I, I, I, I, I, P, P, I],
             "cavs_schedule_trace_from_lists": [I, I, I, I, P, I, P, P, P, P, I, P, I],
             "cavs_session_timing": [P, C.c_char_p, C.POINTER(F)],
+            "cavs_session_get_dropout_steps": [P, C.POINTER(C.c_ulonglong)],
+            "cavs_session_set_dropout_steps": [P, C.c_ulonglong],
             "cavs_session_counter": [P, C.c_char_p, C.POINTER(C.c_double)],
             "cavs_session_profile": [P, I],
             "cavs_session_profile_read": [P, C.c_char_p, C.POINTER(C.c_double), C.POINTER(C.c_double)],
@@ -203,7 +205,7 @@ class Session:
     is the parameter "W.momentum" / "U.momentum" (`param`, `set_params`); ortho_lr 0 is step's lr, ortho_momentum 0 is 0.95,
     negative none.
     dropout: the share of what the vertices push that is dropped before the softmax head in steps with a backward pass, drawn from
-    dropout_seed, the number of such steps before this one, the vertex and the column (`cavs_dropout`).
+    dropout_seed, the number of such steps before this one (`dropout_steps`, for checkpoints), the vertex and the column (`cavs_dropout`).
     block: the inner width of a residual block before the head, h + drop(drop(act(rms(h) Wup^T + bup)) Wdown^T + bdown), with the
     parameters "gnorm" [H], "Wup" [block, H], "bup", "Wdown" [H, block], "bdown"; dropout is then of the block, not of the head's input."""
 
@@ -249,6 +251,18 @@ class Session:
         a = np.empty(shape, np.float32)
         _check(lib().cavs_session_get_grad(self._h, name.encode(), a.ctypes.data, a.size), f"get_grad({name})")
         return a
+
+    @property
+    def dropout_steps(self):
+        """The steps with a backward pass so far, which dropout's masks are drawn from (of sessions with dropout): goes into a checkpoint, and is set in the
+        session that goes on from it"""
+        n = C.c_ulonglong()
+        _check(lib().cavs_session_get_dropout_steps(self._h, C.byref(n)), "cavs_session_get_dropout_steps")
+        return n.value
+
+    @dropout_steps.setter
+    def dropout_steps(self, n):
+        _check(lib().cavs_session_set_dropout_steps(self._h, n), "cavs_session_set_dropout_steps")
 
     def step(self, graph, x=None, labels=None, backward=True, lr=0.0):
         """x / labels: numpy arrays (host feeds) or torch CUDA tensors (already in HBM)."""

@@ -113,7 +113,7 @@ typedef struct {
   float ortho_momentum; /* 0 = 0.95, negative = none */
   float ortho_decay;    /* weight decay */
   /* Softmax loss: the share of what the vertices push that is dropped before the head in steps with a backward pass (cavs_dropout; vertex i, declared column j, p = dropout,
-   * seed = dropout_seed, step = the session's steps with a backward pass before this one).  0 = none, below 1.  "graph_out" is what was pushed, "dgraph_out" its gradient; steps
+   * seed = dropout_seed, step = the session's steps with a backward pass before this one, cavs_session_set_dropout_steps).  0 = none, below 1.  "graph_out" is what was pushed, "dgraph_out" its gradient; steps
    * without a backward pass drop nothing.  The head runs in one piece then (head_chunks). */
   float dropout;
   unsigned dropout_seed;
@@ -142,6 +142,10 @@ int cavs_session_destroy(cavs_session *s);
 int cavs_session_set_param(cavs_session *s, const char *name, const float *host, size_t n);
 int cavs_session_get_param(cavs_session *s, const char *name, float *host, size_t n);
 int cavs_session_get_grad(cavs_session *s, const char *name, float *host, size_t n);
+/* The steps with a backward pass that a session with dropout has made, which its masks are drawn from (synchronises): part of a checkpoint, and set in the session that goes
+ * on from there.  Of a session without dropout both are refused. */
+int cavs_session_get_dropout_steps(cavs_session *s, unsigned long long *steps);
+int cavs_session_set_dropout_steps(cavs_session *s, unsigned long long steps);
 
 /* One pass of F over the batch (C_Run of the train op, cavs/frontend/c_api.cc:149-172):
  * schedule, forward rounds, loss head, and if `backward` the gradient rounds and the

@@ -1,7 +1,7 @@
 // Y = R + drop(act(X W^T + b)) and its gradients: products with everything that follows them in their epilogue.
 //
 //   forward   Z = X W^T + b, Y = R + drop(act(Z))
-//   backward  D = drop(dY) . act'(Z), dX = D W, dW = D^T X, db = sums of D's columns
+//   backward  D = drop(dY . act'(Z)), dX = D W, dW = D^T X, db = sums of D's columns
 //
 // Tiles are made of the transposed product, so that a lane of the 32x32 instruction holds neighbouring values of a row of the result: after an
 // exchange with the lane 32 away eight of them, which is what bias, residual and results are read and written in, and what one call of the dropout's
@@ -182,10 +182,10 @@ __global__ __launch_bounds__(256) void grad_kernel(GradJob<T> g, PackJob<T> x, P
     }
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = d[e];
+    for (int e = 0; e < 8; e++) v[e] = g.act ? d[e] * slope_of<P == 1>(g.act, z[e]) : d[e];
     if (g.m.t && left > 0) drop8(g.m, draws_of(g.m, step, row_id(g.m, row), col >> 3), v);
 #pragma unroll
-    for (int e = 0; e < 8; e++) tile[r][8 * piece + e] = e < left ? g.act ? v[e] * slope_of<P == 1>(g.act, z[e]) : v[e] : 0.f;
+    for (int e = 0; e < 8; e++) tile[r][8 * piece + e] = e < left ? v[e] : 0.f;
   }
   __syncthreads();
   if (g.o.p) pack_tile<P>(tile, g.o, PackedOut{}, r0, k0, g.orows, g.N);
@@ -392,11 +392,11 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(GradJob<u16> g, u16 *D) 
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] = d[i][e];
-        if (g.m.t) drop8(g.m, draws_of(g.m, step, row_id(g.m, row), col >> 3), v);
         if (g.act) {
 #pragma unroll
           for (int e = 0; e < 8; e++) v[e] *= slope_of<true>(g.act, z[i][e]);
         }
+        if (g.m.t) drop8(g.m, draws_of(g.m, step, row_id(g.m, row), col >> 3), v);
 #pragma unroll
         for (int e = 0; e < 8; e++) s[e] += v[e];
         if (D) Eight<u16>::store(D + (long)row * g.N + col, v, 8);

@@ -460,7 +460,7 @@ int cavs_norm_residual_bwd(int type, const cavs_norm_desc *d, const void *s, int
 
 /* FullyConnected (cavs/backend/op_impl_fullyconnected_cublas.cc:71-79, gradients :150-163) with what follows it:
  *   Z = X W^T + b;  Y = R + drop(act(Z))            X [n,K], W [N,K], b [N], Z and R and Y [n,N]
- *   D = drop(dY) . act'(Z);  dX = D W;  dW = D^T X;  db = sum of D's rows;  the gradient of R is dY
+ *   D = drop(dY . act'(Z));  dX = D W;  dW = D^T X;  db = sum of D's rows;  the gradient of R is dY
  * b, R and mask may be NULL; Z NULL: not kept (_bwd reads it unless act is CAVS_ACT_NONE, _fwd writes it; Y is made of Z before it is rounded).  What is
  * NULL of dX, dW and db is not computed (_bwd reads X for dW, W for dX).  Y may be R, with its row stride; otherwise outputs may overlap neither inputs nor each other.
  * CAVS_F32: products as sums of bf16 parts in full fp32 precision (the arithmetic of cavs_sgemm).  CAVS_BF16: products of bf16 values in fp32 accumulators; D

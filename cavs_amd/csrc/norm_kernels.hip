@@ -6,8 +6,8 @@
 //   d weight = sum over rows of d x . v^,  d bias = sum over rows of d x
 //
 // A row is held by L lanes, eight neighbouring values of each in registers, so that memory is read and written once.  The sums of a row are made in 64
-// bits: of values and squares at once (mean and variance from one trip across the lanes, without loss for any mean below 2^20 deviations), and squares of any float
-// fit.  Bound by HBM, of few rows by the trips across the lanes: fp32 7088 x 512 forward 11.4 us, 5.1 TB/s; bf16 gradients of 16384 x 4096 168, 4.8 TB/s, arithmetic 61 %
+// bits: of values and squares at once (mean and variance from one trip across the lanes; a mean of 2^13 deviations costs nothing, beyond that 1 / deviation is off by
+// 2^-52 (mean / deviation)^2 of it, 2^-12 at 2^20), and squares of any float fit.  Bound by HBM, of few rows by the trips across the lanes: fp32 7088 x 512 forward 11.5 us, 5.0 TB/s; bf16 gradients of 16384 x 4096 169, 4.8 TB/s, arithmetic 64 %
 // busy; fp32 gradients of 2371 x 1001 with everything 25, 3.0 TB/s (198 workgroups of three turns, and a launch for the sums).
 #include <cmath>
 #include <type_traits>

@@ -423,7 +423,7 @@ int cavs_dropout_advance(unsigned long long *step_word, unsigned long long by, v
  *         D = ds + d<pre(s), dx>/ds;  dr = D;  dgate = scale z . D (of a row of values the sum over rows);  dy, dpost_w, dpost_b through
  *         dz = scale gate . D;  dpre_w, dpre_b: sums over rows.  What is NULL is not computed; r and, where nothing needs it, y are not read.
  *         dr may be ds, dx or s, dy may be y, dgate_rows may be gate_rows, with their row stride; otherwise what is written may overlap nothing else.
- * Sums of a row, and its mean, variance and their like, in 64 bits; sums over rows in fp32, per workgroup and then across them.  w <= 16384, n < 2^22.
+ * Sums of a row, and its mean, variance and their like, in 64 bits (of a mean beyond 2^13 deviations 1 / deviation is off by 2^-52 (mean / deviation)^2); sums over rows in fp32, per workgroup and then across them.  w <= 16384, n < 2^22.
  * n = 0 is allowed (gradients that are sums become 0).  An infinity or a NaN in a row makes NaN of what depends on the row.
  * The workspace of _bwd: 16-byte aligned, at least cavs_norm_residual_workspace(n, w) bytes on this device (not read where no sums over rows are wanted);
  * for the next call on the same stream to reuse, not for one that overlaps in time. */

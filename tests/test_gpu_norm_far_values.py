@@ -33,3 +33,12 @@ def test_gradients_whose_products_are_beyond_a_float(type_, post, pre, w):
     if post == "none":
         names.remove("dgate")  # (10^25 times 10^18 is no float)
     c.hold(c.run_backward(names), *c.backward())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [8192.0, -8000.0])
+def test_means_thousands_of_deviations_from_zero(offset):
+    """as far as sums of values and of their squares in 64 bits give a deviation a float's rounding"""
+    c = Case("f32", 40, 777, "layer", "layer", "none", residual=False, offset=offset, scale=1.0)
+    c.hold(c.run_forward(), *c.forward())
+    c.hold(c.run_backward(c.names()), *c.backward())

@@ -7,9 +7,9 @@
 // exchange with the lane 32 away eight of them, which is what bias, residual and results are read and written in, and what one call of the dropout's
 // generator is for.
 //
-// Measured, whole calls: bf16 8192 x 8192 x 4096 onto a residual with dropout 388 us, 1420 TFLOP/s (matrix pipe 72 % busy at the clock power leaves, 1.83 GHz); gradients of
-// 4096 x 2048 x 8192 through gelu and dropout 247 (products 200, 1370 TFLOP/s; D 50); fp32 gradients of 7088 x 512 x 2048 194 (products 143, 208 TFLOP/s of fp32;
-// packing 44; joining parts 12); one token of 2048 x 8192 in bf16 8.6, 3.9 TB/s. Gradients' products are bound by the matrix pipe, D and packing by HBM, few rows by W's bytes.
+// Measured, whole calls: bf16 8192 x 8192 x 4096 onto a residual with dropout 386 us, 1420 TFLOP/s (matrix pipe 72 % busy at the clock power leaves, 1.83 GHz); gradients of
+// 4096 x 2048 x 8192 through gelu and dropout 245 (products 198, 1390 TFLOP/s; D 50); fp32 gradients of 7088 x 512 x 2048 194 (products 140, 212 TFLOP/s of fp32;
+// packing 45; joining parts 12); one token of 2048 x 8192 in bf16 8.6, 3.9 TB/s. Gradients' products are bound by the matrix pipe, D and packing by HBM, few rows by W's bytes.
 #include <cmath>
 
 #include "activations.h"
@@ -364,7 +364,7 @@ __global__ __launch_bounds__(T::THREADS, T::EU) void direct_back_kernel(DirectJo
 }
 
 // D is rounded to bf16 before its two products, once (here and in grad_kernel<1>): what bf16 leaves off would be a second part in both, twice the instructions of the
-// matrix pipe, which has 200 of the 247 us of 4096 x 2048 x 8192.  There dX and dW are off by 0.00235 of their norm with it, by 0.00166, their own rounding,
+// matrix pipe, which has 198 of the 245 us of 4096 x 2048 x 8192.  There dX and dW are off by 0.00235 of their norm with it, by 0.00166, their own rounding,
 // without.  db is summed before it.
 // D as it lies (write: bf16, rows of N), and sums of its columns over 64 rows each [stretches of rows][N]; 256 columns a workgroup
 __global__ __launch_bounds__(256) void grad_rows_kernel(GradJob<u16> g, u16 *D) {
@@ -778,11 +778,11 @@ Plan direct_plan_of(int n, int K, int N, int back) {
 }
 
 // Whether a forward pass reads W where it lies (few_rows_kernel) or goes by tiles.  ns a k of its workgroups, one a compute unit: bf16 1.0 + 0.05 a row of X,
-// fp32 3.0 + 0.04 and 0.0013 a row squared (8192 x 2048 with 1, 16, 32, 64 rows: 1.0 1.6 2.5 4.2, 3.2 3.7 5.6 10.8); tiles cost what their model says, and what packing W and X takes.  us of
-// few rows / of tiles: bf16 2048 x 8192 with 1 row 6.9 / 10.8, 16 9.5 / 11.7, 64 20 / 15.5; 8192 x 2048 with 16 16 / 13.4; 1000 x 1000 with 157 5.8 / 13.6, 512
+// fp32 3.0 + 0.04 and 0.0013 a row squared (8192 x 2048 with 1, 16, 32, 64 rows: 1.0 1.6 2.5 4.2, 3.2 3.7 5.6 10.8); tiles cost what their model says, and what packing W and X takes.  us, without bias and
+// what follows it, of few rows (64 a workgroup) / of tiles: bf16 2048 x 8192 with 1 row 6.9 / 10.8, 16 9.5 / 11.7, 64 20 / 15.5; 8192 x 2048 with 16 16 / 13.4; 1000 x 1000 with 157 5.8 / 13.6, 512
 // 10.5 / 14.1; 512 x 2048 with 512 12.4 / 8.4; fp32 2048 x 8192 with 1 16 / 46, 32 29 / 48, 64 50 / 48; 300 x 777 with 157 7.1 / 12.3, 512 x 2048 with 256 15.5 / 17.7.
-// Rows of a workgroup, 16, 32 or 64, by the same figures: where 64 leave compute units idle W is read by more of them (from the caches).  us of 64 / of what this takes: fp32
-// 157 x 300 x 777 7.1 / 5.6, 98 x 1918 x 352 18 / 9.3, 40 x 2048 x 2048 24 / 16, 32 x 8192 x 2048 50 / 35, bf16 64 x 4096 x 640 11 / 9.
+// Rows of a workgroup, 16, 32 or 64, by the same figures: where 64 leave compute units idle W is read by more of them (from the caches).  us, so, of 64 / of what this takes:
+// fp32 157 x 300 x 777 7.1 / 5.6, 98 x 1918 x 352 18 / 8.8, 40 x 2048 x 2048 24 / 17, 32 x 8192 x 2048 50 / 35, bf16 64 x 4096 x 640 11 / 9.
 struct Few {
   int blocks;  // of sixteen rows of X, of a workgroup: 1, 2 or 4
   double us;

@@ -226,8 +226,8 @@ void *cavs_session_stream(cavs_session *s);
  * of the last step. keys: "gather_rows" "scatter_rows" "gemm_flops" (separate GEMM launches: 2*M*N*K
  * of the reference's products) "gemm_flops_hinted" (the part of those that multiplies blocks known
  * to be zero or unused -- the forget-gate columns of the leaves -- and is skipped tile by tile)
- * "round_flops" (products inside fused round launches) "rounds" "launches" (the head without logits, several of them, counts as
- * one); "tail_rounds" (rounds,
+ * "round_flops" (products inside fused round launches) "rounds" "launches" (the head without logits, and each call of the block's
+ * operators, several of them, count as one); "tail_rounds" (rounds,
  * forward and backward, that ran inside cavs_treelstm_tail_* launches) "tail_launches"; "plan_hits" /
  * "plan_misses" of the plan cache since the session was created; "scheduler" (who produced the last
  * step's lists: 0 host scheduler, 1 device scheduler, 2 plan cache); "tail_ready" (1 when the session may

@@ -143,7 +143,7 @@ int cavs_session_set_param(cavs_session *s, const char *name, const float *host,
 int cavs_session_get_param(cavs_session *s, const char *name, float *host, size_t n);
 int cavs_session_get_grad(cavs_session *s, const char *name, float *host, size_t n);
 /* The steps with a backward pass that a session with dropout has made, which its masks are drawn from (synchronises): part of a checkpoint, and set in the session that goes
- * on from there.  Of a session without dropout both are refused. */
+ * on from there.  Steps whose updates were skipped, as the error of a launch that gave up says, are counted too.  Of a session without dropout both are refused. */
 int cavs_session_get_dropout_steps(cavs_session *s, unsigned long long *steps);
 int cavs_session_set_dropout_steps(cavs_session *s, unsigned long long steps);
 
